@@ -365,6 +365,94 @@ int rf_decode_attention(const float* dQ, const uint16_t* dK, const uint16_t* dV,
 int rf_decode_attention_noalloc(const float* dQ, const uint16_t* dK, const uint16_t* dV, int ctx, int n_heads,
                                 int n_kv_heads, int head_dim, int batch, float* dOut, void* stream);
 
+/* ---- verification of drafted tokens (speculative decoding) -------------------------
+ * One pass over the weights can check several drafted tokens at once: their queries
+ * and keys are normalised and rotated (rf_qk_norm_rope), their K/V rows go into the
+ * cache behind the history (rf_kv_cache_write), every drafted token attends to the
+ * history and to its own ancestors (rf_tree_attention), and after the choice the rows
+ * of the accepted path are written again at consecutive positions, the others with
+ * position -1.  No counterpart in the reference (one token per forward).
+ *
+ * All pointers are device pointers; nothing is copied to or from the host and no call
+ * waits for the GPU, so every call can be captured in a CUDA graph.  Calls on
+ * different streams are independent of one another.  Strides are elements between two
+ * tokens' rows (0: rows without gaps); a token's heads are contiguous, [head][head_dim].
+ * Values that live on the device (positions, lengths) are checked there: a row whose
+ * position or length is out of range is left out and raises rf_verify_error_word. */
+
+/* element types of activations (ggml ids; bf16 is no weight type of the engine) */
+#define RF_ACT_F32 0
+#define RF_ACT_F16 1
+#define RF_ACT_BF16 30
+
+/* Per-head RMS norm and position rotation of queries and keys, one pass:
+ * y = x / sqrt(mean(x^2) + eps) * w per head, where the weight (head_dim f32) is given
+ * (NULL: y = x); then, for i < rot_dim / 2 and (c, s) = rope[position][i],
+ *   out[i] = y[i] c - y[i + rot_dim/2] s,  out[i + rot_dim/2] = y[i] s + y[i + rot_dim/2] c
+ * (the engine's half-split rotation, compute.rs:440-456), and out[i] = y[i] from rot_dim on.
+ * f32 arithmetic, one rounding to `act_type` at the end.
+ * q [n_tokens][n_heads][head_dim], k [n_tokens][n_kv_heads][head_dim] (k and k_out may be
+ * NULL with n_kv_heads 0); the outputs may be the inputs themselves with the same strides,
+ * any other overlap is undefined.  head_dim even, 2..256; rot_dim even, 0..head_dim
+ * (rope and positions may be NULL at 0).  rope: [rope_len][rot_dim/2][cos, sin] f32, 8-byte
+ * aligned; positions: n_tokens int32 in [0, rope_len), else the token's rows are not written. */
+int rf_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int act_type, uint32_t n_tokens,
+                    uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint64_t q_stride, uint64_t k_stride,
+                    uint64_t q_out_stride, uint64_t k_out_stride, const float* q_norm, const float* k_norm, float eps,
+                    const float* rope, uint32_t rope_len, uint32_t rot_dim, const int32_t* positions, void* stream);
+
+/* One layer's K/V cache in the caller's memory, head-major like the engine's:
+ *   RF_TYPE_F16   k, v: [seq][kv_head][position][head_dim] f16; scales NULL
+ *   RF_TYPE_Q8_0  k, v: the same shape in int8; k_scale, v_scale:
+ *                 [seq][kv_head][position][head_dim/32] f16
+ * Q8_0 is GGUF's block (32 elements, one f16 scale) with the scales in a plane of their
+ * own, so that rows stay 16-byte aligned.  The value of a code is code * scale rounded to
+ * f16, here as in every reader.  head_dim: a multiple of 32 up to 256.  All planes are
+ * 16-byte aligned. */
+typedef struct rf_kv_view {
+  int type;
+  uint32_t n_seqs, n_kv_heads, head_dim, capacity; /* capacity: positions per sequence */
+  void *k, *v, *k_scale, *v_scale;
+} rf_kv_view;
+
+/* Row r (k, v: [n_rows][n_kv_heads][head_dim], 16-byte aligned rows) goes to position
+ * pos[r] of sequence seq[r] (seq NULL: sequence 0).  pos[r] < 0: the row is not kept.  Two
+ * rows of one call must not name the same place.
+ * Q8_0: x is limited to +-65472 (so that every value read back is a finite f16); per 32
+ * elements a = max|x|, scale = f16(a / 127), code = rint(x * (1 / scale)) limited to +-127,
+ * 0 where the scale is 0.  A block that holds a NaN gets a NaN scale.  F16: rounded to
+ * nearest, beyond 65504 to infinity. */
+int rf_kv_cache_write(const rf_kv_view* cache, const void* k, const void* v, int act_type, uint32_t n_rows,
+                      uint64_t k_stride, uint64_t v_stride, const int32_t* seq, const int32_t* pos, void* stream);
+/* The same rows back (kv_cache.rs:452-480 get_k_range / get_v_range over any positions);
+ * k_out or v_out may be NULL.  Rows with pos[r] < 0 read as zeros. */
+int rf_kv_cache_read(const rf_kv_view* cache, void* k_out, void* v_out, int act_type, uint32_t n_rows,
+                     uint64_t k_stride, uint64_t v_stride, const int32_t* seq, const int32_t* pos, void* stream);
+
+/* Attention of n_tokens drafted tokens of each of n_seqs sequences (sequence b of the
+ * cache) over its history and over the drafts:
+ *   out[t] = sum_p softmax_p(scale * q[t] . k[p]) v[p]
+ * over the positions p < hist_len[b], which every token sees, and the drafts' own
+ * positions p = hist_len[b] + j, j < n_draft[b], where bit j%32 of
+ * mask[(b * n_tokens + t) * ceil(n_tokens/32) + j/32] is set.  mask NULL: a chain, j <= t.
+ * n_draft NULL: n_tokens each.  Tokens t >= n_draft[b], and tokens that see nothing, get
+ * zeros.  What a token does not see never reaches its output, whatever the cache holds
+ * there (NaN included).
+ * q, out [n_seqs * n_tokens][n_heads][head_dim], 16-byte aligned rows; n_heads a multiple of
+ * the cache's n_kv_heads (any group size); head_dim 64 or 128 (RF_EUNSUPPORTED otherwise);
+ * 1 <= n_tokens <= 1024.  scale > 0, or 0 for 1/sqrt(head_dim).  f32 sums and softmax; f32
+ * queries and probabilities enter the products with 22 bits, f16 and bf16 ones with 11.
+ * Sequences whose lengths do not fit the cache get zeros and raise the error word.
+ * Scratch for split histories comes from the library's own stream-ordered memory pool. */
+int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act_type, uint32_t n_seqs,
+                      uint32_t n_tokens, uint32_t n_heads, uint64_t q_stride, uint64_t out_stride,
+                      const int32_t* hist_len, const int32_t* n_draft, const uint32_t* mask, float scale,
+                      void* stream);
+/* Error word of the four calls above on the current device (synchronises it, reads, clears):
+ * bit 0 = a bounded wait of rf_tree_attention gave up, so some output since the last read is
+ * unspecified; bit 1 = a position, sequence or length on the device was out of range. */
+int rf_verify_error_word(uint32_t* word);
+
 #ifdef __cplusplus
 }
 #endif

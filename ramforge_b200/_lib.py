@@ -21,6 +21,7 @@ ERROR_NAMES = {
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K = 0, 1, 2, 8, 12, 13, 14
 TYPE_Q2_K, TYPE_Q3_K = 10, 11
 TYPE_Q5_0, TYPE_Q8_K = 6, 15  # stored as f32
+ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 30  # element types of activations
 ROLE_NAMES = ["attn_norm", "attn_q", "attn_k", "attn_v", "attn_output", "ffn_norm", "ffn_gate", "ffn_up", "ffn_down"]
 # rf_layer_load roles 0-11: the nine weights, then the optional qwen2 Q/K/V biases
 LAYER_VIEW_NAMES = ROLE_NAMES + ["attn_q.bias", "attn_k.bias", "attn_v.bias"]
@@ -39,6 +40,7 @@ EXPORTS = [
     "rf_bench_layer_kernels", "rf_tp_unique_id", "rf_tp_peer_sum", "rf_matrix_create", "rf_matrix_destroy", "rf_matrix_device_bytes",
     "rf_qmatvec", "rf_qgemm", "rf_qgemm_error_word", "rf_decode_attention", "rf_decode_attention_noalloc",
     "rf_should_keep_resident", "rf_layer_read_plan", "rf_plan_residency", "rf_set_layer_cache",
+    "rf_qk_norm_rope", "rf_kv_cache_write", "rf_kv_cache_read", "rf_tree_attention", "rf_verify_error_word",
 ]
 
 
@@ -90,6 +92,17 @@ class PlannedTensor(ctypes.Structure):
 class ReadPlanTotals(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in ("logical_tensor_count", "logical_bytes", "physical_bytes", "gap_bytes",
                                                "reusable_group_buffer_bytes")]
+
+
+class KvView(ctypes.Structure):
+    """rf_kv_view: one layer's K/V cache in device memory the caller owns (device addresses; scales 0 for f16)."""
+    _fields_ = [("type", ctypes.c_int), ("n_seqs", ctypes.c_uint32), ("n_kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("capacity", ctypes.c_uint32), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+
+    def __init__(self, type: int, k_ptr: int, v_ptr: int, k_scale_ptr: int, v_scale_ptr: int, n_seqs: int,
+                 n_kv_heads: int, head_dim: int, capacity: int):
+        super().__init__(type, n_seqs, n_kv_heads, head_dim, capacity, k_ptr, v_ptr, k_scale_ptr, v_scale_ptr)
 
 
 class ResidencyStats(ctypes.Structure):
@@ -163,6 +176,13 @@ def lib():
             "rf_qgemm_error_word": (c_int, [u32p]),
             "rf_decode_attention": (c_int, [vp, vp, vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
             "rf_decode_attention_noalloc": (c_int, [vp, vp, vp, c_int, c_int, c_int, c_int, c_int, vp, vp]),
+            "rf_qk_norm_rope": (c_int, [vp, vp, vp, vp, c_int, c_u32, c_u32, c_u32, c_u32, c_u64, c_u64, c_u64, c_u64,
+                                        vp, vp, ctypes.c_float, vp, c_u32, c_u32, vp, vp]),
+            "rf_kv_cache_write": (c_int, [ctypes.POINTER(KvView), vp, vp, c_int, c_u32, c_u64, c_u64, vp, vp, vp]),
+            "rf_kv_cache_read": (c_int, [ctypes.POINTER(KvView), vp, vp, c_int, c_u32, c_u64, c_u64, vp, vp, vp]),
+            "rf_tree_attention": (c_int, [ctypes.POINTER(KvView), vp, vp, c_int, c_u32, c_u32, c_u32, c_u64, c_u64,
+                                          vp, vp, vp, ctypes.c_float, vp]),
+            "rf_verify_error_word": (c_int, [u32p]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)

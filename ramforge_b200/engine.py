@@ -15,7 +15,7 @@ from typing import Iterable, Sequence
 import numpy as np
 
 from . import _lib
-from ._lib import RfError, check, lib
+from ._lib import KvView, RfError, check, lib
 
 _f32p = ctypes.POINTER(ctypes.c_float)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
@@ -321,4 +321,47 @@ def decode_attention(q_ptr: int, k_ptr: int, v_ptr: int, ctx: int, n_heads: int,
     check(lib().rf_decode_attention(q_ptr, k_ptr, v_ptr, ctx, n_heads, n_kv_heads, head_dim, batch, out_ptr, stream))
 
 
-__all__ = ["DecodeEngine", "QMatrix", "decode_attention", "selftest_wait", "tp_unique_id", "RfError"]
+def qk_norm_rope(q_ptr: int, k_ptr: int, q_out_ptr: int, k_out_ptr: int, act_type: int, n_tokens: int, n_heads: int,
+                 n_kv_heads: int, head_dim: int, rope_ptr: int, rope_len: int, positions_ptr: int, q_norm_ptr: int = 0,
+                 k_norm_ptr: int = 0, eps: float = 1e-6, rot_dim: int | None = None, q_stride: int = 0,
+                 k_stride: int = 0, q_out_stride: int = 0, k_out_stride: int = 0, stream: int = 0):
+    """Per-head RMS norm and rotation of queries and keys (rf_qk_norm_rope); device pointers, act_type one of
+    _lib.ACT_*, rot_dim None for the whole head, strides in elements (0: rows without gaps)."""
+    check(lib().rf_qk_norm_rope(q_ptr, k_ptr, q_out_ptr, k_out_ptr, act_type, n_tokens, n_heads, n_kv_heads, head_dim,
+                                q_stride, k_stride, q_out_stride, k_out_stride, q_norm_ptr, k_norm_ptr, eps, rope_ptr,
+                                rope_len, head_dim if rot_dim is None else rot_dim, positions_ptr, stream))
+
+
+def kv_cache_write(cache: KvView, k_ptr: int, v_ptr: int, act_type: int, n_rows: int, pos_ptr: int, seq_ptr: int = 0,
+                   k_stride: int = 0, v_stride: int = 0, stream: int = 0):
+    """K/V rows into a cache, quantised on the way where it is Q8_0 (rf_kv_cache_write); rows with a negative
+    position are not kept."""
+    check(lib().rf_kv_cache_write(cache, k_ptr, v_ptr, act_type, n_rows, k_stride, v_stride, seq_ptr, pos_ptr, stream))
+
+
+def kv_cache_read(cache: KvView, k_out_ptr: int, v_out_ptr: int, act_type: int, n_rows: int, pos_ptr: int,
+                  seq_ptr: int = 0, k_stride: int = 0, v_stride: int = 0, stream: int = 0):
+    """Rows of a cache as numbers (rf_kv_cache_read); rows with a negative position are zeros."""
+    check(lib().rf_kv_cache_read(cache, k_out_ptr, v_out_ptr, act_type, n_rows, k_stride, v_stride, seq_ptr, pos_ptr,
+                                 stream))
+
+
+def tree_attention(cache: KvView, q_ptr: int, out_ptr: int, act_type: int, n_seqs: int, n_tokens: int, n_heads: int,
+                   hist_len_ptr: int, n_draft_ptr: int = 0, mask_ptr: int = 0, scale: float = 0.0, q_stride: int = 0,
+                   out_stride: int = 0, stream: int = 0):
+    """Attention of drafted tokens over a cached history and their own ancestors (rf_tree_attention); mask 0: a
+    chain, scale 0: 1 / sqrt(head_dim)."""
+    check(lib().rf_tree_attention(cache, q_ptr, out_ptr, act_type, n_seqs, n_tokens, n_heads, q_stride, out_stride,
+                                  hist_len_ptr, n_draft_ptr, mask_ptr, scale, stream))
+
+
+def verify_error_word() -> int:
+    """Error word of the four calls above (rf_verify_error_word): bit 0 a wait gave up, bit 1 an index on the device
+    was out of range; reading clears it."""
+    w = ctypes.c_uint32()
+    check(lib().rf_verify_error_word(ctypes.byref(w)))
+    return w.value
+
+
+__all__ = ["DecodeEngine", "KvView", "QMatrix", "decode_attention", "kv_cache_read", "kv_cache_write", "qk_norm_rope",
+           "selftest_wait", "tp_unique_id", "tree_attention", "verify_error_word", "RfError"]
