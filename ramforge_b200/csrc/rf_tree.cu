@@ -7,6 +7,10 @@
 // the output sum, rescaled when m grows.
 #include <cuda_bf16.h>
 
+#include <mutex>
+#include <type_traits>
+#include <unordered_map>
+
 #include "rf_device.cuh"
 #include "rf_verify.h"
 
@@ -41,73 +45,624 @@ __device__ __forceinline__ void act_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void act_put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void act_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Element d of the cache row `slot` (value = code * scale rounded to f16).
-template <bool Q8>
-__device__ __forceinline__ float kv_value(const void* plane, const void* scale, uint64_t slot, uint32_t D, uint32_t d) {
-  if constexpr (Q8) {
-    const float s = __half2float(((const __half*)scale)[slot * (D / 32) + d / 32]);
-    return __half2float(__float2half_rn((float)((const int8_t*)plane)[slot * D + d] * s));
-  } else {
-    return __half2float(((const __half*)plane)[slot * D + d]);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------------------
+// The work split.  A unit is (sequence b, KV head h, row tile rt): up to ROWS of the
+// n_b * G query rows (G query heads share a KV head; row r = token r / G, head r % G)
+// against all its keys, in tiles of KT.  All tiles of all units, in that order, are
+// cut into equal contiguous ranges, one a CTA (of as many CTAs as there are tiles, at
+// most gridDim.x), whatever the histories: the lengths are read on the device.  A unit that lies in one CTA is finished there; the
+// others leave partial results that tree_merge_kernel adds in order of the keys, so
+// results do not depend on timing.  A CTA leaves at most two: slot 0 for the unit its
+// range starts inside of, slot 1 for the one it ends inside of.
+// ---------------------------------------------------------------------------
+template <int KT, int ROWS>
+struct Split {
+  static __device__ __forceinline__ uint32_t tiles(uint32_t L, uint32_t n) { return n ? (L + n + KT - 1) / KT : 0; }
+  static __device__ __forceinline__ uint32_t row_tiles(const TreeArgs& a, uint32_t n) {
+    return (n * (a.n_heads / a.c.n_kv_heads) + ROWS - 1) / ROWS;
+  }
+  static __device__ __forceinline__ uint64_t work(const TreeArgs& a, uint32_t b) {
+    if (b >= a.n_seqs) return 0;
+    uint32_t L, n;
+    seq_lengths(a, b, &L, &n);
+    return (uint64_t)tiles(L, n) * row_tiles(a, n) * a.c.n_kv_heads;
+  }
+  // Whole warp: the tiles of all sequences, and (through *before) those of the sequences before b.
+  static __device__ __forceinline__ uint64_t total(const TreeArgs& a, uint32_t b, uint64_t* before) {
+    uint64_t t = 0, p = 0;
+    for (uint32_t i = threadIdx.x & 31; i < a.n_seqs; i += 32) {
+      const uint64_t w = work(a, i);
+      t += w;
+      if (i < b) p += w;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+      p += __shfl_xor_sync(0xffffffffu, p, o);
+    }
+    *before = p;
+    return t;
+  }
+  // Whole warp: the sequence that holds tile w, and w's offset in it.
+  static __device__ __forceinline__ uint32_t locate(const TreeArgs& a, uint64_t w, uint64_t* offset) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint64_t acc = 0;
+    for (uint32_t base = 0; base < a.n_seqs; base += 32) {
+      uint64_t s = work(a, base + lane);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, acc + s > w);
+      if (past) {
+        const int first = __ffs(past) - 1;
+        const uint64_t low = first ? __shfl_sync(0xffffffffu, s, first - 1) : 0;
+        *offset = w - acc - low;
+        return base + first;
+      }
+      acc += __shfl_sync(0xffffffffu, s, 31);
+    }
+    *offset = 0;
+    return a.n_seqs;
+  }
+};
+
+// Floats of one partial result: ROWS x D output sums, then ROWS maxima and ROWS sums.
+constexpr size_t part_floats(int rows, int D) { return (size_t)rows * (D + 2); }
+
+// Visibility of position p for token t of sequence b (p < L + n).
+__device__ __forceinline__ bool sees(const TreeArgs& a, uint32_t b, uint32_t t, uint32_t L, uint32_t p) {
+  if (p < L) return true;
+  const uint32_t j = p - L;
+  return a.mask ? (a.mask[((uint64_t)b * a.n_tokens + t) * a.words + j / 32] >> (j % 32)) & 1u : j <= t;
+}
+
+// ---------------------------------------------------------------------------
+// Few query rows a KV head: tree_rows_kernel.
+//
+// The keys' bytes bound it, so they go from HBM straight into the registers that
+// mma.sync reads, and nothing else is staged.  A warp takes MB * 16 keys a step and
+// computes S^T = K Q^T (keys are the MMA's rows, query rows its 8 * NB columns) and
+// O^T += V^T P^T.  The order of the summed index is free in both products, so a lane's
+// A fragments are whole 16-byte pieces of a row: for K the head's dimensions are
+// assigned to the k index so that lane c of a group of four holds consecutive ones, and
+// for V the dimensions are assigned to the m index so that lane group g does.
+// Scores leave the MMA with keys along the lanes' groups; movmatrix turns the 8 x 8
+// blocks of P into the B fragments of the second product.
+// Softmax in base 2 with a running reference m that is only raised (and the sums
+// rescaled) when some score passes it by 2^8; weights are 2^(s - m + 7), below 2^15, so
+// that f16 keeps 11 bits of every weight down to 2^-21 of the largest.
+// ---------------------------------------------------------------------------
+constexpr float kRaise = 8.f, kWeightBias = 7.f;
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 ld_stream16(const void* p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(p));
+  return u;
+}
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+  uint2 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
+  return u;
+}
+
+// Two biased bytes (code + 128) in the low halves of 0x64xx become 1024 + 128 + code; the
+// subtraction is exact, the product rounds once: the value the cache format defines.
+__device__ __forceinline__ uint32_t q8_pair(uint32_t biased, __half2 d) {
+  const __half2 code = __hsub2(bits_h2(biased), __float2half2_rn(1152.f));
+  return h2_bits(__hmul2(code, d));
+}
+
+// Shapes of one step of a warp over a cache of type Q8 and head dimension D.
+template <bool Q8, int D>
+struct Step {
+  static constexpr int MB = Q8 ? 2 : 1;                    // 16-key blocks
+  static constexpr int KEYS = 16 * MB;
+  static constexpr int KW = Q8 ? D / 16 : D / 8;           // 32-bit words of one key's K in a lane
+  static constexpr int VW = Q8 ? D / 32 : D / 16;          // ... of one key's V
+  static constexpr int KS = D / 16;                        // k steps of S, m blocks of O
+};
+constexpr int kRowWarps = 4;
+
+// Query rows as B fragments: row g of block nb, the dimensions lane c holds of a key.
+// f32 and bf16 rows are first scaled by a power of two to a largest magnitude in [1, 2),
+// which f16 holds; f32 keeps a second f16 term.  *exp2 is the scale that was taken out.
+template <class T, bool Q8, int D, bool SPLIT>
+__device__ __forceinline__ void load_query(const T* row, bool live, uint32_t c, uint32_t (&hi)[Step<Q8, D>::KS][2],
+                                           uint32_t (&lo)[SPLIT ? Step<Q8, D>::KS : 1][2], float* exp2) {
+  constexpr int KS = Step<Q8, D>::KS;
+  float v[KS][4];
+  float top = 0.f;
+#pragma unroll
+  for (int k = 0; k < KS; k++) {
+    const uint32_t d = Q8 ? 64 * (k / 4) + 16 * c + 4 * (k % 4) : 32 * (k / 2) + 8 * c + 4 * (k % 2);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[k][i] = live ? act_get(row + d + i) : 0.f;
+      top = fmaxf(top, fabsf(v[k][i]));
+    }
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  float down = 1.f, up = 1.f;
+  if constexpr (!std::is_same<T, __half>::value) {
+    if (top > 0.f && top < INFINITY) {
+      const int e = ilogbf(top);
+      // in two factors: 2^-e alone leaves f32 for the smallest rows
+      down = ldexpf(1.f, -(e / 2)), up = ldexpf(1.f, e);
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[k][i] = v[k][i] * down * ldexpf(1.f, -(e - e / 2));
+    }
+  }
+  *exp2 = up;
+#pragma unroll
+  for (int k = 0; k < KS; k++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const __half2 h = __floats2half2_rn(v[k][2 * i], v[k][2 * i + 1]);
+      hi[k][i] = h2_bits(h);
+      if constexpr (SPLIT) {
+        const float2 f = __half22float2(h);
+        lo[k][i] = h2_bits(__floats2half2_rn(v[k][2 * i] - f.x, v[k][2 * i + 1] - f.y));
+      }
+    }
+}
+
+template <class T, bool Q8, int D, int NB>
+__global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_kernel(TreeArgs a, float* __restrict__ part) {
+  using S = Step<Q8, D>;
+  constexpr bool SPLIT = std::is_same<T, float>::value;
+  constexpr int ROWS = 8 * NB, KT = S::KEYS * kRowWarps, MB = S::MB, KS = S::KS, KW = S::KW, VW = S::VW;
+  using Sp = Split<KT, ROWS>;
+  __shared__ __align__(16) float s_o[kRowWarps][ROWS][D];
+  __shared__ float s_m[kRowWarps][ROWS], s_l[kRowWarps][ROWS];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  griddep_launch();
+  uint64_t ignore, rem;
+  const uint64_t all = Sp::total(a, 0, &ignore);
+  const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, all);  // no CTA without a tile
+  if (blockIdx.x >= ctas) return;
+  uint64_t w = all * blockIdx.x / ctas;
+  const uint64_t w_end = all * (blockIdx.x + 1) / ctas;
+  uint32_t b = Sp::locate(a, w, &rem);
+  const uint32_t G = a.n_heads / a.c.n_kv_heads;
+
+  while (w < w_end) {
+    uint32_t L, n;
+    seq_lengths(a, b, &L, &n);
+    const uint32_t tiles = Sp::tiles(L, n), rts = Sp::row_tiles(a, n), end = L + n;
+    const uint32_t unit = (uint32_t)(rem / tiles), h = unit / rts, rt = unit % rts, k0 = (uint32_t)(rem % tiles);
+    const uint32_t k1 = (uint32_t)min((uint64_t)tiles, k0 + (w_end - w));
+    const uint32_t r0 = rt * ROWS, nrows = min((uint32_t)ROWS, n * G - r0);
+    const uint64_t base = ((uint64_t)b * a.c.n_kv_heads + h) * a.c.capacity;
+    const uint8_t* kp = (const uint8_t*)a.c.k + base * D * (Q8 ? 1 : 2);
+    const uint8_t* vp = (const uint8_t*)a.c.v + base * D * (Q8 ? 1 : 2);
+    const __half* ksp = Q8 ? (const __half*)a.c.k_scale + base * (D / 32) : nullptr;
+    const __half* vsp = Q8 ? (const __half*)a.c.v_scale + base * (D / 32) : nullptr;
+
+    uint32_t qh[NB][KS][2], ql[NB][SPLIT ? KS : 1][2];
+    float coef[NB][2];  // score -> base-2 exponent, of this lane's rows 2c and 2c + 1 of each block
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+      const uint32_t r = 8 * nb + g, rr = r0 + r;
+      const bool live = r < nrows;
+      float up;
+      load_query<T, Q8, D, SPLIT>(
+          (const T*)a.q + ((uint64_t)b * a.n_tokens + (live ? rr / G : 0)) * a.q_stride + (h * G + (live ? rr % G : 0)) * D,
+          live, c, qh[nb], ql[nb], &up);
+      const float cf = a.scale * 1.44269504f * up;
+      coef[nb][0] = __shfl_sync(0xffffffffu, cf, 8 * c);
+      coef[nb][1] = __shfl_sync(0xffffffffu, cf, 8 * c + 4);
+    }
+    float o[KS][NB][4], m[NB][2], l[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+      for (int i = 0; i < KS; i++) o[i][nb][0] = o[i][nb][1] = o[i][nb][2] = o[i][nb][3] = 0.f;
+      m[nb][0] = m[nb][1] = -INFINITY;
+      l[nb][0] = l[nb][1] = 0.f;
+    }
+
+    uint32_t kr[2 * MB][KW], vr[4 * MB][VW], vs[4 * MB];
+    uint2 ks[2 * MB];
+    // keys past the end are read from the last one (in bounds) and masked below
+    auto load_k = [&](uint32_t kb) {
+#pragma unroll
+      for (int i = 0; i < 2 * MB; i++) {
+        const uint64_t key = min(kb + g + 8 * i, end - 1);
+        const uint8_t* p = kp + key * D * (Q8 ? 1 : 2) + 16 * c;
+#pragma unroll
+        for (int j = 0; j < KW / 4; j++) {
+          const uint4 u = ld_stream16(p + 64 * j);
+          kr[i][4 * j] = u.x, kr[i][4 * j + 1] = u.y, kr[i][4 * j + 2] = u.z, kr[i][4 * j + 3] = u.w;
+        }
+        if constexpr (Q8) {
+          if constexpr (D == 128)
+            ks[i] = ld_stream8(ksp + key * 4);
+          else
+            ks[i].x = __ldg((const uint32_t*)(ksp + key * 2));
+        }
+      }
+    };
+    // V keys of the lane: 16 kb + {2c, 2c+1, 2c+8, 2c+9}
+    auto v_key = [&](uint32_t kb, int i) { return kb + 16 * (i / 4) + 2 * c + (i % 2) + 8 * ((i / 2) % 2); };
+    auto load_v = [&](uint32_t kb) {
+#pragma unroll
+      for (int i = 0; i < 4 * MB; i++) {
+        const uint64_t key = min(v_key(kb, i), end - 1);
+        if constexpr (Q8 && D == 64) {
+          const uint2 u = ld_stream8(vp + key * D + 8 * g);
+          vr[i][0] = u.x, vr[i][1] = u.y;
+        } else {
+          const uint8_t* p = vp + key * D * (Q8 ? 1 : 2) + 16 * g;
+#pragma unroll
+          for (int j = 0; j < VW / 4; j++) {
+            const uint4 u = ld_stream16(p + 128 * j);
+            vr[i][4 * j] = u.x, vr[i][4 * j + 1] = u.y, vr[i][4 * j + 2] = u.z, vr[i][4 * j + 3] = u.w;
+          }
+        }
+        if constexpr (Q8) vs[i] = __ldg((const unsigned short*)vsp + key * (D / 32) + g / (D == 128 ? 2 : 4));
+      }
+    };
+
+    const uint32_t kb0 = k0 * KT + warp * S::KEYS;
+    if (kb0 < end) {
+      load_k(kb0);
+      load_v(kb0);
+    }
+    for (uint32_t tile = k0; tile < k1; tile++) {
+      const uint32_t kb = tile * KT + warp * S::KEYS;
+      if (kb >= end) break;
+      const bool more = tile + 1 < k1 && kb + KT < end;
+      const bool edge = kb + S::KEYS > L;  // holds drafts or the end: masks apply
+      // ---- S^T = K Q^T
+      float s[MB][NB][4];
+#pragma unroll
+      for (int mb = 0; mb < MB; mb++) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) s[mb][nb][0] = s[mb][nb][1] = s[mb][nb][2] = s[mb][nb][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          uint32_t f[4];
+          if constexpr (Q8) {  // word k of the lane's piece: four codes, two a half2
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const uint32_t x = kr[2 * mb + i][k] ^ 0x80808080u;
+              const uint32_t sw = k / 4 ? ks[2 * mb + i].y : ks[2 * mb + i].x;
+              const __half2 d = bits_h2(__byte_perm(sw, sw, c >= 2 ? 0x3232 : 0x1010));
+              f[i] = q8_pair(__byte_perm(x, 0x64646464u, 0x4140), d);
+              f[2 + i] = q8_pair(__byte_perm(x, 0x64646464u, 0x4342), d);
+            }
+          } else {
+            f[0] = kr[2 * mb][2 * k], f[1] = kr[2 * mb + 1][2 * k];
+            f[2] = kr[2 * mb][2 * k + 1], f[3] = kr[2 * mb + 1][2 * k + 1];
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) {
+            mma16816(s[mb][nb], f, qh[nb][k][0], qh[nb][k][1]);
+            if constexpr (SPLIT) mma16816(s[mb][nb], f, ql[nb][k][0], ql[nb][k][1]);
+          }
+        }
+      }
+      if (more) load_k(kb + KT);
+      // ---- weights
+      bool raise = false;
+#pragma unroll
+      for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float x = s[mb][nb][e] * coef[nb][e & 1];
+            if (edge) {
+              const uint32_t p = kb + 16 * mb + 8 * (e >> 1) + g, r = 8 * nb + 2 * c + (e & 1);
+              if (p >= end || r >= nrows || !sees(a, b, (r0 + r) / G, L, p)) x = -INFINITY;
+            }
+            s[mb][nb][e] = x;
+            raise |= x > m[nb][e & 1] + kRaise;
+          }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            float top = m[nb][x];
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) top = fmaxf(top, fmaxf(s[mb][nb][x], s[mb][nb][2 + x]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float f = top == -INFINITY ? 1.f : ex2(m[nb][x] - top);
+            m[nb][x] = top;
+            l[nb][x] *= f;
+#pragma unroll
+            for (int i = 0; i < KS; i++) o[i][nb][x] *= f, o[i][nb][2 + x] *= f;
+          }
+      }
+      uint32_t ph[MB][NB][2], pl[MB][SPLIT ? NB : 1][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) {
+        const float ref[2] = {(m[nb][0] == -INFINITY ? 0.f : m[nb][0]) - kWeightBias,
+                              (m[nb][1] == -INFINITY ? 0.f : m[nb][1]) - kWeightBias};
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            s[mb][nb][e] = ex2(s[mb][nb][e] - ref[e & 1]);
+            l[nb][e & 1] += s[mb][nb][e];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const __half2 p2 = __floats2half2_rn(s[mb][nb][2 * i], s[mb][nb][2 * i + 1]);
+            ph[mb][nb][i] = transpose8x8(h2_bits(p2));
+            if constexpr (SPLIT) {
+              const float2 f = __half22float2(p2);
+              pl[mb][nb][i] =
+                  transpose8x8(h2_bits(__floats2half2_rn(s[mb][nb][2 * i] - f.x, s[mb][nb][2 * i + 1] - f.y)));
+            }
+          }
+        }
+      }
+      // ---- O^T += V^T P^T
+      bool wild = false;  // a V element of a masked step is not finite
+#pragma unroll
+      for (int mb = 0; mb < MB; mb++) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+          // m block i: dimensions 2i and 2i + 1 of the lane group's piece; keys in pairs
+          uint32_t f[4];
+#pragma unroll
+          for (int pr = 0; pr < 2; pr++) {
+            const int ka = 4 * mb + 2 * pr;
+            if constexpr (Q8) {
+              const __half2 d = bits_h2(vs[ka] | (vs[ka + 1] << 16));
+              const uint32_t x = vr[ka][i / 2], y = vr[ka + 1][i / 2];
+              const uint32_t e0 = __byte_perm(x, y, i & 1 ? 0x0602 : 0x0400), e1 = __byte_perm(x, y, i & 1 ? 0x0703 : 0x0501);
+              f[2 * pr] = q8_pair((e0 & 0x00ff00ffu) ^ 0x64806480u, d);
+              f[2 * pr + 1] = q8_pair((e1 & 0x00ff00ffu) ^ 0x64806480u, d);
+            } else {
+              f[2 * pr] = __byte_perm(vr[ka][i], vr[ka + 1][i], 0x5410);
+              f[2 * pr + 1] = __byte_perm(vr[ka][i], vr[ka + 1][i], 0x7632);
+            }
+          }
+          if (edge) {  // what is masked must not reach the sums, 0 * NaN included: see below
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+              const bool w0 = (f[x] & 0x7c00u) == 0x7c00u, w1 = (f[x] & 0x7c000000u) == 0x7c000000u;
+              wild |= w0 || w1;
+              if (w0) f[x] &= 0xffff0000u;
+              if (w1) f[x] &= 0x0000ffffu;
+            }
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) {
+            mma16816(o[i][nb], f, ph[mb][nb][0], ph[mb][nb][1]);
+            if constexpr (SPLIT) mma16816(o[i][nb], f, pl[mb][nb][0], pl[mb][nb][1]);
+          }
+        }
+      }
+      if (edge && __any_sync(0xffffffffu, wild)) {
+        // rare: the elements that were left out above, added for the rows that do see them
+        for (int kk = 0; kk < S::KEYS; kk++) {
+          const uint64_t key = kb + kk;
+          const bool in = key < end;
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) {
+            float p[2] = {0.f, 0.f};
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float x = __shfl_sync(0xffffffffu, s[mb][nb][e], 4 * (kk & 7) + c);
+                if (kk / 16 == mb && ((kk >> 3) & 1) == (e >> 1)) p[e & 1] = x;
+              }
+            if (!in) continue;
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+              for (int y = 0; y < 2; y++) {
+                const uint32_t d = Q8 ? g * (D / 8) + 2 * i + y : 64 * (i / 4) + 8 * g + 2 * (i % 4) + y;
+                float v;
+                if constexpr (Q8)
+                  v = __half2float(__float2half_rn((float)((const int8_t*)vp)[key * D + d] *
+                                                   __half2float(vsp[key * (D / 32) + d / 32])));
+                else
+                  v = __half2float(((const __half*)vp)[key * D + d]);
+                if (!(fabsf(v) < INFINITY)) {
+#pragma unroll
+                  for (int x = 0; x < 2; x++)
+                    if (p[x] != 0.f) o[i][nb][2 * y + x] += p[x] * v;
+                }
+              }
+          }
+        }
+      }
+      if (more) load_v(kb + KT);
+    }
+
+    // ---- the CTA's warps together
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        float t = l[nb][x];
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        t += __shfl_xor_sync(0xffffffffu, t, 8);
+        t += __shfl_xor_sync(0xffffffffu, t, 16);
+        const uint32_t r = 8 * nb + 2 * c + x;
+        if (g == 0) s_m[warp][r] = m[nb][x], s_l[warp][r] = t;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+          const uint32_t d = Q8 ? g * (D / 8) + 2 * i : 64 * (i / 4) + 8 * g + 2 * (i % 4);
+          *reinterpret_cast<float2*>(&s_o[warp][r][d]) = make_float2(o[i][nb][x], o[i][nb][2 + x]);
+        }
+      }
+    __syncthreads();
+    const bool whole = k0 == 0 && k1 == tiles;
+    float* slot = part + (2 * (size_t)blockIdx.x + (k0 > 0 ? 0 : 1)) * part_floats(ROWS, D);
+    for (uint32_t x = threadIdx.x; x < nrows * (D / 4); x += 32 * kRowWarps) {
+      const uint32_t r = x / (D / 4), d = x % (D / 4) * 4;
+      float M = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kRowWarps; i++) M = fmaxf(M, s_m[i][r]);
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
+#pragma unroll
+      for (int i = 0; i < kRowWarps; i++) {
+        const float f = M == -INFINITY ? 1.f : ex2(s_m[i][r] - M);
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[i][r][d]);
+        den += s_l[i][r] * f;
+        num.x += v.x * f, num.y += v.y * f, num.z += v.z * f, num.w += v.w * f;
+      }
+      if (whole) {
+        const uint32_t rr = r0 + r;
+        T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + rr / G) * a.out_stride + (h * G + rr % G) * D + d;
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        act_put(out, num.x * inv), act_put(out + 1, num.y * inv), act_put(out + 2, num.z * inv), act_put(out + 3, num.w * inv);
+      } else {
+        *reinterpret_cast<float4*>(slot + (size_t)r * D + d) = num;
+        if (d == 0) slot[ROWS * D + r] = M, slot[ROWS * D + ROWS + r] = den;
+      }
+    }
+    __syncthreads();
+    w += k1 - k0;
+    rem += k1 - k0;
+    if (rem == (uint64_t)tiles * rts * a.c.n_kv_heads && w < w_end) {
+      rem = 0;
+      do b++;
+      while (Sp::work(a, b) == 0);
+    }
   }
 }
 
-// One CTA a (token, query head): warps take the keys in turn, lanes the head's dimensions.
-template <class T, bool Q8, int D>
-__global__ void __launch_bounds__(128) tree_simple_kernel(TreeArgs a) {
+// ---------------------------------------------------------------------------
+// One CTA a (token, query head): adds the partial results of a unit that several of
+// the first kernel's CTAs shared (`grid` of them), and writes the zeros of tokens past a sequence's drafts.
+// ---------------------------------------------------------------------------
+template <class T, int D, int KT, int ROWS>
+__global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
+  using Sp = Split<KT, ROWS>;
   constexpr int E = D / 32;
+  __shared__ float s_o[4][D], s_l[4];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t h = blockIdx.x % a.n_heads, bt = blockIdx.x / a.n_heads, b = bt / a.n_tokens, t = bt % a.n_tokens;
-  const uint32_t kh = h / (a.n_heads / a.c.n_kv_heads);
+  const uint32_t hq = blockIdx.x % a.n_heads, bt = blockIdx.x / a.n_heads, b = bt / a.n_tokens, t = bt % a.n_tokens;
+  const uint32_t G = a.n_heads / a.c.n_kv_heads, h = hq / G, r = t * G + hq % G;
+  T* out = (T*)a.out + bt * a.out_stride + (uint64_t)hq * D;
   uint32_t L, n;
   seq_lengths(a, b, &L, &n);
-  const T* q = (const T*)a.q + bt * a.q_stride + h * D;
-  T* out = (T*)a.out + bt * a.out_stride + h * D;
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; e++) qv[e] = act_get(q + lane + 32 * e) * a.scale, o[e] = 0.f;
-  const uint64_t base = ((uint64_t)b * a.c.n_kv_heads + kh) * a.c.capacity;
-  const uint32_t end = t < n ? L + n : 0;
-  for (uint32_t p = warp; p < end; p += 4) {
-    if (p >= L) {
-      const uint32_t j = p - L;
-      const bool see = a.mask ? (a.mask[(uint64_t)bt * a.words + j / 32] >> (j % 32)) & 1u : j <= t;
-      if (!see) continue;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) s = fmaf(qv[e], kv_value<Q8>(a.c.k, a.c.k_scale, base + p, D, lane + 32 * e), s);
-#pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float c = expf(m - ref), w = expf(s - ref);
-    l = l * c + w;
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = o[e] * c + w * kv_value<Q8>(a.c.v, a.c.v_scale, base + p, D, lane + 32 * e);
-    m = mn;
+  if (t >= n) {
+    if (threadIdx.x < D) act_put(out + threadIdx.x, 0.f);
+    return;
   }
-  __shared__ float sm[4], sl[4], so[4][D];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
+  uint64_t before;
+  const uint64_t all = Sp::total(a, b, &before);
+  const uint32_t tiles = Sp::tiles(L, n);
+  const uint64_t u0 = before + ((uint64_t)h * Sp::row_tiles(a, n) + r / ROWS) * tiles, u1 = u0 + tiles;
+  const uint32_t ctas = (uint32_t)min((uint64_t)grid, all);  // CTA c holds [all c / ctas, all (c+1) / ctas)
+  const uint32_t c0 = (uint32_t)(((u0 + 1) * ctas - 1) / all), c1 = (uint32_t)((u1 * ctas - 1) / all);
+  if (c0 == c1) return;
+  griddep_wait();
+  const uint32_t rl = r % ROWS;
+  auto slot = [&](uint32_t c) { return part + (2 * (size_t)c + (c == c0 ? 1 : 0)) * part_floats(ROWS, D); };
+  float M = -INFINITY;
+  for (uint32_t c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(slot(c) + ROWS * D + rl));
 #pragma unroll
-  for (int e = 0; e < E; e++) so[warp][lane + 32 * e] = o[e];
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float acc[E], den = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e++) acc[e] = 0.f;
+#pragma unroll 4
+  for (uint32_t c = c0 + warp; c <= c1; c += 4) {
+    const float* s = slot(c);
+    const float f = M == -INFINITY ? 1.f : ex2(__ldcg(s + ROWS * D + rl) - M);
+    den += __ldcg(s + ROWS * D + ROWS + rl) * f;
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] += __ldcg(s + (size_t)rl * D + lane + 32 * e) * f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) s_o[warp][lane + 32 * e] = acc[e];
+  if (lane == 0) s_l[warp] = den;
   __syncthreads();
-  for (uint32_t d = threadIdx.x; d < D; d += 128) {
-    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), ref = M == -INFINITY ? 0.f : M;
-    float num = 0.f, den = 0.f;
-    for (int w = 0; w < 4; w++) {
-      const float c = expf(sm[w] - ref);
-      num += so[w][d] * c;
-      den += sl[w] * c;
-    }
-    act_put(out + d, den == 0.f ? 0.f : num / den);
+  if (threadIdx.x < D) {
+    const uint32_t d = threadIdx.x;
+    const float l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+    act_put(out + d, l == 0.f ? 0.f : (s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) / l);
   }
+}
+
+// Scratch of one call: allocated and freed in stream order from a pool of this library's own
+// that keeps its memory, so calls on any stream, and captured ones, never share a buffer.
+int scratch_pool(cudaMemPool_t* out) {
+  static std::mutex mu;
+  static std::unordered_map<int, cudaMemPool_t> pools;
+  int dev = 0;
+  RF_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = pools.find(dev);
+  if (it == pools.end()) {
+    cudaMemPoolProps p = {};
+    p.allocType = cudaMemAllocationTypePinned;
+    p.location.type = cudaMemLocationTypeDevice;
+    p.location.id = dev;
+    cudaMemPool_t pool;
+    RF_CUDA(cudaMemPoolCreate(&pool, &p));
+    uint64_t keep = UINT64_MAX;
+    RF_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+    it = pools.emplace(dev, pool).first;
+  }
+  *out = it->second;
+  return RF_OK;
+}
+
+template <class T, bool Q8, int D, int NB>
+int run_rows(cudaStream_t st, const TreeArgs& a) {
+  constexpr int ROWS = 8 * NB, KT = Step<Q8, D>::KEYS * kRowWarps;
+  const uint32_t ctas = (uint32_t)num_sms() * (NB == 1 ? 3 : 2);
+  cudaMemPool_t pool;
+  RF_TRY(scratch_pool(&pool));
+  void* part = nullptr;
+  RF_CUDA(cudaMallocFromPoolAsync(&part, 2 * (size_t)ctas * part_floats(ROWS, D) * sizeof(float), pool, st));
+  cudaError_t e = launch_k(Launch{st, false}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
+                           (float*)part);
+  if (e == cudaSuccess)
+    e = launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS>, dim3(a.n_seqs * a.n_tokens * a.n_heads), dim3(128),
+                 0, a, (const float*)part, ctas);
+  const cudaError_t f = cudaFreeAsync(part, st);
+  RF_CUDA(e);
+  RF_CUDA(f);
+  return RF_OK;
 }
 
 template <class T, bool Q8>
-cudaError_t launch_tree(const Launch& L, const TreeArgs& a) {
-  const dim3 grid(a.n_seqs * a.n_tokens * a.n_heads);
-  return launch_k(L, a.c.head_dim == 128 ? tree_simple_kernel<T, Q8, 128> : tree_simple_kernel<T, Q8, 64>, grid,
-                  dim3(128), 0, a);
+int run_tree(cudaStream_t st, const TreeArgs& a) {
+  const uint32_t rows = a.n_tokens * (a.n_heads / a.c.n_kv_heads);
+  if (a.c.head_dim == 128) return rows <= 8 ? run_rows<T, Q8, 128, 1>(st, a) : run_rows<T, Q8, 128, 2>(st, a);
+  return rows <= 8 ? run_rows<T, Q8, 64, 1>(st, a) : run_rows<T, Q8, 64, 2>(st, a);
 }
 
 }  // namespace
@@ -149,14 +704,13 @@ int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act
   a.hist_len = hist_len, a.n_draft = n_draft, a.mask = mask;
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
   RF_TRY(verify_error_ptr(&a.err));
-  const Launch L{(cudaStream_t)stream, false};
+  const cudaStream_t st = (cudaStream_t)stream;
   const bool q8 = cache->type == RF_TYPE_Q8_0;
   switch (act_type) {
-    case RF_ACT_F32: RF_CUDA((q8 ? launch_tree<float, true> : launch_tree<float, false>)(L, a)); break;
-    case RF_ACT_F16: RF_CUDA((q8 ? launch_tree<__half, true> : launch_tree<__half, false>)(L, a)); break;
-    default: RF_CUDA((q8 ? launch_tree<__nv_bfloat16, true> : launch_tree<__nv_bfloat16, false>)(L, a));
+    case RF_ACT_F32: return q8 ? run_tree<float, true>(st, a) : run_tree<float, false>(st, a);
+    case RF_ACT_F16: return q8 ? run_tree<__half, true>(st, a) : run_tree<__half, false>(st, a);
+    default: return q8 ? run_tree<__nv_bfloat16, true>(st, a) : run_tree<__nv_bfloat16, false>(st, a);
   }
-  return RF_OK;
 }
 
 }  // extern "C"
