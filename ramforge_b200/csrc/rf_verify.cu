@@ -172,6 +172,75 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(NormRopeArgs a) {
   }
 }
 
+// Whole-head or no rotation, 16-byte aligned rows: lane x of a group of `lanes` holds the
+// 16-byte piece x of the head's first half and of its second half, so each pair to rotate
+// sits in one lane.  A group takes kHeads heads of one token together: their loads are all
+// in flight at once, and the table row and the weights are read once for all of them.
+constexpr int kHeads = 4;
+
+template <class T>
+__global__ void __launch_bounds__(256) norm_rope_vec_kernel(NormRopeArgs a, uint32_t lanes, uint32_t q_groups,
+                                                            uint32_t groups) {
+  constexpr int V = Act<T>::kVec;
+  const uint32_t idx = blockIdx.x * 256 + threadIdx.x;
+  uint32_t item = idx / lanes;
+  const uint32_t x = idx % lanes, D = a.head_dim;
+  bool live = item < a.n_tokens * groups;
+  if (!live) item = 0;
+  const uint32_t t = item / groups, gr = item % groups;
+  const bool is_q = gr < q_groups;
+  const uint32_t h0 = (is_q ? gr : gr - q_groups) * kHeads, heads = is_q ? a.n_heads : a.n_kv_heads;
+  const T* src = (const T*)(is_q ? a.q : a.k) + t * (is_q ? a.q_stride : a.k_stride) + (size_t)h0 * D + x * V;
+  T* dst = (T*)(is_q ? a.q_out : a.k_out) + t * (is_q ? a.q_out_stride : a.k_out_stride) + (size_t)h0 * D + x * V;
+  const float* nw = is_q ? a.q_norm : a.k_norm;
+  uint4 raw[kHeads][2];
+#pragma unroll
+  for (int i = 0; i < kHeads; i++)
+    if (live && h0 + i < heads) {
+      raw[i][0] = *reinterpret_cast<const uint4*>(src + i * D);
+      raw[i][1] = *reinterpret_cast<const uint4*>(src + i * D + D / 2);
+    } else {
+      raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+    }
+  const float2* row;
+  live = rope_row(a, t, &row) && live;
+  float cs[V], sn[V], w[2][V];
+#pragma unroll
+  for (int j = 0; j < V; j += 2) {
+    const float4 f = row && live ? __ldg(reinterpret_cast<const float4*>(row + x * V + j)) : make_float4(1.f, 0.f, 1.f, 0.f);
+    cs[j] = f.x, sn[j] = f.y, cs[j + 1] = f.z, sn[j + 1] = f.w;
+  }
+#pragma unroll
+  for (int s = 0; s < 2; s++)
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 f = nw ? __ldg(reinterpret_cast<const float4*>(nw + s * (D / 2) + x * V + j)) : make_float4(1.f, 1.f, 1.f, 1.f);
+      w[s][j] = f.x, w[s][j + 1] = f.y, w[s][j + 2] = f.z, w[s][j + 3] = f.w;
+    }
+#pragma unroll
+  for (int i = 0; i < kHeads; i++) {
+    float v[2][V];
+    Act<T>::unpack(raw[i][0], v[0]);
+    Act<T>::unpack(raw[i][1], v[1]);
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; j++) ss = fmaf(v[0][j], v[0][j], fmaf(v[1][j], v[1][j], ss));
+    for (uint32_t o = lanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = nw ? 1.f / sqrtf(ss / (float)D + a.eps) : 1.f;
+    float y[2][V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const float p = v[0][j] * r * w[0][j], q = v[1][j] * r * w[1][j];
+      y[0][j] = row ? p * cs[j] - q * sn[j] : p;
+      y[1][j] = row ? p * sn[j] + q * cs[j] : q;
+    }
+    if (live && h0 + i < heads) {
+      *reinterpret_cast<uint4*>(dst + i * D) = Act<T>::pack(y[0]);
+      *reinterpret_cast<uint4*>(dst + i * D + D / 2) = Act<T>::pack(y[1]);
+    }
+  }
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -332,6 +401,18 @@ int check_kv_rows(const rf_kv_view* c, const void* k, const void* v, int act_typ
 
 template <class T>
 cudaError_t launch_norm_rope(const Launch& L, const NormRopeArgs& a) {
+  const uint32_t v = Act<T>::kVec, lanes = a.head_dim / 2 / v;
+  bool vec = a.head_dim % (2 * v) == 0 && lanes <= 32 && !(lanes & (lanes - 1)) &&
+             (a.rot_dim == 0 || a.rot_dim == a.head_dim);
+  for (const void* p : {a.q, a.k, (const void*)a.q_out, (const void*)a.k_out, (const void*)a.q_norm, (const void*)a.k_norm,
+                        (const void*)a.rope})
+    vec = vec && aligned_to(p, 16);
+  for (uint64_t s : {a.q_stride, a.k_stride, a.q_out_stride, a.k_out_stride}) vec = vec && s % v == 0;
+  if (vec) {
+    const uint32_t qg = (a.n_heads + kHeads - 1) / kHeads, groups = qg + (a.n_kv_heads + kHeads - 1) / kHeads;
+    const uint32_t threads = a.n_tokens * groups * lanes;
+    return launch_k(L, norm_rope_vec_kernel<T>, dim3((threads + 255) / 256), dim3(256), 0, a, lanes, qg, groups);
+  }
   const uint32_t warps = a.n_tokens * (a.n_heads + a.n_kv_heads);
   return launch_k(L, norm_rope_any_kernel<T>, dim3((warps + 7) / 8), dim3(256), 0, a);
 }
