@@ -5,124 +5,13 @@
 // the whole history p < L, and the drafts p = L + j whose bit j is set in its mask row.
 // One pass over the keys carries the running maximum m, the sum l of exp(s - m) and
 // the output sum, rescaled when m grows.
-#include <cuda_bf16.h>
-
 #include <mutex>
 #include <type_traits>
-#include <unordered_map>
 
-#include "rf_device.cuh"
-#include "rf_verify.h"
+#include "rf_tree.cuh"
 
 namespace rf {
 namespace {
-
-struct TreeArgs {
-  rf_kv_view c;
-  const void* q;
-  void* out;
-  uint64_t q_stride, out_stride;
-  uint32_t n_seqs, n_tokens, n_heads, words;  // words: mask words per token
-  const int32_t *hist_len, *n_draft;
-  const uint32_t* mask;
-  float scale;
-  unsigned* err;
-};
-
-// History length and draft count of sequence b; (0, 0) and the error bit where they do not fit the cache.
-__device__ __forceinline__ void seq_lengths(const TreeArgs& a, uint32_t b, uint32_t* hist, uint32_t* drafts) {
-  const int32_t L = a.hist_len[b], n = a.n_draft ? a.n_draft[b] : (int32_t)a.n_tokens;
-  const bool ok = L >= 0 && n >= 0 && (uint32_t)n <= a.n_tokens && (uint64_t)L + (uint64_t)n <= a.c.capacity;
-  if (!ok) atomicOr(a.err, kVerifyRange);
-  *hist = ok ? (uint32_t)L : 0;
-  *drafts = ok ? (uint32_t)n : 0;
-}
-
-__device__ __forceinline__ float act_get(const float* p) { return *p; }
-__device__ __forceinline__ float act_get(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ float act_get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void act_put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void act_put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void act_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// ---------------------------------------------------------------------------
-// The work split.  A unit is (sequence b, KV head h, row tile rt): up to ROWS of the
-// n_b * G query rows (G query heads share a KV head; row r = token r / G, head r % G)
-// against all its keys, in tiles of KT.  All tiles of all units, in that order, are
-// cut into equal contiguous ranges, one a CTA (of as many CTAs as there are tiles, at
-// most gridDim.x), whatever the histories: the lengths are read on the device.  A unit that lies in one CTA is finished there; the
-// others leave partial results that tree_merge_kernel adds in order of the keys, so
-// results do not depend on timing.  A CTA leaves at most two: slot 0 for the unit its
-// range starts inside of, slot 1 for the one it ends inside of.
-// ---------------------------------------------------------------------------
-template <int KT, int ROWS>
-struct Split {
-  static __device__ __forceinline__ uint32_t tiles(uint32_t L, uint32_t n) { return n ? (L + n + KT - 1) / KT : 0; }
-  static __device__ __forceinline__ uint32_t row_tiles(const TreeArgs& a, uint32_t n) {
-    return (n * (a.n_heads / a.c.n_kv_heads) + ROWS - 1) / ROWS;
-  }
-  static __device__ __forceinline__ uint64_t work(const TreeArgs& a, uint32_t b) {
-    if (b >= a.n_seqs) return 0;
-    uint32_t L, n;
-    seq_lengths(a, b, &L, &n);
-    return (uint64_t)tiles(L, n) * row_tiles(a, n) * a.c.n_kv_heads;
-  }
-  // Whole warp: the tiles of all sequences, and (through *before) those of the sequences before b.
-  static __device__ __forceinline__ uint64_t total(const TreeArgs& a, uint32_t b, uint64_t* before) {
-    uint64_t t = 0, p = 0;
-    for (uint32_t i = threadIdx.x & 31; i < a.n_seqs; i += 32) {
-      const uint64_t w = work(a, i);
-      t += w;
-      if (i < b) p += w;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      t += __shfl_xor_sync(0xffffffffu, t, o);
-      p += __shfl_xor_sync(0xffffffffu, p, o);
-    }
-    *before = p;
-    return t;
-  }
-  // Whole warp: the sequence that holds tile w, and w's offset in it.
-  static __device__ __forceinline__ uint32_t locate(const TreeArgs& a, uint64_t w, uint64_t* offset) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint64_t acc = 0;
-    for (uint32_t base = 0; base < a.n_seqs; base += 32) {
-      uint64_t s = work(a, base + lane);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t up = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += up;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, acc + s > w);
-      if (past) {
-        const int first = __ffs(past) - 1;
-        const uint64_t low = first ? __shfl_sync(0xffffffffu, s, first - 1) : 0;
-        *offset = w - acc - low;
-        return base + first;
-      }
-      acc += __shfl_sync(0xffffffffu, s, 31);
-    }
-    *offset = 0;
-    return a.n_seqs;
-  }
-};
-
-// Floats of one partial result: ROWS x D output sums, then ROWS maxima and ROWS sums.
-constexpr size_t part_floats(int rows, int D) { return (size_t)rows * (D + 2); }
-
-// Visibility of position p for token t of sequence b (p < L + n).
-__device__ __forceinline__ bool sees(const TreeArgs& a, uint32_t b, uint32_t t, uint32_t L, uint32_t p) {
-  if (p < L) return true;
-  const uint32_t j = p - L;
-  return a.mask ? (a.mask[((uint64_t)b * a.n_tokens + t) * a.words + j / 32] >> (j % 32)) & 1u : j <= t;
-}
 
 // ---------------------------------------------------------------------------
 // Few query rows a KV head: tree_rows_kernel.
@@ -136,11 +25,7 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, uint32_t b, uint32_t t, 
 // for V the dimensions are assigned to the m index so that lane group g does.
 // Scores leave the MMA with keys along the lanes' groups; movmatrix turns the 8 x 8
 // blocks of P into the B fragments of the second product.
-// Softmax in base 2 with a running reference m that is only raised (and the sums
-// rescaled) when some score passes it by 2^8; weights are 2^(s - m + 7), below 2^15, so
-// that f16 keeps 11 bits of every weight down to 2^-21 of the largest.
 // ---------------------------------------------------------------------------
-constexpr float kRaise = 8.f, kWeightBias = 7.f;
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
@@ -238,26 +123,15 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
   using S = Step<Q8, D>;
   constexpr bool SPLIT = std::is_same<T, float>::value;
   constexpr int ROWS = 8 * NB, KT = S::KEYS * kRowWarps, MB = S::MB, KS = S::KS, KW = S::KW, VW = S::VW;
-  using Sp = Split<KT, ROWS>;
   __shared__ __align__(16) float s_o[kRowWarps][ROWS][D];
   __shared__ float s_m[kRowWarps][ROWS], s_l[kRowWarps][ROWS];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   griddep_launch();
-  uint64_t ignore, rem;
-  const uint64_t all = Sp::total(a, 0, &ignore);
-  const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, all);  // no CTA without a tile
-  if (blockIdx.x >= ctas) return;
-  uint64_t w = all * blockIdx.x / ctas;
-  const uint64_t w_end = all * (blockIdx.x + 1) / ctas;
-  uint32_t b = Sp::locate(a, w, &rem);
   const uint32_t G = a.n_heads / a.c.n_kv_heads;
-
-  while (w < w_end) {
-    uint32_t L, n;
-    seq_lengths(a, b, &L, &n);
-    const uint32_t tiles = Sp::tiles(L, n), rts = Sp::row_tiles(a, n), end = L + n;
-    const uint32_t unit = (uint32_t)(rem / tiles), h = unit / rts, rt = unit % rts, k0 = (uint32_t)(rem % tiles);
-    const uint32_t k1 = (uint32_t)min((uint64_t)tiles, k0 + (w_end - w));
+  Walk<KT, ROWS> walk(a);
+  Segment sg;
+  while (walk.next(a, &sg)) {
+    const uint32_t b = sg.b, h = sg.h, L = sg.hist, n = sg.drafts, end = sg.end, k0 = sg.k0, k1 = sg.k1, rt = sg.rt;
     const uint32_t r0 = rt * ROWS, nrows = min((uint32_t)ROWS, n * G - r0);
     const uint64_t base = ((uint64_t)b * a.c.n_kv_heads + h) * a.c.capacity;
     const uint8_t* kp = (const uint8_t*)a.c.k + base * D * (Q8 ? 1 : 2);
@@ -523,7 +397,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
         }
       }
     __syncthreads();
-    const bool whole = k0 == 0 && k1 == tiles;
+    const bool whole = sg.whole();
     float* slot = part + (2 * (size_t)blockIdx.x + (k0 > 0 ? 0 : 1)) * part_floats(ROWS, D);
     for (uint32_t x = threadIdx.x; x < nrows * (D / 4); x += 32 * kRowWarps) {
       const uint32_t r = x / (D / 4), d = x % (D / 4) * 4;
@@ -550,103 +424,15 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       }
     }
     __syncthreads();
-    w += k1 - k0;
-    rem += k1 - k0;
-    if (rem == (uint64_t)tiles * rts * a.c.n_kv_heads && w < w_end) {
-      rem = 0;
-      do b++;
-      while (Sp::work(a, b) == 0);
-    }
   }
-}
-
-// ---------------------------------------------------------------------------
-// One CTA a (token, query head): adds the partial results of a unit that several of
-// the first kernel's CTAs shared (`grid` of them), and writes the zeros of tokens past a sequence's drafts.
-// ---------------------------------------------------------------------------
-template <class T, int D, int KT, int ROWS>
-__global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
-  using Sp = Split<KT, ROWS>;
-  constexpr int E = D / 32;
-  __shared__ float s_o[4][D], s_l[4];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t hq = blockIdx.x % a.n_heads, bt = blockIdx.x / a.n_heads, b = bt / a.n_tokens, t = bt % a.n_tokens;
-  const uint32_t G = a.n_heads / a.c.n_kv_heads, h = hq / G, r = t * G + hq % G;
-  T* out = (T*)a.out + bt * a.out_stride + (uint64_t)hq * D;
-  uint32_t L, n;
-  seq_lengths(a, b, &L, &n);
-  if (t >= n) {
-    if (threadIdx.x < D) act_put(out + threadIdx.x, 0.f);
-    return;
-  }
-  uint64_t before;
-  const uint64_t all = Sp::total(a, b, &before);
-  const uint32_t tiles = Sp::tiles(L, n);
-  const uint64_t u0 = before + ((uint64_t)h * Sp::row_tiles(a, n) + r / ROWS) * tiles, u1 = u0 + tiles;
-  const uint32_t ctas = (uint32_t)min((uint64_t)grid, all);  // CTA c holds [all c / ctas, all (c+1) / ctas)
-  const uint32_t c0 = (uint32_t)(((u0 + 1) * ctas - 1) / all), c1 = (uint32_t)((u1 * ctas - 1) / all);
-  if (c0 == c1) return;
-  griddep_wait();
-  const uint32_t rl = r % ROWS;
-  auto slot = [&](uint32_t c) { return part + (2 * (size_t)c + (c == c0 ? 1 : 0)) * part_floats(ROWS, D); };
-  float M = -INFINITY;
-  for (uint32_t c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(slot(c) + ROWS * D + rl));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float acc[E], den = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; e++) acc[e] = 0.f;
-#pragma unroll 4
-  for (uint32_t c = c0 + warp; c <= c1; c += 4) {
-    const float* s = slot(c);
-    const float f = M == -INFINITY ? 1.f : ex2(__ldcg(s + ROWS * D + rl) - M);
-    den += __ldcg(s + ROWS * D + ROWS + rl) * f;
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[e] += __ldcg(s + (size_t)rl * D + lane + 32 * e) * f;
-  }
-#pragma unroll
-  for (int e = 0; e < E; e++) s_o[warp][lane + 32 * e] = acc[e];
-  if (lane == 0) s_l[warp] = den;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    const uint32_t d = threadIdx.x;
-    const float l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-    act_put(out + d, l == 0.f ? 0.f : (s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) / l);
-  }
-}
-
-// Scratch of one call: allocated and freed in stream order from a pool of this library's own
-// that keeps its memory, so calls on any stream, and captured ones, never share a buffer.
-int scratch_pool(cudaMemPool_t* out) {
-  static std::mutex mu;
-  static std::unordered_map<int, cudaMemPool_t> pools;
-  int dev = 0;
-  RF_CUDA(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lk(mu);
-  auto it = pools.find(dev);
-  if (it == pools.end()) {
-    cudaMemPoolProps p = {};
-    p.allocType = cudaMemAllocationTypePinned;
-    p.location.type = cudaMemLocationTypeDevice;
-    p.location.id = dev;
-    cudaMemPool_t pool;
-    RF_CUDA(cudaMemPoolCreate(&pool, &p));
-    uint64_t keep = UINT64_MAX;
-    RF_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
-    it = pools.emplace(dev, pool).first;
-  }
-  *out = it->second;
-  return RF_OK;
 }
 
 template <class T, bool Q8, int D, int NB>
 int run_rows(cudaStream_t st, const TreeArgs& a) {
   constexpr int ROWS = 8 * NB, KT = Step<Q8, D>::KEYS * kRowWarps;
   const uint32_t ctas = (uint32_t)num_sms() * (NB == 1 ? 3 : 2);
-  cudaMemPool_t pool;
-  RF_TRY(scratch_pool(&pool));
   void* part = nullptr;
-  RF_CUDA(cudaMallocFromPoolAsync(&part, 2 * (size_t)ctas * part_floats(ROWS, D) * sizeof(float), pool, st));
+  RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(ROWS, D) * sizeof(float), st));
   cudaError_t e = launch_k(Launch{st, false}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
                            (float*)part);
   if (e == cudaSuccess)
@@ -666,6 +452,33 @@ int run_tree(cudaStream_t st, const TreeArgs& a) {
 }
 
 }  // namespace
+
+int scratch_alloc(void** out, size_t bytes, cudaStream_t st) {
+  constexpr int kDevices = 64;
+  static std::mutex mu;
+  static cudaMemPool_t pools[kDevices];
+  int dev = 0;
+  RF_CUDA(cudaGetDevice(&dev));
+  if (dev >= kDevices) return set_error(RF_EUNSUPPORTED, "device %d is beyond the %d that have a scratch pool", dev, kDevices);
+  std::lock_guard<std::mutex> lk(mu);
+  if (!pools[dev]) {
+    cudaMemPoolProps p = {};
+    p.allocType = cudaMemAllocationTypePinned;
+    p.location.type = cudaMemLocationTypeDevice;
+    p.location.id = dev;
+    cudaMemPool_t pool;
+    RF_CUDA(cudaMemPoolCreate(&pool, &p));
+    uint64_t keep = UINT64_MAX;
+    RF_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+    pools[dev] = pool;
+  }
+  const cudaError_t e = cudaMallocFromPoolAsync(out, bytes, pools[dev], st);
+  if (e != cudaSuccess)
+    return set_error(e == cudaErrorMemoryAllocation ? RF_ENOMEM : RF_ECUDA, "%zu bytes of attention scratch: %s", bytes,
+                     cudaGetErrorString(e));
+  return RF_OK;
+}
+
 }  // namespace rf
 
 using namespace rf;
@@ -705,6 +518,7 @@ int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
   RF_TRY(verify_error_ptr(&a.err));
   const cudaStream_t st = (cudaStream_t)stream;
+  if (n_tokens * (n_heads / cache->n_kv_heads) > 16) return run_tree_tc(act_type, a, st);
   const bool q8 = cache->type == RF_TYPE_Q8_0;
   switch (act_type) {
     case RF_ACT_F32: return q8 ? run_tree<float, true>(st, a) : run_tree<float, false>(st, a);

@@ -1,0 +1,856 @@
+// rf_tree_tc.cu - rf_tree_attention for many query rows a KV head, on the 5th-generation
+// tensor cores.
+//
+// With R = drafted tokens x query heads a KV head, every cached byte takes part in about
+// R (f16) or 1.9 R (Q8_0) multiply-adds, so from some tens of rows on the products bound the
+// call, not HBM.  A CTA (one an SM) works on RT x 128 query rows of one KV head against a run
+// of 128-key tiles:
+//
+//   S[128 rows][128 keys] = Q K^T   A = Q, B = K, both K-major in shared memory
+//   O[128 rows][D]       += P V     A = P in tensor memory, B = V, MN-major in shared memory
+//
+// Both S and O live in tensor memory (512 columns: two S, two O), so a thread owns one
+// row of S, its softmax needs no exchange, and P goes back over S's columns.  K and V
+// tiles have the same layout in shared memory ([128 keys][64 dimensions] blocks of 128-byte
+// rows, 128-byte swizzle): read along the head they are K-major, read along the keys MN-major.
+//
+// Two groups of four warps do the softmax.  RT = 2: each has a row tile of its own and both
+// share every K and V tile.  RT = 1 (at most 128 rows, or f32): both have the same rows and
+// take the even and the odd key tiles, and are joined at the end.
+//
+//   warp 0        loads: f16 tiles by tensor copies, Q8_0 codes by plain bulk copies
+//   warp 1        all tcgen05.mma
+//   warps 2, 3    f16: V tiles that hold drafts or the end are made finite (below)
+//   warps 4 - 11  softmax, queries, outputs
+//   warps 12 - 15 Q8_0: codes * scales -> f16 operand tiles, one key a thread
+//
+// f32 queries and weights are split into two f16 terms, and each product into two MMAs.
+// What a row does not see has weight 0, and 0 * NaN would still be NaN: elements of drafts'
+// V rows that are not finite are replaced by 0 in shared memory, and a flag makes the
+// epilogue add them to the rows that do see them.
+//
+// Every wait is bounded (about a second): on expiry the kernel raises bit 0 of the error word,
+// all roles run through their loops without waiting or issuing, the copies and MMAs in
+// flight are waited for (bounded again), tensor memory is freed and the kernel returns.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "rf_tc.cuh"
+#include "rf_tree.cuh"
+
+namespace rf {
+namespace {
+
+constexpr int TK = 128;                      // keys of a tile, rows of a row tile
+constexpr uint32_t kOperandBytes = 224 * 1024;
+constexpr uint32_t kBlockBytes = TK * 128;   // one [128][64] f16 block
+constexpr uint32_t kAuxBytes = 2560;
+
+template <class T, bool Q8, int D, int RT>
+struct Shape {
+  static constexpr bool SPLIT = std::is_same<T, float>::value;
+  static constexpr int ROWS = TK * RT;
+  static constexpr int THREADS = Q8 ? 512 : 384;
+  static constexpr uint32_t TILE = TK * D * 2;
+  static constexpr uint32_t RAW = TK * D;
+  static constexpr uint32_t QBYTES = TILE * RT * (SPLIT ? 2 : 1);
+  // raw tiles in flight: one row tile is bound by the cache's bytes, two by the products
+  static constexpr int NRAW = Q8 ? (RT == 2 && D == 128 ? 2 : 4) : 0;
+  static constexpr int kFit = (kOperandBytes - QBYTES - NRAW * RAW) / TILE;
+  static constexpr int NSLOT = kFit < 6 ? kFit : 6;
+  static constexpr uint32_t SMEM = kOperandBytes + kAuxBytes;
+  static constexpr int LEAD = RT == 1 ? 2 : 1;  // K tiles loaded ahead of the first V tile
+};
+
+// ---- tensor memory ------------------------------------------------------------------
+// 32x32b accesses: the thread's lane (32 * (warp % 4) + lane), consecutive columns.
+__device__ __forceinline__ void tmem_ld_64(uint32_t addr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+      "}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+      "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32"
+      "};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- operands -------------------------------------------------------------------------
+// 128-byte swizzled operand: 8-row groups 1024 bytes apart; MN-major blocks of 64 elements
+// kBlockBytes apart (ignored for K-major, where a k step stays inside one 128-byte row).
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(kBlockBytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16, f16 operands, f32 accumulator, M = 128; b_mn: B is MN-major.
+constexpr uint32_t idesc_f16(int N, bool b_mn) {
+  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(TK >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  tc_mma_bf16(d, a, b, idesc, acc);  // the operand type is the descriptor's
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// 16-byte piece `c` (of D / 8) of row r in an operand tile.
+__device__ __forceinline__ uint32_t sw128_offset(uint32_t r, uint32_t c) {
+  return (c >> 3) * kBlockBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Non-finite f16 halves of a word replaced by 0.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x, bool* wild) {
+  const bool lo = (x & 0x7c00u) == 0x7c00u, hi = (x & 0x7c000000u) == 0x7c000000u;
+  *wild |= lo || hi;
+  return x & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+}
+
+// ---- shared-memory bookkeeping -----------------------------------------------------------
+template <class S>
+struct Bars {
+  uint64_t full[S::NSLOT], free[S::NSLOT];
+  uint64_t raw_full[S::NRAW ? S::NRAW : 1], raw_free[S::NRAW ? S::NRAW : 1];
+  uint64_t q_full, s_full[2], p_full[2], pv_done[2], fix_ask, fix_done, drain;
+  uint32_t tmem, stop, wild, fix_slot;
+  float ml[2][TK][2];
+};
+
+// A position in a ring of N slots: its index and the parity of its current use.
+template <int N>
+struct Ring {
+  uint32_t s = 0, phase = 0;
+  __device__ __forceinline__ void advance() {
+    if (++s == N) s = 0, phase ^= 1;
+  }
+};
+
+// Bounded wait for the phase of `bar` with `parity`; false once any wait of the CTA gave up.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+  const long long t0 = clock64();
+  while (!tc_mbar_try_wait(bar, parity)) {
+    if (*stop) return false;
+    if (clock64() - t0 > 2000000000LL) {
+      *stop = 1;
+      atomicOr(err, kVerifyTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+  const uint32_t b = tc_smem_u32(bar);
+  return tc_mbar_try_wait(b, parity) || wait_slow(b, parity, stop, err);
+}
+
+// The e-th tile a segment of nt key tiles loads (2 nt of them): LEAD K tiles, then V and K in turn.
+__device__ __forceinline__ void item_at(uint32_t e, uint32_t nt, uint32_t lead, bool* is_v, uint32_t* i) {
+  const uint32_t first = min(lead, nt);
+  if (e < first) {
+    *is_v = false, *i = e;
+    return;
+  }
+  const uint32_t x = e - first, pairs = nt - first;
+  if (x < 2 * pairs)
+    *is_v = !(x & 1), *i = x & 1 ? first + x / 2 : x / 2;
+  else
+    *is_v = true, *i = x - pairs;
+}
+
+// Bit i: token t sees draft j0 + i (drafts below 0 are history, drafts from n on do not exist).
+__device__ __forceinline__ uint32_t seen32(const uint32_t* mask_row, uint32_t words, uint32_t t, int j0, int n) {
+  if (j0 >= n) return 0;
+  if (j0 <= -32) return ~0u;
+  uint32_t v;
+  if (!mask_row) {
+    const int count = (int)t - j0 + 1;
+    v = count <= 0 ? 0 : count >= 32 ? ~0u : (1u << count) - 1;
+  } else if (j0 >= 0) {
+    const uint32_t w = j0 >> 5, sh = j0 & 31;
+    v = mask_row[w] >> sh;
+    if (sh && w + 1 < words) v |= mask_row[w + 1] << (32 - sh);
+  } else {
+    v = (mask_row[0] << -j0) | ((1u << -j0) - 1);
+  }
+  return n - j0 < 32 ? v & ((1u << (n - j0)) - 1) : v;
+}
+
+// 16 bytes of a row as f32 (8 or 4 values).
+template <class T>
+__device__ __forceinline__ void act_load8(const T* p, float (&v)[8]) {
+  if constexpr (std::is_same<T, float>::value) {
+    const float4 x = __ldg((const float4*)p), y = __ldg((const float4*)p + 1);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 u = __ldg((const uint4*)p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_h2_rest(float a, float b, uint32_t hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return pack_h2(a - f.x, b - f.y);
+}
+
+template <class T, bool Q8, int D, int RT>
+__global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
+    tree_tc_kernel(const TreeArgs a, float* __restrict__ part, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v) {
+  using S = Shape<T, Q8, D, RT>;
+  constexpr bool SPLIT = S::SPLIT;
+  extern __shared__ __align__(1024) uint8_t tsm[];
+  Bars<S>& B = *reinterpret_cast<Bars<S>*>(tsm + kOperandBytes);
+  static_assert(sizeof(Bars<S>) <= kAuxBytes, "bookkeeping must fit");
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t q_smem = tc_smem_u32(tsm), slots = q_smem + S::QBYTES, raws = slots + S::NSLOT * S::TILE;
+  auto slot_addr = [&](uint32_t s) { return slots + s * S::TILE; };
+  griddep_launch();
+  if (q_smem & 1023u) {  // the swizzle is a function of the address
+    if (tid == 0) atomicOr(a.err, kVerifyTimeout);
+    return;
+  }
+  if (warp == 1) tc_tmem_alloc(tc_smem_u32(&B.tmem), 512);
+  if (tid == 0) {
+    for (int i = 0; i < S::NSLOT; i++) {
+      tc_mbar_init(tc_smem_u32(&B.full[i]), Q8 ? 4 : 1);
+      tc_mbar_init(tc_smem_u32(&B.free[i]), 1);
+    }
+    for (int i = 0; i < S::NRAW; i++) {
+      tc_mbar_init(tc_smem_u32(&B.raw_full[i]), 1);
+      tc_mbar_init(tc_smem_u32(&B.raw_free[i]), 4);
+    }
+    tc_mbar_init(tc_smem_u32(&B.q_full), 256);
+    for (int i = 0; i < 2; i++) {
+      tc_mbar_init(tc_smem_u32(&B.s_full[i]), 1);
+      tc_mbar_init(tc_smem_u32(&B.p_full[i]), 4);
+      tc_mbar_init(tc_smem_u32(&B.pv_done[i]), 1);
+    }
+    tc_mbar_init(tc_smem_u32(&B.fix_ask), 1);
+    tc_mbar_init(tc_smem_u32(&B.fix_done), 2);
+    tc_mbar_init(tc_smem_u32(&B.drain), 1);
+    B.stop = B.wild = 0;
+    tc_fence_barrier_init();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = B.tmem;
+  auto s_col = [&](uint32_t g) { return tmem + 128 * g; };
+  auto o_col = [&](uint32_t g) { return tmem + 256 + 128 * g; };
+  volatile uint32_t* stop = &B.stop;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bar(bar, parity, stop, a.err); };
+  bool ok = true;
+  const uint32_t G = a.n_heads / a.c.n_kv_heads;
+  Walk<TK, S::ROWS> walk(a);
+  Segment sg;
+
+  if (warp == 0) {
+    // ---- loads ------------------------------------------------------------------------
+    if (lane == 0) {
+      constexpr int N = Q8 ? S::NRAW : S::NSLOT;
+      uint64_t* full = Q8 ? B.raw_full : B.full;
+      uint64_t* free = Q8 ? B.raw_free : B.free;
+      Ring<N> ring;
+      uint32_t issued = 0;
+      while (walk.next(a, &sg)) {
+        const uint32_t nt = sg.k1 - sg.k0, plane = sg.b * a.c.n_kv_heads + sg.h;
+        for (uint32_t e = 0; e < 2 * nt; e++) {
+          bool is_v;
+          uint32_t i;
+          item_at(e, nt, S::LEAD, &is_v, &i);
+          ok = ok && wait(&free[ring.s], ring.phase ^ 1);
+          if (ok) {
+            const uint32_t bar = tc_smem_u32(&full[ring.s]), key0 = (sg.k0 + i) * TK;
+            if constexpr (Q8) {  // rows past the capacity are not part of this head (or of the plane)
+              const uint32_t bytes = min((uint32_t)TK, a.c.capacity - key0) * D;
+              const uint8_t* src = (const uint8_t*)(is_v ? a.c.v : a.c.k) + ((uint64_t)plane * a.c.capacity + key0) * D;
+              tc_bulk_g2s(raws + ring.s * S::RAW, src, bytes, bar);
+            } else {
+              tc_mbar_expect_tx(bar, S::TILE);
+#pragma unroll
+              for (int x = 0; x < D / 64; x++)
+                tma_load_3d(slot_addr(ring.s) + x * kBlockBytes, is_v ? &map_v : &map_k, 64 * x, (int)key0, (int)plane, bar);
+            }
+            issued++;
+          }
+          ring.advance();
+        }
+      }
+      if (!ok || *stop) {  // copies nobody waited for must land before the CTA's memory is given up
+        Ring<N> r;
+        for (uint32_t i = 0; i < issued; i++) {
+          if (i + N >= issued) tc_mbar_wait(tc_smem_u32(&full[r.s]), r.phase);
+          r.advance();
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- all MMAs -----------------------------------------------------------------------
+    if (lane == 0) {
+      Ring<S::NSLOT> ring;
+      uint32_t q_phase = 0, fix_phase = 0, pv_count[2] = {0, 0};
+      constexpr uint32_t id_s = idesc_f16(TK, false), id_o = idesc_f16(D, true);
+      auto take = [&]() {
+        const uint32_t s = ring.s;
+        ok = ok && wait(&B.full[s], ring.phase);
+        ring.advance();
+        return s;
+      };
+      // V tiles that hold drafts or the end go through warps 2 and 3 while the softmax runs
+      auto take_v = [&](bool drafts) {
+        const uint32_t s = take();
+        if (!Q8 && drafts && ok) {
+          *(volatile uint32_t*)&B.fix_slot = s;
+          tc_mbar_arrive(tc_smem_u32(&B.fix_ask));
+        }
+        return s;
+      };
+      auto fixed = [&](bool drafts) {
+        if (!Q8 && drafts) {
+          ok = ok && wait(&B.fix_done, fix_phase);
+          fix_phase ^= 1;
+        }
+      };
+      auto release = [&](uint32_t s) {
+        if (ok) tc_commit(tc_smem_u32(&B.free[s]));
+      };
+      // S of group g: P of the tile before sits in the same columns, so its product must be over
+      auto qk = [&](uint32_t g, uint32_t s) {
+        if (pv_count[g]) ok = ok && wait(&B.pv_done[g], (pv_count[g] - 1) & 1);
+        if (!ok) return;
+        tc_fence_after_sync();
+        const uint32_t q = q_smem + (RT == 2 ? g * S::TILE : 0), k = slot_addr(s);
+#pragma unroll
+        for (int term = 0; term < (SPLIT ? 2 : 1); term++)
+#pragma unroll
+          for (int i = 0; i < D / 16; i++) {
+            const uint32_t o = (i / 4) * kBlockBytes + (i % 4) * 32;
+            mma_ss(s_col(g), sw128_desc(q + term * S::TILE + o), sw128_desc(k + o), id_s, term > 0 || i > 0);
+          }
+        tc_commit(tc_smem_u32(&B.s_full[g]));
+      };
+      auto pv = [&](uint32_t g, uint32_t s, bool first, bool drafts) {
+        ok = ok && wait(&B.p_full[g], pv_count[g] & 1);
+        pv_count[g]++;
+        fixed(drafts);
+        if (!ok) return;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < TK / 16; i++) {
+          const uint32_t p = s_col(g) + 64 * (i / 4) + 8 * (i % 4);
+          const uint64_t v = sw128_desc(slot_addr(s) + i * 16 * 128);
+          mma_ts(o_col(g), p, v, id_o, !first || i > 0);
+          if constexpr (SPLIT) mma_ts(o_col(g), p + 32, v, id_o, true);
+        }
+        tc_commit(tc_smem_u32(&B.pv_done[g]));
+      };
+      while (walk.next(a, &sg)) {
+        const uint32_t nt = sg.k1 - sg.k0;
+        const bool two = RT == 2 && sg.drafts * G - sg.rt * S::ROWS > TK;
+        auto drafts_in = [&](uint32_t i) { return (sg.k0 + i + 1) * TK > sg.hist; };
+        ok = ok && wait(&B.q_full, q_phase);
+        q_phase ^= 1;
+        if constexpr (RT == 1) {
+          for (uint32_t i = 0; i < min(2u, nt); i++) {
+            const uint32_t k = take();
+            qk(i, k);
+            release(k);
+          }
+          for (uint32_t i = 0; i < nt; i++) {
+            const uint32_t v = take_v(drafts_in(i));
+            pv(i & 1, v, i < 2, drafts_in(i));
+            release(v);
+            if (i + 2 < nt) {
+              const uint32_t k = take();
+              qk(i & 1, k);
+              release(k);
+            }
+          }
+        } else {
+          uint32_t k = take();
+          qk(0, k);
+          if (two) qk(1, k);
+          release(k);
+          for (uint32_t i = 0; i < nt; i++) {
+            const uint32_t v = take_v(drafts_in(i));
+            const bool more = i + 1 < nt;
+            pv(0, v, i == 0, drafts_in(i));
+            if (more) {
+              k = take();
+              qk(0, k);
+            }
+            if (two) pv(1, v, i == 0, false);
+            release(v);
+            if (more) {
+              if (two) qk(1, k);
+              release(k);
+            }
+          }
+        }
+      }
+      // everything issued is over before tensor and shared memory are given up
+      tc_commit(tc_smem_u32(&B.drain));
+      tc_mbar_wait(tc_smem_u32(&B.drain), 0);
+    }
+  } else if (warp < 4) {
+    // ---- f16 V tiles with drafts or the end: rows past the end 0, drafts' rows finite ------
+    if constexpr (!Q8) {
+      uint32_t phase = 0;
+      while (walk.next(a, &sg)) {
+        for (uint32_t tile = max(sg.k0, sg.hist / TK); tile < sg.k1; tile++) {
+          const uint32_t key0 = tile * TK;
+          ok = __all_sync(~0u, ok && wait(&B.fix_ask, phase));
+          phase ^= 1;
+          if (ok) {
+            const uint32_t from = sg.hist > key0 ? sg.hist - key0 : 0, v = slot_addr(*(volatile uint32_t*)&B.fix_slot);
+            bool wild = false;
+            for (uint32_t x = from * 8 + (tid - 64); x < TK * 8; x += 64) {  // 16-byte pieces, in memory order
+              const bool real = key0 + x / 8 < sg.end;
+#pragma unroll
+              for (int blk = 0; blk < D / 64; blk++) {
+                const uint32_t at = v + blk * kBlockBytes + x * 16;
+                uint4 u = real ? ld_shared16(at) : make_uint4(0, 0, 0, 0);
+                bool odd = !real;
+                u.x = finite_halves(u.x, &odd), u.y = finite_halves(u.y, &odd);
+                u.z = finite_halves(u.z, &odd), u.w = finite_halves(u.w, &odd);
+                if (odd) st_shared16(at, u);
+                wild |= real && odd;
+              }
+            }
+            if (wild) *(volatile uint32_t*)&B.wild = 1;
+          }
+          tc_fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.fix_done));
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ---- softmax ----------------------------------------------------------------------
+    const uint32_t g = (warp - 4) / 4, row = 32 * (warp % 4) + lane, lanes = (32 * (warp % 4)) << 16;
+    uint32_t count = 0;  // tiles of this group so far
+    while (walk.next(a, &sg)) {
+      const uint32_t nt = sg.k1 - sg.k0, n_rows = sg.drafts * G;
+      const uint32_t r = sg.rt * S::ROWS + (RT == 2 ? g * TK : 0) + row;
+      const bool live = r < n_rows, warp_live = r - lane < n_rows;
+      const uint32_t t = live ? r / G : 0, hq = sg.h * G + (live ? r % G : 0);
+      const uint64_t token = (uint64_t)sg.b * a.n_tokens + t;
+      // queries: f32 and bf16 rows are scaled by a power of two to a largest magnitude in [1, 2)
+      float coef = a.scale * 1.44269504f;
+      {
+        const T* q = (const T*)a.q + token * a.q_stride + (uint64_t)hq * D;
+        float down0 = 1.f, down1 = 1.f;
+        if constexpr (!std::is_same<T, __half>::value) {
+          float top = 0.f;
+#pragma unroll 4
+          for (int c = 0; c < D / 8; c++) {
+            float v[8];
+            act_load8(q + 8 * c, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]));
+          }
+          if (top > 0.f && top < INFINITY) {
+            const int e = ilogbf(top);  // in two factors: 2^-e alone leaves f32 for the smallest rows
+            down0 = ldexpf(1.f, -(e / 2)), down1 = ldexpf(1.f, -(e - e / 2));
+            coef *= ldexpf(1.f, e);
+          }
+        }
+        if (RT == 2 || g == 0) {
+          const uint32_t dst = q_smem + (RT == 2 ? g * S::TILE : 0);
+#pragma unroll 4
+          for (int c = 0; c < D / 8; c++) {
+            float v[8];
+            act_load8(q + 8 * c, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = live ? v[i] * down0 * down1 : 0.f;
+            uint4 hi;
+            hi.x = pack_h2(v[0], v[1]), hi.y = pack_h2(v[2], v[3]), hi.z = pack_h2(v[4], v[5]), hi.w = pack_h2(v[6], v[7]);
+            st_shared16(dst + sw128_offset(row, c), hi);
+            if constexpr (SPLIT) {
+              uint4 lo;
+              lo.x = pack_h2_rest(v[0], v[1], hi.x), lo.y = pack_h2_rest(v[2], v[3], hi.y);
+              lo.z = pack_h2_rest(v[4], v[5], hi.z), lo.w = pack_h2_rest(v[6], v[7], hi.w);
+              st_shared16(dst + S::TILE + sw128_offset(row, c), lo);
+            }
+          }
+        }
+        tc_fence_proxy_async();
+        tc_mbar_arrive(tc_smem_u32(&B.q_full));
+      }
+      const uint32_t* mask_row = a.mask ? a.mask + token * a.words : nullptr;
+      const bool two = n_rows - sg.rt * S::ROWS > TK;
+      const uint32_t mine = RT == 1 ? (nt + 1 - g) / 2 : (g == 0 || two ? nt : 0);
+      float m = -INFINITY, l = 0.f;
+      for (uint32_t x = 0; x < mine; x++, count++) {
+        const uint32_t key0 = (sg.k0 + (RT == 1 ? 2 * x + g : x)) * TK;
+        const bool edge = key0 + TK > sg.hist;
+        ok = __all_sync(~0u, ok && wait(&B.s_full[g], count & 1));
+        if (ok && warp_live) {
+          tc_fence_after_sync();
+          float top = -INFINITY;
+          uint32_t see[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            see[i] = edge ? seen32(mask_row, a.words, t, (int)(key0 + 32 * i) - (int)sg.hist, (int)sg.drafts) : ~0u;
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            uint32_t s[64];
+            tmem_ld_64(s_col(g) + lanes + 64 * half, s);
+#pragma unroll
+            for (int i = 0; i < 64; i++) {
+              float v = __uint_as_float(s[i]);
+              if (edge && !((see[2 * half + i / 32] >> (i % 32)) & 1)) v = -INFINITY;
+              top = fmaxf(top, v);
+            }
+          }
+          top *= coef;
+          if (__any_sync(0xffffffffu, top > m + kRaise)) {
+            const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+            m = m2;
+            l *= f;
+            if (x > 0) {
+              ok = __all_sync(~0u, ok && wait(&B.pv_done[g], (count - 1) & 1));
+              tc_fence_after_sync();
+#pragma unroll
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32(o_col(g) + lanes + c, o);
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st_32(o_col(g) + lanes + c, o);
+              }
+            }
+          }
+          const float ref = (m == -INFINITY ? 0.f : m) - kWeightBias;
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            uint32_t s[64], p[32];
+            tmem_ld_64(s_col(g) + lanes + 64 * half, s);
+#pragma unroll
+            for (int i = 0; i < 64; i++) {
+              float v = ex2(fmaf(__uint_as_float(s[i]), coef, -ref));
+              if (edge && !((see[2 * half + i / 32] >> (i % 32)) & 1)) v = 0.f;
+              l += v;
+              s[i] = __float_as_uint(v);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) p[i] = pack_h2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+            tmem_st_32(s_col(g) + lanes + 64 * half, p);
+            if constexpr (SPLIT) {
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                p[i] = pack_h2_rest(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), p[i]);
+              tmem_st_32(s_col(g) + lanes + 64 * half + 32, p);
+            }
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.p_full[g]));
+      }
+      if (mine) ok = __all_sync(~0u, ok && wait(&B.pv_done[g], (count - 1) & 1));
+      // ---- output: RT = 1 joins the two groups, each writing half of the dimensions
+      bool has[2] = {mine > 0, false};
+      float f[2] = {1.f, 0.f}, M = m, den = l;
+      uint32_t src0 = o_col(g);
+      if constexpr (RT == 1) {
+        B.ml[g][row][0] = m, B.ml[g][row][1] = l;
+        __syncwarp();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        has[0] = true, has[1] = nt > 1;
+        const float m0 = B.ml[0][row][0], m1 = B.ml[1][row][0];
+        M = fmaxf(m0, m1);
+        f[0] = M == -INFINITY ? 1.f : ex2(m0 - M), f[1] = M == -INFINITY ? 1.f : ex2(m1 - M);
+        den = B.ml[0][row][1] * f[0] + B.ml[1][row][1] * f[1];
+        src0 = o_col(0);
+      }
+      if (ok && warp_live && has[0]) {
+        tc_fence_after_sync();
+        const bool whole = sg.whole();
+        const float inv = !whole ? 1.f : den == 0.f ? 0.f : 1.f / den;
+        float* slot = part + (2 * (size_t)blockIdx.x + (sg.k0 > 0 ? 0 : 1)) * part_floats(S::ROWS, D);
+        const uint32_t rl = r - sg.rt * S::ROWS;
+        constexpr int DIMS = RT == 1 ? D / 2 : D;
+        const uint32_t d0 = RT == 1 ? g * DIMS : 0;
+        const bool wild = *(volatile uint32_t*)&B.wild != 0;
+#pragma unroll 1
+        for (uint32_t d = d0; d < d0 + DIMS; d += 32) {
+          uint32_t o[32];
+          float v[32];
+          tmem_ld_32(src0 + lanes + d, o);
+#pragma unroll
+          for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * f[0];
+          if (has[1]) {
+            tmem_ld_32(o_col(1) + lanes + d, o);
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[i] = fmaf(__uint_as_float(o[i]), f[1], v[i]);
+          }
+          if (!live) continue;
+          if (wild) {  // rare: what was left out of the drafts' V, for the rows that see it
+            const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
+            for (uint32_t p = max(sg.hist, sg.k0 * TK); p < min(sg.end, sg.k1 * TK); p++) {
+              if (!sees(a, sg.b, t, sg.hist, p)) continue;
+#pragma unroll
+              for (int i = 0; i < 32; i++) {
+                const uint64_t at = (base + p) * D + d + i;
+                float y;
+                if constexpr (Q8)
+                  y = __half2float(__float2half_rn((float)((const int8_t*)a.c.v)[at] *
+                                                   __half2float(((const __half*)a.c.v_scale)[at / 32])));
+                else
+                  y = __half2float(((const __half*)a.c.v)[at]);
+                if (!(fabsf(y) < INFINITY)) v[i] += y;
+              }
+            }
+          }
+          if (whole) {
+            T* out = (T*)a.out + token * a.out_stride + (uint64_t)hq * D + d;
+#pragma unroll
+            for (int i = 0; i < 32; i += 16 / sizeof(T)) {
+              __align__(16) T w[16 / sizeof(T)];
+#pragma unroll
+              for (int j = 0; j < (int)(16 / sizeof(T)); j++) act_put(&w[j], v[i + j] * inv);
+              *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(w);
+            }
+          } else {
+            float* dst = slot + (size_t)rl * D + d;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            if (d == 0) slot[S::ROWS * D + rl] = M, slot[S::ROWS * D + S::ROWS + rl] = den;
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if constexpr (RT == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+  } else {
+    // ---- Q8_0 tiles to f16: thread = key; pieces taken in an order that keeps the eight
+    // lanes of a shared-memory phase on different banks, for the codes and for the tile
+    if constexpr (Q8) {
+      const uint32_t key = tid - 384;
+      Ring<S::NRAW> rr;
+      Ring<S::NSLOT> ring;
+      while (walk.next(a, &sg)) {
+        const uint32_t nt = sg.k1 - sg.k0;
+        const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
+        // scales of the e-th tile's key; 0 past the end, so that those rows become 0
+        auto scales = [&](uint32_t e) {
+          uint2 s = make_uint2(0, 0);
+          if (e >= 2 * nt) return s;
+          bool is_v;
+          uint32_t i;
+          item_at(e, nt, S::LEAD, &is_v, &i);
+          const uint32_t p = (sg.k0 + i) * TK + key;
+          if (p >= sg.end) return s;
+          const __half* plane = (const __half*)(is_v ? a.c.v_scale : a.c.k_scale) + (base + p) * (D / 32);
+          if constexpr (D == 128)
+            s = __ldg((const uint2*)plane);
+          else
+            s.x = __ldg((const uint32_t*)plane);
+          return s;
+        };
+        uint2 s0 = scales(0), s1 = scales(1);
+        for (uint32_t e = 0; e < 2 * nt; e++) {
+          bool is_v;
+          uint32_t i;
+          item_at(e, nt, S::LEAD, &is_v, &i);
+          const uint2 sc = s0;
+          s0 = s1;
+          s1 = scales(e + 2);
+          const uint32_t p = (sg.k0 + i) * TK + key;
+          const bool draft_v = is_v && p >= sg.hist;
+          ok = __all_sync(~0u, ok && wait(&B.raw_full[rr.s], rr.phase) && wait(&B.free[ring.s], ring.phase ^ 1));
+          if (ok) {
+            const uint32_t raw = raws + rr.s * S::RAW + key * D, dst = slot_addr(ring.s);
+            bool wild = false;
+#pragma unroll
+            for (int j = 0; j < D / 16; j++) {
+              const uint32_t c = (j + lane) & (D / 16 - 1);
+              const uint4 u = ld_shared16(raw + 16 * c);
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w}, sw = c >= 4 ? sc.y : sc.x;
+              const uint32_t db = __byte_perm(sw, sw, c & 2 ? 0x3232 : 0x1010);
+              const __half2 d = *reinterpret_cast<const __half2*>(&db);
+              uint32_t h[8];
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                // biased bytes under an exponent of 1024: 1152 + code, exact; the product rounds once
+                const uint32_t b = w[k] ^ 0x80808080u;
+                uint32_t lo = __byte_perm(b, 0x64646464u, 0x4140), hi = __byte_perm(b, 0x64646464u, 0x4342);
+                const __half2 bias = __float2half2_rn(1152.f);
+                const __half2 x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), bias), d);
+                const __half2 y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), bias), d);
+                h[2 * k] = *reinterpret_cast<const uint32_t*>(&x), h[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+              if (draft_v) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) h[k] = finite_halves(h[k], &wild);
+              }
+              st_shared16(dst + sw128_offset(key, 2 * c), make_uint4(h[0], h[1], h[2], h[3]));
+              st_shared16(dst + sw128_offset(key, 2 * c + 1), make_uint4(h[4], h[5], h[6], h[7]));
+            }
+            if (wild) *(volatile uint32_t*)&B.wild = 1;
+          }
+          tc_fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tc_mbar_arrive(tc_smem_u32(&B.full[ring.s]));
+            tc_mbar_arrive(tc_smem_u32(&B.raw_free[rr.s]));
+          }
+          rr.advance();
+          ring.advance();
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tc_tmem_dealloc(tmem, 512);
+  }
+}
+
+// Tensor map of an f16 plane [heads][capacity][D], copied in boxes of 64 dimensions x 128 positions.
+int plane_map(CUtensorMap* map, const void* p, const rf_kv_view& c) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static void* fn = nullptr;
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    RF_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !f) return set_error(RF_ECUDA, "cuTensorMapEncodeTiled is not available");
+    fn = f;
+  }
+  const cuuint64_t dims[3] = {c.head_dim, c.capacity, (cuuint64_t)c.n_seqs * c.n_kv_heads};
+  const cuuint64_t strides[2] = {2ull * c.head_dim, 2ull * c.head_dim * c.capacity};
+  const cuuint32_t box[3] = {64, TK, 1}, step[3] = {1, 1, 1};
+  const CUresult r = ((Encode)fn)(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(RF_ECUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+  return RF_OK;
+}
+
+template <class T, bool Q8, int D, int RT>
+int run(cudaStream_t st, const TreeArgs& a) {
+  using S = Shape<T, Q8, D, RT>;
+  CUtensorMap mk{}, mv{};
+  if constexpr (!Q8) {
+    RF_TRY(plane_map(&mk, a.c.k, a.c));
+    RF_TRY(plane_map(&mv, a.c.v, a.c));
+  }
+  auto* k = tree_tc_kernel<T, Q8, D, RT>;
+  RF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+  const uint32_t ctas = (uint32_t)num_sms();
+  void* part = nullptr;
+  RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(S::ROWS, D) * sizeof(float), st));
+  cudaError_t e = launch_k(Launch{st, false}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
+  if (e == cudaSuccess)
+    e = launch_k(Launch{st, true}, tree_merge_kernel<T, D, TK, S::ROWS>, dim3(a.n_seqs * a.n_tokens * a.n_heads), dim3(128),
+                 0, a, (const float*)part, ctas);
+  const cudaError_t f = cudaFreeAsync(part, st);
+  RF_CUDA(e);
+  RF_CUDA(f);
+  return RF_OK;
+}
+
+template <class T, bool Q8, int D>
+int run_shape(cudaStream_t st, const TreeArgs& a) {
+  // f32 splits its queries, which takes the second row tile's place in shared memory
+  if constexpr (!std::is_same<T, float>::value)
+    if (a.n_tokens * (a.n_heads / a.c.n_kv_heads) > TK) return run<T, Q8, D, 2>(st, a);
+  return run<T, Q8, D, 1>(st, a);
+}
+
+template <class T>
+int run_type(cudaStream_t st, const TreeArgs& a) {
+  const bool q8 = a.c.type == RF_TYPE_Q8_0;
+  if (a.c.head_dim == 128) return q8 ? run_shape<T, true, 128>(st, a) : run_shape<T, false, 128>(st, a);
+  return q8 ? run_shape<T, true, 64>(st, a) : run_shape<T, false, 64>(st, a);
+}
+
+}  // namespace
+
+int run_tree_tc(int act_type, const TreeArgs& a, cudaStream_t st) {
+  switch (act_type) {
+    case RF_ACT_F32: return run_type<float>(st, a);
+    case RF_ACT_F16: return run_type<__half>(st, a);
+    default: return run_type<__nv_bfloat16>(st, a);
+  }
+}
+
+}  // namespace rf
