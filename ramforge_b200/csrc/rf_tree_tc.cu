@@ -65,39 +65,25 @@ struct Shape {
 
 // ---- tensor memory ------------------------------------------------------------------
 // 32x32b accesses: the thread's lane (32 * (warp % 4) + lane), consecutive columns.
-__device__ __forceinline__ void tmem_ld_64(uint32_t addr, uint32_t (&r)[64]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
-      "}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
-      "}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
+}
+// The loads before are complete; the registers pass through so that no use moves above the wait.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -111,7 +97,6 @@ __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t (&r)[32
       "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- operands -------------------------------------------------------------------------
@@ -155,6 +140,28 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   return v;
 }
 
+// ---- pairs of f32 in one instruction ------------------------------------------------------
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Non-finite f16 halves of a word replaced by 0.
 __device__ __forceinline__ uint32_t finite_halves(uint32_t x, bool* wild) {
   const bool lo = (x & 0x7c00u) == 0x7c00u, hi = (x & 0x7c000000u) == 0x7c000000u;
@@ -182,7 +189,7 @@ struct Ring {
 };
 
 // Bounded wait for the phase of `bar` with `parity`; false once any wait of the CTA gave up.
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
   const long long t0 = clock64();
   while (!tc_mbar_try_wait(bar, parity)) {
     if (*stop) return false;
@@ -312,6 +319,10 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   Walk<TK, S::ROWS> walk(a);
   Segment sg;
 
+  // Registers: a softmax thread holds a whole row of S.  The shares add up to what the block was
+  // launched with: 512 x 128 = 128 x (56 + 88 + 2 x 184), 384 x 168 = 128 x (72 + 2 x 216).
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 56 : 72));
   if (warp == 0) {
     // ---- loads ------------------------------------------------------------------------
     if (lane == 0) {
@@ -389,11 +400,11 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         tc_fence_after_sync();
         const uint32_t q = q_smem + (RT == 2 ? g * S::TILE : 0), k = slot_addr(s);
 #pragma unroll
-        for (int term = 0; term < (SPLIT ? 2 : 1); term++)
+        for (int term = SPLIT ? 1 : 0; term >= 0; term--)  // the small term first: the sum truncates at its own size
 #pragma unroll
           for (int i = 0; i < D / 16; i++) {
             const uint32_t o = (i / 4) * kBlockBytes + (i % 4) * 32;
-            mma_ss(s_col(g), sw128_desc(q + term * S::TILE + o), sw128_desc(k + o), id_s, term > 0 || i > 0);
+            mma_ss(s_col(g), sw128_desc(q + term * S::TILE + o), sw128_desc(k + o), id_s, (SPLIT && term == 0) || i > 0);
           }
         tc_commit(tc_smem_u32(&B.s_full[g]));
       };
@@ -460,7 +471,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       tc_commit(tc_smem_u32(&B.drain));
       tc_mbar_wait(tc_smem_u32(&B.drain), 0);
     }
-  } else if (warp < 4) {
+  } else {
     // ---- f16 V tiles with drafts or the end: rows past the end 0, drafts' rows finite ------
     if constexpr (!Q8) {
       uint32_t phase = 0;
@@ -493,7 +504,9 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         }
       }
     }
+  }
   } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8 ? 184 : 216));
     // ---- softmax ----------------------------------------------------------------------
     const uint32_t g = (warp - 4) / 4, row = 32 * (warp % 4) + lane, lanes = (32 * (warp % 4)) << 16;
     uint32_t count = 0;  // tiles of this group so far
@@ -520,7 +533,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           if (top > 0.f && top < INFINITY) {
             const int e = ilogbf(top);  // in two factors: 2^-e alone leaves f32 for the smallest rows
             down0 = ldexpf(1.f, -(e / 2)), down1 = ldexpf(1.f, -(e - e / 2));
-            coef *= ldexpf(1.f, e);
+            coef = fmaxf(coef * ldexpf(1.f, e), 1.17549435e-38f);  // not 0: a masked score stays -inf
           }
         }
         if (RT == 2 || g == 0) {
@@ -555,23 +568,27 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         ok = __all_sync(~0u, ok && wait(&B.s_full[g], count & 1));
         if (ok && warp_live) {
           tc_fence_after_sync();
-          float top = -INFINITY;
-          uint32_t see[4];
+          uint32_t s[TK];
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            see[i] = edge ? seen32(mask_row, a.words, t, (int)(key0 + 32 * i) - (int)sg.hist, (int)sg.drafts) : ~0u;
+          for (int i = 0; i < TK; i += 32) tmem_ld_32(s_col(g) + lanes + i, s + i);
+          tmem_wait_ld(s);
+          if (edge) {
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            uint32_t s[64];
-            tmem_ld_64(s_col(g) + lanes + 64 * half, s);
+            for (int i = 0; i < TK / 32; i++) {
+              const uint32_t see =
+                  seen32(mask_row, a.words, t, (int)(key0 + 32 * i) - (int)sg.hist, (int)sg.drafts);
 #pragma unroll
-            for (int i = 0; i < 64; i++) {
-              float v = __uint_as_float(s[i]);
-              if (edge && !((see[2 * half + i / 32] >> (i % 32)) & 1)) v = -INFINITY;
-              top = fmaxf(top, v);
+              for (int j = 0; j < 32; j++)
+                if (!((see >> j) & 1)) s[32 * i + j] = 0xff800000u;
             }
           }
-          top *= coef;
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < TK; i += 8)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              tops[j] = max3(tops[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * coef;
           if (__any_sync(0xffffffffu, top > m + kRaise)) {
             const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
             m = m2;
@@ -579,38 +596,40 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
             if (x > 0) {
               ok = __all_sync(~0u, ok && wait(&B.pv_done[g], (count - 1) & 1));
               tc_fence_after_sync();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_ld_32(o_col(g) + lanes + c, o);
+                tmem_wait_ld(o);
 #pragma unroll
                 for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                 tmem_st_32(o_col(g) + lanes + c, o);
               }
             }
           }
-          const float ref = (m == -INFINITY ? 0.f : m) - kWeightBias;
+          const float ref = kWeightBias - (m == -INFINITY ? 0.f : m);
+          const float2 coef2 = make_float2(coef, coef), ref2 = make_float2(ref, ref);
+          float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            uint32_t s[64], p[32];
-            tmem_ld_64(s_col(g) + lanes + 64 * half, s);
+            uint32_t p[32];
 #pragma unroll
-            for (int i = 0; i < 64; i++) {
-              float v = ex2(fmaf(__uint_as_float(s[i]), coef, -ref));
-              if (edge && !((see[2 * half + i / 32] >> (i % 32)) & 1)) v = 0.f;
-              l += v;
-              s[i] = __float_as_uint(v);
+            for (int i = 0; i < 32; i++) {
+              uint32_t* w = &s[64 * half + 2 * i];
+              float2 v = fma2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), coef2, ref2);
+              v.x = ex2(v.x), v.y = ex2(v.y);
+              sum[i & 1] = add2(sum[i & 1], v);
+              p[i] = pack_h2(v.x, v.y);
+              if constexpr (SPLIT) w[0] = pack_h2_rest(v.x, v.y, p[i]);
             }
-#pragma unroll
-            for (int i = 0; i < 32; i++) p[i] = pack_h2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
             tmem_st_32(s_col(g) + lanes + 64 * half, p);
             if constexpr (SPLIT) {
 #pragma unroll
-              for (int i = 0; i < 32; i++)
-                p[i] = pack_h2_rest(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), p[i]);
+              for (int i = 0; i < 32; i++) p[i] = s[64 * half + 2 * i];
               tmem_st_32(s_col(g) + lanes + 64 * half + 32, p);
             }
           }
+          l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
         }
         tc_fence_before_sync();
@@ -641,37 +660,21 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         const uint32_t rl = r - sg.rt * S::ROWS;
         constexpr int DIMS = RT == 1 ? D / 2 : D;
         const uint32_t d0 = RT == 1 ? g * DIMS : 0;
-        const bool wild = *(volatile uint32_t*)&B.wild != 0;
 #pragma unroll 1
         for (uint32_t d = d0; d < d0 + DIMS; d += 32) {
           uint32_t o[32];
           float v[32];
           tmem_ld_32(src0 + lanes + d, o);
+          tmem_wait_ld(o);
 #pragma unroll
           for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * f[0];
           if (has[1]) {
             tmem_ld_32(o_col(1) + lanes + d, o);
+            tmem_wait_ld(o);
 #pragma unroll
             for (int i = 0; i < 32; i++) v[i] = fmaf(__uint_as_float(o[i]), f[1], v[i]);
           }
           if (!live) continue;
-          if (wild) {  // rare: what was left out of the drafts' V, for the rows that see it
-            const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
-            for (uint32_t p = max(sg.hist, sg.k0 * TK); p < min(sg.end, sg.k1 * TK); p++) {
-              if (!sees(a, sg.b, t, sg.hist, p)) continue;
-#pragma unroll
-              for (int i = 0; i < 32; i++) {
-                const uint64_t at = (base + p) * D + d + i;
-                float y;
-                if constexpr (Q8)
-                  y = __half2float(__float2half_rn((float)((const int8_t*)a.c.v)[at] *
-                                                   __half2float(((const __half*)a.c.v_scale)[at / 32])));
-                else
-                  y = __half2float(((const __half*)a.c.v)[at]);
-                if (!(fabsf(y) < INFINITY)) v[i] += y;
-              }
-            }
-          }
           if (whole) {
             T* out = (T*)a.out + token * a.out_stride + (uint64_t)hq * D + d;
 #pragma unroll
@@ -689,6 +692,30 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
             if (d == 0) slot[S::ROWS * D + rl] = M, slot[S::ROWS * D + S::ROWS + rl] = den;
           }
         }
+        if (*(volatile uint32_t*)&B.wild && live) {  // rare: what was left out of the drafts' V, for the rows that see it
+          const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
+#pragma unroll 1
+          for (uint32_t p = max(sg.hist, sg.k0 * TK); p < min(sg.end, sg.k1 * TK); p++) {
+            if (!sees(a, sg.b, t, sg.hist, p)) continue;
+#pragma unroll 1
+            for (uint32_t d = d0; d < d0 + DIMS; d++) {
+              const uint64_t at = (base + p) * D + d;
+              float y;
+              if constexpr (Q8)
+                y = __half2float(__float2half_rn((float)((const int8_t*)a.c.v)[at] *
+                                                 __half2float(((const __half*)a.c.v_scale)[at / 32])));
+              else
+                y = __half2float(((const __half*)a.c.v)[at]);
+              if (fabsf(y) < INFINITY) continue;
+              if (whole) {
+                T* out = (T*)a.out + token * a.out_stride + (uint64_t)hq * D + d;
+                act_put(out, act_get(out) + y);
+              } else {
+                slot[(size_t)rl * D + d] += y;
+              }
+            }
+          }
+        }
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -698,6 +725,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     // ---- Q8_0 tiles to f16: thread = key; pieces taken in an order that keeps the eight
     // lanes of a shared-memory phase on different banks, for the codes and for the tile
     if constexpr (Q8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(88));
       const uint32_t key = tid - 384;
       Ring<S::NRAW> rr;
       Ring<S::NSLOT> ring;
