@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
         const float inv = den == 0.f ? 0.f : 1.f / den;
         act_put(out, num.x * inv), act_put(out + 1, num.y * inv), act_put(out + 2, num.z * inv), act_put(out + 3, num.w * inv);
       } else {
-        *reinterpret_cast<float4*>(slot + (size_t)r * D + d) = num;
+        *reinterpret_cast<float4*>(slot + part_at<ROWS>(d, r)) = num;
         if (d == 0) slot[ROWS * D + r] = M, slot[ROWS * D + ROWS + r] = den;
       }
     }
@@ -436,8 +436,7 @@ int run_rows(cudaStream_t st, const TreeArgs& a) {
   cudaError_t e = launch_k(Launch{st, false}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
                            (float*)part);
   if (e == cudaSuccess)
-    e = launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS>, dim3(a.n_seqs * a.n_tokens * a.n_heads), dim3(128),
-                 0, a, (const float*)part, ctas);
+    e = launch_merge<T, D, KT, ROWS>(st, a, (const float*)part, ctas);
   const cudaError_t f = cudaFreeAsync(part, st);
   RF_CUDA(e);
   RF_CUDA(f);

@@ -22,7 +22,7 @@ struct TreeArgs {
 
 // History length and draft count of sequence b; (0, 0) and the error bit where they do not fit the cache.
 __device__ __forceinline__ void seq_lengths(const TreeArgs& a, uint32_t b, uint32_t* hist, uint32_t* drafts) {
-  const int32_t L = a.hist_len[b], n = a.n_draft ? a.n_draft[b] : (int32_t)a.n_tokens;
+  const int32_t L = __ldg(a.hist_len + b), n = a.n_draft ? __ldg(a.n_draft + b) : (int32_t)a.n_tokens;
   const bool ok = L >= 0 && n >= 0 && (uint32_t)n <= a.n_tokens && (uint64_t)L + (uint64_t)n <= a.c.capacity;
   if (!ok) atomicOr(a.err, kVerifyRange);
   *hist = ok ? (uint32_t)L : 0;
@@ -105,6 +105,26 @@ struct Split {
   }
 };
 
+// Equal ranges of `all` tiles: the first `more` CTAs take `each` + 1, the others `each`.
+struct Ranges {
+  uint64_t all, each, more;
+  uint32_t ctas;  // as many as there are tiles, at most the grid
+  __device__ __forceinline__ Ranges(uint64_t all_, uint32_t grid) : all(all_), each(0), more(0) {
+    ctas = all < grid ? (uint32_t)all : grid;
+    if (!ctas) return;
+    each = all >> 32 ? all / ctas : (uint32_t)all / ctas;
+    more = all - each * ctas;
+  }
+  __device__ __forceinline__ uint64_t begin(uint32_t c) const { return each * c + min((uint64_t)c, more); }
+  __device__ __forceinline__ uint32_t holder(uint64_t tile) const {  // the CTA of a tile
+    const uint64_t wide = more * (each + 1);
+    return tile < wide ? div(tile, each + 1) : (uint32_t)more + div(tile - wide, each);
+  }
+  static __device__ __forceinline__ uint32_t div(uint64_t x, uint64_t y) {
+    return (x | y) >> 32 ? (uint32_t)(x / y) : (uint32_t)x / (uint32_t)y;
+  }
+};
+
 // A run of consecutive key tiles of one unit: what a CTA works on at a time.
 struct Segment {
   uint32_t b, h, rt;          // sequence, KV head, row tile
@@ -117,21 +137,20 @@ struct Segment {
 template <int KT, int ROWS>
 struct Walk {
   using Sp = Split<KT, ROWS>;
-  uint64_t w, w_end, rem;
+  uint64_t left, rem;  // tiles left, and the next one's offset in sequence b
   uint32_t b;
   // Whole warp.
   __device__ __forceinline__ Walk(const TreeArgs& a) {
     uint64_t ignore;
-    const uint64_t all = Sp::total(a, 0, &ignore);
-    const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, all);  // no CTA without a tile
-    w = w_end = 0;
-    if (blockIdx.x >= ctas) return;
-    w = all * blockIdx.x / ctas;
-    w_end = all * (blockIdx.x + 1) / ctas;
+    const Ranges r(Sp::total(a, 0, &ignore), gridDim.x);
+    left = 0;
+    if (blockIdx.x >= r.ctas) return;
+    const uint64_t w = r.begin(blockIdx.x);
+    left = r.begin(blockIdx.x + 1) - w;
     b = Sp::locate(a, w, &rem);
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, Segment* s) {
-    if (w >= w_end) return false;
+    if (!left) return false;
     uint32_t L, n;
     seq_lengths(a, b, &L, &n);
     uint32_t tiles = Sp::tiles(L, n), rts = Sp::row_tiles(a, n);
@@ -141,20 +160,23 @@ struct Walk {
       seq_lengths(a, b, &L, &n);
       tiles = Sp::tiles(L, n), rts = Sp::row_tiles(a, n);
     }
-    const uint32_t unit = (uint32_t)(rem / tiles);
-    s->b = b, s->h = unit / rts, s->rt = unit % rts;
-    s->k0 = (uint32_t)(rem % tiles);
-    s->k1 = (uint32_t)min((uint64_t)tiles, s->k0 + (w_end - w));
+    const uint32_t unit = Ranges::div(rem, tiles);
+    s->b = b, s->h = unit / rts, s->rt = unit - s->h * rts;
+    s->k0 = (uint32_t)(rem - (uint64_t)unit * tiles);
+    s->k1 = (uint32_t)min((uint64_t)tiles, s->k0 + left);
     s->tiles = tiles;
     s->hist = L, s->drafts = n, s->end = L + n;
-    w += s->k1 - s->k0;
+    left -= s->k1 - s->k0;
     rem += s->k1 - s->k0;
     return true;
   }
 };
 
-// Floats of one partial result: ROWS x D output sums, then ROWS maxima and ROWS sums.
+// One partial result: output sums as [D / 4][ROWS] of 4 floats (rows side by side, so that
+// threads that own a row write and read 16-byte pieces in a run), then ROWS maxima and ROWS sums.
 constexpr size_t part_floats(int rows, int D) { return (size_t)rows * (D + 2); }
+template <int ROWS>
+__device__ __forceinline__ size_t part_at(uint32_t d, uint32_t r) { return ((size_t)(d / 4) * ROWS + r) * 4; }
 
 // Visibility of position p for token t of sequence b (p < L + n).
 __device__ __forceinline__ bool sees(const TreeArgs& a, uint32_t b, uint32_t t, uint32_t L, uint32_t p) {
@@ -169,58 +191,66 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, uint32_t b, uint32_t t, 
 constexpr float kRaise = 8.f, kWeightBias = 7.f;
 
 // ---------------------------------------------------------------------------
-// One CTA a (token, query head): adds the partial results of a unit that several of
-// the first kernel's CTAs shared (`grid` of them), and writes the zeros of tokens past a sequence's drafts.
+// Joins the partial results of the units that several of the first kernel's CTAs shared
+// (`grid` of them), in order of the keys, and writes the zeros of tokens past a sequence's drafts.
+// A CTA takes 8 rows of a (sequence, KV head) and 32 dimensions, four threads to each piece
+// of 4: each adds every fourth partial result.  What bounds it is latency, so many small CTAs.
 // ---------------------------------------------------------------------------
 template <class T, int D, int KT, int ROWS>
-__global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
+__global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
   using Sp = Split<KT, ROWS>;
-  constexpr int E = D / 32;
-  __shared__ float s_o[4][D], s_l[4];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t hq = blockIdx.x % a.n_heads, bt = blockIdx.x / a.n_heads, b = bt / a.n_tokens, t = bt % a.n_tokens;
-  const uint32_t G = a.n_heads / a.c.n_kv_heads, h = hq / G, r = t * G + hq % G;
-  T* out = (T*)a.out + bt * a.out_stride + (uint64_t)hq * D;
+  __shared__ float4 s_o[4][64];
+  __shared__ float s_l[4][8];
+  const uint32_t tid = threadIdx.x, rx = tid & 7, dx = (tid >> 3) & 7, cx = tid >> 6;
+  const uint32_t G = a.n_heads / a.c.n_kv_heads, groups = (a.n_tokens * G + 7) / 8;
+  const uint32_t bh = blockIdx.x / groups, r0 = (blockIdx.x - bh * groups) * 8;
+  const uint32_t b = bh / a.c.n_kv_heads, h = bh - b * a.c.n_kv_heads;
+  const uint32_t r = r0 + rx, t = r / G, hq = h * G + (r - t * G), d = blockIdx.y * 32 + dx * 4;
+  T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d;
   uint32_t L, n;
   seq_lengths(a, b, &L, &n);
-  if (t >= n) {
-    if (threadIdx.x < D) act_put(out + threadIdx.x, 0.f);
-    return;
-  }
+  if (r < a.n_tokens * G && t >= n && cx == 0) act_put(out, 0.f), act_put(out + 1, 0.f), act_put(out + 2, 0.f), act_put(out + 3, 0.f);
+  if (r0 >= n * G) return;
   uint64_t before;
-  const uint64_t all = Sp::total(a, b, &before);
+  const Ranges ranges(Sp::total(a, b, &before), grid);
   const uint32_t tiles = Sp::tiles(L, n);
-  const uint64_t u0 = before + ((uint64_t)h * Sp::row_tiles(a, n) + r / ROWS) * tiles, u1 = u0 + tiles;
-  const uint32_t ctas = (uint32_t)min((uint64_t)grid, all);  // CTA c holds [all c / ctas, all (c+1) / ctas)
-  const uint32_t c0 = (uint32_t)(((u0 + 1) * ctas - 1) / all), c1 = (uint32_t)((u1 * ctas - 1) / all);
-  if (c0 == c1) return;
+  const uint64_t u0 = before + ((uint64_t)h * Sp::row_tiles(a, n) + r0 / ROWS) * tiles;
+  const uint32_t c0 = ranges.holder(u0), c1 = ranges.holder(u0 + tiles - 1);
+  if (c0 == c1) return;  // finished by its CTA
   griddep_wait();
   const uint32_t rl = r % ROWS;
   auto slot = [&](uint32_t c) { return part + (2 * (size_t)c + (c == c0 ? 1 : 0)) * part_floats(ROWS, D); };
   float M = -INFINITY;
-  for (uint32_t c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(slot(c) + ROWS * D + rl));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float acc[E], den = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; e++) acc[e] = 0.f;
-#pragma unroll 4
-  for (uint32_t c = c0 + warp; c <= c1; c += 4) {
+#pragma unroll 8
+  for (uint32_t c = c0; c <= c1; c++) M = fmaxf(M, __ldcg(slot(c) + ROWS * D + rl));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.f;
+#pragma unroll 8
+  for (uint32_t c = c0 + cx; c <= c1; c += 4) {
     const float* s = slot(c);
     const float f = M == -INFINITY ? 1.f : ex2(__ldcg(s + ROWS * D + rl) - M);
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(s + part_at<ROWS>(d, rl)));
     den += __ldcg(s + ROWS * D + ROWS + rl) * f;
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[e] += __ldcg(s + (size_t)rl * D + lane + 32 * e) * f;
+    acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
   }
-#pragma unroll
-  for (int e = 0; e < E; e++) s_o[warp][lane + 32 * e] = acc[e];
-  if (lane == 0) s_l[warp] = den;
+  s_o[cx][tid & 63] = acc;
+  if (dx == 0) s_l[cx][rx] = den;
   __syncthreads();
-  if (threadIdx.x < D) {
-    const uint32_t d = threadIdx.x;
-    const float l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-    act_put(out + d, l == 0.f ? 0.f : (s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) / l);
+  if (cx == 0 && t < n) {
+#pragma unroll
+    for (int i = 1; i < 4; i++) {
+      const float4 v = s_o[i][tid];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    }
+    const float l = s_l[0][rx] + s_l[1][rx] + s_l[2][rx] + s_l[3][rx], inv = l == 0.f ? 0.f : 1.f / l;
+    act_put(out, acc.x * inv), act_put(out + 1, acc.y * inv), act_put(out + 2, acc.z * inv), act_put(out + 3, acc.w * inv);
   }
+}
+template <class T, int D, int KT, int ROWS>
+cudaError_t launch_merge(cudaStream_t st, const TreeArgs& a, const float* part, uint32_t grid) {
+  const uint32_t groups = (a.n_tokens * (a.n_heads / a.c.n_kv_heads) + 7) / 8;
+  return launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS>, dim3(a.n_seqs * a.c.n_kv_heads * groups, D / 32),
+                  dim3(256), 0, a, part, grid);
 }
 
 // Scratch of one call: allocated in stream order from a pool of this library's own that keeps

@@ -9,8 +9,10 @@
 //   S[128 rows][128 keys] = Q K^T   A = Q, B = K, both K-major in shared memory
 //   O[128 rows][D]       += P V     A = P in tensor memory, B = V, MN-major in shared memory
 //
-// Both S and O live in tensor memory (512 columns: two S, two O), so a thread owns one
-// row of S, its softmax needs no exchange, and P goes back over S's columns.  K and V
+// Both S and O live in tensor memory, so a thread owns one row of S, its softmax needs no
+// exchange, and P goes back over S's columns.  All 512 columns are used: two O, and for each
+// group of softmax warps two S of 64 keys (the halves of a tile), so that the next scores of a
+// half are computed while the softmax is at the other half.  K and V
 // tiles have the same layout in shared memory ([128 keys][64 dimensions] blocks of 128-byte
 // rows, 128-byte swizzle): read along the head they are K-major, read along the keys MN-major.
 //
@@ -19,8 +21,8 @@
 // take the even and the odd key tiles, and are joined at the end.
 //
 //   warp 0        loads: f16 tiles by tensor copies, Q8_0 codes by plain bulk copies
-//   warp 1        all tcgen05.mma
-//   warps 2, 3    f16: V tiles that hold drafts or the end are made finite (below)
+//   warps 1, 2    tcgen05.mma, one warp a group
+//   warp 3        f16: V tiles that hold drafts or the end are made finite (below)
 //   warps 4 - 11  softmax, queries, outputs
 //   warps 12 - 15 Q8_0: codes * scales -> f16 operand tiles, one key a thread
 //
@@ -134,6 +136,9 @@ __device__ __forceinline__ uint32_t sw128_offset(uint32_t r, uint32_t c) {
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ void st_shared8(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -169,13 +174,22 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t x, bool* wild) {
   return x & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
 }
 
+// The value of lane 0, which the compiler then keeps in a uniform register.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
+// True in one lane of the (whole) warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+  return p != 0;
+}
+
 // ---- shared-memory bookkeeping -----------------------------------------------------------
 template <class S>
-struct Bars {
-  uint64_t full[S::NSLOT], free[S::NSLOT];
+struct Bars {  // [group][half of the key tile]
+  uint64_t full[S::NSLOT], free[S::NSLOT], fix[S::NSLOT];
   uint64_t raw_full[S::NRAW ? S::NRAW : 1], raw_free[S::NRAW ? S::NRAW : 1];
-  uint64_t q_full, s_full[2], p_full[2], pv_done[2], fix_ask, fix_done, drain;
-  uint32_t tmem, stop, wild, fix_slot;
+  uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2][2], drain;
+  uint32_t tmem, stop, wild, pad;
   float ml[2][TK][2];
 };
 
@@ -189,7 +203,7 @@ struct Ring {
 };
 
 // Bounded wait for the phase of `bar` with `parity`; false once any wait of the CTA gave up.
-__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
   const long long t0 = clock64();
   while (!tc_mbar_try_wait(bar, parity)) {
     if (*stop) return false;
@@ -238,23 +252,19 @@ __device__ __forceinline__ uint32_t seen32(const uint32_t* mask_row, uint32_t wo
   return n - j0 < 32 ? v & ((1u << (n - j0)) - 1) : v;
 }
 
-// 16 bytes of a row as f32 (8 or 4 values).
+// 16 bytes of a row as f32.
 template <class T>
-__device__ __forceinline__ void act_load8(const T* p, float (&v)[8]) {
-  if constexpr (std::is_same<T, float>::value) {
-    const float4 x = __ldg((const float4*)p), y = __ldg((const float4*)p + 1);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-  } else {
-    const uint4 u = __ldg((const uint4*)p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void act_unpack(const uint4& u, float (&v)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
+  for (int i = 0; i < 4; i++) {
+    if constexpr (std::is_same<T, float>::value) {
+      v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    } else {
+      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
 }
@@ -280,6 +290,8 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   const uint32_t q_smem = tc_smem_u32(tsm), slots = q_smem + S::QBYTES, raws = slots + S::NSLOT * S::TILE;
   auto slot_addr = [&](uint32_t s) { return slots + s * S::TILE; };
   griddep_launch();
+  Walk<TK, S::ROWS> walk(a);
+  if (!walk.left) return;
   if (q_smem & 1023u) {  // the swizzle is a function of the address
     if (tid == 0) atomicOr(a.err, kVerifyTimeout);
     return;
@@ -288,21 +300,21 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   if (tid == 0) {
     for (int i = 0; i < S::NSLOT; i++) {
       tc_mbar_init(tc_smem_u32(&B.full[i]), Q8 ? 4 : 1);
-      tc_mbar_init(tc_smem_u32(&B.free[i]), 1);
+      tc_mbar_init(tc_smem_u32(&B.free[i]), Q8 ? 2 : 3);  // both MMA warps, and warp 3
+      tc_mbar_init(tc_smem_u32(&B.fix[i]), 1);
     }
     for (int i = 0; i < S::NRAW; i++) {
       tc_mbar_init(tc_smem_u32(&B.raw_full[i]), 1);
       tc_mbar_init(tc_smem_u32(&B.raw_free[i]), 4);
     }
     tc_mbar_init(tc_smem_u32(&B.q_full), 256);
-    for (int i = 0; i < 2; i++) {
-      tc_mbar_init(tc_smem_u32(&B.s_full[i]), 1);
-      tc_mbar_init(tc_smem_u32(&B.p_full[i]), 4);
-      tc_mbar_init(tc_smem_u32(&B.pv_done[i]), 1);
-    }
-    tc_mbar_init(tc_smem_u32(&B.fix_ask), 1);
-    tc_mbar_init(tc_smem_u32(&B.fix_done), 2);
-    tc_mbar_init(tc_smem_u32(&B.drain), 1);
+    for (int g = 0; g < 2; g++)
+      for (int h = 0; h < 2; h++) {
+        tc_mbar_init(tc_smem_u32(&B.s_full[g][h]), 1);
+        tc_mbar_init(tc_smem_u32(&B.p_full[g][h]), 4);
+        tc_mbar_init(tc_smem_u32(&B.pv_done[g][h]), 1);
+      }
+    tc_mbar_init(tc_smem_u32(&B.drain), 2);
     B.stop = B.wild = 0;
     tc_fence_barrier_init();
   }
@@ -310,19 +322,14 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = B.tmem;
-  auto s_col = [&](uint32_t g) { return tmem + 128 * g; };
+  auto s_col = [&](uint32_t g, uint32_t h) { return tmem + 128 * g + 64 * h; };
   auto o_col = [&](uint32_t g) { return tmem + 256 + 128 * g; };
   volatile uint32_t* stop = &B.stop;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bar(bar, parity, stop, a.err); };
   bool ok = true;
   const uint32_t G = a.n_heads / a.c.n_kv_heads;
-  Walk<TK, S::ROWS> walk(a);
   Segment sg;
 
-  // Registers: a softmax thread holds a whole row of S.  The shares add up to what the block was
-  // launched with: 512 x 128 = 128 x (56 + 88 + 2 x 184), 384 x 168 = 128 x (72 + 2 x 216).
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 56 : 72));
   if (warp == 0) {
     // ---- loads ------------------------------------------------------------------------
     if (lane == 0) {
@@ -363,127 +370,126 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         }
       }
     }
-  } else if (warp == 1) {
-    // ---- all MMAs -----------------------------------------------------------------------
-    if (lane == 0) {
-      Ring<S::NSLOT> ring;
-      uint32_t q_phase = 0, fix_phase = 0, pv_count[2] = {0, 0};
-      constexpr uint32_t id_s = idesc_f16(TK, false), id_o = idesc_f16(D, true);
-      auto take = [&]() {
-        const uint32_t s = ring.s;
-        ok = ok && wait(&B.full[s], ring.phase);
-        ring.advance();
-        return s;
-      };
-      // V tiles that hold drafts or the end go through warps 2 and 3 while the softmax runs
-      auto take_v = [&](bool drafts) {
-        const uint32_t s = take();
-        if (!Q8 && drafts && ok) {
-          *(volatile uint32_t*)&B.fix_slot = s;
-          tc_mbar_arrive(tc_smem_u32(&B.fix_ask));
-        }
-        return s;
-      };
-      auto fixed = [&](bool drafts) {
-        if (!Q8 && drafts) {
-          ok = ok && wait(&B.fix_done, fix_phase);
-          fix_phase ^= 1;
-        }
-      };
-      auto release = [&](uint32_t s) {
-        if (ok) tc_commit(tc_smem_u32(&B.free[s]));
-      };
-      // S of group g: P of the tile before sits in the same columns, so its product must be over
-      auto qk = [&](uint32_t g, uint32_t s) {
-        if (pv_count[g]) ok = ok && wait(&B.pv_done[g], (pv_count[g] - 1) & 1);
-        if (!ok) return;
-        tc_fence_after_sync();
-        const uint32_t q = q_smem + (RT == 2 ? g * S::TILE : 0), k = slot_addr(s);
+  } else if (warp < 3) {
+    // ---- MMAs of one group -----------------------------------------------------------------
+    // The whole warp runs the loop with values the compiler knows to be the same in every
+    // lane, so that descriptors stay in uniform registers, and one elected lane issues.  With
+    // both groups in one lane's loop each MMA cost 110 cycles of issue, more than it takes to
+    // run, and the tensor core waited (256 tokens over 32768: 472 us).
+    const uint32_t g = warp - 1;
+    Ring<S::NSLOT> ring;
+    uint32_t q_phase = 0, fix_phase = 0;
+    uint32_t done = 0;  // tiles of this group so far
+    constexpr uint32_t id_s = idesc_f16(TK / 2, false), id_o = idesc_f16(D, true);
+    const uint32_t s_base = uniform(s_col(g, 0)), o_base = uniform(o_col(g)), base = uniform(q_smem);
+    auto slot_at = [&](uint32_t s) { return base + S::QBYTES + s * S::TILE; };
+    auto until = [&](uint64_t* bar, uint32_t parity) { ok = __all_sync(~0u, ok && wait(bar, parity)); };
+    // The next tile of the ring; a tile with work of this group goes back with its last MMA, others at once.
+    auto take = [&](bool used) {
+      const uint32_t s = ring.s;
+      until(&B.full[s], ring.phase);
+      ring.advance();
+      if (!used && elect_one()) tc_mbar_arrive(tc_smem_u32(&B.free[s]));
+      return s;
+    };
+    auto release = [&](uint32_t s) {
+      if (ok && elect_one()) tc_commit(tc_smem_u32(&B.free[s]));
+    };
+    // S of a half; P of the tile before sat in the same columns, its product is over
+    auto qk = [&](uint32_t h, uint32_t s) {
+      if (!ok) return;
+      const uint64_t q = sw128_desc(base + (RT == 2 ? g * S::TILE : 0)), k = sw128_desc(slot_at(s) + h * (TK / 2) * 128);
+      const uint32_t d = s_base + 64 * h;
+      if (elect_one()) {
 #pragma unroll
         for (int term = SPLIT ? 1 : 0; term >= 0; term--)  // the small term first: the sum truncates at its own size
 #pragma unroll
           for (int i = 0; i < D / 16; i++) {
             const uint32_t o = (i / 4) * kBlockBytes + (i % 4) * 32;
-            mma_ss(s_col(g), sw128_desc(q + term * S::TILE + o), sw128_desc(k + o), id_s, (SPLIT && term == 0) || i > 0);
+            mma_ss(d, q + ((term * S::TILE + o) >> 4), k + (o >> 4), id_s, (SPLIT && term == 0) || i > 0);
           }
-        tc_commit(tc_smem_u32(&B.s_full[g]));
-      };
-      auto pv = [&](uint32_t g, uint32_t s, bool first, bool drafts) {
-        ok = ok && wait(&B.p_full[g], pv_count[g] & 1);
-        pv_count[g]++;
-        fixed(drafts);
-        if (!ok) return;
-        tc_fence_after_sync();
-#pragma unroll
-        for (int i = 0; i < TK / 16; i++) {
-          const uint32_t p = s_col(g) + 64 * (i / 4) + 8 * (i % 4);
-          const uint64_t v = sw128_desc(slot_addr(s) + i * 16 * 128);
-          mma_ts(o_col(g), p, v, id_o, !first || i > 0);
-          if constexpr (SPLIT) mma_ts(o_col(g), p + 32, v, id_o, true);
-        }
-        tc_commit(tc_smem_u32(&B.pv_done[g]));
-      };
-      while (walk.next(a, &sg)) {
-        const uint32_t nt = sg.k1 - sg.k0;
-        const bool two = RT == 2 && sg.drafts * G - sg.rt * S::ROWS > TK;
-        auto drafts_in = [&](uint32_t i) { return (sg.k0 + i + 1) * TK > sg.hist; };
-        ok = ok && wait(&B.q_full, q_phase);
-        q_phase ^= 1;
-        if constexpr (RT == 1) {
-          for (uint32_t i = 0; i < min(2u, nt); i++) {
-            const uint32_t k = take();
-            qk(i, k);
-            release(k);
-          }
-          for (uint32_t i = 0; i < nt; i++) {
-            const uint32_t v = take_v(drafts_in(i));
-            pv(i & 1, v, i < 2, drafts_in(i));
-            release(v);
-            if (i + 2 < nt) {
-              const uint32_t k = take();
-              qk(i & 1, k);
-              release(k);
-            }
-          }
-        } else {
-          uint32_t k = take();
-          qk(0, k);
-          if (two) qk(1, k);
-          release(k);
-          for (uint32_t i = 0; i < nt; i++) {
-            const uint32_t v = take_v(drafts_in(i));
-            const bool more = i + 1 < nt;
-            pv(0, v, i == 0, drafts_in(i));
-            if (more) {
-              k = take();
-              qk(0, k);
-            }
-            if (two) pv(1, v, i == 0, false);
-            release(v);
-            if (more) {
-              if (two) qk(1, k);
-              release(k);
-            }
-          }
-        }
+        tc_commit(tc_smem_u32(&B.s_full[g][h]));
       }
-      // everything issued is over before tensor and shared memory are given up
+    };
+    auto pv = [&](uint32_t h, uint32_t s, bool first) {
+      if (!ok) return;
+      tc_fence_after_sync();
+      const uint64_t v = sw128_desc(slot_at(s) + h * (TK / 2) * 128);
+      const uint32_t p = s_base + 64 * h;
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < TK / 32; i++) {
+          if constexpr (SPLIT) mma_ts(o_base, p + 32 + 8 * i, v + i * (16 * 128 >> 4), id_o, !first || i > 0);
+          mma_ts(o_base, p + 8 * i, v + i * (16 * 128 >> 4), id_o, SPLIT || !first || i > 0);
+        }
+        tc_commit(tc_smem_u32(&B.pv_done[g][h]));
+      }
+    };
+    while (walk.next(a, &sg)) {
+      const uint32_t nt = uniform(sg.k1 - sg.k0), k0 = uniform(sg.k0), hist = uniform(sg.hist);
+      constexpr uint32_t step = RT == 1 ? 2 : 1;
+      const bool work = RT == 1 ? g < nt : g == 0 || uniform(sg.drafts * G - sg.rt * S::ROWS) > TK;
+      auto mine = [&](uint32_t i) { return RT == 1 ? (i & 1) == g : work; };
+      if (work) until(&B.q_full, q_phase);
+      q_phase ^= 1;
+      if (done)  // the products of the segment before are over (also awaited by the softmax)
+        for (uint32_t h = 0; h < 2; h++) until(&B.pv_done[g][h], (done - 1) & 1);
+      tc_fence_after_sync();
+      for (uint32_t i = 0; i < min((uint32_t)S::LEAD, nt); i++) {
+        const uint32_t k = take(mine(i));
+        if (!mine(i)) continue;
+        qk(0, k);
+        qk(1, k);
+        release(k);
+      }
+      // a half's P V, then, that being over, the next scores in its columns
+      for (uint32_t i = 0; i < nt; i++) {
+        const bool drafts = (k0 + i + 1) * TK > hist, more = i + step < nt;
+        const uint32_t v = take(mine(i));
+        const uint32_t fix_bit = (fix_phase >> v) & 1;
+        if (!Q8 && drafts) fix_phase ^= 1u << v;
+        uint32_t k = 0;
+        if (!mine(i)) {
+          if (more) take(false);
+          continue;
+        }
+        for (uint32_t h = 0; h < 2; h++) {
+          until(&B.p_full[g][h], done & 1);
+          if (!Q8 && drafts && h == 0) until(&B.fix[v], fix_bit);
+          pv(h, v, i < step && h == 0);
+          if (h == 1) release(v);
+          if (!more) continue;
+          if (h == 0) k = take(true);
+          until(&B.pv_done[g][h], done & 1);
+          tc_fence_after_sync();
+          qk(h, k);
+          if (h == 1) release(k);
+        }
+        done++;
+      }
+    }
+    // everything issued is over before tensor and shared memory are given up
+    if (elect_one()) {
       tc_commit(tc_smem_u32(&B.drain));
       tc_mbar_wait(tc_smem_u32(&B.drain), 0);
     }
-  } else {
+  } else if (warp == 3) {
     // ---- f16 V tiles with drafts or the end: rows past the end 0, drafts' rows finite ------
     if constexpr (!Q8) {
-      uint32_t phase = 0;
+      Ring<S::NSLOT> ring;
       while (walk.next(a, &sg)) {
-        for (uint32_t tile = max(sg.k0, sg.hist / TK); tile < sg.k1; tile++) {
-          const uint32_t key0 = tile * TK;
-          ok = __all_sync(~0u, ok && wait(&B.fix_ask, phase));
-          phase ^= 1;
-          if (ok) {
-            const uint32_t from = sg.hist > key0 ? sg.hist - key0 : 0, v = slot_addr(*(volatile uint32_t*)&B.fix_slot);
+        const uint32_t nt = sg.k1 - sg.k0;
+        for (uint32_t e = 0; e < 2 * nt; e++) {
+          bool is_v;
+          uint32_t i;
+          item_at(e, nt, S::LEAD, &is_v, &i);
+          const uint32_t key0 = (sg.k0 + i) * TK;
+          ok = __all_sync(~0u, ok && wait(&B.full[ring.s], ring.phase));
+          if (ok && is_v && key0 + TK > sg.hist) {
+            const uint32_t from = sg.hist > key0 ? sg.hist - key0 : 0, v = slot_addr(ring.s);
             bool wild = false;
-            for (uint32_t x = from * 8 + (tid - 64); x < TK * 8; x += 64) {  // 16-byte pieces, in memory order
+#pragma unroll 2
+            for (uint32_t x = from * 8 + lane; x < TK * 8; x += 32) {  // 16-byte pieces, in memory order
               const bool real = key0 + x / 8 < sg.end;
 #pragma unroll
               for (int blk = 0; blk < D / 64; blk++) {
@@ -497,206 +503,232 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
               }
             }
             if (wild) *(volatile uint32_t*)&B.wild = 1;
+            tc_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.fix[ring.s]));
           }
-          tc_fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.fix_done));
+          if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.free[ring.s]));
+          ring.advance();
         }
       }
     }
-  }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8 ? 184 : 216));
     // ---- softmax ----------------------------------------------------------------------
-    const uint32_t g = (warp - 4) / 4, row = 32 * (warp % 4) + lane, lanes = (32 * (warp % 4)) << 16;
-    uint32_t count = 0;  // tiles of this group so far
+    const uint32_t g = (warp - 4) / 4, w32 = 32 * (warp % 4), row = w32 + lane, lanes = w32 << 16;
+    const uint32_t q_tile = q_smem + (RT == 2 ? g * S::TILE : 0);
+    constexpr uint32_t CPR = D * sizeof(T) / 16;  // 16-byte pieces of a row of activations
+    constexpr uint32_t RPI = 32 / CPR;            // rows a warp moves at a time
+    uint32_t count = 0;                           // tiles of this group so far
     while (walk.next(a, &sg)) {
       const uint32_t nt = sg.k1 - sg.k0, n_rows = sg.drafts * G;
-      const uint32_t r = sg.rt * S::ROWS + (RT == 2 ? g * TK : 0) + row;
-      const bool live = r < n_rows, warp_live = r - lane < n_rows;
-      const uint32_t t = live ? r / G : 0, hq = sg.h * G + (live ? r % G : 0);
-      const uint64_t token = (uint64_t)sg.b * a.n_tokens + t;
-      // queries: f32 and bf16 rows are scaled by a power of two to a largest magnitude in [1, 2)
+      const uint32_t r_base = sg.rt * S::ROWS + (RT == 2 ? g * TK : 0) + w32;  // the warp's first row
+      const uint32_t r = r_base + lane;
+      const bool live = r < n_rows, warp_live = r_base < n_rows;
+      const uint32_t t = live ? r / G : 0;
+      // element offset of row x's head in a tensor of token stride `stride`
+      auto row_at = [&](uint32_t x, uint64_t stride) {
+        const uint32_t tx = x / G;
+        return ((uint64_t)sg.b * a.n_tokens + tx) * stride + (uint64_t)(sg.h * G + (x - tx * G)) * D;
+      };
+      // queries, a few rows of the warp at a time: f32 and bf16 rows are scaled by a power of
+      // two to a largest magnitude in [1, 2)
       float coef = a.scale * 1.44269504f;
       {
-        const T* q = (const T*)a.q + token * a.q_stride + (uint64_t)hq * D;
-        float down0 = 1.f, down1 = 1.f;
-        if constexpr (!std::is_same<T, __half>::value) {
-          float top = 0.f;
-#pragma unroll 4
-          for (int c = 0; c < D / 8; c++) {
-            float v[8];
-            act_load8(q + 8 * c, v);
+        constexpr int BATCH = 32 / RPI < 8 ? 32 / RPI : 8;
+        constexpr int PIECE = 16 / sizeof(T);
+        const uint32_t sub = lane / CPR, c = lane % CPR;
+        int e_mine = 0;
+#pragma unroll 1
+        for (int b0 = 0; b0 < (int)(32 / RPI); b0 += BATCH) {
+          uint4 u[BATCH];
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]));
+          for (int i = 0; i < BATCH; i++) {
+            const uint32_t x = r_base + (b0 + i) * RPI + sub;
+            u[i] = x < n_rows ? __ldg(reinterpret_cast<const uint4*>((const T*)a.q + row_at(x, a.q_stride)) + c)
+                              : make_uint4(0, 0, 0, 0);
           }
-          if (top > 0.f && top < INFINITY) {
-            const int e = ilogbf(top);  // in two factors: 2^-e alone leaves f32 for the smallest rows
-            down0 = ldexpf(1.f, -(e / 2)), down1 = ldexpf(1.f, -(e - e / 2));
-            coef = fmaxf(coef * ldexpf(1.f, e), 1.17549435e-38f);  // not 0: a masked score stays -inf
-          }
-        }
-        if (RT == 2 || g == 0) {
-          const uint32_t dst = q_smem + (RT == 2 ? g * S::TILE : 0);
-#pragma unroll 4
-          for (int c = 0; c < D / 8; c++) {
-            float v[8];
-            act_load8(q + 8 * c, v);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = live ? v[i] * down0 * down1 : 0.f;
-            uint4 hi;
-            hi.x = pack_h2(v[0], v[1]), hi.y = pack_h2(v[2], v[3]), hi.z = pack_h2(v[4], v[5]), hi.w = pack_h2(v[6], v[7]);
-            st_shared16(dst + sw128_offset(row, c), hi);
-            if constexpr (SPLIT) {
-              uint4 lo;
-              lo.x = pack_h2_rest(v[0], v[1], hi.x), lo.y = pack_h2_rest(v[2], v[3], hi.y);
-              lo.z = pack_h2_rest(v[4], v[5], hi.z), lo.w = pack_h2_rest(v[6], v[7], hi.w);
-              st_shared16(dst + S::TILE + sw128_offset(row, c), lo);
+          for (int i = 0; i < BATCH; i++) {
+            float v[PIECE];
+            act_unpack<T>(u[i], v);
+            if constexpr (!std::is_same<T, __half>::value) {
+              float top = 0.f;
+#pragma unroll
+              for (int j = 0; j < PIECE; j++) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+              for (uint32_t o = CPR / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+              const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
+              // in two factors: 2^-e alone leaves f32 for the smallest rows
+              const float d0 = ldexpf(1.f, -(e / 2)), d1 = ldexpf(1.f, -(e - e / 2));
+#pragma unroll
+              for (int j = 0; j < PIECE; j++) v[j] = v[j] * d0 * d1;
+              const int et = __shfl_sync(~0u, e, (lane % RPI) * CPR);
+              if ((int)(lane / RPI) == b0 + i) e_mine = et;
+            }
+            if (RT == 2 || g == 0) {
+              const uint32_t x = w32 + (b0 + i) * RPI + sub;
+              if constexpr (SPLIT) {  // 4 elements: half of a 16-byte piece of f16
+                const uint32_t at = sw128_offset(x, c / 2) + 8 * (c & 1);
+                const uint32_t h0 = pack_h2(v[0], v[1]), h1 = pack_h2(v[2], v[3]);
+                st_shared8(q_tile + at, h0, h1);
+                st_shared8(q_tile + S::TILE + at, pack_h2_rest(v[0], v[1], h0), pack_h2_rest(v[2], v[3], h1));
+              } else {
+                st_shared16(q_tile + sw128_offset(x, c), make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]),
+                                                                    pack_h2(v[4], v[5]), pack_h2(v[6], v[7])));
+              }
             }
           }
         }
+        if constexpr (!std::is_same<T, __half>::value)
+          coef = fmaxf(coef * ldexpf(1.f, e_mine), 1.17549435e-38f);  // not 0: a masked score stays -inf
         tc_fence_proxy_async();
         tc_mbar_arrive(tc_smem_u32(&B.q_full));
       }
-      const uint32_t* mask_row = a.mask ? a.mask + token * a.words : nullptr;
+      const uint32_t* mask_row = a.mask ? a.mask + ((uint64_t)sg.b * a.n_tokens + t) * a.words : nullptr;
       const bool two = n_rows - sg.rt * S::ROWS > TK;
       const uint32_t mine = RT == 1 ? (nt + 1 - g) / 2 : (g == 0 || two ? nt : 0);
       float m = -INFINITY, l = 0.f;
       for (uint32_t x = 0; x < mine; x++, count++) {
         const uint32_t key0 = (sg.k0 + (RT == 1 ? 2 * x + g : x)) * TK;
         const bool edge = key0 + TK > sg.hist;
-        ok = __all_sync(~0u, ok && wait(&B.s_full[g], count & 1));
-        if (ok && warp_live) {
-          tc_fence_after_sync();
-          uint32_t s[TK];
-#pragma unroll
-          for (int i = 0; i < TK; i += 32) tmem_ld_32(s_col(g) + lanes + i, s + i);
-          tmem_wait_ld(s);
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < TK / 32; i++) {
-              const uint32_t see =
-                  seen32(mask_row, a.words, t, (int)(key0 + 32 * i) - (int)sg.hist, (int)sg.drafts);
-#pragma unroll
-              for (int j = 0; j < 32; j++)
-                if (!((see >> j) & 1)) s[32 * i + j] = 0xff800000u;
-            }
-          }
-          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < TK; i += 8)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              tops[j] = max3(tops[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
-          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * coef;
-          if (__any_sync(0xffffffffu, top > m + kRaise)) {
-            const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
-            m = m2;
-            l *= f;
-            if (x > 0) {
-              ok = __all_sync(~0u, ok && wait(&B.pv_done[g], (count - 1) & 1));
-              tc_fence_after_sync();
 #pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld_32(o_col(g) + lanes + c, o);
-                tmem_wait_ld(o);
+        for (uint32_t h = 0; h < 2; h++) {
+          const uint32_t scores = s_col(g, h) + lanes;
+          ok = __all_sync(~0u, ok && wait(&B.s_full[g][h], count & 1));
+          if (ok && warp_live) {
+            tc_fence_after_sync();
+            uint32_t s[TK / 2];
+            tmem_ld_32(scores, s);
+            tmem_ld_32(scores + 32, s + 32);
+            tmem_wait_ld(s);
+            if (edge) {
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st_32(o_col(g) + lanes + c, o);
+              for (int i = 0; i < 2; i++) {
+                const uint32_t see = seen32(mask_row, a.words, t, (int)(key0 + 64 * h + 32 * i) - (int)sg.hist, (int)sg.drafts);
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                  if (!((see >> j) & 1)) s[32 * i + j] = 0xff800000u;
               }
             }
-          }
-          const float ref = kWeightBias - (m == -INFINITY ? 0.f : m);
-          const float2 coef2 = make_float2(coef, coef), ref2 = make_float2(ref, ref);
-          float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
+            for (int i = 0; i < TK / 2; i += 8)
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                tops[j] = max3(tops[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * coef;
+            if (__any_sync(~0u, top > m + kRaise)) {
+              const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+              m = m2;
+              l *= f;
+              if (x + h > 0) {  // all products issued so far are in O before it is rescaled
+                ok = __all_sync(~0u, ok && wait(&B.pv_done[g][h ^ 1], (h ? count : count - 1) & 1));
+                tc_fence_after_sync();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld_32(o_col(g) + lanes + c, o);
+                  tmem_wait_ld(o);
+#pragma unroll
+                  for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_st_32(o_col(g) + lanes + c, o);
+                }
+              }
+            }
+            const float ref = kWeightBias - (m == -INFINITY ? 0.f : m);
+            const float2 coef2 = make_float2(coef, coef), ref2 = make_float2(ref, ref);
+            float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-              uint32_t* w = &s[64 * half + 2 * i];
-              float2 v = fma2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), coef2, ref2);
+              float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
               v.x = ex2(v.x), v.y = ex2(v.y);
               sum[i & 1] = add2(sum[i & 1], v);
               p[i] = pack_h2(v.x, v.y);
-              if constexpr (SPLIT) w[0] = pack_h2_rest(v.x, v.y, p[i]);
+              if constexpr (SPLIT) s[i] = pack_h2_rest(v.x, v.y, p[i]);
             }
-            tmem_st_32(s_col(g) + lanes + 64 * half, p);
+            tmem_st_32(scores, p);
             if constexpr (SPLIT) {
 #pragma unroll
-              for (int i = 0; i < 32; i++) p[i] = s[64 * half + 2 * i];
-              tmem_st_32(s_col(g) + lanes + 64 * half + 32, p);
+              for (int i = 0; i < 32; i++) p[i] = s[i];
+              tmem_st_32(scores + 32, p);
             }
+            l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            tmem_wait_st();
           }
-          l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.p_full[g][h]));
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc_mbar_arrive(tc_smem_u32(&B.p_full[g]));
       }
-      if (mine) ok = __all_sync(~0u, ok && wait(&B.pv_done[g], (count - 1) & 1));
+      if (mine) ok = __all_sync(~0u, ok && wait(&B.pv_done[g][1], (count - 1) & 1));
       // ---- output: RT = 1 joins the two groups, each writing half of the dimensions
-      bool has[2] = {mine > 0, false};
-      float f[2] = {1.f, 0.f}, M = m, den = l;
-      uint32_t src0 = o_col(g);
+      const bool joined = RT == 1 && nt > 1;
+      float f0 = 1.f, f1 = 0.f, M = m, den = l;
       if constexpr (RT == 1) {
         B.ml[g][row][0] = m, B.ml[g][row][1] = l;
         __syncwarp();
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        has[0] = true, has[1] = nt > 1;
         const float m0 = B.ml[0][row][0], m1 = B.ml[1][row][0];
         M = fmaxf(m0, m1);
-        f[0] = M == -INFINITY ? 1.f : ex2(m0 - M), f[1] = M == -INFINITY ? 1.f : ex2(m1 - M);
-        den = B.ml[0][row][1] * f[0] + B.ml[1][row][1] * f[1];
-        src0 = o_col(0);
+        f0 = M == -INFINITY ? 1.f : ex2(m0 - M), f1 = M == -INFINITY ? 1.f : ex2(m1 - M);
+        den = B.ml[0][row][1] * f0 + B.ml[1][row][1] * f1;
       }
-      if (ok && warp_live && has[0]) {
+      if (ok && warp_live && (RT == 1 || mine)) {
         tc_fence_after_sync();
         const bool whole = sg.whole();
-        const float inv = !whole ? 1.f : den == 0.f ? 0.f : 1.f / den;
+        if (whole) f0 *= den == 0.f ? 0.f : 1.f / den, f1 *= den == 0.f ? 0.f : 1.f / den;
         float* slot = part + (2 * (size_t)blockIdx.x + (sg.k0 > 0 ? 0 : 1)) * part_floats(S::ROWS, D);
         const uint32_t rl = r - sg.rt * S::ROWS;
-        constexpr int DIMS = RT == 1 ? D / 2 : D;
+        constexpr uint32_t DIMS = RT == 1 ? D / 2 : D;
         const uint32_t d0 = RT == 1 ? g * DIMS : 0;
 #pragma unroll 1
         for (uint32_t d = d0; d < d0 + DIMS; d += 32) {
           uint32_t o[32];
           float v[32];
-          tmem_ld_32(src0 + lanes + d, o);
+          tmem_ld_32(o_col(RT == 1 ? 0 : g) + lanes + d, o);
           tmem_wait_ld(o);
 #pragma unroll
-          for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * f[0];
-          if (has[1]) {
+          for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * f0;
+          if (joined) {
             tmem_ld_32(o_col(1) + lanes + d, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = fmaf(__uint_as_float(o[i]), f[1], v[i]);
+            for (int i = 0; i < 32; i++) v[i] = fmaf(__uint_as_float(o[i]), f1, v[i]);
           }
-          if (!live) continue;
-          if (whole) {
-            T* out = (T*)a.out + token * a.out_stride + (uint64_t)hq * D + d;
+          if (whole) {  // through the query's place in shared memory, to whole rows
+            constexpr int PIECE = 16 / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 32; i += 16 / sizeof(T)) {
-              __align__(16) T w[16 / sizeof(T)];
+            for (int i = 0; i < 32 / PIECE; i++) {
+              __align__(16) T w[PIECE];
 #pragma unroll
-              for (int j = 0; j < (int)(16 / sizeof(T)); j++) act_put(&w[j], v[i + j] * inv);
-              *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(w);
+              for (int j = 0; j < PIECE; j++) act_put(&w[j], v[PIECE * i + j]);
+              const uint32_t c = d / PIECE + i;
+              st_shared16(q_tile + row * (CPR * 16) + ((c ^ (row & 7)) << 4), *reinterpret_cast<const uint4*>(w));
             }
-          } else {
-            float* dst = slot + (size_t)rl * D + d;
+          } else if (live) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            if (d == 0) slot[S::ROWS * D + rl] = M, slot[S::ROWS * D + S::ROWS + rl] = den;
+              *reinterpret_cast<float4*>(slot + part_at<S::ROWS>(d + i, rl)) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           }
         }
-        if (*(volatile uint32_t*)&B.wild && live) {  // rare: what was left out of the drafts' V, for the rows that see it
+        if (whole) {
+          constexpr uint32_t CH = DIMS * sizeof(T) / 16, RP = 32 / CH;  // pieces of the group's part of a row
+          __syncwarp();
+#pragma unroll 4
+          for (uint32_t i = 0; i < 32 / RP; i++) {
+            const uint32_t x = i * RP + lane / CH, c = d0 * sizeof(T) / 16 + lane % CH;
+            const uint4 u = ld_shared16(q_tile + (w32 + x) * (CPR * 16) + ((c ^ (x & 7)) << 4));
+            if (r_base + x < n_rows) *(reinterpret_cast<uint4*>((T*)a.out + row_at(r_base + x, a.out_stride)) + c) = u;
+          }
+        } else if (live && d0 == 0) {
+          slot[S::ROWS * D + rl] = M, slot[S::ROWS * D + S::ROWS + rl] = den;
+        }
+        if (__any_sync(~0u, *(volatile uint32_t*)&B.wild)) {  // rare: what was left out of the drafts' V
           const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
 #pragma unroll 1
           for (uint32_t p = max(sg.hist, sg.k0 * TK); p < min(sg.end, sg.k1 * TK); p++) {
-            if (!sees(a, sg.b, t, sg.hist, p)) continue;
+            if (!live || !sees(a, sg.b, t, sg.hist, p)) continue;
 #pragma unroll 1
             for (uint32_t d = d0; d < d0 + DIMS; d++) {
               const uint64_t at = (base + p) * D + d;
@@ -708,10 +740,10 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
                 y = __half2float(((const __half*)a.c.v)[at]);
               if (fabsf(y) < INFINITY) continue;
               if (whole) {
-                T* out = (T*)a.out + token * a.out_stride + (uint64_t)hq * D + d;
+                T* out = (T*)a.out + row_at(r, a.out_stride) + d;
                 act_put(out, act_get(out) + y);
               } else {
-                slot[(size_t)rl * D + d] += y;
+                slot[part_at<S::ROWS>(d, rl) + d % 4] += y;
               }
             }
           }
@@ -725,7 +757,6 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     // ---- Q8_0 tiles to f16: thread = key; pieces taken in an order that keeps the eight
     // lanes of a shared-memory phase on different banks, for the codes and for the tile
     if constexpr (Q8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(88));
       const uint32_t key = tid - 384;
       Ring<S::NRAW> rr;
       Ring<S::NSLOT> ring;
@@ -762,10 +793,13 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           if (ok) {
             const uint32_t raw = raws + rr.s * S::RAW + key * D, dst = slot_addr(ring.s);
             bool wild = false;
+            uint4 codes[D / 16];
+#pragma unroll
+            for (int j = 0; j < D / 16; j++) codes[j] = ld_shared16(raw + 16 * ((j + lane) & (D / 16 - 1)));
 #pragma unroll
             for (int j = 0; j < D / 16; j++) {
               const uint32_t c = (j + lane) & (D / 16 - 1);
-              const uint4 u = ld_shared16(raw + 16 * c);
+              const uint4 u = codes[j];
               const uint32_t w[4] = {u.x, u.y, u.z, u.w}, sw = c >= 4 ? sc.y : sc.x;
               const uint32_t db = __byte_perm(sw, sw, c & 2 ? 0x3232 : 0x1010);
               const __half2 d = *reinterpret_cast<const __half2*>(&db);
@@ -848,8 +882,7 @@ int run(cudaStream_t st, const TreeArgs& a) {
   RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(S::ROWS, D) * sizeof(float), st));
   cudaError_t e = launch_k(Launch{st, false}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
   if (e == cudaSuccess)
-    e = launch_k(Launch{st, true}, tree_merge_kernel<T, D, TK, S::ROWS>, dim3(a.n_seqs * a.n_tokens * a.n_heads), dim3(128),
-                 0, a, (const float*)part, ctas);
+    e = launch_merge<T, D, TK, S::ROWS>(st, a, (const float*)part, ctas);
   const cudaError_t f = cudaFreeAsync(part, st);
   RF_CUDA(e);
   RF_CUDA(f);
