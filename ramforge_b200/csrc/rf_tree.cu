@@ -92,17 +92,14 @@ __device__ __forceinline__ void load_query(const T* row, bool live, uint32_t c, 
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  float down = 1.f, up = 1.f;
+  float up = 1.f;
   if constexpr (!std::is_same<T, __half>::value) {
-    if (top > 0.f && top < INFINITY) {
-      const int e = ilogbf(top);
-      // in two factors: 2^-e alone leaves f32 for the smallest rows
-      down = ldexpf(1.f, -(e / 2)), up = ldexpf(1.f, e);
+    float down;
+    pow2_scale(top, &down, &up);
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+    for (int k = 0; k < KS; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[k][i] = v[k][i] * down * ldexpf(1.f, -(e - e / 2));
-    }
+      for (int i = 0; i < 4; i++) v[k][i] *= down;
   }
   *exp2 = up;
 #pragma unroll
@@ -127,7 +124,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
   __shared__ float s_m[kRowWarps][ROWS], s_l[kRowWarps][ROWS];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   griddep_launch();
-  const uint32_t G = a.n_heads / a.c.n_kv_heads;
+  const uint32_t G = a.group;
   Walk<KT, ROWS> walk(a);
   Segment sg;
   while (walk.next(a, &sg)) {
@@ -147,7 +144,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       const bool live = r < nrows;
       float up;
       load_query<T, Q8, D, SPLIT>(
-          (const T*)a.q + ((uint64_t)b * a.n_tokens + (live ? rr / G : 0)) * a.q_stride + (h * G + (live ? rr % G : 0)) * D,
+          (const T*)a.q + ((uint64_t)b * a.n_tokens + (live ? group_div(a, rr) : 0)) * a.q_stride + (h * G + (live ? rr - group_div(a, rr) * G : 0)) * D,
           live, c, qh[nb], ql[nb], &up);
       const float cf = a.scale * 1.44269504f * up;
       coef[nb][0] = __shfl_sync(0xffffffffu, cf, 8 * c);
@@ -255,7 +252,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
             float x = s[mb][nb][e] * coef[nb][e & 1];
             if (edge) {
               const uint32_t p = kb + 16 * mb + 8 * (e >> 1) + g, r = 8 * nb + 2 * c + (e & 1);
-              if (p >= end || r >= nrows || !sees(a, b, (r0 + r) / G, L, p)) x = -INFINITY;
+              if (p >= end || r >= nrows || !sees(a, b, group_div(a, r0 + r), L, p)) x = -INFINITY;
             }
             s[mb][nb][e] = x;
             raise |= x > m[nb][e & 1] + kRaise;
@@ -415,7 +412,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       }
       if (whole) {
         const uint32_t rr = r0 + r;
-        T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + rr / G) * a.out_stride + (h * G + rr % G) * D + d;
+        const uint32_t t = group_div(a, rr);
+        T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (h * G + rr - t * G) * D + d;
         const float inv = den == 0.f ? 0.f : 1.f / den;
         act_put(out, num.x * inv), act_put(out + 1, num.y * inv), act_put(out + 2, num.z * inv), act_put(out + 3, num.w * inv);
       } else {
@@ -445,7 +443,7 @@ int run_rows(cudaStream_t st, const TreeArgs& a) {
 
 template <class T, bool Q8>
 int run_tree(cudaStream_t st, const TreeArgs& a) {
-  const uint32_t rows = a.n_tokens * (a.n_heads / a.c.n_kv_heads);
+  const uint32_t rows = a.n_tokens * a.group;
   if (a.c.head_dim == 128) return rows <= 8 ? run_rows<T, Q8, 128, 1>(st, a) : run_rows<T, Q8, 128, 2>(st, a);
   return rows <= 8 ? run_rows<T, Q8, 64, 1>(st, a) : run_rows<T, Q8, 64, 2>(st, a);
 }
@@ -499,6 +497,8 @@ int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act
   if (!n_heads || n_heads % cache->n_kv_heads)
     return set_error(RF_EINVAL, "%u query heads are no multiple of %u KV heads", n_heads, cache->n_kv_heads);
   if (!(scale >= 0.f) || scale > 3.0e38f) return set_error(RF_EINVAL, "scale must be positive, or 0 for 1/sqrt(head_dim)");
+  if (n_heads / cache->n_kv_heads > kMaxGroup)
+    return set_error(RF_EUNSUPPORTED, "%u query heads a KV head, at most %u", n_heads / cache->n_kv_heads, kMaxGroup);
   const uint64_t row = (uint64_t)n_heads * cache->head_dim;
   if (!q_stride) q_stride = row;
   if (!out_stride) out_stride = row;
@@ -514,10 +514,12 @@ int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act
   a.q_stride = q_stride, a.out_stride = out_stride;
   a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.n_heads = n_heads, a.words = (n_tokens + 31) / 32;
   a.hist_len = hist_len, a.n_draft = n_draft, a.mask = mask;
+  a.group = n_heads / cache->n_kv_heads;
+  a.group_magic = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
   RF_TRY(verify_error_ptr(&a.err));
   const cudaStream_t st = (cudaStream_t)stream;
-  if (n_tokens * (n_heads / cache->n_kv_heads) > 16) return run_tree_tc(act_type, a, st);
+  if (n_tokens * a.group > 16) return run_tree_tc(act_type, a, st);
   const bool q8 = cache->type == RF_TYPE_Q8_0;
   switch (act_type) {
     case RF_ACT_F32: return q8 ? run_tree<float, true>(st, a) : run_tree<float, false>(st, a);

@@ -16,9 +16,16 @@ struct TreeArgs {
   uint32_t n_seqs, n_tokens, n_heads, words;  // words: mask words per token
   const int32_t *hist_len, *n_draft;
   const uint32_t* mask;
+  uint32_t group, group_magic;  // query heads a KV head, and ceil(2^32 / group)
   float scale;
   unsigned* err;
 };
+
+// r / group for a query row r < 1024 * group, group <= kMaxGroup: the magic's excess times r stays below 2^32.
+constexpr uint32_t kMaxGroup = 1024;
+__device__ __forceinline__ uint32_t group_div(const TreeArgs& a, uint32_t r) {
+  return a.group == 1 ? r : __umulhi(r, a.group_magic);
+}
 
 // History length and draft count of sequence b; (0, 0) and the error bit where they do not fit the cache.
 __device__ __forceinline__ void seq_lengths(const TreeArgs& a, uint32_t b, uint32_t* hist, uint32_t* drafts) {
@@ -42,6 +49,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The powers of two that take a row of largest magnitude `top` to [1, 4) and back (1 for 0, infinity
+// and NaN): products with them are exact.
+__device__ __forceinline__ void pow2_scale(float top, float* down, float* up) {
+  const int e = top > 0.f && top < INFINITY ? min(max(__float_as_int(top) >> 23, 1), 253) : 127;  // biased exponent
+  *down = __int_as_float((254 - e) << 23);
+  *up = __int_as_float(e << 23);
+}
+
 // ---------------------------------------------------------------------------
 // The work split.  A unit is (sequence b, KV head h, row tile rt): up to ROWS of the
 // n_b * G query rows (G query heads share a KV head; row r = token r / G, head r % G)
@@ -56,7 +71,7 @@ template <int KT, int ROWS>
 struct Split {
   static __device__ __forceinline__ uint32_t tiles(uint32_t L, uint32_t n) { return n ? (L + n + KT - 1) / KT : 0; }
   static __device__ __forceinline__ uint32_t row_tiles(const TreeArgs& a, uint32_t n) {
-    return (n * (a.n_heads / a.c.n_kv_heads) + ROWS - 1) / ROWS;
+    return (n * a.group + ROWS - 1) / ROWS;
   }
   static __device__ __forceinline__ uint64_t work(const TreeArgs& a, uint32_t b) {
     if (b >= a.n_seqs) return 0;
@@ -66,6 +81,8 @@ struct Split {
   }
   // Whole warp: the tiles of all sequences, and (through *before) those of the sequences before b.
   static __device__ __forceinline__ uint64_t total(const TreeArgs& a, uint32_t b, uint64_t* before) {
+    *before = 0;
+    if (a.n_seqs == 1) return work(a, 0);
     uint64_t t = 0, p = 0;
     for (uint32_t i = threadIdx.x & 31; i < a.n_seqs; i += 32) {
       const uint64_t w = work(a, i);
@@ -83,6 +100,8 @@ struct Split {
   // Whole warp: the sequence that holds tile w, and w's offset in it.
   static __device__ __forceinline__ uint32_t locate(const TreeArgs& a, uint64_t w, uint64_t* offset) {
     const uint32_t lane = threadIdx.x & 31;
+    *offset = w;
+    if (a.n_seqs == 1) return 0;
     uint64_t acc = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 32) {
       uint64_t s = work(a, base + lane);
@@ -193,24 +212,33 @@ constexpr float kRaise = 8.f, kWeightBias = 7.f;
 // ---------------------------------------------------------------------------
 // Joins the partial results of the units that several of the first kernel's CTAs shared
 // (`grid` of them), in order of the keys, and writes the zeros of tokens past a sequence's drafts.
-// A CTA takes 8 rows of a (sequence, KV head) and 32 dimensions, four threads to each piece
-// of 4: each adds every fourth partial result.  What bounds it is latency, so many small CTAs.
+// A CTA takes 8 rows of a (sequence, KV head) and DPC dimensions; four threads share each
+// piece of 4 dimensions, each adding every fourth partial result against a maximum of its own.
+// Latency bounds it: a thread requests kAhead partial results with their maxima and sums at
+// once.  Many rows are better served by fewer CTAs (DPC = D), few by more (32): 24 against
+// 9 us at 1024 rows x 8 KV heads, 3 against 5 us at 64 x 8.
 // ---------------------------------------------------------------------------
-template <class T, int D, int KT, int ROWS>
+template <class T, int D, int KT, int ROWS, int DPC>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
   using Sp = Split<KT, ROWS>;
+  constexpr int X = DPC / 32, kAhead = X == 1 ? 6 : 3;
   __shared__ float4 s_o[4][64];
-  __shared__ float s_l[4][8];
+  __shared__ float2 s_ml[4][8];
   const uint32_t tid = threadIdx.x, rx = tid & 7, dx = (tid >> 3) & 7, cx = tid >> 6;
-  const uint32_t G = a.n_heads / a.c.n_kv_heads, groups = (a.n_tokens * G + 7) / 8;
+  const uint32_t groups = (a.n_tokens * a.group + 7) / 8;
   const uint32_t bh = blockIdx.x / groups, r0 = (blockIdx.x - bh * groups) * 8;
   const uint32_t b = bh / a.c.n_kv_heads, h = bh - b * a.c.n_kv_heads;
-  const uint32_t r = r0 + rx, t = r / G, hq = h * G + (r - t * G), d = blockIdx.y * 32 + dx * 4;
-  T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d;
+  const uint32_t r = r0 + rx, t = group_div(a, r), hq = h * a.group + (r - t * a.group), d0 = blockIdx.y * DPC + dx * 4;
+  T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d0;
   uint32_t L, n;
   seq_lengths(a, b, &L, &n);
-  if (r < a.n_tokens * G && t >= n && cx == 0) act_put(out, 0.f), act_put(out + 1, 0.f), act_put(out + 2, 0.f), act_put(out + 3, 0.f);
-  if (r0 >= n * G) return;
+  if (t < a.n_tokens && t >= n && cx == 0) {
+#pragma unroll
+    for (int x = 0; x < X; x++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) act_put(out + 32 * x + i, 0.f);
+  }
+  if (r0 >= n * a.group) return;
   uint64_t before;
   const Ranges ranges(Sp::total(a, b, &before), grid);
   const uint32_t tiles = Sp::tiles(L, n);
@@ -219,38 +247,79 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float
   if (c0 == c1) return;  // finished by its CTA
   griddep_wait();
   const uint32_t rl = r % ROWS;
-  auto slot = [&](uint32_t c) { return part + (2 * (size_t)c + (c == c0 ? 1 : 0)) * part_floats(ROWS, D); };
-  float M = -INFINITY;
-#pragma unroll 8
-  for (uint32_t c = c0; c <= c1; c++) M = fmaxf(M, __ldcg(slot(c) + ROWS * D + rl));
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.f;
-#pragma unroll 8
-  for (uint32_t c = c0 + cx; c <= c1; c += 4) {
-    const float* s = slot(c);
-    const float f = M == -INFINITY ? 1.f : ex2(__ldcg(s + ROWS * D + rl) - M);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(s + part_at<ROWS>(d, rl)));
-    den += __ldcg(s + ROWS * D + ROWS + rl) * f;
-    acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
-  }
-  s_o[cx][tid & 63] = acc;
-  if (dx == 0) s_l[cx][rx] = den;
-  __syncthreads();
-  if (cx == 0 && t < n) {
+  float M = -INFINITY, den = 0.f;
+  float4 acc[X];
 #pragma unroll
-    for (int i = 1; i < 4; i++) {
-      const float4 v = s_o[i][tid];
-      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+  for (int x = 0; x < X; x++) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t c = c0 + cx; c <= c1; c += 4 * kAhead) {
+    float m[kAhead], l[kAhead];
+    float4 v[kAhead][X];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+      const uint32_t ck = c + 4 * k;
+      m[k] = -INFINITY, l[k] = 0.f;
+#pragma unroll
+      for (int x = 0; x < X; x++) v[k][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ck <= c1) {
+        const float* s = part + (2 * (size_t)ck + (ck == c0 ? 1 : 0)) * part_floats(ROWS, D);
+        m[k] = __ldcg(s + ROWS * D + rl), l[k] = __ldcg(s + ROWS * D + ROWS + rl);
+#pragma unroll
+        for (int x = 0; x < X; x++) v[k][x] = __ldcg(reinterpret_cast<const float4*>(s + part_at<ROWS>(d0 + 32 * x, rl)));
+      }
     }
-    const float l = s_l[0][rx] + s_l[1][rx] + s_l[2][rx] + s_l[3][rx], inv = l == 0.f ? 0.f : 1.f / l;
-    act_put(out, acc.x * inv), act_put(out + 1, acc.y * inv), act_put(out + 2, acc.z * inv), act_put(out + 3, acc.w * inv);
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) top = fmaxf(top, m[k]);
+    const float old = top == -INFINITY ? 1.f : ex2(M - top);
+    M = top;
+    den *= old;
+#pragma unroll
+    for (int x = 0; x < X; x++) acc[x].x *= old, acc[x].y *= old, acc[x].z *= old, acc[x].w *= old;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+      const float f = top == -INFINITY ? 1.f : ex2(m[k] - top);
+      den += l[k] * f;
+#pragma unroll
+      for (int x = 0; x < X; x++)
+        acc[x].x += v[k][x].x * f, acc[x].y += v[k][x].y * f, acc[x].z += v[k][x].z * f, acc[x].w += v[k][x].w * f;
+    }
+  }
+  if (dx == 0) s_ml[cx][rx] = make_float2(M, den);
+  float f[4], inv = 0.f;
+#pragma unroll
+  for (int x = 0; x < X; x++) {
+    if (x) __syncthreads();
+    s_o[cx][tid & 63] = acc[x];
+    __syncthreads();
+    if (cx == 0 && t < n) {
+      if (x == 0) {
+        float top = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = fmaxf(top, s_ml[i][rx].x);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          f[i] = top == -INFINITY ? 1.f : ex2(s_ml[i][rx].x - top);
+          l += s_ml[i][rx].y * f[i];
+        }
+        inv = l == 0.f ? 0.f : 1.f / l;
+      }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float4 v = s_o[i][tid];
+        o.x += v.x * f[i], o.y += v.y * f[i], o.z += v.z * f[i], o.w += v.w * f[i];
+      }
+      T* p = out + 32 * x;
+      act_put(p, o.x * inv), act_put(p + 1, o.y * inv), act_put(p + 2, o.z * inv), act_put(p + 3, o.w * inv);
+    }
   }
 }
 template <class T, int D, int KT, int ROWS>
 cudaError_t launch_merge(cudaStream_t st, const TreeArgs& a, const float* part, uint32_t grid) {
-  const uint32_t groups = (a.n_tokens * (a.n_heads / a.c.n_kv_heads) + 7) / 8;
-  return launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS>, dim3(a.n_seqs * a.c.n_kv_heads * groups, D / 32),
-                  dim3(256), 0, a, part, grid);
+  const uint32_t blocks = a.n_seqs * a.c.n_kv_heads * ((a.n_tokens * a.group + 7) / 8);
+  if (blocks > 2 * (uint32_t)num_sms())
+    return launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS, D>, dim3(blocks), dim3(256), 0, a, part, grid);
+  return launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS, 32>, dim3(blocks, D / 32), dim3(256), 0, a, part, grid);
 }
 
 // Scratch of one call: allocated in stream order from a pool of this library's own that keeps

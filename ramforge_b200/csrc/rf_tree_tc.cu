@@ -48,6 +48,10 @@ constexpr int TK = 128;                      // keys of a tile, rows of a row ti
 constexpr uint32_t kOperandBytes = 224 * 1024;
 constexpr uint32_t kBlockBytes = TK * 128;   // one [128][64] f16 block
 constexpr uint32_t kAuxBytes = 2560;
+#ifndef KP
+#define KP 3
+#endif
+constexpr int kPoly = KP, kPolyOf = 16;
 
 template <class T, bool Q8, int D, int RT>
 struct Shape {
@@ -57,8 +61,7 @@ struct Shape {
   static constexpr uint32_t TILE = TK * D * 2;
   static constexpr uint32_t RAW = TK * D;
   static constexpr uint32_t QBYTES = TILE * RT * (SPLIT ? 2 : 1);
-  // raw tiles in flight: one row tile is bound by the cache's bytes, two by the products
-  static constexpr int NRAW = Q8 ? (RT == 2 && D == 128 ? 2 : 4) : 0;
+  static constexpr int NRAW = Q8 ? 4 : 0;  // raw tiles in flight
   static constexpr int kFit = (kOperandBytes - QBYTES - NRAW * RAW) / TILE;
   static constexpr int NSLOT = kFit < 6 ? kFit : 6;
   static constexpr uint32_t SMEM = kOperandBytes + kAuxBytes;
@@ -165,6 +168,32 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+// 2^x on the multiply-add pipe, x <= 127: 2^n * 2^f with n = round(x) and a degree-4 polynomial of 2^f
+// on [-1/2, 1/2] (least maximum relative error, fitted: 2.7e-6, against f16's 4.9e-4).  NaN stays NaN; below
+// -126 the result is 2^-126.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  const float2 magic = make_float2(12582912.f, 12582912.f), less = make_float2(-12582912.f, -12582912.f);
+  const float2 t = add2(x, magic), n = add2(t, less);
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = make_float2(0.0095701013f, 0.0095701013f);
+  p = fma2(p, f, make_float2(0.0559178605f, 0.0559178605f));
+  p = fma2(p, f, make_float2(0.2402474433f, 0.2402474433f));
+  p = fma2(p, f, make_float2(0.6931218147f, 0.6931218147f));
+  p = fma2(p, f, make_float2(0.9999992847f, 0.9999992847f));
+  const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+  return mul2(p, scale);
 }
 
 // Non-finite f16 halves of a word replaced by 0.
@@ -327,7 +356,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   volatile uint32_t* stop = &B.stop;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bar(bar, parity, stop, a.err); };
   bool ok = true;
-  const uint32_t G = a.n_heads / a.c.n_kv_heads;
+  const uint32_t G = a.group;
   Segment sg;
 
   if (warp == 0) {
@@ -524,10 +553,10 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       const uint32_t r_base = sg.rt * S::ROWS + (RT == 2 ? g * TK : 0) + w32;  // the warp's first row
       const uint32_t r = r_base + lane;
       const bool live = r < n_rows, warp_live = r_base < n_rows;
-      const uint32_t t = live ? r / G : 0;
+      const uint32_t t = live ? group_div(a, r) : 0;
       // element offset of row x's head in a tensor of token stride `stride`
       auto row_at = [&](uint32_t x, uint64_t stride) {
-        const uint32_t tx = x / G;
+        const uint32_t tx = group_div(a, x);
         return ((uint64_t)sg.b * a.n_tokens + tx) * stride + (uint64_t)(sg.h * G + (x - tx * G)) * D;
       };
       // queries, a few rows of the warp at a time: f32 and bf16 rows are scaled by a power of
@@ -537,7 +566,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         constexpr int BATCH = 32 / RPI < 8 ? 32 / RPI : 8;
         constexpr int PIECE = 16 / sizeof(T);
         const uint32_t sub = lane / CPR, c = lane % CPR;
-        int e_mine = 0;
+        float up_mine = 1.f;
 #pragma unroll 1
         for (int b0 = 0; b0 < (int)(32 / RPI); b0 += BATCH) {
           uint4 u[BATCH];
@@ -557,13 +586,12 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
               for (int j = 0; j < PIECE; j++) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
               for (uint32_t o = CPR / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-              const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
-              // in two factors: 2^-e alone leaves f32 for the smallest rows
-              const float d0 = ldexpf(1.f, -(e / 2)), d1 = ldexpf(1.f, -(e - e / 2));
+              float down, up;
+              pow2_scale(top, &down, &up);
 #pragma unroll
-              for (int j = 0; j < PIECE; j++) v[j] = v[j] * d0 * d1;
-              const int et = __shfl_sync(~0u, e, (lane % RPI) * CPR);
-              if ((int)(lane / RPI) == b0 + i) e_mine = et;
+              for (int j = 0; j < PIECE; j++) v[j] *= down;
+              up = __shfl_sync(~0u, up, (lane % RPI) * CPR);
+              if ((int)(lane / RPI) == b0 + i) up_mine = up;
             }
             if (RT == 2 || g == 0) {
               const uint32_t x = w32 + (b0 + i) * RPI + sub;
@@ -580,7 +608,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           }
         }
         if constexpr (!std::is_same<T, __half>::value)
-          coef = fmaxf(coef * ldexpf(1.f, e_mine), 1.17549435e-38f);  // not 0: a masked score stays -inf
+          coef = fmaxf(coef * up_mine, 1.17549435e-38f);  // not 0: a masked score stays -inf
         tc_fence_proxy_async();
         tc_mbar_arrive(tc_smem_u32(&B.q_full));
       }
@@ -642,7 +670,10 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i++) {
               float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
-              v.x = ex2(v.x), v.y = ex2(v.y);
+              if (!SPLIT && i % kPolyOf < kPoly)
+                v = ex2_poly(v);
+              else
+                v.x = ex2(v.x), v.y = ex2(v.y);
               sum[i & 1] = add2(sum[i & 1], v);
               p[i] = pack_h2(v.x, v.y);
               if constexpr (SPLIT) s[i] = pack_h2_rest(v.x, v.y, p[i]);
@@ -791,18 +822,27 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           const bool draft_v = is_v && p >= sg.hist;
           ok = __all_sync(~0u, ok && wait(&B.raw_full[rr.s], rr.phase) && wait(&B.free[ring.s], ring.phase ^ 1));
           if (ok) {
-            const uint32_t raw = raws + rr.s * S::RAW + key * D, dst = slot_addr(ring.s);
+            // piece j of the lane's turn is piece c = j ^ lm of its key: the eight lanes of a phase
+            // meet different banks when they read it and when they write its two f16 pieces
+            constexpr uint32_t N = D / 16;
+            const uint32_t lm = lane & (N - 1), l7 = lane & 7;
+            const uint32_t raw = (raws + rr.s * S::RAW + key * D) + lm * 16;
+            const uint32_t lane_at = slot_addr(ring.s) + key * 128 + ((((2 * lm) ^ l7) & 7) << 4);
+            const uint32_t near = lane_at + (lm >> 2) * kBlockBytes, far = lane_at + ((lm >> 2) ^ 1) * kBlockBytes;
+            uint32_t scale[N / 2];  // of the pieces 2i, 2i + 1 of the turn, twice in a word
+#pragma unroll
+            for (uint32_t i = 0; i < N / 2; i++) {
+              const uint32_t blk = i ^ (lm >> 1), w = blk & 2 ? sc.y : sc.x;
+              scale[i] = __byte_perm(w, w, blk & 1 ? 0x3232 : 0x1010);
+            }
+            uint4 codes[N];
+#pragma unroll
+            for (uint32_t j = 0; j < N; j++) codes[j] = ld_shared16(raw ^ (16 * j));
             bool wild = false;
-            uint4 codes[D / 16];
 #pragma unroll
-            for (int j = 0; j < D / 16; j++) codes[j] = ld_shared16(raw + 16 * ((j + lane) & (D / 16 - 1)));
-#pragma unroll
-            for (int j = 0; j < D / 16; j++) {
-              const uint32_t c = (j + lane) & (D / 16 - 1);
-              const uint4 u = codes[j];
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w}, sw = c >= 4 ? sc.y : sc.x;
-              const uint32_t db = __byte_perm(sw, sw, c & 2 ? 0x3232 : 0x1010);
-              const __half2 d = *reinterpret_cast<const __half2*>(&db);
+            for (uint32_t j = 0; j < N; j++) {
+              const uint32_t w[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
+              const __half2 d = *reinterpret_cast<const __half2*>(&scale[j / 2]);
               uint32_t h[8];
 #pragma unroll
               for (int k = 0; k < 4; k++) {
@@ -818,8 +858,9 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 8; k++) h[k] = finite_halves(h[k], &wild);
               }
-              st_shared16(dst + sw128_offset(key, 2 * c), make_uint4(h[0], h[1], h[2], h[3]));
-              st_shared16(dst + sw128_offset(key, 2 * c + 1), make_uint4(h[4], h[5], h[6], h[7]));
+              const uint32_t at = (N == 8 && j >= 4 ? far : near) ^ (((2 * j) & 7) << 4);
+              st_shared16(at, make_uint4(h[0], h[1], h[2], h[3]));
+              st_shared16(at ^ 16, make_uint4(h[4], h[5], h[6], h[7]));
             }
             if (wild) *(volatile uint32_t*)&B.wild = 1;
           }
@@ -893,7 +934,7 @@ template <class T, bool Q8, int D>
 int run_shape(cudaStream_t st, const TreeArgs& a) {
   // f32 splits its queries, which takes the second row tile's place in shared memory
   if constexpr (!std::is_same<T, float>::value)
-    if (a.n_tokens * (a.n_heads / a.c.n_kv_heads) > TK) return run<T, Q8, D, 2>(st, a);
+    if (a.n_tokens * a.group > TK) return run<T, Q8, D, 2>(st, a);
   return run<T, Q8, D, 1>(st, a);
 }
 
