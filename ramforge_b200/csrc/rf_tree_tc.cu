@@ -48,10 +48,7 @@ constexpr int TK = 128;                      // keys of a tile, rows of a row ti
 constexpr uint32_t kOperandBytes = 224 * 1024;
 constexpr uint32_t kBlockBytes = TK * 128;   // one [128][64] f16 block
 constexpr uint32_t kAuxBytes = 2560;
-#ifndef KP
-#define KP 3
-#endif
-constexpr int kPoly = KP, kPolyOf = 16;
+constexpr int kPoly = 3, kPolyOf = 16;  // pairs of weights, of every 16, on the multiply-add pipe
 
 template <class T, bool Q8, int D, int RT>
 struct Shape {

@@ -6,6 +6,9 @@
 // and written once, so HBM bounds the long calls and launch latency the short ones.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "rf_device.cuh"
 #include "rf_verify.h"
 
@@ -101,6 +104,15 @@ struct Act<__nv_bfloat16> {
   }
 };
 
+// 16 bytes that this call reads once.
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(p));
+  return u;
+}
+
 // ---------------------------------------------------------------------------
 // Per-head norm and rotation.
 // ---------------------------------------------------------------------------
@@ -172,67 +184,103 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(NormRopeArgs a) {
   }
 }
 
+// Pairs of f32 in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+
 // Whole-head or no rotation, 16-byte aligned rows: lane x of a group of `lanes` holds the
 // 16-byte piece x of the head's first half and of its second half, so each pair to rotate
-// sits in one lane.  A group takes kHeads heads of one token together: their loads are all
-// in flight at once, and the table row and the weights are read once for all of them.
-constexpr int kHeads = 4;
+// sits in one lane.  A group takes kHeads heads of one token together: their loads are all in
+// flight at once, and the products of weights and table are formed once for all of them.
+constexpr int kHeads = 2, kNormThreads = 128;
 
 template <class T>
-__global__ void __launch_bounds__(256) norm_rope_vec_kernel(NormRopeArgs a, uint32_t lanes, uint32_t q_groups,
-                                                            uint32_t groups) {
+__global__ void __launch_bounds__(kNormThreads) norm_rope_vec_kernel(NormRopeArgs a, uint32_t lanes, uint32_t q_groups,
+                                                                      uint32_t groups) {
   constexpr int V = Act<T>::kVec;
-  const uint32_t idx = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t idx = blockIdx.x * kNormThreads + threadIdx.x, D = a.head_dim;
   uint32_t item = idx / lanes;
-  const uint32_t x = idx % lanes, D = a.head_dim;
+  const uint32_t x = idx - item * lanes;
   bool live = item < a.n_tokens * groups;
   if (!live) item = 0;
-  const uint32_t t = item / groups, gr = item % groups;
+  const uint32_t t = item / groups, gr = item - t * groups;
   const bool is_q = gr < q_groups;
   const uint32_t h0 = (is_q ? gr : gr - q_groups) * kHeads, heads = is_q ? a.n_heads : a.n_kv_heads;
   const T* src = (const T*)(is_q ? a.q : a.k) + t * (is_q ? a.q_stride : a.k_stride) + (size_t)h0 * D + x * V;
   T* dst = (T*)(is_q ? a.q_out : a.k_out) + t * (is_q ? a.q_out_stride : a.k_out_stride) + (size_t)h0 * D + x * V;
   const float* nw = is_q ? a.q_norm : a.k_norm;
+  const int32_t pos = a.rot_dim ? __ldg(a.pos + t) : 0;
   uint4 raw[kHeads][2];
 #pragma unroll
-  for (int i = 0; i < kHeads; i++)
+  for (int i = 0; i < kHeads; i++) {
+    raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
     if (live && h0 + i < heads) {
       raw[i][0] = *reinterpret_cast<const uint4*>(src + i * D);
       raw[i][1] = *reinterpret_cast<const uint4*>(src + i * D + D / 2);
-    } else {
-      raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
     }
-  const float2* row;
-  live = rope_row(a, t, &row) && live;
-  float cs[V], sn[V], w[2][V];
+  }
+  const bool turn = a.rot_dim != 0;
+  if (turn && (pos < 0 || (uint32_t)pos >= a.rope_len)) {
+    if (live) atomicOr(a.err, kVerifyRange);
+    live = false;
+  }
+  // out of the halves v0, v1:  r (v0 w0c - v1 w1s)  and  r (v1 w1c + v0 w0s)
+  float2 w0c[V / 2], w1c[V / 2], w0s[V / 2], w1s[V / 2];
 #pragma unroll
-  for (int j = 0; j < V; j += 2) {
-    const float4 f = row && live ? __ldg(reinterpret_cast<const float4*>(row + x * V + j)) : make_float4(1.f, 0.f, 1.f, 0.f);
-    cs[j] = f.x, sn[j] = f.y, cs[j + 1] = f.z, sn[j + 1] = f.w;
+  for (int j = 0; j < V / 2; j += 2) {
+    const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+    const float4 a0 = nw ? __ldg(reinterpret_cast<const float4*>(nw + x * V + 2 * j)) : one;
+    const float4 a1 = nw ? __ldg(reinterpret_cast<const float4*>(nw + D / 2 + x * V + 2 * j)) : one;
+    w0c[j] = make_float2(a0.x, a0.y), w0c[j + 1] = make_float2(a0.z, a0.w);
+    w1c[j] = make_float2(a1.x, a1.y), w1c[j + 1] = make_float2(a1.z, a1.w);
+  }
+  if (turn) {
+    const float2* row = a.rope + (size_t)(live ? pos : 0) * (D / 2) + x * V;
+#pragma unroll
+    for (int j = 0; j < V / 2; j++) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(row + 2 * j));
+      const float2 c = make_float2(f.x, f.z), s = make_float2(f.y, f.w);
+      w0s[j] = mul2(w0c[j], s), w1s[j] = mul2(w1c[j], make_float2(-f.y, -f.w));
+      w0c[j] = mul2(w0c[j], c), w1c[j] = mul2(w1c[j], c);
+    }
   }
 #pragma unroll
-  for (int s = 0; s < 2; s++)
-#pragma unroll
-    for (int j = 0; j < V; j += 4) {
-      const float4 f = nw ? __ldg(reinterpret_cast<const float4*>(nw + s * (D / 2) + x * V + j)) : make_float4(1.f, 1.f, 1.f, 1.f);
-      w[s][j] = f.x, w[s][j + 1] = f.y, w[s][j + 2] = f.z, w[s][j + 3] = f.w;
-    }
-#pragma unroll
   for (int i = 0; i < kHeads; i++) {
-    float v[2][V];
-    Act<T>::unpack(raw[i][0], v[0]);
-    Act<T>::unpack(raw[i][1], v[1]);
-    float ss = 0.f;
+    float2 v[2][V / 2];
 #pragma unroll
-    for (int j = 0; j < V; j++) ss = fmaf(v[0][j], v[0][j], fmaf(v[1][j], v[1][j], ss));
+    for (int s = 0; s < 2; s++) {
+      float f[V];
+      Act<T>::unpack(raw[i][s], f);
+#pragma unroll
+      for (int j = 0; j < V / 2; j++) v[s][j] = make_float2(f[2 * j], f[2 * j + 1]);
+    }
+    float2 ss2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < V / 2; j++) ss2 = fma2(v[0][j], v[0][j], fma2(v[1][j], v[1][j], ss2));
+    float ss = ss2.x + ss2.y;
     for (uint32_t o = lanes / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = nw ? 1.f / sqrtf(ss / (float)D + a.eps) : 1.f;
+    const float r1 = nw ? 1.f / sqrtf(ss / (float)D + a.eps) : 1.f;
+    const float2 r = make_float2(r1, r1);
     float y[2][V];
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      const float p = v[0][j] * r * w[0][j], q = v[1][j] * r * w[1][j];
-      y[0][j] = row ? p * cs[j] - q * sn[j] : p;
-      y[1][j] = row ? p * sn[j] + q * cs[j] : q;
+    for (int j = 0; j < V / 2; j++) {
+      float2 u = mul2(v[0][j], w0c[j]), z = mul2(v[1][j], w1c[j]);
+      if (turn) u = fma2(v[1][j], w1s[j], u), z = fma2(v[0][j], w0s[j], z);
+      u = mul2(u, r), z = mul2(z, r);
+      y[0][2 * j] = u.x, y[0][2 * j + 1] = u.y, y[1][2 * j] = z.x, y[1][2 * j + 1] = z.y;
     }
     if (live && h0 + i < heads) {
       *reinterpret_cast<uint4*>(dst + i * D) = Act<T>::pack(y[0]);
@@ -244,8 +292,10 @@ __global__ void __launch_bounds__(256) norm_rope_vec_kernel(NormRopeArgs a, uint
 }  // namespace
 
 // ---------------------------------------------------------------------------
-// The cache.  A thread handles 16 elements of one head of one row, for K or for V:
-// half a Q8_0 block, so a pair of neighbouring lanes shares a scale.
+// The cache.  A lane handles 16 elements of one head of a row at a time, for K or for V: a 16-byte
+// piece of codes, half a Q8_0 block, so a pair of neighbouring lanes shares a scale.  A position has
+// to arrive before the row it names can be asked for, so CTAs stay and go from row to row: while a
+// row is converted, the next one and the position after that are on their way.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -254,57 +304,111 @@ struct KvRowsArgs {
   const void *k, *v;  // write: sources; read: destinations (may be null)
   uint64_t k_stride, v_stride;
   const int32_t *seq, *pos;
-  uint32_t n_rows;
+  uint32_t n_rows, per_head, per_row;  // 16-element pieces of a head and of a row (K and V)
+  bool wide;                           // activations' rows are 32-byte aligned
   unsigned* err;
 };
 
-// Element offset of (seq, head, pos 0..) rows in a plane, or -1: not kept (pos < 0), -2: out of range.
-__device__ __forceinline__ int64_t kv_row(const KvRowsArgs& a, uint32_t row, uint32_t h) {
-  const int32_t p = a.pos[row], s = a.seq ? a.seq[row] : 0;
-  if (p < 0) return -1;
-  if ((uint32_t)p >= a.c.capacity || s < 0 || (uint32_t)s >= a.c.n_seqs) {
-    atomicOr(a.err, kVerifyRange);
-    return -2;
+constexpr int kKvThreads = 256, kKvCtas = 4, kKvRows = 2;  // CTAs an SM; rows of a thread in flight
+
+// Thread (x, y) of a CTA: piece x of a row's K and V pieces (blockIdx.y counts runs of kKvThreads), row y
+// of every `rows` the CTA takes at a time.
+struct KvPlace {
+  bool in, is_v;
+  uint32_t x, h, c;  // piece of the K or V row, its head, piece of the head
+  uint32_t row, step;
+  __device__ __forceinline__ KvPlace(const KvRowsArgs& a) {
+    const uint32_t width = min(a.per_row, (uint32_t)kKvThreads), y = threadIdx.x / width;
+    const uint32_t at = blockIdx.y * kKvThreads + (threadIdx.x - y * width), half = a.per_row / 2, rows = kKvThreads / width;
+    in = at < a.per_row && y < rows;
+    is_v = at >= half;
+    x = is_v ? at - half : at;
+    h = x / a.per_head;
+    c = x - h * a.per_head;
+    row = blockIdx.x * rows + y;
+    step = gridDim.x * rows;
   }
-  return ((int64_t)s * a.c.n_kv_heads + h) * a.c.capacity + p;
+};
+
+// Place of a row: its position and sequence, then (out of range: the error bit) its cache row, or -1.
+struct KvAddr {
+  int32_t pos, seq;
+};
+__device__ __forceinline__ KvAddr kv_addr(const KvRowsArgs& a, uint32_t row) {
+  KvAddr p{-1, 0};
+  if (row < a.n_rows) p.pos = __ldg(a.pos + row), p.seq = a.seq ? __ldg(a.seq + row) : 0;
+  return p;
+}
+__device__ __forceinline__ int64_t kv_slot(const KvRowsArgs& a, KvAddr p, uint32_t h) {
+  if (p.pos < 0) return -1;
+  if ((uint32_t)p.pos >= a.c.capacity || p.seq < 0 || (uint32_t)p.seq >= a.c.n_seqs) {
+    atomicOr(a.err, kVerifyRange);
+    return -1;
+  }
+  return ((int64_t)p.seq * a.c.n_kv_heads + h) * a.c.capacity + p.pos;
 }
 
-template <class T, bool Q8>
-__global__ void __launch_bounds__(256) kv_write_kernel(KvRowsArgs a) {
-  const uint32_t lph = a.c.head_dim / 16, per = a.c.n_kv_heads * lph;
-  const uint32_t idx = blockIdx.x * 256 + threadIdx.x;
-  const uint32_t total = 2 * a.n_rows * per;
-  const bool in = idx < total;
-  const uint32_t at = in ? idx : 0;
-  const uint32_t rk = at / per, x = at % per, row = rk >> 1, h = x / lph, c16 = x % lph;
-  const bool is_v = rk & 1;
-  const int64_t slot = kv_row(a, row, h);
-  const bool live = in && slot >= 0;
-  constexpr int NV = 16 / Act<T>::kVec;
-  float v[16];
-  if (live) {
-    const T* src = (const T*)(is_v ? a.v : a.k) + row * (is_v ? a.v_stride : a.k_stride) + (size_t)x * 16;
+// 16 activations: two or four 16-byte loads or stores, or half as many of 32 bytes.
+template <class T>
+struct Acts16 {
+  static constexpr int N = 16 / Act<T>::kVec;
+  uint4 u[N];
+  __device__ __forceinline__ void load(const T* p, bool wide) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
+    for (int i = 0; i < N; i += 2) {
+      const uint4* q = reinterpret_cast<const uint4*>(p) + i;
+      if (wide)
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(u[i].x), "=r"(u[i].y), "=r"(u[i].z), "=r"(u[i].w), "=r"(u[i + 1].x), "=r"(u[i + 1].y),
+                       "=r"(u[i + 1].z), "=r"(u[i + 1].w)
+                     : "l"(q));
+      else
+        u[i] = __ldg(q), u[i + 1] = __ldg(q + 1);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, bool wide) const {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      uint4* q = reinterpret_cast<uint4*>(p) + i;
+      if (wide)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(q), "r"(u[i].x), "r"(u[i].y), "r"(u[i].z),
+                     "r"(u[i].w), "r"(u[i + 1].x), "r"(u[i + 1].y), "r"(u[i + 1].z), "r"(u[i + 1].w)
+                     : "memory");
+      else
+        q[0] = u[i], q[1] = u[i + 1];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[16]) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
       float f[Act<T>::kVec];
-      Act<T>::unpack(reinterpret_cast<const uint4*>(src)[i], f);
+      Act<T>::unpack(u[i], f);
 #pragma unroll
       for (int j = 0; j < Act<T>::kVec; j++) v[i * Act<T>::kVec + j] = f[j];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = 0.f;
   }
-  if constexpr (!Q8) {
-    if (!live) return;
-    __half* dst = (__half*)(is_v ? a.c.v : a.c.k) + slot * a.c.head_dim + c16 * 16;
+  __device__ __forceinline__ void put(const float (&v)[16]) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      float f[8];
+    for (int i = 0; i < N; i++) {
+      float f[Act<T>::kVec];
 #pragma unroll
-      for (int j = 0; j < 8; j++) f[j] = v[8 * i + j];
-      reinterpret_cast<uint4*>(dst)[i] = Act<__half>::pack(f);
+      for (int j = 0; j < Act<T>::kVec; j++) f[j] = v[i * Act<T>::kVec + j];
+      u[i] = Act<T>::pack(f);
     }
+  }
+};
+
+template <class T, bool Q8>
+__device__ __forceinline__ void kv_store(const KvRowsArgs& a, const KvPlace& p, int64_t slot, const Acts16<T>& in) {
+  float v[16];
+  in.get(v);
+  const uint64_t at = (uint64_t)slot * a.c.head_dim + p.c * 16;
+  if constexpr (!Q8) {
+    if (slot < 0) return;
+    __half* dst = (__half*)(p.is_v ? a.c.v : a.c.k) + at;
+    Acts16<__half> out;
+    out.put(v);
+    out.store(dst, false);
   } else {
     float amax = 0.f;
     bool nan = false;
@@ -314,70 +418,136 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvRowsArgs a) {
       v[i] = fminf(fmaxf(v[i], -65472.f), 65472.f);
       amax = fmaxf(amax, fabsf(v[i]));
     }
-    if (nan) amax = __int_as_float(0x7fffffff);
-    const float other = __shfl_xor_sync(0xffffffffu, amax, 1);
-    amax = amax != amax || other != other ? __int_as_float(0x7fffffff) : fmaxf(amax, other);
+    // a NaN's bits are above every number's, so the maximum of the bits keeps it
+    int bits = nan ? 0x7fffffff : __float_as_int(amax);
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
     // the scale is kept in f16 (GGUF's block): its 11 bits cost at most 2^-11 of a code step per code,
     // and codes are taken against the rounded scale
-    const __half d = __float2half_rn(__fdiv_rn(amax, 127.f));
+    const __half d = __float2half_rn(__fdiv_rn(__int_as_float(bits), 127.f));
     const float df = __half2float(d), inv = df > 0.f ? __fdiv_rn(1.f, df) : 0.f;
-    if (!live) return;
+    if (slot < 0) return;
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      w[i] = 0;
+      uint32_t b[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int code = min(127, max(-127, __float2int_rn(__fmul_rn(v[4 * i + j], inv))));
-        w[i] |= ((uint32_t)code & 0xffu) << (8 * j);
-      }
+      for (int j = 0; j < 4; j++)  // round to nearest even by the sum's own rounding: the code is its low byte
+        b[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(v[4 * i + j], inv), -127.f), 127.f), 12582912.f));
+      w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
-    *reinterpret_cast<uint4*>((int8_t*)(is_v ? a.c.v : a.c.k) + slot * a.c.head_dim + c16 * 16) =
-        make_uint4(w[0], w[1], w[2], w[3]);
-    if (!(c16 & 1)) ((__half*)(is_v ? a.c.v_scale : a.c.k_scale))[slot * (a.c.head_dim / 32) + c16 / 2] = d;
+    *reinterpret_cast<uint4*>((int8_t*)(p.is_v ? a.c.v : a.c.k) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (!(p.c & 1)) ((__half*)(p.is_v ? a.c.v_scale : a.c.k_scale))[slot * (a.c.head_dim / 32) + p.c / 2] = d;
   }
 }
 
 template <class T, bool Q8>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvRowsArgs a) {
-  const uint32_t lph = a.c.head_dim / 16, per = a.c.n_kv_heads * lph;
-  const uint32_t idx = blockIdx.x * 256 + threadIdx.x;
-  if (idx >= 2 * a.n_rows * per) return;
-  const uint32_t rk = idx / per, x = idx % per, row = rk >> 1, h = x / lph, c16 = x % lph;
-  const bool is_v = rk & 1;
-  T* dst = (T*)(is_v ? a.v : a.k);
-  if (!dst) return;
-  dst += row * (is_v ? a.v_stride : a.k_stride) + (size_t)x * 16;
-  const int64_t slot = kv_row(a, row, h);
-  float v[16];
+__global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvRowsArgs a) {
+  const KvPlace p(a);
+  const T* src = (const T*)(p.is_v ? a.v : a.k) + p.x * 16;
+  const uint64_t stride = p.is_v ? a.v_stride : a.k_stride;
+  Acts16<T> cur[kKvRows] = {}, next[kKvRows] = {};
+  KvAddr at[kKvRows], at_next[kKvRows];
+  auto fetch = [&](uint32_t row, Acts16<T>(&u)[kKvRows], KvAddr(&w)[kKvRows]) {
 #pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = 0.f;
-  if (slot >= 0) {
-    if constexpr (Q8) {
-      const uint4 u = *reinterpret_cast<const uint4*>((const int8_t*)(is_v ? a.c.v : a.c.k) + slot * a.c.head_dim + c16 * 16);
-      const float d = __half2float(((const __half*)(is_v ? a.c.v_scale : a.c.k_scale))[slot * (a.c.head_dim / 32) + c16 / 2]);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < kKvRows; i++) {
+      const uint32_t r = row + i * p.step;
+      w[i] = kv_addr(a, p.in ? r : a.n_rows);
+      if (p.in && r < a.n_rows) u[i].load(src + r * stride, a.wide);
+    }
+  };
+  fetch(p.row, cur, at);
+  // all lanes of a warp go round as often as the CTA's first row does: shuffles inside
+  for (uint32_t row = p.row, first = blockIdx.x * (kKvThreads / min(a.per_row, (uint32_t)kKvThreads)); first < a.n_rows;
+       row += kKvRows * p.step, first += kKvRows * p.step) {
+    fetch(row + kKvRows * p.step, next, at_next);
 #pragma unroll
-      for (int i = 0; i < 16; i++)  // code * scale is exact in f32 (8 x 11 bits), then one rounding to f16
-        v[i] = __half2float(__float2half_rn((float)(int8_t)((w[i / 4] >> (8 * (i % 4))) & 0xffu) * d));
-    } else {
-      const uint4* p = reinterpret_cast<const uint4*>((const __half*)(is_v ? a.c.v : a.c.k) + slot * a.c.head_dim + c16 * 16);
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        float f[8];
-        Act<__half>::unpack(p[i], f);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[8 * i + j] = f[j];
-      }
+    for (int i = 0; i < kKvRows; i++) {
+      kv_store<T, Q8>(a, p, p.in ? kv_slot(a, at[i], p.h) : -1, cur[i]);
+      cur[i] = next[i], at[i] = at_next[i];
     }
   }
-  constexpr int NV = 16 / Act<T>::kVec;
+}
+
+// A cache piece as it is stored: 16 codes and their scale, or 16 f16.
+template <bool Q8>
+struct KvRaw {
+  uint4 u[Q8 ? 1 : 2];
+  __half d;
+};
+
+template <class T, bool Q8>
+__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvRowsArgs a) {
+  const KvPlace p(a);
+  T* dst = (T*)(p.is_v ? a.v : a.k);
+  if (!dst || !p.in) return;
+  dst += p.x * 16;
+  const uint64_t stride = p.is_v ? a.v_stride : a.k_stride;
+  const void* plane = p.is_v ? a.c.v : a.c.k;
+  const __half* scales = (const __half*)(p.is_v ? a.c.v_scale : a.c.k_scale);
+  auto fetch = [&](KvAddr w) {
+    KvRaw<Q8> x = {};
+    const int64_t slot = kv_slot(a, w, p.h);
+    if (slot < 0) return x;
+    const uint64_t at = (uint64_t)slot * a.c.head_dim + p.c * 16;
+    if constexpr (Q8) {
+      x.u[0] = ld_once((const int8_t*)plane + at);
+      x.d = __ldg(scales + slot * (a.c.head_dim / 32) + p.c / 2);
+    } else {
+      const uint4* q = reinterpret_cast<const uint4*>((const __half*)plane + at);
+      x.u[0] = __ldg(q), x.u[1] = __ldg(q + 1);
+    }
+    return x;
+  };
+  KvRaw<Q8> cur[kKvRows];
+  KvAddr at[kKvRows];
 #pragma unroll
-  for (int i = 0; i < NV; i++) {
-    float f[Act<T>::kVec];
+  for (int i = 0; i < kKvRows; i++) at[i] = kv_addr(a, p.row + i * p.step);
 #pragma unroll
-    for (int j = 0; j < Act<T>::kVec; j++) f[j] = v[i * Act<T>::kVec + j];
-    reinterpret_cast<uint4*>(dst)[i] = Act<T>::pack(f);
+  for (int i = 0; i < kKvRows; i++) {
+    cur[i] = fetch(at[i]);
+    at[i] = kv_addr(a, p.row + (kKvRows + i) * p.step);
+  }
+  for (uint32_t row = p.row; row < a.n_rows; row += kKvRows * p.step) {
+    KvRaw<Q8> next[kKvRows];
+#pragma unroll
+    for (int i = 0; i < kKvRows; i++) {
+      next[i] = fetch(at[i]);
+      at[i] = kv_addr(a, row + (2 * kKvRows + i) * p.step);
+    }
+#pragma unroll
+    for (int i = 0; i < kKvRows; i++) {
+      const uint32_t r = row + i * p.step;
+      Acts16<__half> out;
+      if constexpr (Q8) {
+        // biased bytes under an exponent of 1024: 1152 + code, exact; the product with the scale rounds once to f16
+        const __half2 d2 = __half2half2(cur[i].d), bias = __float2half2_rn(1152.f);
+        const uint32_t w[4] = {cur[i].u[0].x, cur[i].u[0].y, cur[i].u[0].z, cur[i].u[0].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t b = w[k] ^ 0x80808080u;
+          uint32_t lo = __byte_perm(b, 0x64646464u, 0x4140), hi = __byte_perm(b, 0x64646464u, 0x4342);
+          const __half2 x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), bias), d2);
+          const __half2 y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), bias), d2);
+          h[2 * k] = *reinterpret_cast<const uint32_t*>(&x), h[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        out.u[0] = make_uint4(h[0], h[1], h[2], h[3]), out.u[1] = make_uint4(h[4], h[5], h[6], h[7]);
+      } else {
+        out.u[0] = cur[i].u[0], out.u[1] = cur[i].u[1];
+      }
+      if (r < a.n_rows) {
+        if constexpr (std::is_same<T, __half>::value) {
+          out.store(dst + r * stride, a.wide);
+        } else {
+          float v[16];
+          out.get(v);
+          Acts16<T> o;
+          o.put(v);
+          o.store(dst + r * stride, a.wide);
+        }
+      }
+      cur[i] = next[i];
+    }
   }
 }
 
@@ -395,7 +565,7 @@ int check_kv_rows(const rf_kv_view* c, const void* k, const void* v, int act_typ
     if (*s * es % 16) return set_error(RF_EINVAL, "row stride %llu is not a multiple of 16 bytes", (unsigned long long)*s);
   }
   if (!aligned_to(k, 16) || !aligned_to(v, 16)) return set_error(RF_EINVAL, "K/V rows must be 16-byte aligned");
-  if (2ull * n_rows * row / 16 > 0x7fffffffull) return set_error(RF_EINVAL, "%u rows are too many for one call", n_rows);
+  if (2ull * n_rows * row / 4 > 0x7fffffffull) return set_error(RF_EINVAL, "%u rows are too many for one call", n_rows);
   return RF_OK;
 }
 
@@ -410,20 +580,26 @@ cudaError_t launch_norm_rope(const Launch& L, const NormRopeArgs& a) {
   for (uint64_t s : {a.q_stride, a.k_stride, a.q_out_stride, a.k_out_stride}) vec = vec && s % v == 0;
   if (vec) {
     const uint32_t qg = (a.n_heads + kHeads - 1) / kHeads, groups = qg + (a.n_kv_heads + kHeads - 1) / kHeads;
-    const uint32_t threads = a.n_tokens * groups * lanes;
-    return launch_k(L, norm_rope_vec_kernel<T>, dim3((threads + 255) / 256), dim3(256), 0, a, lanes, qg, groups);
+    const uint64_t threads = (uint64_t)a.n_tokens * groups * lanes;
+    return launch_k(L, norm_rope_vec_kernel<T>, dim3((uint32_t)((threads + kNormThreads - 1) / kNormThreads)),
+                    dim3(kNormThreads), 0, a, lanes, qg, groups);
   }
   const uint32_t warps = a.n_tokens * (a.n_heads + a.n_kv_heads);
   return launch_k(L, norm_rope_any_kernel<T>, dim3((warps + 7) / 8), dim3(256), 0, a);
 }
 
 template <class T>
-cudaError_t launch_kv_rows(const Launch& L, const KvRowsArgs& a, bool write) {
-  const uint32_t threads = 2 * a.n_rows * (a.c.n_kv_heads * (a.c.head_dim / 16));
+cudaError_t launch_kv_rows(const Launch& L, KvRowsArgs a, bool write) {
+  a.per_head = a.c.head_dim / 16;
+  a.per_row = 2 * a.c.n_kv_heads * a.per_head;
+  a.wide = aligned_to(a.k, 32) && aligned_to(a.v, 32) && a.k_stride * sizeof(T) % 32 == 0 && a.v_stride * sizeof(T) % 32 == 0;
   const bool q8 = a.c.type == RF_TYPE_Q8_0;
   auto* k = write ? (q8 ? kv_write_kernel<T, true> : kv_write_kernel<T, false>)
                   : (q8 ? kv_read_kernel<T, true> : kv_read_kernel<T, false>);
-  return launch_k(L, k, dim3((threads + 255) / 256), dim3(256), 0, a);
+  const uint32_t width = std::min(a.per_row, (uint32_t)kKvThreads), rows = kKvThreads / width;
+  const uint32_t cols = (a.per_row + kKvThreads - 1) / kKvThreads;
+  const uint32_t most = std::max(1u, (uint32_t)num_sms() * kKvCtas / cols);  // CTAs stay for as many rows as there are
+  return launch_k(L, k, dim3(std::min((a.n_rows + rows - 1) / rows, most), cols), dim3(kKvThreads), 0, a);
 }
 
 int run_kv_rows(const rf_kv_view* cache, const void* k, const void* v, int act_type, uint32_t n_rows, uint64_t k_stride,
