@@ -61,6 +61,9 @@ __device__ __forceinline__ uint32_t q8_pair(uint32_t biased, __half2 d) {
   return h2_bits(__hmul2(code, d));
 }
 
+// A block whose largest code could leave f16, or whose scale is no number.
+__device__ __forceinline__ bool wild_scale(uint32_t half_bits) { return (half_bits & 0x7fffu) > 0x6007u; }  // 515.5
+
 // Shapes of one step of a warp over a cache of type Q8 and head dimension D.
 template <bool Q8, int D>
 struct Step {
@@ -123,6 +126,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
   __shared__ __align__(16) float s_o[kRowWarps][ROWS][D];
   __shared__ float s_m[kRowWarps][ROWS], s_l[kRowWarps][ROWS];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const uint32_t k_half = c >= 2 ? 0x3232 : 0x1010;  // which of a word's two scales the lane's dimensions have
   griddep_launch();
   const uint32_t G = a.group;
   Walk<KT, ROWS> walk(a);
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       load_query<T, Q8, D, SPLIT>(
           (const T*)a.q + ((uint64_t)b * a.n_tokens + (live ? group_div(a, rr) : 0)) * a.q_stride + (h * G + (live ? rr - group_div(a, rr) * G : 0)) * D,
           live, c, qh[nb], ql[nb], &up);
-      const float cf = a.scale * 1.44269504f * up;
+      const float cf = fmaxf(a.scale * 1.44269504f * up, 1.17549435e-38f);  // not 0: a masked score stays -inf
       coef[nb][0] = __shfl_sync(0xffffffffu, cf, 8 * c);
       coef[nb][1] = __shfl_sync(0xffffffffu, cf, 8 * c + 4);
     }
@@ -159,49 +163,74 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       l[nb][0] = l[nb][1] = 0.f;
     }
 
+    // The lane's pieces: K of keys g + 8 i, V of keys 2c + {0, 1, 8, 9} + 16 i of a step.  Whole
+    // steps of the history are read at constant offsets from pointers that move with the
+    // steps; a step that holds drafts or the end reads the last key in place of what is past it.
+    constexpr uint32_t KB = D * (Q8 ? 1 : 2);  // bytes of a row
+    constexpr uint32_t VO = Q8 && D == 64 ? 8 : 16;
     uint32_t kr[2 * MB][KW], vr[4 * MB][VW], vs[4 * MB];
     uint2 ks[2 * MB];
-    // keys past the end are read from the last one (in bounds) and masked below
-    auto load_k = [&](uint32_t kb) {
+    auto v_off = [](int i) { return 16 * (i / 4) + (i % 2) + 8 * ((i / 2) % 2); };
+    auto get_k = [&](int i, const uint8_t* p, const __half* sp) {
 #pragma unroll
-      for (int i = 0; i < 2 * MB; i++) {
-        const uint64_t key = min(kb + g + 8 * i, end - 1);
-        const uint8_t* p = kp + key * D * (Q8 ? 1 : 2) + 16 * c;
-#pragma unroll
-        for (int j = 0; j < KW / 4; j++) {
-          const uint4 u = ld_stream16(p + 64 * j);
-          kr[i][4 * j] = u.x, kr[i][4 * j + 1] = u.y, kr[i][4 * j + 2] = u.z, kr[i][4 * j + 3] = u.w;
-        }
-        if constexpr (Q8) {
-          if constexpr (D == 128)
-            ks[i] = ld_stream8(ksp + key * 4);
-          else
-            ks[i].x = __ldg((const uint32_t*)(ksp + key * 2));
-        }
+      for (int j = 0; j < KW / 4; j++) {
+        const uint4 u = ld_stream16(p + 64 * j);
+        kr[i][4 * j] = u.x, kr[i][4 * j + 1] = u.y, kr[i][4 * j + 2] = u.z, kr[i][4 * j + 3] = u.w;
+      }
+      if constexpr (Q8) {
+        if constexpr (D == 128)
+          ks[i] = ld_stream8(sp);
+        else
+          ks[i].x = __ldg((const uint32_t*)sp);
       }
     };
-    // V keys of the lane: 16 kb + {2c, 2c+1, 2c+8, 2c+9}
-    auto v_key = [&](uint32_t kb, int i) { return kb + 16 * (i / 4) + 2 * c + (i % 2) + 8 * ((i / 2) % 2); };
-    auto load_v = [&](uint32_t kb) {
+    auto get_v = [&](int i, const uint8_t* p, const __half* sp) {
+      if constexpr (Q8 && D == 64) {
+        const uint2 u = ld_stream8(p);
+        vr[i][0] = u.x, vr[i][1] = u.y;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4 * MB; i++) {
-        const uint64_t key = min(v_key(kb, i), end - 1);
-        if constexpr (Q8 && D == 64) {
-          const uint2 u = ld_stream8(vp + key * D + 8 * g);
-          vr[i][0] = u.x, vr[i][1] = u.y;
-        } else {
-          const uint8_t* p = vp + key * D * (Q8 ? 1 : 2) + 16 * g;
-#pragma unroll
-          for (int j = 0; j < VW / 4; j++) {
-            const uint4 u = ld_stream16(p + 128 * j);
-            vr[i][4 * j] = u.x, vr[i][4 * j + 1] = u.y, vr[i][4 * j + 2] = u.z, vr[i][4 * j + 3] = u.w;
-          }
+        for (int j = 0; j < VW / 4; j++) {
+          const uint4 u = ld_stream16(p + 128 * j);
+          vr[i][4 * j] = u.x, vr[i][4 * j + 1] = u.y, vr[i][4 * j + 2] = u.z, vr[i][4 * j + 3] = u.w;
         }
-        if constexpr (Q8) vs[i] = __ldg((const unsigned short*)vsp + key * (D / 32) + g / (D == 128 ? 2 : 4));
       }
+      if constexpr (Q8) vs[i] = __ldg((const unsigned short*)sp);
+    };
+    auto inner = [&](uint32_t kb) { return kb + S::KEYS <= L; };
+    const uint32_t kb0 = k0 * KT + warp * S::KEYS;
+    const uint8_t *kl = kp + (uint64_t)(kb0 + g) * KB + 16 * c, *vl = vp + (uint64_t)(kb0 + 2 * c) * KB + VO * g;
+    const __half* ksl = Q8 ? ksp + (uint64_t)(kb0 + g) * (D / 32) : nullptr;
+    const __half* vsl = Q8 ? vsp + (uint64_t)(kb0 + 2 * c) * (D / 32) + g / (D == 128 ? 2 : 4) : nullptr;
+    auto load_k = [&](uint32_t kb) {
+      if (inner(kb)) {
+#pragma unroll
+        for (int i = 0; i < 2 * MB; i++) get_k(i, kl + 8 * i * KB, Q8 ? ksl + 8 * i * (D / 32) : nullptr);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * MB; i++) {
+          const uint64_t key = min(kb + g + 8 * i, end - 1);
+          get_k(i, kp + key * KB + 16 * c, Q8 ? ksp + key * (D / 32) : nullptr);
+        }
+      }
+      kl += KT * KB;
+      if constexpr (Q8) ksl += KT * (D / 32);
+    };
+    auto load_v = [&](uint32_t kb) {
+      if (inner(kb)) {
+#pragma unroll
+        for (int i = 0; i < 4 * MB; i++) get_v(i, vl + v_off(i) * KB, Q8 ? vsl + v_off(i) * (D / 32) : nullptr);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * MB; i++) {
+          const uint64_t key = min(kb + 2 * c + v_off(i), end - 1);
+          get_v(i, vp + key * KB + VO * g, Q8 ? vsp + key * (D / 32) + g / (D == 128 ? 2 : 4) : nullptr);
+        }
+      }
+      vl += KT * KB;
+      if constexpr (Q8) vsl += KT * (D / 32);
     };
 
-    const uint32_t kb0 = k0 * KT + warp * S::KEYS;
     if (kb0 < end) {
       load_k(kb0);
       load_v(kb0);
@@ -210,7 +239,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       const uint32_t kb = tile * KT + warp * S::KEYS;
       if (kb >= end) break;
       const bool more = tile + 1 < k1 && kb + KT < end;
-      const bool edge = kb + S::KEYS > L;  // holds drafts or the end: masks apply
+      const bool edge = !inner(kb);  // holds drafts or the end: masks apply
       // ---- S^T = K Q^T
       float s[MB][NB][4];
 #pragma unroll
@@ -225,7 +254,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
             for (int i = 0; i < 2; i++) {
               const uint32_t x = kr[2 * mb + i][k] ^ 0x80808080u;
               const uint32_t sw = k / 4 ? ks[2 * mb + i].y : ks[2 * mb + i].x;
-              const __half2 d = bits_h2(__byte_perm(sw, sw, c >= 2 ? 0x3232 : 0x1010));
+              const __half2 d = bits_h2(__byte_perm(sw, sw, k_half));
               f[i] = q8_pair(__byte_perm(x, 0x64646464u, 0x4140), d);
               f[2 + i] = q8_pair(__byte_perm(x, 0x64646464u, 0x4342), d);
             }
@@ -242,34 +271,40 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       }
       if (more) load_k(kb + KT);
       // ---- weights
-      bool raise = false;
+      if (edge) {
 #pragma unroll
-      for (int mb = 0; mb < MB; mb++)
+        for (int mb = 0; mb < MB; mb++)
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++)
+          for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            float x = s[mb][nb][e] * coef[nb][e & 1];
-            if (edge) {
+            for (int e = 0; e < 4; e++) {
               const uint32_t p = kb + 16 * mb + 8 * (e >> 1) + g, r = 8 * nb + 2 * c + (e & 1);
-              if (p >= end || r >= nrows || !sees(a, b, group_div(a, r0 + r), L, p)) x = -INFINITY;
+              if (p >= end || r >= nrows || !sees(a, b, group_div(a, r0 + r), L, p)) s[mb][nb][e] = -INFINITY;
             }
-            s[mb][nb][e] = x;
-            raise |= x > m[nb][e & 1] + kRaise;
-          }
+      }
+      bool raise = false;
+      float top[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          top[nb][x] = -INFINITY;
+#pragma unroll
+          for (int mb = 0; mb < MB; mb++) top[nb][x] = fmaxf(top[nb][x], fmaxf(s[mb][nb][x], s[mb][nb][2 + x]));
+          top[nb][x] *= coef[nb][x];
+          raise |= top[nb][x] > m[nb][x] + kRaise;
+        }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
           for (int x = 0; x < 2; x++) {
-            float top = m[nb][x];
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++) top = fmaxf(top, fmaxf(s[mb][nb][x], s[mb][nb][2 + x]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float f = top == -INFINITY ? 1.f : ex2(m[nb][x] - top);
-            m[nb][x] = top;
+            float t = fmaxf(m[nb][x], top[nb][x]);
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+            const float f = t == -INFINITY ? 1.f : ex2(m[nb][x] - t);
+            m[nb][x] = t;
             l[nb][x] *= f;
 #pragma unroll
             for (int i = 0; i < KS; i++) o[i][nb][x] *= f, o[i][nb][2 + x] *= f;
@@ -278,13 +313,13 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
       uint32_t ph[MB][NB][2], pl[MB][SPLIT ? NB : 1][2];
 #pragma unroll
       for (int nb = 0; nb < NB; nb++) {
-        const float ref[2] = {(m[nb][0] == -INFINITY ? 0.f : m[nb][0]) - kWeightBias,
-                              (m[nb][1] == -INFINITY ? 0.f : m[nb][1]) - kWeightBias};
+        const float ref[2] = {kWeightBias - (m[nb][0] == -INFINITY ? 0.f : m[nb][0]),
+                              kWeightBias - (m[nb][1] == -INFINITY ? 0.f : m[nb][1])};
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            s[mb][nb][e] = ex2(s[mb][nb][e] - ref[e & 1]);
+            s[mb][nb][e] = ex2(fmaf(s[mb][nb][e], coef[nb][e & 1], ref[e & 1]));
             l[nb][e & 1] += s[mb][nb][e];
           }
 #pragma unroll
@@ -299,8 +334,24 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
           }
         }
       }
+      // what is masked must not reach the sums, 0 * NaN included: V that is not finite (Q8_0: blocks that may
+      // not be, by their scale) counts as 0 here, and is added below for the rows that see it
+      bool wild = false;
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4 * MB; i++) {
+          if constexpr (Q8) {
+            if (wild_scale(vs[i])) vs[i] = 0, wild = true;
+          } else {
+#pragma unroll
+            for (int j = 0; j < VW; j++) {
+              if ((vr[i][j] & 0x7c00u) == 0x7c00u) vr[i][j] &= 0xffff0000u, wild = true;
+              if ((vr[i][j] & 0x7c000000u) == 0x7c000000u) vr[i][j] &= 0x0000ffffu, wild = true;
+            }
+          }
+        }
+      }
       // ---- O^T += V^T P^T
-      bool wild = false;  // a V element of a masked step is not finite
 #pragma unroll
       for (int mb = 0; mb < MB; mb++) {
 #pragma unroll
@@ -311,7 +362,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
           for (int pr = 0; pr < 2; pr++) {
             const int ka = 4 * mb + 2 * pr;
             if constexpr (Q8) {
-              const __half2 d = bits_h2(vs[ka] | (vs[ka + 1] << 16));
+              const __half2 d = bits_h2(__byte_perm(vs[ka], vs[ka + 1], 0x5410));
               const uint32_t x = vr[ka][i / 2], y = vr[ka + 1][i / 2];
               const uint32_t e0 = __byte_perm(x, y, i & 1 ? 0x0602 : 0x0400), e1 = __byte_perm(x, y, i & 1 ? 0x0703 : 0x0501);
               f[2 * pr] = q8_pair((e0 & 0x00ff00ffu) ^ 0x64806480u, d);
@@ -321,15 +372,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
               f[2 * pr + 1] = __byte_perm(vr[ka][i], vr[ka + 1][i], 0x7632);
             }
           }
-          if (edge) {  // what is masked must not reach the sums, 0 * NaN included: see below
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-              const bool w0 = (f[x] & 0x7c00u) == 0x7c00u, w1 = (f[x] & 0x7c000000u) == 0x7c000000u;
-              wild |= w0 || w1;
-              if (w0) f[x] &= 0xffff0000u;
-              if (w1) f[x] &= 0x0000ffffu;
-            }
-          }
 #pragma unroll
           for (int nb = 0; nb < NB; nb++) {
             mma16816(o[i][nb], f, ph[mb][nb][0], ph[mb][nb][1]);
@@ -337,8 +379,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
           }
         }
       }
-      if (edge && __any_sync(0xffffffffu, wild)) {
-        // rare: the elements that were left out above, added for the rows that do see them
+      if (__any_sync(0xffffffffu, wild)) {
         for (int kk = 0; kk < S::KEYS; kk++) {
           const uint64_t key = kb + kk;
           const bool in = key < end;
@@ -359,12 +400,16 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
               for (int y = 0; y < 2; y++) {
                 const uint32_t d = Q8 ? g * (D / 8) + 2 * i + y : 64 * (i / 4) + 8 * g + 2 * (i % 4) + y;
                 float v;
-                if constexpr (Q8)
-                  v = __half2float(__float2half_rn((float)((const int8_t*)vp)[key * D + d] *
-                                                   __half2float(vsp[key * (D / 32) + d / 32])));
-                else
+                bool left_out;
+                if constexpr (Q8) {
+                  const __half sc = vsp[key * (D / 32) + d / 32];
+                  left_out = wild_scale(__half_as_ushort(sc));
+                  v = __half2float(__float2half_rn((float)((const int8_t*)vp)[key * D + d] * __half2float(sc)));
+                } else {
                   v = __half2float(((const __half*)vp)[key * D + d]);
-                if (!(fabsf(v) < INFINITY)) {
+                  left_out = !(fabsf(v) < INFINITY);
+                }
+                if (left_out) {
 #pragma unroll
                   for (int x = 0; x < 2; x++)
                     if (p[x] != 0.f) o[i][nb][2 * y + x] += p[x] * v;
