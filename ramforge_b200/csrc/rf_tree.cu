@@ -64,10 +64,27 @@ __device__ __forceinline__ uint32_t q8_pair(uint32_t biased, __half2 d) {
 // A block whose largest code could leave f16, or whose scale is no number.
 __device__ __forceinline__ bool wild_scale(uint32_t half_bits) { return (half_bits & 0x7fffu) > 0x6007u; }  // 515.5
 
-// Shapes of one step of a warp over a cache of type Q8 and head dimension D.
-template <bool Q8, int D>
+// The four codes of a word without those whose product with the scale is not finite.
+__device__ __noinline__ uint32_t finite_codes(uint32_t w, uint32_t half_bits) {
+  const float d = __half2float(__ushort_as_half((unsigned short)half_bits));
+#pragma unroll 1
+  for (int i = 0; i < 32; i += 8) {
+    const float v = __half2float(__float2half_rn((float)(int8_t)(w >> i) * d));
+    if (!(fabsf(v) < INFINITY)) w &= ~(0xffu << i);
+  }
+  return w;
+}
+
+// Shapes of one step of a warp over a cache of type Q8, head dimension D
+// and NB blocks of 8 query rows, with the CTAs of an SM.  Q8_0 is bound by the decode's
+// instructions, so it wants more warps: one row over 131072 positions of 128 dimensions takes
+// 59 us with 16 keys a step and four CTAs, 64 with 32 and three, 87 with 32 and four (spills);
+// of 64 dimensions 35 with 32 and four, 40 with 16 and four.  f16 is bound by HBM: 87 us
+// (0.94 of the copy rate) with three CTAs, 96 with four.
+template <bool Q8, int D, int NB>
 struct Step {
-  static constexpr int MB = Q8 ? 2 : 1;                    // 16-key blocks
+  static constexpr int MB = !Q8 || (D == 128 && NB == 1) ? 1 : 2;  // 16-key blocks
+  static constexpr int CTAS = NB == 2 ? 2 : Q8 ? 4 : 3;
   static constexpr int KEYS = 16 * MB;
   static constexpr int KW = Q8 ? D / 16 : D / 8;           // 32-bit words of one key's K in a lane
   static constexpr int VW = Q8 ? D / 32 : D / 16;          // ... of one key's V
@@ -79,9 +96,9 @@ constexpr int kRowWarps = 4;
 // f32 and bf16 rows are first scaled by a power of two to a largest magnitude in [1, 2),
 // which f16 holds; f32 keeps a second f16 term.  *exp2 is the scale that was taken out.
 template <class T, bool Q8, int D, bool SPLIT>
-__device__ __forceinline__ void load_query(const T* row, bool live, uint32_t c, uint32_t (&hi)[Step<Q8, D>::KS][2],
-                                           uint32_t (&lo)[SPLIT ? Step<Q8, D>::KS : 1][2], float* exp2) {
-  constexpr int KS = Step<Q8, D>::KS;
+__device__ __forceinline__ void load_query(const T* row, bool live, uint32_t c, uint32_t (&hi)[D / 16][2],
+                                           uint32_t (&lo)[SPLIT ? D / 16 : 1][2], float* exp2) {
+  constexpr int KS = D / 16;
   float v[KS][4];
   float top = 0.f;
 #pragma unroll
@@ -119,15 +136,19 @@ __device__ __forceinline__ void load_query(const T* row, bool live, uint32_t c, 
 }
 
 template <class T, bool Q8, int D, int NB>
-__global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_kernel(TreeArgs a, float* __restrict__ part) {
-  using S = Step<Q8, D>;
+__global__ void __launch_bounds__(32 * kRowWarps, Step<Q8, D, NB>::CTAS)
+    tree_rows_kernel(TreeArgs a, float* __restrict__ part) {
+  using S = Step<Q8, D, NB>;
   constexpr bool SPLIT = std::is_same<T, float>::value;
   constexpr int ROWS = 8 * NB, KT = S::KEYS * kRowWarps, MB = S::MB, KS = S::KS, KW = S::KW, VW = S::VW;
   __shared__ __align__(16) float s_o[kRowWarps][ROWS][D];
   __shared__ float s_m[kRowWarps][ROWS], s_l[kRowWarps][ROWS];
+  __shared__ int s_wild;  // a V element of a draft is not finite
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const uint32_t k_half = c >= 2 ? 0x3232 : 0x1010;  // which of a word's two scales the lane's dimensions have
   griddep_launch();
+  if (threadIdx.x == 0) s_wild = 0;
+  __syncthreads();
   const uint32_t G = a.group;
   Walk<KT, ROWS> walk(a);
   Segment sg;
@@ -334,14 +355,19 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
           }
         }
       }
-      // what is masked must not reach the sums, 0 * NaN included: V that is not finite (Q8_0: blocks that may
-      // not be, by their scale) counts as 0 here, and is added below for the rows that see it
-      bool wild = false;
+      // what is masked must not reach the sums, 0 * NaN included: V elements that are not finite count
+      // as 0 here, and the rows that see them get them when the results are written
       if (edge) {
+        bool wild = false;
 #pragma unroll
         for (int i = 0; i < 4 * MB; i++) {
           if constexpr (Q8) {
-            if (wild_scale(vs[i])) vs[i] = 0, wild = true;
+            if (wild_scale(vs[i])) {
+              wild = true;
+#pragma unroll
+              for (int j = 0; j < VW; j++) vr[i][j] = finite_codes(vr[i][j], vs[i]);
+              if ((vs[i] & 0x7c00u) == 0x7c00u) vs[i] = 0;
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < VW; j++) {
@@ -350,6 +376,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
             }
           }
         }
+        if (wild) s_wild = 1;
       }
       // ---- O^T += V^T P^T
 #pragma unroll
@@ -376,45 +403,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
           for (int nb = 0; nb < NB; nb++) {
             mma16816(o[i][nb], f, ph[mb][nb][0], ph[mb][nb][1]);
             if constexpr (SPLIT) mma16816(o[i][nb], f, pl[mb][nb][0], pl[mb][nb][1]);
-          }
-        }
-      }
-      if (__any_sync(0xffffffffu, wild)) {
-        for (int kk = 0; kk < S::KEYS; kk++) {
-          const uint64_t key = kb + kk;
-          const bool in = key < end;
-#pragma unroll
-          for (int nb = 0; nb < NB; nb++) {
-            float p[2] = {0.f, 0.f};
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const float x = __shfl_sync(0xffffffffu, s[mb][nb][e], 4 * (kk & 7) + c);
-                if (kk / 16 == mb && ((kk >> 3) & 1) == (e >> 1)) p[e & 1] = x;
-              }
-            if (!in) continue;
-#pragma unroll
-            for (int i = 0; i < KS; i++)
-#pragma unroll
-              for (int y = 0; y < 2; y++) {
-                const uint32_t d = Q8 ? g * (D / 8) + 2 * i + y : 64 * (i / 4) + 8 * g + 2 * (i % 4) + y;
-                float v;
-                bool left_out;
-                if constexpr (Q8) {
-                  const __half sc = vsp[key * (D / 32) + d / 32];
-                  left_out = wild_scale(__half_as_ushort(sc));
-                  v = __half2float(__float2half_rn((float)((const int8_t*)vp)[key * D + d] * __half2float(sc)));
-                } else {
-                  v = __half2float(((const __half*)vp)[key * D + d]);
-                  left_out = !(fabsf(v) < INFINITY);
-                }
-                if (left_out) {
-#pragma unroll
-                  for (int x = 0; x < 2; x++)
-                    if (p[x] != 0.f) o[i][nb][2 * y + x] += p[x] * v;
-                }
-              }
           }
         }
       }
@@ -455,6 +443,23 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
         den += s_l[i][r] * f;
         num.x += v.x * f, num.y += v.y * f, num.z += v.z * f, num.w += v.w * f;
       }
+      if (s_wild) {
+        const uint32_t t = group_div(a, r0 + r);
+        for (uint32_t p = max(L, k0 * KT); p < min(end, k1 * KT); p++) {
+          if (!sees(a, b, t, L, p)) continue;
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint64_t at = (uint64_t)p * D + d + i;
+            if constexpr (Q8)
+              v[i] = __half2float(__float2half_rn((float)((const int8_t*)vp)[at] * __half2float(vsp[at / 32])));
+            else
+              v[i] = __half2float(((const __half*)vp)[at]);
+            if (fabsf(v[i]) < INFINITY) v[i] = 0.f;
+          }
+          num.x += v[0], num.y += v[1], num.z += v[2], num.w += v[3];
+        }
+      }
       if (whole) {
         const uint32_t rr = r0 + r;
         const uint32_t t = group_div(a, rr);
@@ -472,8 +477,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, NB == 1 ? 3 : 2) tree_rows_ker
 
 template <class T, bool Q8, int D, int NB>
 int run_rows(cudaStream_t st, const TreeArgs& a) {
-  constexpr int ROWS = 8 * NB, KT = Step<Q8, D>::KEYS * kRowWarps;
-  const uint32_t ctas = (uint32_t)num_sms() * (NB == 1 ? 3 : 2);
+  constexpr int ROWS = 8 * NB, KT = Step<Q8, D, NB>::KEYS * kRowWarps;
+  const uint32_t ctas = (uint32_t)num_sms() * Step<Q8, D, NB>::CTAS;
   void* part = nullptr;
   RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(ROWS, D) * sizeof(float), st));
   cudaError_t e = launch_k(Launch{st, false}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
