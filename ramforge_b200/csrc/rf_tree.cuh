@@ -230,6 +230,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float
   const uint32_t b = bh / a.c.n_kv_heads, h = bh - b * a.c.n_kv_heads;
   const uint32_t r = r0 + rx, t = group_div(a, r), hq = h * a.group + (r - t * a.group), d0 = blockIdx.y * DPC + dx * 4;
   T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d0;
+  griddep_launch();
+  // the lengths were there before the first kernel began; every CTA waits for it before it ends, so
+  // that whoever waits for this kernel has waited for both
   uint32_t L, n;
   seq_lengths(a, b, &L, &n);
   if (t < a.n_tokens && t >= n && cx == 0) {
@@ -238,14 +241,14 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float
 #pragma unroll
       for (int i = 0; i < 4; i++) act_put(out + 32 * x + i, 0.f);
   }
-  if (r0 >= n * a.group) return;
   uint64_t before;
   const Ranges ranges(Sp::total(a, b, &before), grid);
   const uint32_t tiles = Sp::tiles(L, n);
   const uint64_t u0 = before + ((uint64_t)h * Sp::row_tiles(a, n) + r0 / ROWS) * tiles;
-  const uint32_t c0 = ranges.holder(u0), c1 = ranges.holder(u0 + tiles - 1);
-  if (c0 == c1) return;  // finished by its CTA
+  const bool mine = r0 < n * a.group;
+  const uint32_t c0 = mine ? ranges.holder(u0) : 0, c1 = mine ? ranges.holder(u0 + tiles - 1) : 0;
   griddep_wait();
+  if (c0 == c1) return;  // no rows, or finished by its CTA
   const uint32_t rl = r % ROWS;
   float M = -INFINITY, den = 0.f;
   float4 acc[X];

@@ -136,6 +136,10 @@ __device__ __forceinline__ uint32_t sw128_offset(uint32_t r, uint32_t c) {
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+// 16 bytes from global to shared memory, asynchronously; the last 16 - bytes as zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, uint64_t src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void st_shared8(uint32_t addr, uint32_t x, uint32_t y) {
   asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
 }
@@ -315,13 +319,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t q_smem = tc_smem_u32(tsm), slots = q_smem + S::QBYTES, raws = slots + S::NSLOT * S::TILE;
   auto slot_addr = [&](uint32_t s) { return slots + s * S::TILE; };
-  griddep_launch();
-  Walk<TK, S::ROWS> walk(a);
-  if (!walk.left) return;
-  if (q_smem & 1023u) {  // the swizzle is a function of the address
-    if (tid == 0) atomicOr(a.err, kVerifyTimeout);
-    return;
-  }
+  // (all that is above the wait overlaps the kernel before)
   if (warp == 1) tc_tmem_alloc(tc_smem_u32(&B.tmem), 512);
   if (tid == 0) {
     for (int i = 0; i < S::NSLOT; i++) {
@@ -344,6 +342,11 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     B.stop = B.wild = 0;
     tc_fence_barrier_init();
   }
+  griddep_launch();
+  griddep_wait();
+  Walk<TK, S::ROWS> walk(a);
+  Segment sg;
+  bool work_left = walk.next(a, &sg);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -354,7 +357,6 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bar(bar, parity, stop, a.err); };
   bool ok = true;
   const uint32_t G = a.group;
-  Segment sg;
 
   if (warp == 0) {
     // ---- loads ------------------------------------------------------------------------
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       uint64_t* free = Q8 ? B.raw_free : B.free;
       Ring<N> ring;
       uint32_t issued = 0;
-      while (walk.next(a, &sg)) {
+      for (; work_left; work_left = walk.next(a, &sg)) {
         const uint32_t nt = sg.k1 - sg.k0, plane = sg.b * a.c.n_kv_heads + sg.h;
         for (uint32_t e = 0; e < 2 * nt; e++) {
           bool is_v;
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         tc_commit(tc_smem_u32(&B.pv_done[g][h]));
       }
     };
-    while (walk.next(a, &sg)) {
+    for (; work_left; work_left = walk.next(a, &sg)) {
       const uint32_t nt = uniform(sg.k1 - sg.k0), k0 = uniform(sg.k0), hist = uniform(sg.hist);
       constexpr uint32_t step = RT == 1 ? 2 : 1;
       const bool work = RT == 1 ? g < nt : g == 0 || uniform(sg.drafts * G - sg.rt * S::ROWS) > TK;
@@ -503,7 +505,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     // ---- f16 V tiles with drafts or the end: rows past the end 0, drafts' rows finite ------
     if constexpr (!Q8) {
       Ring<S::NSLOT> ring;
-      while (walk.next(a, &sg)) {
+      for (; work_left; work_left = walk.next(a, &sg)) {
         const uint32_t nt = sg.k1 - sg.k0;
         for (uint32_t e = 0; e < 2 * nt; e++) {
           bool is_v;
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     constexpr uint32_t CPR = D * sizeof(T) / 16;  // 16-byte pieces of a row of activations
     constexpr uint32_t RPI = 32 / CPR;            // rows a warp moves at a time
     uint32_t count = 0;                           // tiles of this group so far
-    while (walk.next(a, &sg)) {
+    for (; work_left; work_left = walk.next(a, &sg)) {
       const uint32_t nt = sg.k1 - sg.k0, n_rows = sg.drafts * G;
       const uint32_t r_base = sg.rt * S::ROWS + (RT == 2 ? g * TK : 0) + w32;  // the warp's first row
       const uint32_t r = r_base + lane;
@@ -556,28 +558,38 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         const uint32_t tx = group_div(a, x);
         return ((uint64_t)sg.b * a.n_tokens + tx) * stride + (uint64_t)(sg.h * G + (x - tx * G)) * D;
       };
-      // queries, a few rows of the warp at a time: f32 and bf16 rows are scaled by a power of
-      // two to a largest magnitude in [1, 2)
+      // queries: the warp moves RPI of its rows at a time.  f16 rows go straight to shared memory; f32
+      // and bf16 rows are scaled by a power of two to a largest magnitude in [1, 4).  Small code: what
+      // runs once is bound by the fetch of its instructions.
       float coef = a.scale * 1.44269504f;
       {
-        constexpr int BATCH = 32 / RPI < 8 ? 32 / RPI : 8;
         constexpr int PIECE = 16 / sizeof(T);
         const uint32_t sub = lane / CPR, c = lane % CPR;
+        const uint64_t mine_at = live ? (uint64_t)((const T*)a.q + row_at(r, a.q_stride)) : 0;
         float up_mine = 1.f;
-#pragma unroll 1
-        for (int b0 = 0; b0 < (int)(32 / RPI); b0 += BATCH) {
-          uint4 u[BATCH];
-#pragma unroll
-          for (int i = 0; i < BATCH; i++) {
-            const uint32_t x = r_base + (b0 + i) * RPI + sub;
-            u[i] = x < n_rows ? __ldg(reinterpret_cast<const uint4*>((const T*)a.q + row_at(x, a.q_stride)) + c)
-                              : make_uint4(0, 0, 0, 0);
+        if constexpr (std::is_same<T, __half>::value) {
+          if (RT == 2 || g == 0) {
+#pragma unroll 4
+            for (uint32_t i = 0; i < 32 / RPI; i++) {
+              const uint32_t x = i * RPI + sub;
+              const uint64_t at = __shfl_sync(~0u, mine_at, x);
+              cp_async16(q_tile + sw128_offset(w32 + x, c), at ? at + 16 * c : (uint64_t)a.q, at ? 16 : 0);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
           }
+        } else {
+#pragma unroll 1
+          for (uint32_t b0 = 0; b0 < 32 / RPI; b0 += 8) {
+            uint4 u[8];
 #pragma unroll
-          for (int i = 0; i < BATCH; i++) {
-            float v[PIECE];
-            act_unpack<T>(u[i], v);
-            if constexpr (!std::is_same<T, __half>::value) {
+            for (uint32_t i = 0; i < 8; i++) {
+              const uint64_t at = __shfl_sync(~0u, mine_at, (b0 + i) * RPI + sub);
+              u[i] = at ? __ldg(reinterpret_cast<const uint4*>(at) + c) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+              float v[PIECE];
+              act_unpack<T>(u[i], v);
               float top = 0.f;
 #pragma unroll
               for (int j = 0; j < PIECE; j++) top = fmaxf(top, fabsf(v[j]));
@@ -588,18 +600,18 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
 #pragma unroll
               for (int j = 0; j < PIECE; j++) v[j] *= down;
               up = __shfl_sync(~0u, up, (lane % RPI) * CPR);
-              if ((int)(lane / RPI) == b0 + i) up_mine = up;
-            }
-            if (RT == 2 || g == 0) {
-              const uint32_t x = w32 + (b0 + i) * RPI + sub;
-              if constexpr (SPLIT) {  // 4 elements: half of a 16-byte piece of f16
-                const uint32_t at = sw128_offset(x, c / 2) + 8 * (c & 1);
-                const uint32_t h0 = pack_h2(v[0], v[1]), h1 = pack_h2(v[2], v[3]);
-                st_shared8(q_tile + at, h0, h1);
-                st_shared8(q_tile + S::TILE + at, pack_h2_rest(v[0], v[1], h0), pack_h2_rest(v[2], v[3], h1));
-              } else {
-                st_shared16(q_tile + sw128_offset(x, c), make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]),
-                                                                    pack_h2(v[4], v[5]), pack_h2(v[6], v[7])));
+              if (lane / RPI == b0 + i) up_mine = up;
+              if (RT == 2 || g == 0) {
+                const uint32_t x = w32 + (b0 + i) * RPI + sub;
+                if constexpr (SPLIT) {  // 4 elements: half of a 16-byte piece of f16
+                  const uint32_t at = sw128_offset(x, c / 2) + 8 * (c & 1);
+                  const uint32_t h0 = pack_h2(v[0], v[1]), h1 = pack_h2(v[2], v[3]);
+                  st_shared8(q_tile + at, h0, h1);
+                  st_shared8(q_tile + S::TILE + at, pack_h2_rest(v[0], v[1], h0), pack_h2_rest(v[2], v[3], h1));
+                } else {
+                  st_shared16(q_tile + sw128_offset(x, c), make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]),
+                                                                      pack_h2(v[4], v[5]), pack_h2(v[6], v[7])));
+                }
               }
             }
           }
@@ -788,7 +800,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       const uint32_t key = tid - 384;
       Ring<S::NRAW> rr;
       Ring<S::NSLOT> ring;
-      while (walk.next(a, &sg)) {
+      for (; work_left; work_left = walk.next(a, &sg)) {
         const uint32_t nt = sg.k1 - sg.k0;
         const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
         // scales of the e-th tile's key; 0 past the end, so that those rows become 0
@@ -918,7 +930,7 @@ int run(cudaStream_t st, const TreeArgs& a) {
   const uint32_t ctas = (uint32_t)num_sms();
   void* part = nullptr;
   RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(S::ROWS, D) * sizeof(float), st));
-  cudaError_t e = launch_k(Launch{st, false}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
+  cudaError_t e = launch_k(Launch{st, true}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
   if (e == cudaSuccess)
     e = launch_merge<T, D, TK, S::ROWS>(st, a, (const float*)part, ctas);
   const cudaError_t f = cudaFreeAsync(part, st);
