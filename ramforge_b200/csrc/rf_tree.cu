@@ -485,7 +485,7 @@ int run_rows(cudaStream_t st, const TreeArgs& a) {
   cudaError_t e = launch_k(Launch{st, true}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
                            (float*)part);
   if (e == cudaSuccess)
-    e = launch_merge<T, D, KT, ROWS>(st, a, (const float*)part, ctas);
+    e = launch_merge<T, D, KT, ROWS>(st, a, (const float*)part, ctas, cudaSharedmemCarveoutDefault);
   const cudaError_t f = cudaFreeAsync(part, st);
   RF_CUDA(e);
   RF_CUDA(f);

@@ -60,51 +60,94 @@ __device__ __forceinline__ void pow2_scale(float top, float* down, float* up) {
 // ---------------------------------------------------------------------------
 // The work split.  A unit is (sequence b, KV head h, row tile rt): up to ROWS of the
 // n_b * G query rows (G query heads share a KV head; row r = token r / G, head r % G)
-// against all its keys, in tiles of KT.  All tiles of all units, in that order, are
-// cut into equal contiguous ranges, one a CTA (of as many CTAs as there are tiles, at
-// most gridDim.x), whatever the histories: the lengths are read on the device.  A unit that lies in one CTA is finished there; the
-// others leave partial results that tree_merge_kernel adds in order of the keys, so
-// results do not depend on timing.  A CTA leaves at most two: slot 0 for the unit its
-// range starts inside of, slot 1 for the one it ends inside of.
+// against all its keys, in tiles of KT.  The lengths are read on the device, and every warp
+// that needs the plan computes it.  Two ways to give the units to the CTAs:
+//
+//   by quota   each CTA gets at most `quota` tiles of one unit: the smallest quota for which the
+//              grid has CTAs enough.  Nobody changes unit, which costs a CTA about 4 us.
+//   in a row   all tiles of all units, in order, in equal ranges: the best balance, at the cost
+//              of CTAs that end one unit and begin another.  For a quota that would be over
+//              the even share by more than kSwitch tiles (or more units than CTAs).
+//
+// (16 tokens over 4095 Q8_0 positions, 32/8 heads: 20.0 us in a row, 15.4 by quota; 256 tokens over
+// 32768, 64/8 heads: 129 tiles a CTA by quota, 112 in a row.)  A unit that lies in one CTA is
+// finished there; the others leave partial results that tree_merge_kernel adds in order of
+// the keys, so results do not depend on timing.  A CTA leaves at most two: slot 0 for the unit
+// its tiles start inside of, slot 1 for the one they end inside of.
 // ---------------------------------------------------------------------------
+constexpr uint32_t kSwitch = 3;
+
+// x / y, on the short path where both fit 32 bits.
+__device__ __forceinline__ uint32_t div_u(uint64_t x, uint64_t y) {
+  return (x | y) >> 32 ? (uint32_t)(x / y) : (uint32_t)x / (uint32_t)y;
+}
+
+// A run of consecutive key tiles of one unit: what a CTA works on at a time.
+struct Segment {
+  uint32_t b, h, rt;          // sequence, KV head, row tile
+  uint32_t k0, k1, tiles;     // the run [k0, k1) of the unit's tiles
+  uint32_t hist, drafts, end; // lengths of the sequence; end = hist + drafts
+  __device__ bool whole() const { return k0 == 0 && k1 == tiles; }
+};
+
 template <int KT, int ROWS>
-struct Split {
+struct Plan {
+  uint64_t all;         // tiles of all units
+  uint32_t quota;       // most tiles of a CTA; 0: in a row
+  uint32_t ctas;        // in a row: CTAs with work; the first `more` take `each` + 1 tiles, the others `each`
+  uint64_t each, more;
+
   static __device__ __forceinline__ uint32_t tiles(uint32_t L, uint32_t n) { return n ? (L + n + KT - 1) / KT : 0; }
-  static __device__ __forceinline__ uint32_t row_tiles(const TreeArgs& a, uint32_t n) {
-    return (n * a.group + ROWS - 1) / ROWS;
+  static __device__ __forceinline__ uint32_t units(const TreeArgs& a, uint32_t n) {
+    return (n * a.group + ROWS - 1) / ROWS * a.c.n_kv_heads;
   }
-  static __device__ __forceinline__ uint64_t work(const TreeArgs& a, uint32_t b) {
+  // What sequence b takes: tiles (q = 0), or CTAs at a quota of q.
+  static __device__ __forceinline__ uint64_t share(const TreeArgs& a, uint32_t b, uint32_t q) {
     if (b >= a.n_seqs) return 0;
     uint32_t L, n;
     seq_lengths(a, b, &L, &n);
-    return (uint64_t)tiles(L, n) * row_tiles(a, n) * a.c.n_kv_heads;
+    const uint32_t t = tiles(L, n);
+    return (uint64_t)units(a, n) * (q ? (t + q - 1) / q : t);
   }
-  // Whole warp: the tiles of all sequences, and (through *before) those of the sequences before b.
-  static __device__ __forceinline__ uint64_t total(const TreeArgs& a, uint32_t b, uint64_t* before) {
-    *before = 0;
-    if (a.n_seqs == 1) return work(a, 0);
-    uint64_t t = 0, p = 0;
-    for (uint32_t i = threadIdx.x & 31; i < a.n_seqs; i += 32) {
-      const uint64_t w = work(a, i);
-      t += w;
-      if (i < b) p += w;
-    }
+  // Whole warp: the shares of the sequences before `limit`.
+  static __device__ __forceinline__ uint64_t sum(const TreeArgs& a, uint32_t limit, uint32_t q) {
+    if (limit <= 1) return limit ? share(a, 0, q) : 0;
+    uint64_t t = 0;
+    for (uint32_t i = threadIdx.x & 31; i < limit; i += 32) t += share(a, i, q);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      t += __shfl_xor_sync(0xffffffffu, t, o);
-      p += __shfl_xor_sync(0xffffffffu, p, o);
-    }
-    *before = p;
+    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     return t;
   }
-  // Whole warp: the sequence that holds tile w, and w's offset in it.
-  static __device__ __forceinline__ uint32_t locate(const TreeArgs& a, uint64_t w, uint64_t* offset) {
+  // Whole warp.
+  __device__ __forceinline__ Plan(const TreeArgs& a, uint32_t grid) : each(0), more(0) {
+    all = sum(a, a.n_seqs, 0);
+    ctas = all < grid ? (uint32_t)all : grid;
+    quota = 0;
+    if (!ctas) return;
+    each = div_u(all, ctas);
+    more = all - each * ctas;
+    const uint64_t least = each + (more ? 1 : 0);
+    if (least >> 31) return;
+    for (uint32_t q = (uint32_t)least; q <= least + kSwitch; q++)
+      if (sum(a, a.n_seqs, q) <= grid) {
+        quota = q;
+        return;
+      }
+  }
+  __device__ __forceinline__ uint64_t begin(uint32_t c) const { return each * c + min((uint64_t)c, more); }
+  // In a row: the CTA that holds a tile.
+  __device__ __forceinline__ uint32_t holder(uint64_t tile) const {
+    const uint64_t wide = more * (each + 1);
+    return tile < wide ? div_u(tile, each + 1) : (uint32_t)more + div_u(tile - wide, each);
+  }
+  // Whole warp: the sequence whose share holds w (w below the sum of all), and w's offset in it.
+  static __device__ __forceinline__ uint32_t locate(const TreeArgs& a, uint64_t w, uint32_t q, uint64_t* offset) {
     const uint32_t lane = threadIdx.x & 31;
     *offset = w;
-    if (a.n_seqs == 1) return 0;
+    if (a.n_seqs == 1) return w < share(a, 0, q) ? 0 : 1;
     uint64_t acc = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 32) {
-      uint64_t s = work(a, base + lane);
+      uint64_t s = share(a, base + lane, q);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint64_t up = __shfl_up_sync(0xffffffffu, s, o);
@@ -119,74 +162,57 @@ struct Split {
       }
       acc += __shfl_sync(0xffffffffu, s, 31);
     }
-    *offset = 0;
     return a.n_seqs;
   }
-};
-
-// Equal ranges of `all` tiles: the first `more` CTAs take `each` + 1, the others `each`.
-struct Ranges {
-  uint64_t all, each, more;
-  uint32_t ctas;  // as many as there are tiles, at most the grid
-  __device__ __forceinline__ Ranges(uint64_t all_, uint32_t grid) : all(all_), each(0), more(0) {
-    ctas = all < grid ? (uint32_t)all : grid;
-    if (!ctas) return;
-    each = all >> 32 ? all / ctas : (uint32_t)all / ctas;
-    more = all - each * ctas;
-  }
-  __device__ __forceinline__ uint64_t begin(uint32_t c) const { return each * c + min((uint64_t)c, more); }
-  __device__ __forceinline__ uint32_t holder(uint64_t tile) const {  // the CTA of a tile
-    const uint64_t wide = more * (each + 1);
-    return tile < wide ? div(tile, each + 1) : (uint32_t)more + div(tile - wide, each);
-  }
-  static __device__ __forceinline__ uint32_t div(uint64_t x, uint64_t y) {
-    return (x | y) >> 32 ? (uint32_t)(x / y) : (uint32_t)x / (uint32_t)y;
-  }
-};
-
-// A run of consecutive key tiles of one unit: what a CTA works on at a time.
-struct Segment {
-  uint32_t b, h, rt;          // sequence, KV head, row tile
-  uint32_t k0, k1, tiles;     // the run [k0, k1) of the unit's tiles
-  uint32_t hist, drafts, end; // lengths of the sequence; end = hist + drafts
-  __device__ bool whole() const { return k0 == 0 && k1 == tiles; }
 };
 
 // The segments of this CTA, in order.
 template <int KT, int ROWS>
 struct Walk {
-  using Sp = Split<KT, ROWS>;
-  uint64_t left, rem;  // tiles left, and the next one's offset in sequence b
-  uint32_t b;
+  using P = Plan<KT, ROWS>;
+  uint64_t left, rem;  // tiles left (by quota: 1 for the CTA's only segment), and the next one's offset in sequence b
+  uint32_t b, quota;
   // Whole warp.
-  __device__ __forceinline__ Walk(const TreeArgs& a) {
-    uint64_t ignore;
-    const Ranges r(Sp::total(a, 0, &ignore), gridDim.x);
-    left = 0;
-    if (blockIdx.x >= r.ctas) return;
-    const uint64_t w = r.begin(blockIdx.x);
-    left = r.begin(blockIdx.x + 1) - w;
-    b = Sp::locate(a, w, &rem);
+  __device__ __forceinline__ Walk(const TreeArgs& a) : left(0), rem(0), b(0) {
+    const P p(a, gridDim.x);
+    quota = p.quota;
+    if (quota) {
+      b = P::locate(a, blockIdx.x, quota, &rem);
+      left = b < a.n_seqs;
+    } else if (blockIdx.x < p.ctas) {
+      const uint64_t w = p.begin(blockIdx.x);
+      left = p.begin(blockIdx.x + 1) - w;
+      b = P::locate(a, w, 0, &rem);
+    }
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, Segment* s) {
     if (!left) return false;
     uint32_t L, n;
     seq_lengths(a, b, &L, &n);
-    uint32_t tiles = Sp::tiles(L, n), rts = Sp::row_tiles(a, n);
-    while (rem == (uint64_t)tiles * rts * a.c.n_kv_heads) {  // past this sequence (or it has no work)
-      b++;
-      rem = 0;
-      seq_lengths(a, b, &L, &n);
-      tiles = Sp::tiles(L, n), rts = Sp::row_tiles(a, n);
+    uint32_t tiles = P::tiles(L, n), units = P::units(a, n);
+    uint32_t unit;
+    if (quota) {
+      const uint32_t parts = (tiles + quota - 1) / quota, part = (uint32_t)rem % parts;
+      unit = (uint32_t)rem / parts;
+      s->k0 = (uint32_t)((uint64_t)tiles * part / parts), s->k1 = (uint32_t)((uint64_t)tiles * (part + 1) / parts);
+      left = 0;
+    } else {
+      while (rem == (uint64_t)tiles * units) {  // past this sequence (or it has no work)
+        b++;
+        rem = 0;
+        seq_lengths(a, b, &L, &n);
+        tiles = P::tiles(L, n), units = P::units(a, n);
+      }
+      unit = div_u(rem, tiles);
+      s->k0 = (uint32_t)(rem - (uint64_t)unit * tiles);
+      s->k1 = (uint32_t)min((uint64_t)tiles, s->k0 + left);
+      left -= s->k1 - s->k0;
+      rem += s->k1 - s->k0;
     }
-    const uint32_t unit = Ranges::div(rem, tiles);
+    const uint32_t rts = units / a.c.n_kv_heads;
     s->b = b, s->h = unit / rts, s->rt = unit - s->h * rts;
-    s->k0 = (uint32_t)(rem - (uint64_t)unit * tiles);
-    s->k1 = (uint32_t)min((uint64_t)tiles, s->k0 + left);
     s->tiles = tiles;
     s->hist = L, s->drafts = n, s->end = L + n;
-    left -= s->k1 - s->k0;
-    rem += s->k1 - s->k0;
     return true;
   }
 };
@@ -220,7 +246,6 @@ constexpr float kRaise = 8.f, kWeightBias = 7.f;
 // ---------------------------------------------------------------------------
 template <class T, int D, int KT, int ROWS, int DPC>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
-  using Sp = Split<KT, ROWS>;
   constexpr int X = DPC / 32, kAhead = X == 1 ? 6 : 3;
   __shared__ float4 s_o[4][64];
   __shared__ float2 s_ml[4][8];
@@ -241,12 +266,14 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float
 #pragma unroll
       for (int i = 0; i < 4; i++) act_put(out + 32 * x + i, 0.f);
   }
-  uint64_t before;
-  const Ranges ranges(Sp::total(a, b, &before), grid);
-  const uint32_t tiles = Sp::tiles(L, n);
-  const uint64_t u0 = before + ((uint64_t)h * Sp::row_tiles(a, n) + r0 / ROWS) * tiles;
-  const bool mine = r0 < n * a.group;
-  const uint32_t c0 = mine ? ranges.holder(u0) : 0, c1 = mine ? ranges.holder(u0 + tiles - 1) : 0;
+  const Plan<KT, ROWS> plan(a, grid);
+  const uint32_t tiles = plan.tiles(L, n), parts = plan.quota ? (tiles + plan.quota - 1) / plan.quota : tiles;
+  const uint64_t u0 = plan.sum(a, b, plan.quota) + ((uint64_t)h * (plan.units(a, n) / a.c.n_kv_heads) + r0 / ROWS) * parts;
+  uint32_t c0 = 0, c1 = 0;  // the CTAs that shared the unit
+  if (r0 < n * a.group) {
+    c0 = plan.quota ? (uint32_t)u0 : plan.holder(u0);
+    c1 = plan.quota ? (uint32_t)u0 + parts - 1 : plan.holder(u0 + tiles - 1);
+  }
   griddep_wait();
   if (c0 == c1) return;  // no rows, or finished by its CTA
   const uint32_t rl = r % ROWS;
@@ -317,12 +344,15 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float
     }
   }
 }
+// `carveout`: the first kernel's share of shared memory, kept so that the SMs need not change it between the two.
 template <class T, int D, int KT, int ROWS>
-cudaError_t launch_merge(cudaStream_t st, const TreeArgs& a, const float* part, uint32_t grid) {
+cudaError_t launch_merge(cudaStream_t st, const TreeArgs& a, const float* part, uint32_t grid, int carveout) {
   const uint32_t blocks = a.n_seqs * a.c.n_kv_heads * ((a.n_tokens * a.group + 7) / 8);
-  if (blocks > 2 * (uint32_t)num_sms())
-    return launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS, D>, dim3(blocks), dim3(256), 0, a, part, grid);
-  return launch_k(Launch{st, true}, tree_merge_kernel<T, D, KT, ROWS, 32>, dim3(blocks, D / 32), dim3(256), 0, a, part, grid);
+  const bool many = blocks > 2 * (uint32_t)num_sms();
+  auto* k = many ? tree_merge_kernel<T, D, KT, ROWS, D> : tree_merge_kernel<T, D, KT, ROWS, 32>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, carveout);
+  if (e != cudaSuccess) return e;
+  return launch_k(Launch{st, true}, k, dim3(blocks, many ? 1 : D / 32), dim3(256), 0, a, part, grid);
 }
 
 // Scratch of one call: allocated in stream order from a pool of this library's own that keeps

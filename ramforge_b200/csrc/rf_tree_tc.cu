@@ -80,6 +80,16 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t* r) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
+      "}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
 // The loads before are complete; the registers pass through so that no use moves above the wait.
 template <int N>
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[N]) {
@@ -723,23 +733,23 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         constexpr uint32_t DIMS = RT == 1 ? D / 2 : D;
         const uint32_t d0 = RT == 1 ? g * DIMS : 0;
 #pragma unroll 1
-        for (uint32_t d = d0; d < d0 + DIMS; d += 32) {
-          uint32_t o[32];
-          float v[32];
-          tmem_ld_32(o_col(RT == 1 ? 0 : g) + lanes + d, o);
+        for (uint32_t d = d0; d < d0 + DIMS; d += 16) {  // rolled: this code runs from a cold instruction cache
+          uint32_t o[16];
+          float v[16];
+          tmem_ld_16(o_col(RT == 1 ? 0 : g) + lanes + d, o);
           tmem_wait_ld(o);
 #pragma unroll
-          for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * f0;
+          for (int i = 0; i < 16; i++) v[i] = __uint_as_float(o[i]) * f0;
           if (joined) {
-            tmem_ld_32(o_col(1) + lanes + d, o);
+            tmem_ld_16(o_col(1) + lanes + d, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = fmaf(__uint_as_float(o[i]), f1, v[i]);
+            for (int i = 0; i < 16; i++) v[i] = fmaf(__uint_as_float(o[i]), f1, v[i]);
           }
           if (whole) {  // through the query's place in shared memory, to whole rows
             constexpr int PIECE = 16 / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 32 / PIECE; i++) {
+            for (int i = 0; i < 16 / PIECE; i++) {
               __align__(16) T w[PIECE];
 #pragma unroll
               for (int j = 0; j < PIECE; j++) act_put(&w[j], v[PIECE * i + j]);
@@ -748,7 +758,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
             }
           } else if (live) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
+            for (int i = 0; i < 16; i += 4)
               *reinterpret_cast<float4*>(slot + part_at<S::ROWS>(d + i, rl)) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           }
         }
@@ -932,7 +942,7 @@ int run(cudaStream_t st, const TreeArgs& a) {
   RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(S::ROWS, D) * sizeof(float), st));
   cudaError_t e = launch_k(Launch{st, true}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
   if (e == cudaSuccess)
-    e = launch_merge<T, D, TK, S::ROWS>(st, a, (const float*)part, ctas);
+    e = launch_merge<T, D, TK, S::ROWS>(st, a, (const float*)part, ctas, cudaSharedmemCarveoutMaxShared);
   const cudaError_t f = cudaFreeAsync(part, st);
   RF_CUDA(e);
   RF_CUDA(f);
