@@ -122,12 +122,19 @@ struct Plan {
   __device__ __forceinline__ Plan(const TreeArgs& a, uint32_t grid) : each(0), more(0) {
     all = sum(a, a.n_seqs, 0);
     ctas = all < grid ? (uint32_t)all : grid;
-    quota = 0;
-    if (!ctas) return;
+    quota = all <= grid;
+    if (quota) return;
     each = div_u(all, ctas);
     more = all - each * ctas;
     const uint64_t least = each + (more ? 1 : 0);
     if (least >> 31) return;
+    if (a.n_seqs == 1) {
+      uint32_t L, n;
+      seq_lengths(a, 0, &L, &n);
+      const uint32_t u = units(a, n), per = u <= grid ? grid / u : 0, q = per ? (tiles(L, n) + per - 1) / per : 0;
+      if (per && q <= least + kSwitch) quota = q;
+      return;
+    }
     for (uint32_t q = (uint32_t)least; q <= least + kSwitch; q++)
       if (sum(a, a.n_seqs, q) <= grid) {
         quota = q;
