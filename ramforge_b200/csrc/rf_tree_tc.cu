@@ -48,13 +48,17 @@ constexpr int TK = 128;                      // keys of a tile, rows of a row ti
 constexpr uint32_t kOperandBytes = 224 * 1024;
 constexpr uint32_t kBlockBytes = TK * 128;   // one [128][64] f16 block
 constexpr uint32_t kAuxBytes = 2560;
-constexpr int kPoly = 3, kPolyOf = 16;  // pairs of weights, of every 16, on the multiply-add pipe
+constexpr int kPoly = 3;  // pairs of weights, of every 16, on the multiply-add pipe
 
 template <class T, bool Q8, int D, int RT>
 struct Shape {
   static constexpr bool SPLIT = std::is_same<T, float>::value;
   static constexpr int ROWS = TK * RT;
-  static constexpr int THREADS = Q8 ? 512 : 384;
+  // RT = 1 is bound by the cache's bytes: eight warps decode Q8_0 and the softmax gets by with few registers.
+  // RT = 2 is bound by the softmax: a half row of S is held in registers, and four warps decode.
+  static constexpr bool HOLD = RT == 2;
+  static constexpr int SETS = !Q8 ? 0 : RT == 1 ? 2 : 1;
+  static constexpr int THREADS = 384 + 128 * SETS;
   static constexpr uint32_t TILE = TK * D * 2;
   static constexpr uint32_t RAW = TK * D;
   static constexpr uint32_t QBYTES = TILE * RT * (SPLIT ? 2 : 1);
@@ -107,6 +111,15 @@ __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t (&r)[32
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
       "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
       "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
+      "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16"
+      "};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -240,6 +253,9 @@ struct Ring {
   __device__ __forceinline__ void advance() {
     if (++s == N) s = 0, phase ^= 1;
   }
+  __device__ __forceinline__ void retreat() {
+    if (s-- == 0) s = N - 1, phase ^= 1;
+  }
 };
 
 // Bounded wait for the phase of `bar` with `parity`; false once any wait of the CTA gave up.
@@ -290,6 +306,13 @@ __device__ __forceinline__ uint32_t seen32(const uint32_t* mask_row, uint32_t wo
     v = (mask_row[0] << -j0) | ((1u << -j0) - 1);
   }
   return n - j0 < 32 ? v & ((1u << (n - j0)) - 1) : v;
+}
+
+// Scores of the columns whose bit is not set become -infinity.
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t see) {
+#pragma unroll
+  for (int j = 0; j < 32; j++)
+    if (!((see >> j) & 1)) s[j] = 0xff800000u;
 }
 
 // 16 bytes of a row as f32.
@@ -457,8 +480,9 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < TK / 32; i++) {
-          if constexpr (SPLIT) mma_ts(o_base, p + 32 + 8 * i, v + i * (16 * 128 >> 4), id_o, !first || i > 0);
-          mma_ts(o_base, p + 8 * i, v + i * (16 * 128 >> 4), id_o, SPLIT || !first || i > 0);
+          const uint32_t pi = p + (S::HOLD ? 8 * i : 32 * (i / 2) + 8 * (i % 2));
+          if constexpr (SPLIT) mma_ts(o_base, pi + 16, v + i * (16 * 128 >> 4), id_o, !first || i > 0);
+          mma_ts(o_base, pi, v + i * (16 * 128 >> 4), id_o, SPLIT || !first || i > 0);
         }
         tc_commit(tc_smem_u32(&B.pv_done[g][h]));
       }
@@ -644,66 +668,163 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           ok = __all_sync(~0u, ok && wait(&B.s_full[g][h], count & 1));
           if (ok && warp_live) {
             tc_fence_after_sync();
-            uint32_t s[TK / 2];
-            tmem_ld_32(scores, s);
-            tmem_ld_32(scores + 32, s + 32);
-            tmem_wait_ld(s);
-            if (edge) {
+            if constexpr (S::HOLD) {  // all 64 columns in registers, weights in pairs over the first 32 of them
+              uint32_t s[TK / 2];
+              tmem_ld_32(scores, s);
+              tmem_ld_32(scores + 32, s + 32);
+              tmem_wait_ld(s);
+              if (edge) {
 #pragma unroll
-              for (int i = 0; i < 2; i++) {
-                const uint32_t see = seen32(mask_row, a.words, t, (int)(key0 + 64 * h + 32 * i) - (int)sg.hist, (int)sg.drafts);
+                for (int i = 0; i < 2; i++) {
+                  const uint32_t see = seen32(mask_row, a.words, t, (int)(key0 + 64 * h + 32 * i) - (int)sg.hist, (int)sg.drafts);
 #pragma unroll
-                for (int j = 0; j < 32; j++)
-                  if (!((see >> j) & 1)) s[32 * i + j] = 0xff800000u;
+                  for (int j = 0; j < 32; j++)
+                    if (!((see >> j) & 1)) s[32 * i + j] = 0xff800000u;
+                }
               }
-            }
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < TK / 2; i += 8)
+              for (int i = 0; i < TK / 2; i += 8)
 #pragma unroll
-              for (int j = 0; j < 4; j++)
-                tops[j] = max3(tops[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * coef;
-            if (__any_sync(~0u, top > m + kRaise)) {
-              const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
-              m = m2;
-              l *= f;
-              if (x + h > 0) {  // all products issued so far are in O before it is rescaled
-                ok = __all_sync(~0u, ok && wait(&B.pv_done[g][h ^ 1], (h ? count : count - 1) & 1));
-                tc_fence_after_sync();
+                for (int j = 0; j < 4; j++)
+                  tops[j] = max3(tops[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
+              const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * coef;
+              if (__any_sync(~0u, top > m + kRaise)) {
+                const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+                m = m2;
+                l *= f;
+                if (x + h > 0) {  // all products issued so far are in O before it is rescaled
+                  ok = __all_sync(~0u, ok && wait(&B.pv_done[g][h ^ 1], (h ? count : count - 1) & 1));
+                  tc_fence_after_sync();
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tmem_ld_32(o_col(g) + lanes + c, o);
-                  tmem_wait_ld(o);
+                  for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32(o_col(g) + lanes + c, o);
+                    tmem_wait_ld(o);
 #pragma unroll
-                  for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  tmem_st_32(o_col(g) + lanes + c, o);
+                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st_32(o_col(g) + lanes + c, o);
+                  }
+                }
+              }
+              const float ref = kWeightBias - (m == -INFINITY ? 0.f : m);
+              const float2 coef2 = make_float2(coef, coef), ref2 = make_float2(ref, ref);
+              float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+              uint32_t p[32];
+#pragma unroll
+              for (int i = 0; i < 32; i++) {
+                float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
+                if (i % 16 < kPoly)
+                  v = ex2_poly(v);
+                else
+                  v.x = ex2(v.x), v.y = ex2(v.y);
+                sum[i & 1] = add2(sum[i & 1], v);
+                p[i] = pack_h2(v.x, v.y);
+              }
+              tmem_st_32(scores, p);
+              l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            } else {
+              uint32_t see[2] = {~0u, ~0u};
+              if (edge) {
+                const int j0 = (int)(key0 + 64 * h) - (int)sg.hist;
+                see[0] = seen32(mask_row, a.words, t, j0, (int)sg.drafts);
+                see[1] = seen32(mask_row, a.words, t, j0 + 32, (int)sg.drafts);
+              }
+              // Raise the reference to the scores' maximum `top` (base-2 exponents) where some row has to: the sums
+              // and O, with all products issued so far in it, are rescaled.
+              auto raise = [&](float top) {
+                const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+                m = m2;
+                l *= f;
+                if (x + h > 0) {
+                  ok = __all_sync(~0u, ok && wait(&B.pv_done[g][h ^ 1], (h ? count : count - 1) & 1));
+                  tc_fence_after_sync();
+#pragma unroll 1
+                  for (int c = 0; c < D; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld_16(o_col(g) + lanes + c, o);
+                    tmem_wait_ld(o);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st_16(o_col(g) + lanes + c, o);
+                  }
+                }
+                return f;
+              };
+              auto maximum = [&](const uint32_t(&s)[32]) {
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                  for (int j = 0; j < 4; j++)
+                    tops[j] = max3(tops[j], __uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1]));
+                return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+              };
+              // the weights of 32 columns of scores, in pairs
+              auto weigh = [&](uint32_t* s, uint32_t* p) {
+                const float ref = kWeightBias - (m == -INFINITY ? 0.f : m);
+                const float2 coef2 = make_float2(coef, coef), ref2 = make_float2(ref, ref);
+                float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                  float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
+                  if (!SPLIT && i < kPoly)
+                    v = ex2_poly(v);
+                  else
+                    v.x = ex2(v.x), v.y = ex2(v.y);
+                  sum[i & 1] = add2(sum[i & 1], v);
+                  p[i] = pack_h2(v.x, v.y);
+                  if constexpr (SPLIT) s[i] = pack_h2_rest(v.x, v.y, p[i]);
+                }
+                l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+              };
+              // 32 columns at a time, rolled: for the registers and for the instruction cache, which all roles share
+              // (unrolled: 17.4 us for 16 tokens over 4095 Q8_0 positions, rolled 15.9).  Weights go back in pairs over the
+              // first 16 of their 32 columns, the small terms over the others.
+              if constexpr (SPLIT) {  // two passes: a weight once rounded in two terms is not scaled again
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 2; c++) {
+                  uint32_t s[32];
+                  tmem_ld_32(scores + 32 * c, s);
+                  tmem_wait_ld(s);
+                  if (edge) hide(s, see[c]);
+                  top = fmaxf(top, maximum(s));
+                }
+                if (__any_sync(~0u, top * coef > m + kRaise)) raise(top * coef);
+              }
+#pragma unroll 1
+              for (int c = 0; c < 2; c++) {
+                uint32_t s[32], p[16];
+                tmem_ld_32(scores + 32 * c, s);
+                tmem_wait_ld(s);
+                if (edge) hide(s, see[c]);
+                if constexpr (!SPLIT) {
+                  const float top = maximum(s) * coef;
+                  if (__any_sync(~0u, top > m + kRaise)) {
+                    const float f = raise(top);
+                    if (c) {  // the first 32 keys' weights were taken against the old reference
+                      const __half2 f2 = __float2half2_rn(f);
+                      tmem_ld_16(scores, p);
+                      tmem_wait_ld(p);
+#pragma unroll
+                      for (int i = 0; i < 16; i++) {
+                        const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&p[i]), f2);
+                        p[i] = *reinterpret_cast<const uint32_t*>(&w);
+                      }
+                      tmem_st_16(scores, p);
+                    }
+                  }
+                }
+                weigh(s, p);
+                tmem_st_16(scores + 32 * c, p);
+                if constexpr (SPLIT) {
+#pragma unroll
+                  for (int i = 0; i < 16; i++) p[i] = s[i];
+                  tmem_st_16(scores + 32 * c + 16, p);
                 }
               }
             }
-            const float ref = kWeightBias - (m == -INFINITY ? 0.f : m);
-            const float2 coef2 = make_float2(coef, coef), ref2 = make_float2(ref, ref);
-            float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
-            uint32_t p[32];
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-              float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
-              if (!SPLIT && i % kPolyOf < kPoly)
-                v = ex2_poly(v);
-              else
-                v.x = ex2(v.x), v.y = ex2(v.y);
-              sum[i & 1] = add2(sum[i & 1], v);
-              p[i] = pack_h2(v.x, v.y);
-              if constexpr (SPLIT) s[i] = pack_h2_rest(v.x, v.y, p[i]);
-            }
-            tmem_st_32(scores, p);
-            if constexpr (SPLIT) {
-#pragma unroll
-              for (int i = 0; i < 32; i++) p[i] = s[i];
-              tmem_st_32(scores + 32, p);
-            }
-            l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_st();
           }
           tc_fence_before_sync();
@@ -807,7 +928,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     // ---- Q8_0 tiles to f16: thread = key; pieces taken in an order that keeps the eight
     // lanes of a shared-memory phase on different banks, for the codes and for the tile
     if constexpr (Q8) {
-      const uint32_t key = tid - 384;
+      const uint32_t key = (tid - 384) % TK, set = (tid - 384) / TK;  // sets of four warps take the tiles in turn
       Ring<S::NRAW> rr;
       Ring<S::NSLOT> ring;
       for (; work_left; work_left = walk.next(a, &sg)) {
@@ -829,14 +950,15 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
             s.x = __ldg((const uint32_t*)plane);
           return s;
         };
-        uint2 s0 = scales(0), s1 = scales(1);
-        for (uint32_t e = 0; e < 2 * nt; e++) {
+        uint2 s0 = scales(set), s1 = scales(set + S::SETS);
+        if (set) rr.advance(), ring.advance();
+        for (uint32_t e = set; e < 2 * nt; e += S::SETS) {
           bool is_v;
           uint32_t i;
           item_at(e, nt, S::LEAD, &is_v, &i);
           const uint2 sc = s0;
           s0 = s1;
-          s1 = scales(e + 2);
+          s1 = scales(e + 2 * S::SETS);
           const uint32_t p = (sg.k0 + i) * TK + key;
           const bool draft_v = is_v && p >= sg.hist;
           ok = __all_sync(~0u, ok && wait(&B.raw_full[rr.s], rr.phase) && wait(&B.free[ring.s], ring.phase ^ 1));
@@ -847,39 +969,38 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
             const uint32_t lm = lane & (N - 1), l7 = lane & 7;
             const uint32_t raw = (raws + rr.s * S::RAW + key * D) + lm * 16;
             const uint32_t lane_at = slot_addr(ring.s) + key * 128 + ((((2 * lm) ^ l7) & 7) << 4);
-            const uint32_t near = lane_at + (lm >> 2) * kBlockBytes, far = lane_at + ((lm >> 2) ^ 1) * kBlockBytes;
-            uint32_t scale[N / 2];  // of the pieces 2i, 2i + 1 of the turn, twice in a word
-#pragma unroll
-            for (uint32_t i = 0; i < N / 2; i++) {
-              const uint32_t blk = i ^ (lm >> 1), w = blk & 2 ? sc.y : sc.x;
-              scale[i] = __byte_perm(w, w, blk & 1 ? 0x3232 : 0x1010);
-            }
-            uint4 codes[N];
-#pragma unroll
-            for (uint32_t j = 0; j < N; j++) codes[j] = ld_shared16(raw ^ (16 * j));
             bool wild = false;
+#pragma unroll 1
+            for (uint32_t q = 0; q < N / 4; q++) {  // 64 codes at a time, rolled for the instruction cache
+              const uint32_t dst = lane_at + ((lm >> 2) ^ q) * kBlockBytes;
+              uint4 codes[4];
 #pragma unroll
-            for (uint32_t j = 0; j < N; j++) {
-              const uint32_t w[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
-              const __half2 d = *reinterpret_cast<const __half2*>(&scale[j / 2]);
-              uint32_t h[8];
+              for (uint32_t j = 0; j < 4; j++) codes[j] = ld_shared16(raw ^ (64 * q + 16 * j));
 #pragma unroll
-              for (int k = 0; k < 4; k++) {
-                // biased bytes under an exponent of 1024: 1152 + code, exact; the product rounds once
-                const uint32_t b = w[k] ^ 0x80808080u;
-                uint32_t lo = __byte_perm(b, 0x64646464u, 0x4140), hi = __byte_perm(b, 0x64646464u, 0x4342);
-                const __half2 bias = __float2half2_rn(1152.f);
-                const __half2 x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), bias), d);
-                const __half2 y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), bias), d);
-                h[2 * k] = *reinterpret_cast<const uint32_t*>(&x), h[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&y);
+              for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t blk = (2 * q + j / 2) ^ (lm >> 1), sw = blk & 2 ? sc.y : sc.x;
+                const uint32_t db = __byte_perm(sw, sw, blk & 1 ? 0x3232 : 0x1010);
+                const __half2 d = *reinterpret_cast<const __half2*>(&db);
+                const uint32_t w[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  // biased bytes under an exponent of 1024: 1152 + code, exact; the product rounds once
+                  const uint32_t b = w[k] ^ 0x80808080u;
+                  uint32_t lo = __byte_perm(b, 0x64646464u, 0x4140), hi = __byte_perm(b, 0x64646464u, 0x4342);
+                  const __half2 bias = __float2half2_rn(1152.f);
+                  const __half2 x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), bias), d);
+                  const __half2 y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), bias), d);
+                  h[2 * k] = *reinterpret_cast<const uint32_t*>(&x), h[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+                if (draft_v) {
+#pragma unroll
+                  for (int k = 0; k < 8; k++) h[k] = finite_halves(h[k], &wild);
+                }
+                const uint32_t at = dst ^ (((2 * j) & 7) << 4);
+                st_shared16(at, make_uint4(h[0], h[1], h[2], h[3]));
+                st_shared16(at ^ 16, make_uint4(h[4], h[5], h[6], h[7]));
               }
-              if (draft_v) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) h[k] = finite_halves(h[k], &wild);
-              }
-              const uint32_t at = (N == 8 && j >= 4 ? far : near) ^ (((2 * j) & 7) << 4);
-              st_shared16(at, make_uint4(h[0], h[1], h[2], h[3]));
-              st_shared16(at ^ 16, make_uint4(h[4], h[5], h[6], h[7]));
             }
             if (wild) *(volatile uint32_t*)&B.wild = 1;
           }
@@ -889,9 +1010,9 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
             tc_mbar_arrive(tc_smem_u32(&B.full[ring.s]));
             tc_mbar_arrive(tc_smem_u32(&B.raw_free[rr.s]));
           }
-          rr.advance();
-          ring.advance();
+          for (int i = 0; i < S::SETS; i++) rr.advance(), ring.advance();
         }
+        if (set) rr.retreat(), ring.retreat();  // tiles come in pairs: back to the first of the next segment
       }
     }
   }
