@@ -439,7 +439,7 @@ int rf_kv_cache_read(const rf_kv_view* cache, void* k_out, void* v_out, int act_
  * zeros.  What a token does not see never reaches its output, whatever the cache holds
  * there (NaN included).
  * q, out [n_seqs * n_tokens][n_heads][head_dim], 16-byte aligned rows; n_heads a multiple of
- * the cache's n_kv_heads (any group size); head_dim 64 or 128 (RF_EUNSUPPORTED otherwise);
+ * the cache's n_kv_heads, up to 1024 times it; head_dim 64 or 128 (RF_EUNSUPPORTED otherwise);
  * 1 <= n_tokens <= 1024.  scale > 0, or 0 for 1/sqrt(head_dim).  f32 sums and softmax; f32
  * queries and probabilities enter the products with 22 bits, f16 and bf16 ones with 11.
  * Sequences whose lengths do not fit the cache get zeros and raise the error word.

@@ -585,3 +585,15 @@ def test_verify_step_in_a_cuda_graph():
         step()
         assert torch.equal(out, got)
     assert verify_error_word() == 0
+
+
+def test_example_verifies_drafts():
+    """examples/verify_drafts.py: projection, norm and rotation, cache and attention as they are used together."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "verify_drafts.py")
+    spec = importlib.util.spec_from_file_location("verify_drafts", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    # the same values in another order: f32 sums of some 60 terms, far below the 1e-5 the example allows itself
+    assert m.main() <= 1e-5

@@ -73,7 +73,8 @@ TA = dict(q_ptr=P, out_ptr=P, act_type=_lib.ACT_BF16, n_seqs=2, n_tokens=5, n_he
     (dict(out_ptr=0), _lib.RF_EINVAL, "null"), (dict(hist_len_ptr=0), _lib.RF_EINVAL, "null"),
     (dict(n_seqs=3), _lib.RF_EINVAL, "the cache holds 2"), (dict(n_tokens=0), _lib.RF_EINVAL, "1..1024"),
     (dict(n_tokens=1025), _lib.RF_EINVAL, "1..1024"), (dict(n_heads=6), _lib.RF_EINVAL, "no multiple"),
-    (dict(n_heads=0), _lib.RF_EINVAL, "no multiple"), (dict(scale=-0.1), _lib.RF_EINVAL, "scale"),
+    (dict(n_heads=0), _lib.RF_EINVAL, "no multiple"),
+    (dict(n_heads=4 * 1025), _lib.RF_EUNSUPPORTED, "at most 1024"), (dict(scale=-0.1), _lib.RF_EINVAL, "scale"),
     (dict(scale=float("nan")), _lib.RF_EINVAL, "scale"), (dict(scale=float("inf")), _lib.RF_EINVAL, "scale"),
     (dict(q_stride=1000), _lib.RF_EINVAL, "stride"), (dict(out_stride=1028), _lib.RF_EINVAL, "16-byte"),
     (dict(q_ptr=P + 2), _lib.RF_EINVAL, "16-byte")])
