@@ -24,12 +24,18 @@
 //   warps 1, 2    tcgen05.mma, one warp a group
 //   warp 3        f16: V tiles that hold drafts or the end are made finite (below)
 //   warps 4 - 11  softmax, queries, outputs
-//   warps 12 - 15 Q8_0: codes * scales -> f16 operand tiles, one key a thread
+//   warps 12 on   Q8_0: codes * scales -> f16 operand tiles, one key a thread, four warps a tile
 //
 // f32 queries and weights are split into two f16 terms, and each product into two MMAs.
 // What a row does not see has weight 0, and 0 * NaN would still be NaN: elements of drafts'
 // V rows that are not finite are replaced by 0 in shared memory, and a flag makes the
 // epilogue add them to the rows that do see them.
+//
+// What bounds it: with two row tiles the softmax, a half tile's 64 columns taking a warp about 1,100 cycles
+// (230 instructions, 64 of them exponentials, with the waits for tensor memory) against 640 of the tensor
+// core, and the 985 W power cap (1.6 GHz): 256 tokens of 64/8 heads over 32768 f16 positions 305 us, 0.91
+// PFLOP/s.  With one row tile HBM and about 15 us of launch, first tiles and join: 16 tokens over
+// 32768 f16 positions 38 us (20.6 for the bytes).
 //
 // Every wait is bounded (about a second): on expiry the kernel raises bit 0 of the error word,
 // all roles run through their loops without waiting or issuing, the copies and MMAs in
@@ -48,14 +54,14 @@ constexpr int TK = 128;                      // keys of a tile, rows of a row ti
 constexpr uint32_t kOperandBytes = 224 * 1024;
 constexpr uint32_t kBlockBytes = TK * 128;   // one [128][64] f16 block
 constexpr uint32_t kAuxBytes = 2560;
-constexpr int kPoly = 3;  // pairs of weights, of every 16, on the multiply-add pipe
 
 template <class T, bool Q8, int D, int RT>
 struct Shape {
   static constexpr bool SPLIT = std::is_same<T, float>::value;
   static constexpr int ROWS = TK * RT;
-  // RT = 1 is bound by the cache's bytes: eight warps decode Q8_0 and the softmax gets by with few registers.
-  // RT = 2 is bound by the softmax: a half row of S is held in registers, and four warps decode.
+  // RT = 1 is bound by the cache's bytes: eight warps decode Q8_0 (16 tokens over 32768 positions: 40 us, with
+  // four 49) and the softmax gets by with few registers.  RT = 2 is bound by the softmax: a half row of S is held
+  // in registers (256 tokens of 64/8 heads over 32768 f16: 305 us, with 32 columns at a time 344), and four warps decode.
   static constexpr bool HOLD = RT == 2;
   static constexpr int SETS = !Q8 ? 0 : RT == 1 ? 2 : 1;
   static constexpr int THREADS = 384 + 128 * SETS;
@@ -194,31 +200,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-  return d;
-}
-// 2^x on the multiply-add pipe, x <= 127: 2^n * 2^f with n = round(x) and a degree-4 polynomial of 2^f
-// on [-1/2, 1/2] (least maximum relative error, fitted: 2.7e-6, against f16's 4.9e-4).  NaN stays NaN; below
-// -126 the result is 2^-126.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-  const float2 magic = make_float2(12582912.f, 12582912.f), less = make_float2(-12582912.f, -12582912.f);
-  const float2 t = add2(x, magic), n = add2(t, less);
-  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 p = make_float2(0.0095701013f, 0.0095701013f);
-  p = fma2(p, f, make_float2(0.0559178605f, 0.0559178605f));
-  p = fma2(p, f, make_float2(0.2402474433f, 0.2402474433f));
-  p = fma2(p, f, make_float2(0.6931218147f, 0.6931218147f));
-  p = fma2(p, f, make_float2(0.9999992847f, 0.9999992847f));
-  const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
-                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
-  return mul2(p, scale);
-}
 
 // Non-finite f16 halves of a word replaced by 0.
 __device__ __forceinline__ uint32_t finite_halves(uint32_t x, bool* wild) {
@@ -712,10 +693,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
 #pragma unroll
               for (int i = 0; i < 32; i++) {
                 float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
-                if (i % 16 < kPoly)
-                  v = ex2_poly(v);
-                else
-                  v.x = ex2(v.x), v.y = ex2(v.y);
+                v.x = ex2(v.x), v.y = ex2(v.y);
                 sum[i & 1] = add2(sum[i & 1], v);
                 p[i] = pack_h2(v.x, v.y);
               }
@@ -766,10 +744,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                   float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), coef2, ref2);
-                  if (!SPLIT && i < kPoly)
-                    v = ex2_poly(v);
-                  else
-                    v.x = ex2(v.x), v.y = ex2(v.y);
+                  v.x = ex2(v.x), v.y = ex2(v.y);
                   sum[i & 1] = add2(sum[i & 1], v);
                   p[i] = pack_h2(v.x, v.y);
                   if constexpr (SPLIT) s[i] = pack_h2_rest(v.x, v.y, p[i]);
