@@ -146,8 +146,9 @@ __global__ void __launch_bounds__(32 * kRowWarps, Step<Q8, D, NB>::CTAS)
   __shared__ int s_wild;  // a V element of a draft is not finite
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const uint32_t k_half = c >= 2 ? 0x3232 : 0x1010;  // which of a word's two scales the lane's dimensions have
-  griddep_launch();  // of tree_merge_kernel
   if (threadIdx.x == 0) s_wild = 0;
+  griddep_wait();
+  griddep_launch();  // of tree_merge_kernel, which reads the lengths before it waits: not before they are there
   __syncthreads();
   const uint32_t G = a.group;
   Walk<KT, ROWS> walk(a);
@@ -481,7 +482,7 @@ int run_rows(cudaStream_t st, const TreeArgs& a) {
   const uint32_t ctas = (uint32_t)num_sms() * Step<Q8, D, NB>::CTAS;
   void* part = nullptr;
   RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(ROWS, D) * sizeof(float), st));
-  cudaError_t e = launch_k(Launch{st, false}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
+  cudaError_t e = launch_k(Launch{st, true}, tree_rows_kernel<T, Q8, D, NB>, dim3(ctas), dim3(32 * kRowWarps), 0, a,
                            (float*)part);
   if (e == cudaSuccess)
     e = launch_merge<T, D, KT, ROWS>(st, a, (const float*)part, ctas, cudaSharedmemCarveoutDefault);

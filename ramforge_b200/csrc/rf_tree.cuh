@@ -262,8 +262,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float
   const uint32_t b = bh / a.c.n_kv_heads, h = bh - b * a.c.n_kv_heads;
   const uint32_t r = r0 + rx, t = group_div(a, r), hq = h * a.group + (r - t * a.group), d0 = blockIdx.y * DPC + dx * 4;
   T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d0;
-  // the lengths were there before the first kernel began; every CTA waits for that kernel before it
-  // ends, so that whoever waits for this one has waited for both
+  griddep_launch();
+  // the lengths were there before the first kernel began to read; every CTA waits for that kernel
+  // before it ends, so that whoever waits for this one has waited for both
   uint32_t L, n;
   seq_lengths(a, b, &L, &n);
   if (t < a.n_tokens && t >= n && cx == 0) {

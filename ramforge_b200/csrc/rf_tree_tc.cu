@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t q_smem = tc_smem_u32(tsm), slots = q_smem + S::QBYTES, raws = slots + S::NSLOT * S::TILE;
   auto slot_addr = [&](uint32_t s) { return slots + s * S::TILE; };
-  griddep_launch();  // of tree_merge_kernel
+  // what is above the wait overlaps the kernel before
   if (warp == 1) tc_tmem_alloc(tc_smem_u32(&B.tmem), 512);
   if (tid == 0) {
     for (int i = 0; i < S::NSLOT; i++) {
@@ -356,6 +356,8 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
     B.stop = B.wild = 0;
     tc_fence_barrier_init();
   }
+  griddep_wait();
+  griddep_launch();  // of tree_merge_kernel, which reads the lengths before it waits: not before they are there
   Walk<TK, S::ROWS> walk(a);
   Segment sg;
   bool work_left = walk.next(a, &sg);
@@ -1034,7 +1036,7 @@ int run(cudaStream_t st, const TreeArgs& a) {
   const uint32_t ctas = (uint32_t)num_sms();
   void* part = nullptr;
   RF_TRY(scratch_alloc(&part, 2 * (size_t)ctas * part_floats(S::ROWS, D) * sizeof(float), st));
-  cudaError_t e = launch_k(Launch{st, false}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
+  cudaError_t e = launch_k(Launch{st, true}, k, dim3(ctas), dim3(S::THREADS), S::SMEM, a, (float*)part, mk, mv);
   if (e == cudaSuccess)
     e = launch_merge<T, D, TK, S::ROWS>(st, a, (const float*)part, ctas, cudaSharedmemCarveoutMaxShared);
   const cudaError_t f = cudaFreeAsync(part, st);

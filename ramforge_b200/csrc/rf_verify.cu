@@ -2,6 +2,10 @@
 // norm and rotation of queries and keys, and the 8-bit (or f16) cache they write
 // and read.  The attention itself is in rf_tree.cu.
 //
+// Every kernel is launched to begin while the one before it in the stream ends (programmatic
+// launch) and waits for it, whole, before it touches memory: without, 8200 rows into a cache and
+// back took 28.5 us in place of 23.9.
+//
 // All three only move data: a few operations per element, each element read once
 // and written once, so HBM bounds the long calls and launch latency the short ones.
 #include <cuda_bf16.h>
@@ -144,6 +148,8 @@ __device__ __forceinline__ bool rope_row(const NormRopeArgs& a, uint32_t t, cons
 // Any even head_dim, stride and alignment: one warp a head, one element a lane and step.
 template <class T>
 __global__ void __launch_bounds__(256) norm_rope_any_kernel(NormRopeArgs a) {
+  griddep_launch();
+  griddep_wait();
   const uint32_t heads = a.n_heads + a.n_kv_heads, lane = threadIdx.x & 31;
   const uint32_t w = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (w >= a.n_tokens * heads) return;
@@ -213,6 +219,8 @@ template <class T>
 __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_rope_vec_kernel(NormRopeArgs a, uint32_t lane_bits, uint32_t per,
                                                                       uint32_t q_groups, uint32_t groups) {
   constexpr int V = Act<T>::kVec;
+  griddep_launch();
+  griddep_wait();
   const uint32_t idx = blockIdx.x * kNormThreads + threadIdx.x, D = a.head_dim;
   uint32_t item = idx >> lane_bits;
   const uint32_t x = idx & ((1u << lane_bits) - 1);
@@ -458,6 +466,8 @@ __device__ __forceinline__ void kv_store(const KvRowsArgs& a, const KvPlace& p, 
 template <class T, bool Q8>
 __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvRowsArgs a) {
   const KvPlace p(a);
+  griddep_launch();
+  griddep_wait();
   const T* src = (const T*)(p.is_v ? a.v : a.k) + p.x * 16;
   const uint64_t stride = p.is_v ? a.v_stride : a.k_stride;
   Acts16<T> cur[kKvRows] = {}, next[kKvRows] = {};
@@ -493,6 +503,8 @@ struct KvRaw {
 template <class T, bool Q8>
 __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvRowsArgs a) {
   const KvPlace p(a);
+  griddep_launch();
+  griddep_wait();
   T* dst = (T*)(p.is_v ? a.v : a.k);
   if (!dst || !p.in) return;
   dst += p.x * 16;
@@ -633,7 +645,7 @@ int run_kv_rows(const rf_kv_view* cache, const void* k, const void* v, int act_t
   a.seq = seq, a.pos = pos;
   a.n_rows = n_rows;
   RF_TRY(verify_error_ptr(&a.err));
-  const Launch L{(cudaStream_t)stream, false};
+  const Launch L{(cudaStream_t)stream, true};
   switch (act_type) {
     case RF_ACT_F32: RF_CUDA(launch_kv_rows<float>(L, a, write)); break;
     case RF_ACT_F16: RF_CUDA(launch_kv_rows<__half>(L, a, write)); break;
@@ -686,7 +698,7 @@ int rf_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int 
   a.head_dim = head_dim, a.rope_len = rope_len, a.rot_dim = rot_dim;
   a.eps = eps;
   RF_TRY(verify_error_ptr(&a.err));
-  const Launch L{(cudaStream_t)stream, false};
+  const Launch L{(cudaStream_t)stream, true};
   switch (act_type) {
     case RF_ACT_F32: RF_CUDA(launch_norm_rope<float>(L, a)); break;
     case RF_ACT_F16: RF_CUDA(launch_norm_rope<__half>(L, a)); break;

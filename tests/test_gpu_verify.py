@@ -587,6 +587,30 @@ def test_verify_step_in_a_cuda_graph():
     assert verify_error_word() == 0
 
 
+@pytest.mark.parametrize("T,HQ", [(1, 4), (3, 4), (40, 8)])
+def test_tree_lengths_written_just_before(T, HQ):
+    """Lengths, queries and cache rows that the kernels right before in the stream write: call after call with no
+    wait between them, each with its own history."""
+    hk, D, cap = 2, 128, 2000
+    c = random_cache("q8_0", 1, hk, cap, D, 30)
+    q = torch.randn(T, HQ * D, device="cuda", generator=gen(31)).half()
+    hists = [int(x) for x in np.random.RandomState(32).randint(0, cap - T + 1, size=40)]
+    want = [run_tree(c, "f16", 1, T, HQ, [h], None, None, 0, q=q)[1] for h in hists]
+    hl = torch.zeros(1, device="cuda", dtype=torch.int32)
+    q2, outs = torch.zeros_like(q), [torch.empty_like(q) for _ in hists]
+    st = torch.cuda.current_stream().cuda_stream
+    for h, o in zip(hists, outs):
+        q2.copy_(q)
+        hl.fill_(h)
+        tree_attention(c.view, q2.data_ptr(), o.data_ptr(), _lib.ACT_F16, 1, T, HQ, hl.data_ptr(), stream=st)
+        q2.zero_()
+        hl.fill_(-1)
+    torch.cuda.synchronize()
+    for h, o, w in zip(hists, outs, want):
+        assert torch.equal(o, w), h
+    assert verify_error_word() == 0
+
+
 def test_example_verifies_drafts():
     """examples/verify_drafts.py: projection, norm and rotation, cache and attention as they are used together."""
     import importlib.util
