@@ -222,7 +222,7 @@ template <class S>
 struct Bars {  // [group][half of the key tile]
   uint64_t full[S::NSLOT], free[S::NSLOT], fix[S::NSLOT];
   uint64_t raw_full[S::NRAW ? S::NRAW : 1], raw_free[S::NRAW ? S::NRAW : 1];
-  uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2][2], drain;
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drain;
   uint32_t tmem, stop, wild, pad;
   float ml[2][TK][2];
 };
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       tc_mbar_init(tc_smem_u32(&B.raw_full[i]), 1);
       tc_mbar_init(tc_smem_u32(&B.raw_free[i]), 4);
     }
-    tc_mbar_init(tc_smem_u32(&B.q_full), 256);
+    for (int g = 0; g < 2; g++) tc_mbar_init(tc_smem_u32(&B.q_full[g]), 128);
     for (int g = 0; g < 2; g++)
       for (int h = 0; h < 2; h++) {
         tc_mbar_init(tc_smem_u32(&B.s_full[g][h]), 1);
@@ -473,8 +473,10 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       constexpr uint32_t step = RT == 1 ? 2 : 1;
       const bool work = RT == 1 ? g < nt : g == 0 || uniform(sg.drafts * G - sg.rt * S::ROWS) > TK;
       auto mine = [&](uint32_t i) { return RT == 1 ? (i & 1) == g : work; };
-      if (work) until(&B.q_full, q_phase);
-      q_phase ^= 1;
+      if (work) {
+        until(&B.q_full[g], q_phase);
+        q_phase ^= 1;
+      }
       if (done)  // the products of the segment before are over (also awaited by the softmax)
         for (uint32_t h = 0; h < 2; h++) until(&B.pv_done[g][h], (done - 1) & 1);
       tc_fence_after_sync();
@@ -567,6 +569,8 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
       const uint32_t r_base = sg.rt * S::ROWS + (RT == 2 ? g * TK : 0) + w32;  // the warp's first row
       const uint32_t r = r_base + lane;
       const bool live = r < n_rows, warp_live = r_base < n_rows;
+      const bool two = n_rows - sg.rt * S::ROWS > TK;
+      const uint32_t mine = RT == 1 ? (nt + 1 - g) / 2 : (g == 0 || two ? nt : 0);  // tiles of this group
       const uint32_t t = live ? group_div(a, r) : 0;
       // element offset of row x's head in a tensor of token stride `stride`
       auto row_at = [&](uint32_t x, uint64_t stride) {
@@ -634,11 +638,13 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
         if constexpr (!std::is_same<T, __half>::value)
           coef = fmaxf(coef * up_mine, 1.17549435e-38f);  // not 0: a masked score stays -inf
         tc_fence_proxy_async();
-        tc_mbar_arrive(tc_smem_u32(&B.q_full));
+        // Told to the groups with work in this segment alone: phases that a group does not wait for it could not tell
+        // apart, nor may a softmax group without work, which runs ahead, complete the phase of another.
+        if (RT == 1 && g == 0)
+          for (uint32_t i = 0; i < min(nt, 2u); i++) tc_mbar_arrive(tc_smem_u32(&B.q_full[i]));
+        if (RT == 2 && mine) tc_mbar_arrive(tc_smem_u32(&B.q_full[g]));
       }
       const uint32_t* mask_row = a.mask ? a.mask + ((uint64_t)sg.b * a.n_tokens + t) * a.words : nullptr;
-      const bool two = n_rows - sg.rt * S::ROWS > TK;
-      const uint32_t mine = RT == 1 ? (nt + 1 - g) / 2 : (g == 0 || two ? nt : 0);
       float m = -INFINITY, l = 0.f;
       for (uint32_t x = 0; x < mine; x++, count++) {
         const uint32_t key0 = (sg.k0 + (RT == 1 ? 2 * x + g : x)) * TK;

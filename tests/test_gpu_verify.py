@@ -414,6 +414,12 @@ def test_tree_ragged_batches(kind, dtype):
                seed=4)
 
 
+@pytest.mark.parametrize("kind", ["q8_0", "f16"])
+def test_tree_one_key_tile_then_many(kind):
+    """200 tokens over 20000 positions: a CTA whose first unit has one tile left, and the next ones 46."""
+    check_tree(kind, "f32", 1, 200, 28, 4, 128, 20000, None, True, seed=44)
+
+
 @pytest.mark.parametrize("T", [1, 2, 4, 8, 15, 17, 31, 32, 48, 65, 100])
 def test_tree_lengths(T):
     """Row counts around every tile edge (4 query heads a KV head), odd histories."""
