@@ -415,6 +415,20 @@ def test_tree_ragged_batches(kind, dtype):
 
 
 @pytest.mark.parametrize("kind", ["q8_0", "f16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_tree_ctas_that_change_units(kind, dtype):
+    """More work units than SMs: a CTA ends one unit and begins another, with runs of a single key tile and row
+    tiles that are half empty or less among them."""
+    check_tree(kind, dtype, 5, 40, 32, 8, 128, 1100, None, True, seed=40)
+    rs = np.random.RandomState(1)
+    hist = rs.randint(0, 900, 24).tolist()
+    drafts = rs.choice([3, 20, 32, 33, 64], 24, p=[.3, .2, .2, .1, .2]).tolist()
+    check_tree(kind, dtype, 24, 64, 32, 8, 128, hist, drafts, True, seed=41)
+    check_tree(kind, dtype, 24, 64, 32, 8, 64, hist, drafts, False, seed=42)
+    check_tree(kind, dtype, 24, 4, 32, 8, 128, hist, [min(n, 4) for n in drafts], True, seed=43)
+
+
+@pytest.mark.parametrize("kind", ["q8_0", "f16"])
 def test_tree_one_key_tile_then_many(kind):
     """200 tokens over 20000 positions: a CTA whose first unit has one tile left, and the next ones 46."""
     check_tree(kind, "f32", 1, 200, 28, 4, 128, 20000, None, True, seed=44)
