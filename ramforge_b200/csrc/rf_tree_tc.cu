@@ -605,15 +605,15 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           }
         } else {
 #pragma unroll 1
-          for (uint32_t b0 = 0; b0 < 32 / RPI; b0 += 8) {
-            uint4 u[8];
+          for (uint32_t b0 = 0; b0 < 32 / RPI; b0 += 4) {
+            uint4 u[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
+            for (uint32_t i = 0; i < 4; i++) {
               const uint64_t at = __shfl_sync(~0u, mine_at, (b0 + i) * RPI + sub);
               u[i] = at ? __ldg(reinterpret_cast<const uint4*>(at) + c) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
+            for (uint32_t i = 0; i < 4; i++) {
               float v[PIECE];
               act_unpack<T>(u[i], v);
               float top = 0.f;
