@@ -2,6 +2,7 @@
 // split of the work over CTAs, visibility, and the softmax's constants.
 #pragma once
 #include <cuda_bf16.h>
+#include <algorithm>
 
 #include "rf_device.cuh"
 #include "rf_verify.h"
@@ -247,119 +248,133 @@ constexpr float kRaise = 8.f, kWeightBias = 7.f;
 // (`grid` of them), in order of the keys, and writes the zeros of tokens past a sequence's drafts.
 // A CTA takes 8 rows of a (sequence, KV head) and DPC dimensions; four threads share each
 // piece of 4 dimensions, each adding every fourth partial result against a maximum of its own.
-// Latency bounds it: a thread requests kAhead partial results with their maxima and sums at
-// once.  Many rows are better served by fewer CTAs (DPC = D), few by more (32): 24 against
-// 9 us at 1024 rows x 8 KV heads, 3 against 5 us at 64 x 8.
+// Latency bounds it, so that what counts is the number of requests in flight on an SM:
+//   few rows   a CTA for 32 dimensions, kAhead partial results with their maxima and sums
+//              requested at once.  For a grid of up to two CTAs an SM with the registers for all of
+//              them (one token over 131072 Q8_0 positions: 59.1 us with BLOCKS = 2, 60.1 with 4), above it
+//              with as many CTAs an SM as fit (64 tokens over 8192, 32/8 heads: 28.2 with 4, 30.8 with 2).
+//   many rows  a CTA for all dimensions, one partial result at a time, and a grid that fits the SMs,
+//              since each CTA computes the plan: 24 sequences of 64 tokens over 500 positions, 32/8
+//              heads, 81 us; with a CTA for each 8 rows and three partial results ahead 108.
 // ---------------------------------------------------------------------------
-template <class T, int D, int KT, int ROWS, int DPC>
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
-  constexpr int X = DPC / 32, kAhead = X == 1 ? 6 : 3;
+template <class T, int D, int KT, int ROWS, int DPC, int BLOCKS>
+__global__ void __launch_bounds__(256, BLOCKS)
+    tree_merge_kernel(TreeArgs a, const float* __restrict__ part, uint32_t grid) {
+  constexpr int X = DPC / 32, kAhead = X == 1 ? 6 : 1;
   __shared__ float4 s_o[4][64];
   __shared__ float2 s_ml[4][8];
   const uint32_t tid = threadIdx.x, rx = tid & 7, dx = (tid >> 3) & 7, cx = tid >> 6;
   const uint32_t groups = (a.n_tokens * a.group + 7) / 8;
-  const uint32_t bh = blockIdx.x / groups, r0 = (blockIdx.x - bh * groups) * 8;
-  const uint32_t b = bh / a.c.n_kv_heads, h = bh - b * a.c.n_kv_heads;
-  const uint32_t r = r0 + rx, t = group_div(a, r), hq = h * a.group + (r - t * a.group), d0 = blockIdx.y * DPC + dx * 4;
-  T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d0;
+  const uint32_t items = a.n_seqs * a.c.n_kv_heads * groups;
   griddep_launch();
-  // the lengths were there before the first kernel began to read; every CTA waits for that kernel
-  // before it ends, so that whoever waits for this one has waited for both
-  uint32_t L, n;
-  seq_lengths(a, b, &L, &n);
-  if (t < a.n_tokens && t >= n && cx == 0) {
-#pragma unroll
-    for (int x = 0; x < X; x++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) act_put(out + 32 * x + i, 0.f);
-  }
   const Plan<KT, ROWS> plan(a, grid);
-  const uint32_t tiles = plan.tiles(L, n), parts = plan.quota ? (tiles + plan.quota - 1) / plan.quota : tiles;
-  const uint64_t u0 = plan.sum(a, b, plan.quota) + ((uint64_t)h * (plan.units(a, n) / a.c.n_kv_heads) + r0 / ROWS) * parts;
-  uint32_t c0 = 0, c1 = 0;  // the CTAs that shared the unit
-  if (r0 < n * a.group) {
-    c0 = plan.quota ? (uint32_t)u0 : plan.holder(u0);
-    c1 = plan.quota ? (uint32_t)u0 + parts - 1 : plan.holder(u0 + tiles - 1);
-  }
-  griddep_wait();
-  if (c0 == c1) return;  // no rows, or finished by its CTA
-  const uint32_t rl = r % ROWS;
-  float M = -INFINITY, den = 0.f;
-  float4 acc[X];
-#pragma unroll
-  for (int x = 0; x < X; x++) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t c = c0 + cx; c <= c1; c += 4 * kAhead) {
-    float m[kAhead], l[kAhead];
-    float4 v[kAhead][X];
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) {
-      const uint32_t ck = c + 4 * k;
-      m[k] = -INFINITY, l[k] = 0.f;
-#pragma unroll
-      for (int x = 0; x < X; x++) v[k][x] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (ck <= c1) {
-        const float* s = part + (2 * (size_t)ck + (ck == c0 ? 1 : 0)) * part_floats(ROWS, D);
-        m[k] = __ldcg(s + ROWS * D + rl), l[k] = __ldcg(s + ROWS * D + ROWS + rl);
-#pragma unroll
-        for (int x = 0; x < X; x++) v[k][x] = __ldcg(reinterpret_cast<const float4*>(s + part_at<ROWS>(d0 + 32 * x, rl)));
-      }
-    }
-    float top = M;
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) top = fmaxf(top, m[k]);
-    const float old = top == -INFINITY ? 1.f : ex2(M - top);
-    M = top;
-    den *= old;
-#pragma unroll
-    for (int x = 0; x < X; x++) acc[x].x *= old, acc[x].y *= old, acc[x].z *= old, acc[x].w *= old;
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) {
-      const float f = top == -INFINITY ? 1.f : ex2(m[k] - top);
-      den += l[k] * f;
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const uint32_t bh = item / groups, r0 = (item - bh * groups) * 8;
+    const uint32_t b = bh / a.c.n_kv_heads, h = bh - b * a.c.n_kv_heads;
+    const uint32_t r = r0 + rx, t = group_div(a, r), hq = h * a.group + (r - t * a.group), d0 = blockIdx.y * DPC + dx * 4;
+    T* out = (T*)a.out + ((uint64_t)b * a.n_tokens + t) * a.out_stride + (uint64_t)hq * D + d0;
+    // the lengths were there before the first kernel began to read; every CTA waits for that kernel
+    // before it ends, so that whoever waits for this one has waited for both
+    uint32_t L, n;
+    seq_lengths(a, b, &L, &n);
+    if (t < a.n_tokens && t >= n && cx == 0) {
 #pragma unroll
       for (int x = 0; x < X; x++)
-        acc[x].x += v[k][x].x * f, acc[x].y += v[k][x].y * f, acc[x].z += v[k][x].z * f, acc[x].w += v[k][x].w * f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) act_put(out + 32 * x + i, 0.f);
     }
-  }
-  if (dx == 0) s_ml[cx][rx] = make_float2(M, den);
-  float f[4], inv = 0.f;
+    const uint32_t tiles = plan.tiles(L, n), parts = plan.quota ? (tiles + plan.quota - 1) / plan.quota : tiles;
+    uint32_t c0 = 0, c1 = 0;  // the CTAs that shared the unit
+    if (r0 < n * a.group) {
+      const uint64_t unit = (uint64_t)h * (plan.units(a, n) / a.c.n_kv_heads) + r0 / ROWS;
+      const uint64_t u0 = plan.sum(a, b, plan.quota) + unit * parts;
+      c0 = plan.quota ? (uint32_t)u0 : plan.holder(u0);
+      c1 = plan.quota ? (uint32_t)u0 + parts - 1 : plan.holder(u0 + tiles - 1);
+    }
+    griddep_wait();
+    if (c0 == c1) continue;  // no rows, or finished by its CTA
+    const uint32_t rl = r % ROWS;
+    float M = -INFINITY, den = 0.f;
+    float4 acc[X];
 #pragma unroll
-  for (int x = 0; x < X; x++) {
-    if (x) __syncthreads();
-    s_o[cx][tid & 63] = acc[x];
-    __syncthreads();
-    if (cx == 0 && t < n) {
-      if (x == 0) {
-        float top = -INFINITY, l = 0.f;
+    for (int x = 0; x < X; x++) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t c = c0 + cx; c <= c1; c += 4 * kAhead) {
+      float m[kAhead], l[kAhead];
+      float4 v[kAhead][X];
 #pragma unroll
-        for (int i = 0; i < 4; i++) top = fmaxf(top, s_ml[i][rx].x);
+      for (int k = 0; k < kAhead; k++) {
+        const uint32_t ck = c + 4 * k;
+        m[k] = -INFINITY, l[k] = 0.f;
+#pragma unroll
+        for (int x = 0; x < X; x++) v[k][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ck <= c1) {
+          const float* s = part + (2 * (size_t)ck + (ck == c0 ? 1 : 0)) * part_floats(ROWS, D);
+          m[k] = __ldcg(s + ROWS * D + rl), l[k] = __ldcg(s + ROWS * D + ROWS + rl);
+#pragma unroll
+          for (int x = 0; x < X; x++) v[k][x] = __ldcg(reinterpret_cast<const float4*>(s + part_at<ROWS>(d0 + 32 * x, rl)));
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) top = fmaxf(top, m[k]);
+      const float old = top == -INFINITY ? 1.f : ex2(M - top);
+      M = top;
+      den *= old;
+#pragma unroll
+      for (int x = 0; x < X; x++) acc[x].x *= old, acc[x].y *= old, acc[x].z *= old, acc[x].w *= old;
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) {
+        const float f = top == -INFINITY ? 1.f : ex2(m[k] - top);
+        den += l[k] * f;
+#pragma unroll
+        for (int x = 0; x < X; x++)
+          acc[x].x += v[k][x].x * f, acc[x].y += v[k][x].y * f, acc[x].z += v[k][x].z * f, acc[x].w += v[k][x].w * f;
+      }
+    }
+    if (dx == 0) s_ml[cx][rx] = make_float2(M, den);
+    float f[4], inv = 0.f;
+#pragma unroll
+    for (int x = 0; x < X; x++) {
+      if (x) __syncthreads();
+      s_o[cx][tid & 63] = acc[x];
+      __syncthreads();
+      if (cx == 0 && t < n) {
+        if (x == 0) {
+          float top = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; i++) top = fmaxf(top, s_ml[i][rx].x);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            f[i] = top == -INFINITY ? 1.f : ex2(s_ml[i][rx].x - top);
+            l += s_ml[i][rx].y * f[i];
+          }
+          inv = l == 0.f ? 0.f : 1.f / l;
+        }
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          f[i] = top == -INFINITY ? 1.f : ex2(s_ml[i][rx].x - top);
-          l += s_ml[i][rx].y * f[i];
+          const float4 v = s_o[i][tid];
+          o.x += v.x * f[i], o.y += v.y * f[i], o.z += v.z * f[i], o.w += v.w * f[i];
         }
-        inv = l == 0.f ? 0.f : 1.f / l;
+        T* p = out + 32 * x;
+        act_put(p, o.x * inv), act_put(p + 1, o.y * inv), act_put(p + 2, o.z * inv), act_put(p + 3, o.w * inv);
       }
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float4 v = s_o[i][tid];
-        o.x += v.x * f[i], o.y += v.y * f[i], o.z += v.z * f[i], o.w += v.w * f[i];
-      }
-      T* p = out + 32 * x;
-      act_put(p, o.x * inv), act_put(p + 1, o.y * inv), act_put(p + 2, o.z * inv), act_put(p + 3, o.w * inv);
     }
+    __syncthreads();  // of s_ml and s_o, before the next rows
   }
 }
 // `carveout`: the first kernel's share of shared memory, kept so that the SMs need not change it between the two.
 template <class T, int D, int KT, int ROWS>
 cudaError_t launch_merge(cudaStream_t st, const TreeArgs& a, const float* part, uint32_t grid, int carveout) {
-  const uint32_t blocks = a.n_seqs * a.c.n_kv_heads * ((a.n_tokens * a.group + 7) / 8);
-  const bool many = blocks > 2 * (uint32_t)num_sms();
-  auto* k = many ? tree_merge_kernel<T, D, KT, ROWS, D> : tree_merge_kernel<T, D, KT, ROWS, 32>;
+  const uint32_t blocks = a.n_seqs * a.c.n_kv_heads * ((a.n_tokens * a.group + 7) / 8), sms = (uint32_t)num_sms();
+  const bool many = blocks > 2 * sms;
+  auto* k = many                          ? tree_merge_kernel<T, D, KT, ROWS, D, 4>
+            : blocks * (D / 32) > 2 * sms ? tree_merge_kernel<T, D, KT, ROWS, 32, 4>
+                                          : tree_merge_kernel<T, D, KT, ROWS, 32, 2>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, carveout);
   if (e != cudaSuccess) return e;
-  return launch_k(Launch{st, true}, k, dim3(blocks, many ? 1 : D / 32), dim3(256), 0, a, part, grid);
+  return launch_k(Launch{st, true}, k, dim3(many ? std::min(blocks, 4 * sms) : blocks, many ? 1 : D / 32), dim3(256), 0, a,
+                  part, grid);
 }
 
 // Scratch of one call: allocated in stream order from a pool of this library's own that keeps
