@@ -884,6 +884,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           slot[S::ROWS * D + rl] = M, slot[S::ROWS * D + S::ROWS + rl] = den;
         }
         if (__any_sync(~0u, *(volatile uint32_t*)&B.wild)) {  // rare: what was left out of the drafts' V
+          __syncwarp();  // other lanes stored this thread's row
           const uint64_t base = ((uint64_t)sg.b * a.c.n_kv_heads + sg.h) * a.c.capacity;
 #pragma unroll 1
           for (uint32_t p = max(sg.hist, sg.k0 * TK); p < min(sg.end, sg.k1 * TK); p++) {
