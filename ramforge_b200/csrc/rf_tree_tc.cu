@@ -34,8 +34,8 @@
 // What bounds it: with two row tiles the softmax, a half tile's 64 columns taking a warp about 1,100 cycles
 // (230 instructions, 64 of them exponentials, with the waits for tensor memory) against 640 of the tensor
 // core, and the 985 W power cap (1.6 GHz): 256 tokens of 64/8 heads over 32768 f16 positions 305 us, 0.91
-// PFLOP/s.  With one row tile HBM and about 15 us of launch, first tiles and join: 16 tokens over
-// 32768 f16 positions 38 us (20.6 for the bytes).
+// PFLOP/s.  With one row tile HBM and about 15 us of launch, first tiles and join: 5 tokens over
+// 32768 f16 positions 36 us (20.5 for the bytes).
 //
 // Every wait is bounded (about a second): on expiry the kernel raises bit 0 of the error word,
 // all roles run through their loops without waiting or issuing, the copies and MMAs in
@@ -59,9 +59,10 @@ template <class T, bool Q8, int D, int RT>
 struct Shape {
   static constexpr bool SPLIT = std::is_same<T, float>::value;
   static constexpr int ROWS = TK * RT;
-  // RT = 1 is bound by the cache's bytes: eight warps decode Q8_0 (16 tokens over 32768 positions: 40 us, with
-  // four 49) and the softmax gets by with few registers.  RT = 2 is bound by the softmax: a half row of S is held
-  // in registers (256 tokens of 64/8 heads over 32768 f16: 305 us, with 32 columns at a time 344), and four warps decode.
+  // RT = 1 is bound by the cache's bytes: eight warps decode Q8_0 (16 tokens over 32768 positions: 34 us now;
+  // when it took 40, four warps took 49) and the softmax gets by with few registers.  RT = 2 is bound by the
+  // softmax: a half row of S is held in registers (256 tokens of 64/8 heads over 32768 f16: 305 us, with 32 columns
+  // at a time 344), and four warps decode.
   static constexpr bool HOLD = RT == 2;
   static constexpr int SETS = !Q8 ? 0 : RT == 1 ? 2 : 1;
   static constexpr int THREADS = 384 + 128 * SETS;
