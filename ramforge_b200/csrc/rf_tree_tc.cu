@@ -951,7 +951,12 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           s1 = scales(e + 2 * S::SETS);
           const uint32_t p = (sg.k0 + i) * TK + key;
           const bool draft_v = is_v && p >= sg.hist;
-          ok = __all_sync(~0u, ok && wait(&B.raw_full[rr.s], rr.phase) && wait(&B.free[ring.s], ring.phase ^ 1));
+          ok = __all_sync(~0u, ok && wait(&B.raw_full[rr.s], rr.phase));
+          // A parity tells two neighbouring uses of a slot apart, so a set that has not waited for the use before must
+          // know that it has begun.  With an odd number of slots that use was the other set's: its tile is waited for.
+          // (The one before that was this set's own, and done: its raw tile would not have been loaded over else.)
+          if constexpr (S::SETS == 2 && S::NSLOT % 2) ok = __all_sync(~0u, ok && wait(&B.full[ring.s], ring.phase ^ 1));
+          ok = __all_sync(~0u, ok && wait(&B.free[ring.s], ring.phase ^ 1));
           if (ok) {
             // piece j of the lane's turn is piece c = j ^ lm of its key: the eight lanes of a phase
             // meet different banks when they read it and when they write its two f16 pieces
