@@ -373,10 +373,11 @@ int rf_decode_attention_noalloc(const float* dQ, const uint16_t* dK, const uint1
  * of the accepted path are written again at consecutive positions, the others with
  * position -1.  No counterpart in the reference (one token per forward).
  *
- * All pointers are device pointers; nothing is copied to or from the host and no call
- * waits for the GPU, so every call can be captured in a CUDA graph.  Calls on
- * different streams are independent of one another.  Strides are elements between two
- * tokens' rows (0: rows without gaps); a token's heads are contiguous, [head][head_dim].
+ * All pointers are device pointers, aligned to their elements where no more is asked
+ * (RF_EINVAL otherwise); nothing is copied to or from the host and no call waits for the
+ * GPU, so every call can be captured in a CUDA graph.  Calls on different streams are
+ * independent of one another.  Strides are elements between two tokens' rows (0: rows
+ * without gaps); a token's heads are contiguous, [head][head_dim].
  * Values that live on the device (positions, lengths) are checked there: a row whose
  * position or length is out of range is left out and raises rf_verify_error_word. */
 

@@ -556,6 +556,8 @@ int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act
   if (q_stride < row || out_stride < row) return set_error(RF_EINVAL, "a token stride is below its row's elements");
   if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride * es % 16 || out_stride * es % 16)
     return set_error(RF_EINVAL, "query and output rows must be 16-byte aligned");
+  if (!aligned_to(hist_len, 4) || !aligned_to(n_draft, 4) || !aligned_to(mask, 4))
+    return set_error(RF_EINVAL, "lengths and mask words must be 4-byte aligned");
   if ((uint64_t)n_seqs * n_tokens * n_heads > 0x7fffffffull)
     return set_error(RF_EINVAL, "%u x %u tokens of %u heads are too many for one call", n_seqs, n_tokens, n_heads);
   if (!n_seqs) return RF_OK;

@@ -579,11 +579,12 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvRowsArgs a) {
 }
 
 int check_kv_rows(const rf_kv_view* c, const void* k, const void* v, int act_type, uint32_t n_rows, uint64_t* k_stride,
-                  uint64_t* v_stride, const int32_t* pos) {
+                  uint64_t* v_stride, const int32_t* seq, const int32_t* pos) {
   RF_TRY(check_kv_view(c));
   const uint32_t es = act_bytes(act_type);
   if (!es) return set_error(RF_EINVAL, "activation type %d is not F32, F16 or BF16", act_type);
   if (n_rows && !pos) return set_error(RF_EINVAL, "null positions");
+  if (!aligned_to(pos, 4) || !aligned_to(seq, 4)) return set_error(RF_EINVAL, "positions and sequences must be 4-byte aligned");
   const uint64_t row = (uint64_t)c->n_kv_heads * c->head_dim;
   for (uint64_t* s : {k_stride, v_stride}) {
     if (!*s) *s = row;
@@ -636,7 +637,7 @@ cudaError_t launch_kv_rows(const Launch& L, KvRowsArgs a, bool write) {
 
 int run_kv_rows(const rf_kv_view* cache, const void* k, const void* v, int act_type, uint32_t n_rows, uint64_t k_stride,
                 uint64_t v_stride, const int32_t* seq, const int32_t* pos, void* stream, bool write) {
-  RF_TRY(check_kv_rows(cache, k, v, act_type, n_rows, &k_stride, &v_stride, pos));
+  RF_TRY(check_kv_rows(cache, k, v, act_type, n_rows, &k_stride, &v_stride, seq, pos));
   if (!n_rows) return RF_OK;
   KvRowsArgs a{};
   a.c = *cache;
@@ -677,6 +678,8 @@ int rf_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int 
   if (rot_dim && !aligned_to(rope, 8)) return set_error(RF_EINVAL, "the rotation table must be 8-byte aligned");
   if (!aligned_to(q, es) || !aligned_to(k, es) || !aligned_to(q_out, es) || !aligned_to(k_out, es))
     return set_error(RF_EINVAL, "queries and keys must be aligned to their element size");
+  if (!aligned_to(q_norm, 4) || !aligned_to(k_norm, 4) || !aligned_to(positions, 4))
+    return set_error(RF_EINVAL, "norm weights and positions must be 4-byte aligned");
   if (!(eps >= 0.f)) return set_error(RF_EINVAL, "eps must not be negative");
   if (n_heads > 65535 || n_kv_heads > 65535 || (uint64_t)n_tokens * (n_heads + n_kv_heads) > 0x7fffffffull / 32)
     return set_error(RF_EINVAL, "%u tokens of %u + %u heads are too many for one call", n_tokens, n_heads, n_kv_heads);
