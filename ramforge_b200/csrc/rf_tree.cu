@@ -356,12 +356,14 @@ __global__ void __launch_bounds__(32 * kRowWarps, Step<Q8, D, NB>::CTAS)
           }
         }
       }
-      // what is masked must not reach the sums, 0 * NaN included: V elements that are not finite count
-      // as 0 here, and the rows that see them get them when the results are written
+      // what is masked must not reach the sums, 0 * NaN included: drafts' V elements that are not finite
+      // count as 0 here, and the rows that see them get them when the results are written; the history's
+      // stay, since every row sees them
       if (edge) {
         bool wild = false;
 #pragma unroll
         for (int i = 0; i < 4 * MB; i++) {
+          if (kb + 2 * c + v_off(i) < L) continue;
           if constexpr (Q8) {
             if (wild_scale(vs[i])) {
               wild = true;
