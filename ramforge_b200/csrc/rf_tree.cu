@@ -61,8 +61,9 @@ __device__ __forceinline__ uint32_t q8_pair(uint32_t biased, __half2 d) {
   return h2_bits(__hmul2(code, d));
 }
 
-// A block whose largest code could leave f16, or whose scale is no number.
-__device__ __forceinline__ bool wild_scale(uint32_t half_bits) { return (half_bits & 0x7fffu) > 0x6007u; }  // 515.5
+// A block in which a code could leave f16, or whose scale is no number.  The cache's writer makes codes up to 127, but
+// a plane may hold -128: above 511.75 (511.75 * 128 = 65504, the last f16).
+__device__ __forceinline__ bool wild_scale(uint32_t half_bits) { return (half_bits & 0x7fffu) > 0x5fffu; }
 
 // The four codes of a word without those whose product with the scale is not finite.
 __device__ __noinline__ uint32_t finite_codes(uint32_t w, uint32_t half_bits) {

@@ -89,3 +89,38 @@ def test_draft_values_reach_those_that_see_them(T, G, D, dtype, kind):
             spoilt[j, :G, dims] = True
             check(out, ref, dtype, sabs, vmax, hist + T, D, spoilt)
     assert verify_error_word() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [s for s in SHAPES if s[0] > 1])
+@pytest.mark.parametrize("code,scale", [(127, 600.0), (-127, 600.0), (-128, 512.0), (-128, 515.5), (126, -521.0)])
+def test_finite_scales_whose_products_overflow(code, scale, D, dtype, T, G):
+    """A finite Q8_0 scale whose product with one code leaves f16: that element alone is infinite, and reaches only
+    the token that sees it.  The codes go down to -128, which a caller's planes may hold."""
+    hk, j, d = 2, 1, 37
+    sign = 1.0 if code * scale > 0 else -1.0
+    assert abs(code * scale) >= 65520  # rounds to infinity
+    for hist in (0, 3, 131):
+        c = random_cache("q8_0", 1, hk, hist + T + 2, D, hist + 2)
+        vis = np.tril(np.ones((1, T, T), bool))
+        vis[0, :, j] = False
+        vis[0, j, j] = True
+        c.v[0, :, hist + j].clamp_(-5, 5)
+        c.v[0, 0, hist + j, d] = 0
+        c.vs[0, 0, hist + j, d // 32] = scale
+        q, _ = run_tree(c, dtype, 1, T, hk * G, [hist], None, vis, 7)
+        ref, sabs, vmax = attention_ref(c, q, 1, T, hk * G, [hist], [T], vis, D ** -0.5)
+        c.v[0, 0, hist + j, d] = code
+        _, out = run_tree(c, dtype, 1, T, hk * G, [hist], None, vis, 7)
+        spoilt = torch.zeros(T, hk * G, D, dtype=torch.bool, device="cuda")
+        spoilt[j, :G, d] = True
+        rest = torch.arange(T, device="cuda") != j  # they never meet the large values
+        tol = torch.where(rest[:, None, None], 0.0, 1.0).expand(T, hk * G, D)
+        r, o = ref.reshape(T, hk * G, D), out.reshape(T, hk * G, D)
+        low = attention_tolerance(dtype, r, sabs, 6.0, hist + T, D)
+        high = attention_tolerance(dtype, r, sabs, vmax, hist + T, D)
+        tol = torch.where(tol > 0, high, low)
+        assert ((o.double() - r).abs() <= tol)[~spoilt].all()
+        assert (o[spoilt] == sign * float("inf")).all()
+    assert verify_error_word() == 0
