@@ -723,9 +723,12 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
                 see[1] = seen32(mask_row, a.words, t, j0 + 32, (int)sg.drafts);
               }
               // Raise the reference to the scores' maximum `top` (base-2 exponents) where some row has to: the sums
-              // and O, with all products issued so far in it, are rescaled.
+              // and O, with all products issued so far in it, are rescaled.  Weights in f16 may be rescaled too (below):
+              // their references are whole numbers, so that the factor is a power of two and rounds no weight again.
               auto raise = [&](float top) {
-                const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+                float m2 = fmaxf(m, top);
+                if constexpr (!SPLIT) m2 = ceilf(m2);
+                const float f = m2 == -INFINITY ? 1.f : ex2(m - m2);
                 m = m2;
                 l *= f;
                 if (x + h > 0) {
