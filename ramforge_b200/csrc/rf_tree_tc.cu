@@ -42,6 +42,7 @@
 // flight are waited for (bounded again), tensor memory is freed and the kernel returns.
 #include <cuda.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "rf_tc.cuh"
@@ -1028,13 +1029,13 @@ int plane_map(CUtensorMap* map, const void* p, const rf_kv_view& c) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static void* fn = nullptr;
+  static std::atomic<void*> known{nullptr};  // calls may come from several threads
+  void* fn = known.load(std::memory_order_relaxed);
   if (!fn) {
     cudaDriverEntryPointQueryResult q;
-    void* f = nullptr;
-    RF_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q));
-    if (q != cudaDriverEntryPointSuccess || !f) return set_error(RF_ECUDA, "cuTensorMapEncodeTiled is not available");
-    fn = f;
+    RF_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !fn) return set_error(RF_ECUDA, "cuTensorMapEncodeTiled is not available");
+    known.store(fn, std::memory_order_relaxed);
   }
   const cuuint64_t dims[3] = {c.head_dim, c.capacity, (cuuint64_t)c.n_seqs * c.n_kv_heads};
   const cuuint64_t strides[2] = {2ull * c.head_dim, 2ull * c.head_dim * c.capacity};
