@@ -249,10 +249,9 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, uint32_t b, uint32_t t, 
 
 // Softmax in base 2 with a running reference m that is only raised (and the sums
 // rescaled) when some score passes it by 2^kRaise; weights are 2^(s - m + kWeightBias),
-// below 2^15, so that f16 keeps 11 bits of every weight down to 2^-21 of the largest (2^-20 where the
-// reference is a whole number above it).  With f16 and bf16 activations a weight is that one f16, which is
-// what their products take: a second term would double the products (f32 activations have it), and
-// 2^-11 is what f16 outputs round by themselves.
+// below 2^15, so that f16 keeps 11 bits of every weight down to 2^-21 of the largest.  With f16 and bf16
+// activations a weight is that one f16, which is what their products take: a second term would double
+// the products (f32 activations have it), and 2^-11 is what f16 outputs round by themselves.
 constexpr float kRaise = 8.f, kWeightBias = 7.f;
 
 // ---------------------------------------------------------------------------

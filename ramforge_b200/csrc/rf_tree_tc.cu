@@ -724,12 +724,9 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
                 see[1] = seen32(mask_row, a.words, t, j0 + 32, (int)sg.drafts);
               }
               // Raise the reference to the scores' maximum `top` (base-2 exponents) where some row has to: the sums
-              // and O, with all products issued so far in it, are rescaled.  Weights in f16 may be rescaled too (below):
-              // their references are whole numbers, so that the factor is a power of two and rounds no weight again.
+              // and O, with all products issued so far in it, are rescaled.
               auto raise = [&](float top) {
-                float m2 = fmaxf(m, top);
-                if constexpr (!SPLIT) m2 = ceilf(m2);
-                const float f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+                const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2(m - m2);
                 m = m2;
                 l *= f;
                 if (x + h > 0) {
@@ -745,7 +742,6 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
                     tmem_st_16(o_col(g) + lanes + c, o);
                   }
                 }
-                return f;
               };
               auto maximum = [&](const uint32_t(&s)[32]) {
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -774,41 +770,25 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
               // 32 columns at a time, rolled: for the registers and for the instruction cache, which all roles share
               // (unrolled: 17.4 us for 16 tokens over 4095 Q8_0 positions, rolled 15.9).  Weights go back in pairs over the
               // first 16 of their 32 columns, the small terms over the others.
-              if constexpr (SPLIT) {  // two passes: a weight once rounded in two terms is not scaled again
-                float top = -INFINITY;
+              // Two passes: a weight once rounded is not scaled again.  (With 16-bit activations one pass, which rescales
+              // the first 32 keys' weights, takes the same time: 16 tokens over 32768 Q8_0 34.6 us against 35.1, over 4095
+              // 15.1 both, 32 over 32768 f16 39.9 both.)
+              float top = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                  uint32_t s[32];
-                  tmem_ld_32(scores + 32 * c, s);
-                  tmem_wait_ld(s);
-                  if (edge) hide(s, see[c]);
-                  top = fmaxf(top, maximum(s));
-                }
-                if (__any_sync(~0u, top * coef > m + kRaise)) raise(top * coef);
+              for (int c = 0; c < 2; c++) {
+                uint32_t s[32];
+                tmem_ld_32(scores + 32 * c, s);
+                tmem_wait_ld(s);
+                if (edge) hide(s, see[c]);
+                top = fmaxf(top, maximum(s));
               }
+              if (__any_sync(~0u, top * coef > m + kRaise)) raise(top * coef);
 #pragma unroll 1
               for (int c = 0; c < 2; c++) {
                 uint32_t s[32], p[16];
                 tmem_ld_32(scores + 32 * c, s);
                 tmem_wait_ld(s);
                 if (edge) hide(s, see[c]);
-                if constexpr (!SPLIT) {
-                  const float top = maximum(s) * coef;
-                  if (__any_sync(~0u, top > m + kRaise)) {
-                    const float f = raise(top);
-                    if (c) {  // the first 32 keys' weights were taken against the old reference
-                      const __half2 f2 = __float2half2_rn(f);
-                      tmem_ld_16(scores, p);
-                      tmem_wait_ld(p);
-#pragma unroll
-                      for (int i = 0; i < 16; i++) {
-                        const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&p[i]), f2);
-                        p[i] = *reinterpret_cast<const uint32_t*>(&w);
-                      }
-                      tmem_st_16(scores, p);
-                    }
-                  }
-                }
                 weigh(s, p);
                 tmem_st_16(scores + 32 * c, p);
                 if constexpr (SPLIT) {
