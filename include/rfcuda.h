@@ -379,7 +379,8 @@ int rf_decode_attention_noalloc(const float* dQ, const uint16_t* dK, const uint1
  * independent of one another.  Strides are elements between two tokens' rows (0: rows
  * without gaps); a token's heads are contiguous, [head][head_dim].
  * Values that live on the device (positions, lengths) are checked there: a row whose
- * position or length is out of range is left out and raises rf_verify_error_word. */
+ * position, sequence or length is out of range raises rf_verify_error_word; its outputs
+ * are not written by rf_qk_norm_rope and rf_kv_cache_write, and zeros in the other two. */
 
 /* element types of activations (ggml ids; bf16 is no weight type of the engine) */
 #define RF_ACT_F32 0
@@ -426,7 +427,8 @@ typedef struct rf_kv_view {
 int rf_kv_cache_write(const rf_kv_view* cache, const void* k, const void* v, int act_type, uint32_t n_rows,
                       uint64_t k_stride, uint64_t v_stride, const int32_t* seq, const int32_t* pos, void* stream);
 /* The same rows back (kv_cache.rs:452-480 get_k_range / get_v_range over any positions);
- * k_out or v_out may be NULL.  Rows with pos[r] < 0 read as zeros. */
+ * k_out or v_out may be NULL.  Rows with pos[r] < 0 read as zeros, and so do rows whose
+ * position or sequence is out of range. */
 int rf_kv_cache_read(const rf_kv_view* cache, void* k_out, void* v_out, int act_type, uint32_t n_rows,
                      uint64_t k_stride, uint64_t v_stride, const int32_t* seq, const int32_t* pos, void* stream);
 
@@ -438,11 +440,15 @@ int rf_kv_cache_read(const rf_kv_view* cache, void* k_out, void* v_out, int act_
  * mask[(b * n_tokens + t) * ceil(n_tokens/32) + j/32] is set.  mask NULL: a chain, j <= t.
  * n_draft NULL: n_tokens each.  Tokens t >= n_draft[b], and tokens that see nothing, get
  * zeros.  What a token does not see never reaches its output, whatever the cache holds
- * there (NaN included).
+ * there (NaN included).  A value of V that is not finite makes the outputs that see it
+ * not finite (with f32 activations an infinity may come out as NaN).
  * q, out [n_seqs * n_tokens][n_heads][head_dim], 16-byte aligned rows; n_heads a multiple of
  * the cache's n_kv_heads, up to 1024 times it; head_dim 64 or 128 (RF_EUNSUPPORTED otherwise);
  * 1 <= n_tokens <= 1024.  scale > 0, or 0 for 1/sqrt(head_dim).  f32 sums and softmax; f32
  * queries and probabilities enter the products with 22 bits, f16 and bf16 ones with 11.
+ * The products' f32 sums are the tensor core's, which truncate: long histories cost f32
+ * outputs bits (off by 1.2e-6 of their size for 32 tokens over 8192 positions, 8.5e-6 for 64
+ * over 60000, 1.7e-5 for 64 over 131072).
  * Sequences whose lengths do not fit the cache get zeros and raise the error word.
  * Scratch for split histories comes from the library's own stream-ordered memory pool. */
 int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act_type, uint32_t n_seqs,

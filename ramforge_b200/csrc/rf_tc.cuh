@@ -1,8 +1,10 @@
 // rf_tc.cuh - Blackwell tensor-core plumbing (tcgen05 MMA with its accumulator in
 // tensor memory, bulk copies into shared memory completed on mbarriers) for the
-// batched prompt GEMM.  Only the forms used are wrapped: kind::f16 with bf16
-// operands and an f32 accumulator, cta_group::1, K-major operands in the
-// no-swizzle canonical layout, and no cluster multicast anywhere.
+// batched prompt GEMM, the streaming decode attention and the attention of drafted
+// tokens.  Only the forms used are wrapped: kind::f16 with an f32 accumulator (the
+// instruction descriptor says whether the operands are bf16 or f16), cta_group::1, and
+// no cluster multicast anywhere.  tc_smem_desc is the K-major layout without swizzle;
+// rf_tree_tc.cu has its own descriptors for 128-byte swizzled operands.
 #pragma once
 #include <stdint.h>
 
@@ -97,7 +99,8 @@ __host__ __device__ constexpr uint32_t tc_idesc_bf16_f32(int M, int N) {
 }
 
 // ---- MMA, commit, tensor-memory loads ------------------------------------------------
-// D[tmem] (+)= A[smem] x B[smem]^T for one K = 16 step; issued by one thread.
+// D[tmem] (+)= A[smem] x B[smem]^T for one K = 16 step, operands of the type `idesc` gives (bf16 in the
+// prompt GEMM, f16 in rf_tree_tc.cu); issued by one thread.
 __device__ __forceinline__ void tc_mma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                             bool accumulate) {
   asm volatile(

@@ -77,11 +77,12 @@ __device__ __noinline__ uint32_t finite_codes(uint32_t w, uint32_t half_bits) {
 }
 
 // Shapes of one step of a warp over a cache of type Q8, head dimension D
-// and NB blocks of 8 query rows, with the CTAs of an SM.  Q8_0 is bound by the decode's
-// instructions, so it wants more warps: one row over 131072 positions of 128 dimensions takes
-// 59 us with 16 keys a step and four CTAs, 64 with 32 and three, 87 with 32 and four (spills);
-// of 64 dimensions 35 with 32 and four, 40 with 16 and four.  f16 is bound by HBM: 87 us
-// (0.94 of the copy rate) with three CTAs, 96 with four.
+// and NB blocks of 8 query rows, with the CTAs of an SM.  Q8_0 is bound by the latency of its steps: 42 % of
+// a warp's time it waits for loads, one step ahead of their use, and 22 % for the decode's own results, at 16 warps
+// an SM (registers); issue slots are 49 % full and HBM is at 0.72 of the copy rate.  So it wants more warps: one row
+// over 131072 positions of 128 dimensions takes 59 us with 16 keys a step and four CTAs, 64 with 32 and three, 87
+// with 32 and four (spills); of 64 dimensions 35 with 32 and four, 40 with 16 and four.  f16 is bound by HBM: 86 us
+// (0.95 of the copy rate) with three CTAs, 96 with four.
 template <bool Q8, int D, int NB>
 struct Step {
   static constexpr int MB = !Q8 || (D == 128 && NB == 1) ? 1 : 2;  // 16-key blocks

@@ -137,7 +137,7 @@ struct Plan {
       return;
     }
     // No quota does for more units than CTAs, which the largest quota tells (200 single tokens over 500 f16
-    // positions, 32/8 heads: 97 us without that, 87 with it); with few (sequence, head) pairs it is not asked.
+    // positions, 32/8 heads: 97 us without that, 83 to 87 with it); with few (sequence, head) pairs it is not asked.
     constexpr uint32_t kMost = 1u << 31;
     uint32_t q = (uint64_t)a.n_seqs * a.c.n_kv_heads > grid ? kMost : (uint32_t)least;
 #pragma unroll 1
@@ -266,7 +266,7 @@ constexpr float kRaise = 8.f, kWeightBias = 7.f;
 //              with as many CTAs an SM as fit (64 tokens over 8192, 32/8 heads: 28.2 with 4, 30.8 with 2).
 //   many rows  a CTA for all dimensions, one partial result at a time, and a grid that fits the SMs,
 //              since each CTA computes the plan: 24 sequences of 64 tokens over 500 positions, 32/8
-//              heads, 81 us; with a CTA for each 8 rows and three partial results ahead 108.
+//              heads, 80 us; with a CTA for each 8 rows and three partial results ahead 108.
 // ---------------------------------------------------------------------------
 template <class T, int D, int KT, int ROWS, int DPC, int BLOCKS>
 __global__ void __launch_bounds__(256, BLOCKS)

@@ -26,16 +26,22 @@
 //   warps 4 - 11  softmax, queries, outputs
 //   warps 12 on   Q8_0: codes * scales -> f16 operand tiles, one key a thread, four warps a tile
 //
-// f32 queries and weights are split into two f16 terms, and each product into two MMAs.
+// f32 queries and weights are split into two f16 terms, and each product into two MMAs.  The tensor core's f32
+// sums truncate: an f32 output loses about 1.7e-8 of its size for each 16 keys and term that one group of one CTA
+// sums (64 tokens over 60000 positions: 8.5e-6 off, the same in plain f32 4.6e-6).
 // What a row does not see has weight 0, and 0 * NaN would still be NaN: elements of drafts'
 // V rows that are not finite are replaced by 0 in shared memory, and a flag makes the
 // epilogue add them to the rows that do see them.
 //
-// What bounds it: with two row tiles the softmax, a half tile's 64 columns taking a warp about 1,100 cycles
-// (230 instructions, 64 of them exponentials, with the waits for tensor memory) against 640 of the tensor
-// core, and the 985 W power cap (1.6 GHz): 256 tokens of 64/8 heads over 32768 f16 positions 305 us, 0.91
-// PFLOP/s.  With one row tile HBM and about 15 us of launch, first tiles and join: 5 tokens over
-// 32768 f16 positions 36 us (20.5 for the bytes).
+// What bounds it.  Two row tiles, f16: no unit is full.  Of about 3,300 cycles a tile the tensor core works 61 % and a
+// softmax warp 2,100 (230 instructions a half tile, 64 of them exponentials, and the waits for tensor memory);
+// the rest is the chain between them, since P lies over the columns of S: the next scores of a half wait for its P
+// and for the product with it (both MMA warps stand at those barriers about 650 cycles a tile).  The power cap
+// lowers the clock besides: 256 tokens of 64/8 heads over 32768 f16 positions take 260 us in a short run and 305 to 320
+// in a long one (1.06 and 0.87 to 0.91 PFLOP/s).  Two row tiles, Q8_0: the softmax beside the decode, whose instructions it shares the SM
+// with: a half tile takes a softmax warp 1,630 cycles and 280 of waiting, a tile a decoding warp 1,300 and 550 of
+// waiting (400 of them for a free slot).  With one row tile HBM and about 15 us of launch, first tiles and join:
+// 5 tokens over 32768 f16 positions 36 us (20.5 for the bytes).
 //
 // Every wait is bounded (about a second): on expiry the kernel raises bit 0 of the error word,
 // all roles run through their loops without waiting or issuing, the copies and MMAs in
@@ -60,10 +66,10 @@ template <class T, bool Q8, int D, int RT>
 struct Shape {
   static constexpr bool SPLIT = std::is_same<T, float>::value;
   static constexpr int ROWS = TK * RT;
-  // RT = 1 is bound by the cache's bytes: eight warps decode Q8_0 (16 tokens over 32768 positions: 34 us now;
-  // when it took 40, four warps took 49) and the softmax gets by with few registers.  RT = 2 is bound by the
-  // softmax: a half row of S is held in registers (256 tokens of 64/8 heads over 32768 f16: 305 us, with 32 columns
-  // at a time 344), and four warps decode.
+  // RT = 1 has little work a tile: eight warps decode Q8_0 (16 tokens over 32768 positions: 35 us now;
+  // when it took 40, four warps took 49) and the softmax gets by with few registers.  RT = 2 waits for the
+  // softmax more than for loads: a half row of S is held in registers (256 tokens of 64/8 heads over 32768 f16: 305 us,
+  // with 32 columns at a time 344), and four warps decode.
   static constexpr bool HOLD = RT == 2;
   static constexpr int SETS = !Q8 ? 0 : RT == 1 ? 2 : 1;
   static constexpr int THREADS = 384 + 128 * SETS;
