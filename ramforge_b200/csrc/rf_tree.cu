@@ -43,14 +43,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
                : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
                : "l"(p));
   return u;
 }
 __device__ __forceinline__ uint2 ld_stream8(const void* p) {
   uint2 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
   return u;
 }
 
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, Step<Q8, D, NB>::CTAS)
         if constexpr (D == 128)
           ks[i] = ld_stream8(sp);
         else
-          ks[i].x = __ldg((const uint32_t*)sp);
+          ks[i].x = *(const uint32_t*)sp;
       }
     };
     auto get_v = [&](int i, const uint8_t* p, const __half* sp) {
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, Step<Q8, D, NB>::CTAS)
           vr[i][4 * j] = u.x, vr[i][4 * j + 1] = u.y, vr[i][4 * j + 2] = u.z, vr[i][4 * j + 3] = u.w;
         }
       }
-      if constexpr (Q8) vs[i] = __ldg((const unsigned short*)sp);
+      if constexpr (Q8) vs[i] = *(const unsigned short*)sp;
     };
     auto inner = [&](uint32_t kb) { return kb + S::KEYS <= L; };
     const uint32_t kb0 = k0 * KT + warp * S::KEYS;

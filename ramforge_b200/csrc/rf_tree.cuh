@@ -29,6 +29,9 @@ __device__ __forceinline__ uint32_t group_div(const TreeArgs& a, uint32_t r) {
 }
 
 // History length and draft count of sequence b; (0, 0) and the error bit where they do not fit the cache.
+// The read-only path, so that the compiler keeps them in registers: with plain loads, which the error word's
+// atomics make it repeat, a 64-token tree over 32768 Q8_0 takes 59 us in place of 55.  They are read after the
+// wait for the kernel before (tests/test_gpu_verify_chain.py has one that writes them until then).
 __device__ __forceinline__ void seq_lengths(const TreeArgs& a, uint32_t b, uint32_t* hist, uint32_t* drafts) {
   const int32_t L = __ldg(a.hist_len + b), n = a.n_draft ? __ldg(a.n_draft + b) : (int32_t)a.n_tokens;
   const bool ok = L >= 0 && n >= 0 && (uint32_t)n <= a.n_tokens && (uint64_t)L + (uint64_t)n <= a.c.capacity;

@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
               const uint64_t at = __shfl_sync(~0u, mine_at, (b0 + i) * RPI + sub);
-              u[i] = at ? __ldg(reinterpret_cast<const uint4*>(at) + c) : make_uint4(0, 0, 0, 0);
+              u[i] = at ? *(reinterpret_cast<const uint4*>(at) + c) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
@@ -925,9 +925,9 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           if (p >= sg.end) return s;
           const __half* plane = (const __half*)(is_v ? a.c.v_scale : a.c.k_scale) + (base + p) * (D / 32);
           if constexpr (D == 128)
-            s = __ldg((const uint2*)plane);
+            asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(s.x), "=r"(s.y) : "l"(plane));
           else
-            s.x = __ldg((const uint32_t*)plane);
+            asm volatile("ld.global.b32 %0, [%1];" : "=r"(s.x) : "l"(plane));
           return s;
         };
         uint2 s0 = scales(set), s1 = scales(set + S::SETS);

@@ -4,7 +4,8 @@
 //
 // Every kernel is launched to begin while the one before it in the stream ends (programmatic
 // launch) and waits for it, whole, before it touches memory: without, 8200 rows into a cache and
-// back took 28.5 us in place of 23.9.
+// back took 28.5 us in place of 23.9.  What the one before may write is not read through the read-only
+// path (.nc, __ldg), which is for memory that nobody writes while a kernel runs: norm weights and tables.
 //
 // All three only move data: a few operations per element, each element read once
 // and written once, so HBM bounds the long calls and launch latency the short ones.
@@ -111,7 +112,7 @@ struct Act<__nv_bfloat16> {
 // 16 bytes that this call reads once.
 __device__ __forceinline__ uint4 ld_once(const void* p) {
   uint4 u;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
                : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
                : "l"(p));
   return u;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_rope_vec_kernel(
   const T* src = (const T*)(is_q ? a.q : a.k) + t * (is_q ? a.q_stride : a.k_stride) + (size_t)h0 * D + x * V;
   T* dst = (T*)(is_q ? a.q_out : a.k_out) + t * (is_q ? a.q_out_stride : a.k_out_stride) + (size_t)h0 * D + x * V;
   const float* nw = is_q ? a.q_norm : a.k_norm;
-  const int32_t pos = a.rot_dim ? __ldg(a.pos + t) : 0;
+  const int32_t pos = a.rot_dim ? a.pos[t] : 0;
   uint4 raw[kHeads][2];
   auto load = [&](uint32_t h) {
 #pragma unroll
@@ -361,7 +362,7 @@ struct KvAddr {
 };
 __device__ __forceinline__ KvAddr kv_addr(const KvRowsArgs& a, uint32_t row) {
   KvAddr p{-1, 0};
-  if (row < a.n_rows) p.pos = __ldg(a.pos + row), p.seq = a.seq ? __ldg(a.seq + row) : 0;
+  if (row < a.n_rows) p.pos = a.pos[row], p.seq = a.seq ? a.seq[row] : 0;
   return p;
 }
 __device__ __forceinline__ int64_t kv_slot(const KvRowsArgs& a, KvAddr p, uint32_t h) {
@@ -383,12 +384,12 @@ struct Acts16 {
     for (int i = 0; i < N; i += 2) {
       const uint4* q = reinterpret_cast<const uint4*>(p) + i;
       if (wide)
-        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                      : "=r"(u[i].x), "=r"(u[i].y), "=r"(u[i].z), "=r"(u[i].w), "=r"(u[i + 1].x), "=r"(u[i + 1].y),
                        "=r"(u[i + 1].z), "=r"(u[i + 1].w)
                      : "l"(q));
       else
-        u[i] = __ldg(q), u[i + 1] = __ldg(q + 1);
+        u[i] = q[0], u[i + 1] = q[1];
     }
   }
   __device__ __forceinline__ void store(T* p, bool wide) const {
@@ -524,10 +525,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvRowsArgs a) {
     const uint64_t at = (uint64_t)slot * a.c.head_dim + p.c * 16;
     if constexpr (Q8) {
       x.u[0] = ld_once((const int8_t*)plane + at);
-      x.d = __ldg(scales + slot * (a.c.head_dim / 32) + p.c / 2);
+      x.d = scales[slot * (a.c.head_dim / 32) + p.c / 2];
     } else {
       const uint4* q = reinterpret_cast<const uint4*>((const __half*)plane + at);
-      x.u[0] = __ldg(q), x.u[1] = __ldg(q + 1);
+      x.u[0] = q[0], x.u[1] = q[1];
     }
     return x;
   };
