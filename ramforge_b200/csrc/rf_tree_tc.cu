@@ -412,12 +412,11 @@ __global__ void __launch_bounds__(Shape<T, Q8, D, RT>::THREADS, 1)
           ring.advance();
         }
       }
-      if (!ok || *stop) {  // copies nobody waited for must land before the CTA's memory is given up
-        Ring<N> r;
-        for (uint32_t i = 0; i < issued; i++) {
-          if (i + N >= issued) tc_mbar_wait(tc_smem_u32(&full[r.s]), r.phase);
-          r.advance();
-        }
+      // every copy must land before the CTA's memory is given up, also if the other roles' waits give up after this
+      Ring<N> r;
+      for (uint32_t i = 0; i < issued; i++) {
+        if (i + N >= issued) tc_mbar_wait(tc_smem_u32(&full[r.s]), r.phase);
+        r.advance();
       }
     }
   } else if (warp < 3) {
