@@ -37,8 +37,8 @@
 // softmax warp 2,100 (230 instructions a half tile, 64 of them exponentials, and the waits for tensor memory);
 // the rest is the chain between them, since P lies over the columns of S: the next scores of a half wait for its P
 // and for the product with it (both MMA warps stand at those barriers about 650 cycles a tile).  The power cap
-// lowers the clock besides: 256 tokens of 64/8 heads over 32768 f16 positions take 260 us in a short run and 305 to 320
-// in a long one (1.06 and 0.87 to 0.91 PFLOP/s).  Two row tiles, Q8_0: the softmax beside the decode, whose instructions it shares the SM
+// lowers the clock besides: 256 tokens of 64/8 heads over 32768 f16 positions take 260 us in a short run and 305 to 330
+// in a long one (1.06 and 0.84 to 0.91 PFLOP/s).  Two row tiles, Q8_0: the softmax beside the decode, whose instructions it shares the SM
 // with: a half tile takes a softmax warp 1,630 cycles and 280 of waiting, a tile a decoding warp 1,300 and 550 of
 // waiting (400 of them for a free slot).  With one row tile HBM and about 15 us of launch, first tiles and join:
 // 5 tokens over 32768 f16 positions 36 us (20.5 for the bytes).
