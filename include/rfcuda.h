@@ -455,10 +455,87 @@ int rf_tree_attention(const rf_kv_view* cache, const void* q, void* out, int act
                       uint32_t n_tokens, uint32_t n_heads, uint64_t q_stride, uint64_t out_stride,
                       const int32_t* hist_len, const int32_t* n_draft, const uint32_t* mask, float scale,
                       void* stream);
-/* Error word of the four calls above on the current device (synchronises it, reads, clears):
- * bit 0 = a bounded wait of rf_tree_attention gave up, so some output since the last read is
- * unspecified; bit 1 = a position, sequence or length on the device was out of range. */
+/* Error word of the calls of this section and of the two below on the current device
+ * (synchronises it, reads, clears): bit 0 = a bounded wait gave up, so some output since the
+ * last read is unspecified; bit 1 = a position, sequence, length or token on the device was
+ * out of range. */
 int rf_verify_error_word(uint32_t* word);
+
+/* ---- 8-bit rows and their product ----------------------------------------------------
+ * The products of a pass of several tokens (drafts, a prompt) in 8-bit integers: activations
+ * are rows of int8 codes with one f32 scale a token, weights rows of codes with one f32 scale
+ * a channel.  No counterpart in the reference (its activations are f32).  The rules of the
+ * section above hold for pointers, streams, strides and graphs.
+ *
+ * A row y of f32 numbers becomes
+ *   scale = max|y| / 127, 0 where that is below 2^-126;  code = rint(y * (1 / scale)), 0 where scale is 0
+ * in f32, ties to even, codes within +-127.  A row with a number that is not finite has a NaN scale and codes
+ * of 0, so all that is made of it is NaN.  Codes stand for code * scale.  n_cols: 1..65536; strides
+ * in elements (0: n_cols); codes between n_cols and the stride are left as they are. */
+
+/* s = x + add in f32 (add NULL: s = x), rounded to act_type in sum (may be NULL, or x or add itself with the same
+ * stride); then the rows y = (s * weight) * (1 / sqrt(mean(s^2) + eps)) of the f32 sums s
+ * as 8-bit rows: products and reciprocal root rounded to f32, the mean in 64 bits, so that
+ * the codes do not depend on how the work was split.  weight: n_cols f32, NULL: ones.  A row of
+ * zeros with eps 0 counts as one that is not finite. */
+int rf_norm_i8(const void* x, const void* add, void* sum, int act_type, uint32_t n_rows, uint32_t n_cols,
+               uint64_t x_stride, uint64_t add_stride, uint64_t sum_stride, const float* weight, float eps, int8_t* q,
+               uint64_t q_stride, float* scale, void* stream);
+/* y = gate / (1 + exp(-gate)) * up (the SwiGLU of compute.rs:347) as 8-bit rows; y within a few
+ * units of f32's last place.  gate and up may be slices of one projection's rows. */
+int rf_swiglu_i8(const void* gate, const void* up, int act_type, uint32_t n_rows, uint32_t n_cols, uint64_t gate_stride,
+                 uint64_t up_stride, int8_t* q, uint64_t q_stride, float* scale, void* stream);
+/* Rows as they are into the format (weights: one row a channel), and back: out = code * scale. */
+int rf_quantize_i8(const void* x, int act_type, uint32_t n_rows, uint32_t n_cols, uint64_t x_stride, int8_t* q,
+                   uint64_t q_stride, float* scale, void* stream);
+int rf_dequantize_i8(const int8_t* q, const float* scale, void* out, int act_type, uint32_t n_rows, uint32_t n_cols,
+                     uint64_t q_stride, uint64_t out_stride, void* stream);
+/* y[t][n] = (sum_k x[t][k] w[n][k]) * x_scale[t] * w_scale[n] + bias[n] for t < n_tokens, n < n_out:
+ * the sum in whole numbers, exact; then f32 in the order written, rounded to act_type.
+ * bias: n_out f32, or NULL.  x [n_tokens][n_in] and w [n_out][n_in] int8 (any codes, -128 too)
+ * with 16-byte aligned rows (strides multiples of 16); n_in 1..65536; y rows at any
+ * stride >= n_out.  y overlaps no input. */
+int rf_i8_matmul(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const float* bias, void* y,
+                 int act_type, uint32_t n_tokens, uint32_t n_out, uint32_t n_in, uint64_t x_stride, uint64_t w_stride,
+                 uint64_t y_stride, void* stream);
+
+/* ---- the verdict on drafted tokens -----------------------------------------------------
+ * The end of a verification pass: which drafted tokens stand, the token behind them, and the
+ * cache positions of their rows, all on the device.  The rules of the two sections above hold.
+ *
+ * Sequence b has n_draft[b] <= n_tokens drafts (NULL: n_tokens each; n_tokens 0..1024): tokens
+ * [n_seqs][n_tokens], and parent[b][j] < j, the draft that j follows, or -1 where it follows
+ * the history (parent NULL: a chain, j - 1).  Rows of the target: [n_seqs][n_tokens + 1][vocab],
+ * row 0 what it says behind the history, row 1 + j behind draft j.
+ * out_tokens [n_seqs][n_tokens + 1]: the tokens that stand, the one behind them, then -1;
+ * n_accepted [n_seqs]: how many stand; positions [n_seqs][n_tokens] (NULL, or with hist_len):
+ * hist_len[b] + depth for a draft that stands, -1 for the others, as rf_kv_cache_write wants them.
+ * A draft whose token or parent is out of range never stands and raises rf_verify_error_word; a
+ * sequence whose n_draft is out of range gets 0, -1 and -1, and raises it. */
+
+/* By given random numbers, so that the tokens follow the target's probabilities.  target and
+ * draft hold probabilities of prob_type (RF_ACT_*): draft [n_seqs][n_tokens][vocab], row 1 +
+ * parent[b][j] the one that draft j was drawn from (siblings independently, from one row); NULL:
+ * the drafts were certain, each of its token.  At a node with target row p and draft row q the
+ * drafts behind it are tried in order of their index: draft j of token c stands if
+ * accept_u[b][j] * S * q(c) < r(c), where r = p and S = 1 at first; each one that does not
+ * stand changes them to a = a + S (0 at first), r = max(p - a q, 0), S = sum r (certain drafts:
+ * r(c) = 0).  Where none is left, the next token is the least x with r(0) + ... + r(x) > next_u[b] * S, S = sum r
+ * (r = p again where nothing of it is left; numbers below 0 and NaN in p count as 0).  Products and sums in 64
+ * bits.  accept_u [n_seqs][n_tokens] and next_u [n_seqs] are uniform in [0, 1).  A row of the target
+ * without a number above 0 gives the token -1 and raises the error word. */
+int rf_verify_drafts(const void* target, const void* draft, int prob_type, uint32_t vocab, uint32_t n_seqs,
+                     uint32_t n_tokens, uint64_t target_stride, uint64_t draft_stride, const int32_t* tokens,
+                     const int32_t* parent, const int32_t* n_draft, const float* accept_u, const float* next_u,
+                     const int32_t* hist_len, int32_t* out_tokens, int32_t* n_accepted, int32_t* positions, void* stream);
+/* Greedily (the engine's own sampler, sampling.rs:45-56): a draft stands where it is the best token
+ * of its parent's row (largest logit or probability, the first of equal ones; NaN counts as the
+ * least), the lowest index of several.  best [n_seqs][n_tokens + 1] receives the best token of
+ * each row up to n_draft[b]. */
+int rf_verify_greedy(const void* logits, int logit_type, uint32_t vocab, uint32_t n_seqs, uint32_t n_tokens,
+                     uint64_t logits_stride, const int32_t* tokens, const int32_t* parent, const int32_t* n_draft,
+                     const int32_t* hist_len, int32_t* best, int32_t* out_tokens, int32_t* n_accepted, int32_t* positions,
+                     void* stream);
 
 #ifdef __cplusplus
 }

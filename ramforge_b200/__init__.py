@@ -5,10 +5,12 @@ include/rfcuda.h); this package holds its Python host mirror (engine.py),
 ctypes bindings (_lib.py), the synthetic model generator (synth.py) and the
 build script (build.py).
 """
-from .engine import (DecodeEngine, KvView, QMatrix, RfError, decode_attention, kv_cache_read,  # noqa: F401
-                     kv_cache_write, layer_read_plan, qk_norm_rope, selftest_wait, should_keep_resident,
-                     tp_unique_id, tree_attention, verify_error_word)
+from .engine import (DecodeEngine, KvView, QMatrix, RfError, decode_attention, dequantize_i8,  # noqa: F401
+                     i8_matmul, kv_cache_read, kv_cache_write, layer_read_plan, norm_i8, qk_norm_rope, quantize_i8,
+                     selftest_wait, should_keep_resident, swiglu_i8, tp_unique_id, tree_attention, verify_drafts,
+                     verify_error_word, verify_greedy)
 
-__all__ = ["DecodeEngine", "KvView", "QMatrix", "RfError", "decode_attention", "kv_cache_read", "kv_cache_write",
-           "layer_read_plan", "qk_norm_rope", "selftest_wait", "should_keep_resident", "tp_unique_id",
-           "tree_attention", "verify_error_word"]
+__all__ = ["DecodeEngine", "KvView", "QMatrix", "RfError", "decode_attention", "dequantize_i8", "i8_matmul",
+           "kv_cache_read", "kv_cache_write", "layer_read_plan", "norm_i8", "qk_norm_rope", "quantize_i8",
+           "selftest_wait", "should_keep_resident", "swiglu_i8", "tp_unique_id", "tree_attention", "verify_drafts",
+           "verify_error_word", "verify_greedy"]

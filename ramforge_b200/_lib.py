@@ -41,6 +41,8 @@ EXPORTS = [
     "rf_qmatvec", "rf_qgemm", "rf_qgemm_error_word", "rf_decode_attention", "rf_decode_attention_noalloc",
     "rf_should_keep_resident", "rf_layer_read_plan", "rf_plan_residency", "rf_set_layer_cache",
     "rf_qk_norm_rope", "rf_kv_cache_write", "rf_kv_cache_read", "rf_tree_attention", "rf_verify_error_word",
+    "rf_norm_i8", "rf_swiglu_i8", "rf_quantize_i8", "rf_dequantize_i8", "rf_i8_matmul", "rf_verify_drafts",
+    "rf_verify_greedy",
 ]
 
 
@@ -183,6 +185,15 @@ def lib():
             "rf_tree_attention": (c_int, [ctypes.POINTER(KvView), vp, vp, c_int, c_u32, c_u32, c_u32, c_u64, c_u64,
                                           vp, vp, vp, ctypes.c_float, vp]),
             "rf_verify_error_word": (c_int, [u32p]),
+            "rf_norm_i8": (c_int, [vp, vp, vp, c_int, c_u32, c_u32, c_u64, c_u64, c_u64, vp, ctypes.c_float, vp, c_u64,
+                                   vp, vp]),
+            "rf_swiglu_i8": (c_int, [vp, vp, c_int, c_u32, c_u32, c_u64, c_u64, vp, c_u64, vp, vp]),
+            "rf_quantize_i8": (c_int, [vp, c_int, c_u32, c_u32, c_u64, vp, c_u64, vp, vp]),
+            "rf_dequantize_i8": (c_int, [vp, vp, vp, c_int, c_u32, c_u32, c_u64, c_u64, vp]),
+            "rf_i8_matmul": (c_int, [vp, vp, vp, vp, vp, vp, c_int, c_u32, c_u32, c_u32, c_u64, c_u64, c_u64, vp]),
+            "rf_verify_drafts": (c_int, [vp, vp, c_int, c_u32, c_u32, c_u32, c_u64, c_u64, vp, vp, vp, vp, vp, vp, vp,
+                                         vp, vp, vp]),
+            "rf_verify_greedy": (c_int, [vp, c_int, c_u32, c_u32, c_u32, c_u64, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)

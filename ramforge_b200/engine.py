@@ -356,12 +356,69 @@ def tree_attention(cache: KvView, q_ptr: int, out_ptr: int, act_type: int, n_seq
 
 
 def verify_error_word() -> int:
-    """Error word of the four calls above (rf_verify_error_word): bit 0 a wait gave up, bit 1 an index on the device
-    was out of range; reading clears it."""
+    """Error word of the calls on device pointers above and below (rf_verify_error_word): bit 0 a wait gave up, bit 1
+    an index on the device was out of range; reading clears it."""
     w = ctypes.c_uint32()
     check(lib().rf_verify_error_word(ctypes.byref(w)))
     return w.value
 
 
-__all__ = ["DecodeEngine", "KvView", "QMatrix", "decode_attention", "kv_cache_read", "kv_cache_write", "qk_norm_rope",
-           "selftest_wait", "tp_unique_id", "tree_attention", "verify_error_word", "RfError"]
+def norm_i8(x_ptr: int, weight_ptr: int, eps: float, q_ptr: int, scale_ptr: int, act_type: int, n_rows: int,
+            n_cols: int, add_ptr: int = 0, sum_ptr: int = 0, x_stride: int = 0, add_stride: int = 0,
+            sum_stride: int = 0, q_stride: int = 0, stream: int = 0):
+    """Residual addition and RMS norm as 8-bit rows with a scale each (rf_norm_i8); device pointers, strides in
+    elements (0: rows without gaps), weight 0: ones."""
+    check(lib().rf_norm_i8(x_ptr, add_ptr, sum_ptr, act_type, n_rows, n_cols, x_stride, add_stride, sum_stride,
+                           weight_ptr, eps, q_ptr, q_stride, scale_ptr, stream))
+
+
+def swiglu_i8(gate_ptr: int, up_ptr: int, q_ptr: int, scale_ptr: int, act_type: int, n_rows: int, n_cols: int,
+              gate_stride: int = 0, up_stride: int = 0, q_stride: int = 0, stream: int = 0):
+    """silu(gate) * up as 8-bit rows with a scale each (rf_swiglu_i8)."""
+    check(lib().rf_swiglu_i8(gate_ptr, up_ptr, act_type, n_rows, n_cols, gate_stride, up_stride, q_ptr, q_stride,
+                             scale_ptr, stream))
+
+
+def quantize_i8(x_ptr: int, q_ptr: int, scale_ptr: int, act_type: int, n_rows: int, n_cols: int, x_stride: int = 0,
+                q_stride: int = 0, stream: int = 0):
+    """Rows as 8-bit codes with a scale each (rf_quantize_i8)."""
+    check(lib().rf_quantize_i8(x_ptr, act_type, n_rows, n_cols, x_stride, q_ptr, q_stride, scale_ptr, stream))
+
+
+def dequantize_i8(q_ptr: int, scale_ptr: int, out_ptr: int, act_type: int, n_rows: int, n_cols: int,
+                  q_stride: int = 0, out_stride: int = 0, stream: int = 0):
+    """The numbers that 8-bit rows stand for (rf_dequantize_i8)."""
+    check(lib().rf_dequantize_i8(q_ptr, scale_ptr, out_ptr, act_type, n_rows, n_cols, q_stride, out_stride, stream))
+
+
+def i8_matmul(x_ptr: int, x_scale_ptr: int, w_ptr: int, w_scale_ptr: int, y_ptr: int, act_type: int, n_tokens: int,
+              n_out: int, n_in: int, x_stride: int = 0, w_stride: int = 0, y_stride: int = 0, bias_ptr: int = 0,
+              stream: int = 0):
+    """Y = X W^T of 8-bit rows, scales per token and channel (rf_i8_matmul); x and w rows at multiples of 16 bytes."""
+    check(lib().rf_i8_matmul(x_ptr, x_scale_ptr, w_ptr, w_scale_ptr, bias_ptr, y_ptr, act_type, n_tokens, n_out, n_in,
+                             x_stride, w_stride, y_stride, stream))
+
+
+def verify_drafts(target_ptr: int, draft_ptr: int, prob_type: int, vocab: int, n_seqs: int, n_tokens: int,
+                  tokens_ptr: int, accept_u_ptr: int, next_u_ptr: int, out_tokens_ptr: int, n_accepted_ptr: int,
+                  parent_ptr: int = 0, n_draft_ptr: int = 0, hist_len_ptr: int = 0, positions_ptr: int = 0,
+                  target_stride: int = 0, draft_stride: int = 0, stream: int = 0):
+    """Which drafted tokens stand by the target's probabilities and given random numbers, and the token behind them
+    (rf_verify_drafts); parent 0: chains, draft 0: drafts that were certain."""
+    check(lib().rf_verify_drafts(target_ptr, draft_ptr, prob_type, vocab, n_seqs, n_tokens, target_stride,
+                                 draft_stride, tokens_ptr, parent_ptr, n_draft_ptr, accept_u_ptr, next_u_ptr,
+                                 hist_len_ptr, out_tokens_ptr, n_accepted_ptr, positions_ptr, stream))
+
+
+def verify_greedy(logits_ptr: int, logit_type: int, vocab: int, n_seqs: int, n_tokens: int, tokens_ptr: int,
+                  best_ptr: int, out_tokens_ptr: int, n_accepted_ptr: int, parent_ptr: int = 0, n_draft_ptr: int = 0,
+                  hist_len_ptr: int = 0, positions_ptr: int = 0, logits_stride: int = 0, stream: int = 0):
+    """Which drafted tokens are the target's best ones, and the best one behind them (rf_verify_greedy)."""
+    check(lib().rf_verify_greedy(logits_ptr, logit_type, vocab, n_seqs, n_tokens, logits_stride, tokens_ptr,
+                                 parent_ptr, n_draft_ptr, hist_len_ptr, best_ptr, out_tokens_ptr, n_accepted_ptr,
+                                 positions_ptr, stream))
+
+
+__all__ = ["DecodeEngine", "KvView", "QMatrix", "decode_attention", "dequantize_i8", "i8_matmul", "kv_cache_read",
+           "kv_cache_write", "norm_i8", "qk_norm_rope", "quantize_i8", "selftest_wait", "swiglu_i8", "tp_unique_id",
+           "tree_attention", "verify_drafts", "verify_error_word", "verify_greedy", "RfError"]
