@@ -2,10 +2,17 @@
 //
 // The sums are whole 32-bit numbers and exact, so any split of the work gives the same bits:
 //   y[t][n] = f32(f32(f32(sum) * x_scale[t]) * w_scale[n]) + bias[n], rounded to the output's type.
+//
+// The products run on tcgen05 (kind::i8) with channels as the rows of a tile and tokens as its columns: few tokens
+// fill a tile of few columns, and a warp's 32 lanes of the accumulator are 32 consecutive outputs of one token.
+#include <cuda.h>
+
 #include <algorithm>
+#include <atomic>
 
 #include "rf_act.cuh"
 #include "rf_device.cuh"
+#include "rf_tc.cuh"
 #include "rf_verify.h"
 
 namespace rf {
@@ -21,56 +28,284 @@ struct MatmulArgs {
   uint32_t n_tokens, n_out, n_in;
 };
 
-// The simplest form: a CTA has 64 tokens x 64 channels, a thread 4 x 4 of them, 64 elements of both a step.
-template <class T>
-__global__ void __launch_bounds__(256) i8_tile_kernel(MatmulArgs a) {
-  __shared__ uint32_t xs[64][17], ws[64][17];
-  griddep_launch();
-  griddep_wait();
-  const uint32_t tid = threadIdx.x, t0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = tid & 15, ty = tid >> 4;
-  int acc[4][4] = {};
-  for (uint32_t k0 = 0; k0 < a.n_in; k0 += 64) {
-    const uint32_t r = tid >> 2, c = (tid & 3) * 16;
-    auto fetch = [&](uint32_t (*s)[17], const int8_t* base, uint64_t stride, uint32_t row, uint32_t rows) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (row < rows && k0 + c < a.n_in) {
-        u = *reinterpret_cast<const uint4*>(base + row * stride + k0 + c);  // rows end in whole 16-byte pieces
-        uint32_t* w = &u.x;
-        for (uint32_t j = 0; j < 16; j++)
-          if (k0 + c + j >= a.n_in) w[j / 4] &= ~(0xffu << (8 * (j & 3)));
-      }
-      s[r][c / 4] = u.x, s[r][c / 4 + 1] = u.y, s[r][c / 4 + 2] = u.z, s[r][c / 4 + 3] = u.w;
-    };
-    fetch(xs, a.x, a.x_stride, t0 + r, a.n_tokens);
-    fetch(ws, a.w, a.w_stride, n0 + r, a.n_out);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; k++) {
-      int xv[4], wv[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) xv[i] = (int)xs[ty + 16 * i][k], wv[i] = (int)ws[tx + 16 * i][k];
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xv[i], wv[j], acc[i][j]);
+// ---- waits, tensor memory, copies -------------------------------------------------------
+// Bounded wait for the phase of `bar` with `parity`; false once any wait of the CTA gave up.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+  const long long t0 = clock64();
+  while (!tc_mbar_try_wait(bar, parity)) {
+    if (*stop) return false;
+    if (clock64() - t0 > 2000000000LL) {
+      *stop = 1;
+      atomicOr(err, kVerifyTimeout);
+      return false;
     }
-    __syncthreads();
   }
+  return true;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+  const uint32_t b = tc_smem_u32(bar);
+  return tc_mbar_try_wait(b, parity) || wait_slow(b, parity, stop, err);
+}
+// 16 columns of the thread's lane (32 * (warp % 4) + lane).
+__device__ __forceinline__ void tmem_ld_16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
+      "}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < 16; i++) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+// K-major operand of 128-byte rows, 128-byte swizzle: groups of 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+// kind::i8: signed codes, 32-bit sums, M x N.
+__device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) {
+  return 2u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (m >> 4) << 24;
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// 16 bytes at shared address `addr` of the cluster's CTA `rank`.
+__device__ __forceinline__ int4 ld_cluster16(uint32_t addr, uint32_t rank) {
+  int4 v;
+  asm volatile(
+      "{ .reg .b32 a; mapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.b32 {%0,%1,%2,%3}, [a]; }"
+      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+// Four channels n .. n + 3 of token t.
+template <class T>
+__device__ __forceinline__ void put4(const MatmulArgs& a, uint32_t t, uint32_t n, const float (&v)[4], bool wide) {
+  T* y = (T*)a.y + t * a.y_stride + n;
+  if (wide && n + 4 <= a.n_out) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      T h[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) Act<T>::put(h + i, v[i]);
+      *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(h);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (n + i < a.n_out) Act<T>::put(y + i, v[i]);
+  }
+}
+
+constexpr uint32_t TM = 128, TK = 128;  // channels of a tile, elements of a step
+
+// ---------------------------------------------------------------------------
+// One tile a cluster, its elements split over the cluster's CTAs: i8_split_kernel.
+//
+// A CTA has 128 channels x `cols` tokens and a run of the steps; warp 0 copies 128 bytes of each row a step through a
+// ring of `stages`, warp 1 multiplies, and the CTAs' sums meet in shared memory, where each CTA adds and writes its
+// share of the tile.  Tensor memory is given back before the CTAs wait for one another, so that no two clusters can
+// wait for each other's columns, and taken only after the kernel before has ended, whose CTAs may still need it.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kMaxStages = 12;
+
+struct SplitArgs {
+  MatmulArgs a;
+  uint32_t cols, n_tiles, stages, tmem_cols, steps, split;
+  bool wide;  // y takes four outputs at once
+  unsigned* err;
+};
+
+template <class T>
+__global__ void __launch_bounds__(128)
+    i8_split_kernel(const SplitArgs s, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w) {
+  extern __shared__ uint8_t dyn[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  __shared__ uint32_t s_tmem, s_stop;
+  __shared__ float s_x[256], s_w[TM], s_b[TM];
+  const MatmulArgs& a = s.a;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = (tc_smem_u32(dyn) + 1023) & ~1023u, stage = TM * TK + s.cols * TK;
+  const uint32_t rank = blockIdx.x % s.split, tile = blockIdx.x / s.split;
+  const uint32_t n0 = tile / s.n_tiles * TM, t0 = tile % s.n_tiles * s.cols;
+  const uint32_t k0 = s.steps * rank / s.split, k1 = s.steps * (rank + 1) / s.split;
+  if (tid == 0) {
+    for (uint32_t i = 0; i < s.stages; i++) tc_mbar_init(tc_smem_u32(full + i), 1), tc_mbar_init(tc_smem_u32(empty + i), 1);
+    tc_mbar_init(tc_smem_u32(&done), 1);
+    tc_fence_barrier_init();
+    s_stop = 0;
+    for (uint32_t i = k0; i < min(k0 + s.stages, k1); i++) tma_prefetch(&map_w, i * TK, n0);  // into L2: safe before the wait
+  }
+  griddep_wait();
+  if (warp == 2) tc_tmem_alloc(tc_smem_u32(&s_tmem), s.tmem_cols);
+  for (uint32_t t = tid; t < s.cols; t += 128) s_x[t] = t0 + t < a.n_tokens ? a.x_scale[t0 + t] : 0.f;
+  s_w[tid] = n0 + tid < a.n_out ? a.w_scale[n0 + tid] : 0.f;
+  s_b[tid] = a.bias && n0 + tid < a.n_out ? a.bias[n0 + tid] : 0.f;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  griddep_launch();
+  const uint32_t tmem = s_tmem;
+  volatile uint32_t* stop = &s_stop;
+
+  if (warp == 0 && lane == 0) {
+    uint32_t slot = 0, phase = 0, k = k0;
+    for (; k < k1; k++) {
+      if (k >= k0 + s.stages && !wait_bar(empty + slot, phase ^ 1, stop, s.err)) break;
+      const uint32_t bar = tc_smem_u32(full + slot), dst = ring + slot * stage;
+      tc_mbar_expect_tx(bar, stage);
+      tma_load(dst, &map_w, k * TK, n0, bar);
+      tma_load(dst + TM * TK, &map_x, k * TK, t0, bar);
+      if (++slot == s.stages) slot = 0, phase ^= 1;
+    }
+    if (k < k1)  // gave up: the copies in flight are waited for all the same
+      for (uint32_t i = 0; i < min(k - k0, s.stages); i++) {
+        if (slot-- == 0) slot = s.stages - 1, phase ^= 1;
+        tc_mbar_wait(tc_smem_u32(full + slot), phase);
+      }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = idesc_i8(TM, s.cols);
+    uint32_t slot = 0, phase = 0;
+    for (uint32_t k = k0; k < k1; k++) {
+      if (!wait_bar(full + slot, phase, stop, s.err)) break;
+      tc_fence_after_sync();
+      const uint64_t da = operand_desc(ring + slot * stage), db = operand_desc(ring + slot * stage + TM * TK);
+#pragma unroll
+      for (int i = 0; i < 4; i++) mma_i8(tmem, da + 2 * i, db + 2 * i, idesc, k > k0 || i > 0);
+      tc_commit(tc_smem_u32(empty + slot));
+      if (++slot == s.stages) slot = 0, phase ^= 1;
+    }
+    tc_commit(tc_smem_u32(&done));
+  }
+  __syncwarp();
+  const bool good = wait_bar(&done, 0, stop, s.err);
+  if (!good) tc_mbar_wait(tc_smem_u32(&done), 0);
+  tc_fence_after_sync();
+
+  // the sums as [token][channel] over the ring, which all copies and products are through with
+  const uint32_t tokens = min(s.cols, a.n_tokens - t0);
+  __syncwarp();
+  for (uint32_t c = 0; c < tokens; c += 16) {
+    uint32_t r[16];
+    tmem_ld_16(tmem + (warp << 21) + c, r);
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (c + i < tokens) asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + ((c + i) * TM + tid) * 4), "r"(r[i]) : "memory");
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after_sync();
+    tc_tmem_dealloc(tmem, s.tmem_cols);
+  }
+  __syncwarp();
+  if (s.split > 1) cluster_arrive(), cluster_wait();
+  const uint32_t pieces = tokens * (TM / 4);
+  for (uint32_t i = pieces * rank / s.split + tid; i < pieces * (rank + 1) / s.split; i += 128) {
+    int4 sum = make_int4(0, 0, 0, 0);
+    for (uint32_t r = 0; r < s.split; r++) {
+      const int4 v = ld_cluster16(ring + i * 16, r);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const uint32_t t = i / (TM / 4), c = i % (TM / 4) * 4;
+    const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
+    float v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const uint32_t t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (t >= a.n_tokens || n >= a.n_out) continue;
-      float v = __fmul_rn(__fmul_rn((float)acc[i][j], a.x_scale[t]), a.w_scale[n]);
-      if (a.bias) v = __fadd_rn(v, a.bias[n]);
-      Act<T>::put((T*)a.y + t * a.y_stride + n, v);
+      v[j] = __fmul_rn(__fmul_rn((float)acc[j], s_x[t]), s_w[c + j]);
+      if (a.bias) v[j] = __fadd_rn(v[j], s_b[c + j]);
     }
+    if (good) put4<T>(a, t0 + t, n0 + c, v, s.wide);
+  }
+  if (s.split > 1) cluster_arrive(), cluster_wait();
+}
+
+// Tensor map of 8-bit rows, copied in boxes of 128 elements x box_rows.
+int rows_map(CUtensorMap* map, const int8_t* p, uint64_t n_cols, uint64_t n_rows, uint64_t stride, uint32_t box_rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<void*> known{nullptr};  // calls may come from several threads
+  void* fn = known.load(std::memory_order_relaxed);
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    RF_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !fn) return set_error(RF_ECUDA, "cuTensorMapEncodeTiled is not available");
+    known.store(fn, std::memory_order_relaxed);
+  }
+  const cuuint64_t dims[2] = {n_cols, n_rows}, strides[1] = {stride};
+  const cuuint32_t box[2] = {TK, box_rows}, step[2] = {1, 1};
+  const CUresult r = ((Encode)fn)(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, box, step,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(RF_ECUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+  return RF_OK;
 }
 
 template <class T>
-cudaError_t launch(const Launch& L, const MatmulArgs& a) {
-  return launch_k(L, i8_tile_kernel<T>, dim3((a.n_out + 63) / 64, (a.n_tokens + 63) / 64), dim3(256), 0, a);
+int run_split(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
+  SplitArgs s{};
+  s.a = a, s.err = err;
+  s.n_tiles = (a.n_tokens + 255) / 256;
+  s.cols = ((a.n_tokens + s.n_tiles - 1) / s.n_tiles + 15) / 16 * 16;
+  s.n_tiles = (a.n_tokens + s.cols - 1) / s.cols;
+  s.steps = (a.n_in + TK - 1) / TK;
+  s.tmem_cols = s.cols <= 32 ? 32 : s.cols <= 64 ? 64 : s.cols <= 128 ? 128 : 256;
+  s.wide = aligned_to(a.y, 4 * sizeof(T)) && a.y_stride % 4 == 0;
+  const uint32_t stage = (TM + s.cols) * TK, per_sm = s.cols <= 64 ? 2 : 1, m_tiles = (a.n_out + TM - 1) / TM;
+  s.stages = std::min(std::min(((per_sm == 2 ? 108u : 216u) * 1024) / stage, kMaxStages), s.steps);
+  const uint64_t tiles = (uint64_t)m_tiles * s.n_tiles, slots = (uint64_t)num_sms() * per_sm;
+  // the split for which the longest CTA has the least to do, counting what a CTA costs as 8 steps
+  s.split = 1;
+  uint64_t best = ~0ull;
+  for (uint32_t c = 1; c <= 8 && c <= s.steps; c++) {
+    const uint64_t cost = ((tiles * c + slots - 1) / slots) * ((s.steps + c - 1) / c + 8);
+    if (cost < best) best = cost, s.split = c;
+  }
+  if (tiles * s.split > 0x7fffffffull) return set_error(RF_EINVAL, "%u tokens x %u channels are too many for one call", a.n_tokens, a.n_out);
+  CUtensorMap mx{}, mw{};
+  RF_TRY(rows_map(&mx, a.x, a.n_in, a.n_tokens, a.x_stride, s.cols));
+  RF_TRY(rows_map(&mw, a.w, a.n_in, a.n_out, a.w_stride, TM));
+  const size_t smem = 1024 + std::max((size_t)s.stages * stage, (size_t)s.cols * TM * 4);
+  auto* k = i8_split_kernel<T>;
+  RF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(217 * 1024)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((uint32_t)(tiles * s.split));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = s.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = s.split > 1 ? 2 : 1;
+  RF_CUDA(cudaLaunchKernelEx(&cfg, k, s, mx, mw));
+  return RF_OK;
 }
 
 int check_operand(const char* name, const int8_t* p, uint64_t* stride, uint32_t n_in) {
@@ -108,13 +343,14 @@ int rf_i8_matmul(const int8_t* x, const float* x_scale, const int8_t* w, const f
     return set_error(RF_EINVAL, "scales and bias must be 4-byte aligned");
   if (!n_tokens || !n_out) return RF_OK;
   const MatmulArgs a{x, w, x_scale, w_scale, bias, y, x_stride, w_stride, y_stride, n_tokens, n_out, n_in};
-  const Launch L{(cudaStream_t)stream, true};
+  unsigned* err = nullptr;
+  RF_TRY(verify_error_ptr(&err));
+  const cudaStream_t st = (cudaStream_t)stream;
   switch (act_type) {
-    case RF_ACT_F32: RF_CUDA(launch<float>(L, a)); break;
-    case RF_ACT_F16: RF_CUDA(launch<__half>(L, a)); break;
-    default: RF_CUDA(launch<__nv_bfloat16>(L, a));
+    case RF_ACT_F32: return run_split<float>(st, a, err);
+    case RF_ACT_F16: return run_split<__half>(st, a, err);
+    default: return run_split<__nv_bfloat16>(st, a, err);
   }
-  return RF_OK;
 }
 
 }  // extern "C"
