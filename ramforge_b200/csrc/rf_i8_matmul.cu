@@ -242,6 +242,196 @@ __global__ void __launch_bounds__(128)
   if (s.split > 1) cluster_arrive(), cluster_wait();
 }
 
+// ---------------------------------------------------------------------------
+// Many tiles: i8_pair_kernel.
+//
+// A pair of CTAs (cta_group::2) has 256 channels x `cols` tokens: each holds 128 rows of W and half of the tokens'
+// rows of X in its shared memory, and the sums of its channels in its tensor memory, so an SM reads 256 rows a step
+// for 128 x 256 sums where a CTA alone reads 384.  At 8 bits that is what bounds it: 64 bytes a cycle and SM would
+// feed the tensor cores' full rate.  Pairs stay and go from tile to tile; two accumulators, so that warps 4 to 7 write one out
+// while the next fills.  Tokens' tiles come first in the order, so that a W tile is read by all of them at about one time.
+//
+//   warp 0  copies (both CTAs, completing on the first one's barriers)
+//   warp 1  tcgen05.mma (the first CTA, for both)
+//   warps 4 - 7  results
+// ---------------------------------------------------------------------------
+struct PairArgs {
+  MatmulArgs a;
+  uint32_t cols, n_tiles, tiles, stages, steps;
+  unsigned* err;
+};
+
+__device__ __forceinline__ uint32_t map_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// A copy of one of the pair that completes on a barrier of either.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+// Arrive on `bar` of both CTAs when the products issued before are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+      "}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
+}
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256)
+    i8_pair_kernel(const PairArgs s, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w) {
+  extern __shared__ uint8_t dyn[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
+  __shared__ uint32_t s_tmem, s_stop;
+  __shared__ __align__(16) float s_x[4][256];
+  const MatmulArgs& a = s.a;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1, pair = blockIdx.x >> 1;
+  const uint32_t pairs = gridDim.x >> 1, half = s.cols / 2;
+  const uint32_t ring = (tc_smem_u32(dyn) + 1023) & ~1023u, stage = (TM + half) * TK;
+  if (tid == 0) {
+    for (uint32_t i = 0; i < s.stages; i++) tc_mbar_init(tc_smem_u32(full + i), 1), tc_mbar_init(tc_smem_u32(empty + i), 1);
+    for (int i = 0; i < 2; i++) tc_mbar_init(tc_smem_u32(acc_full + i), 1), tc_mbar_init(tc_smem_u32(acc_free + i), 8);
+    tc_fence_barrier_init();
+    s_stop = 0;
+  }
+  griddep_wait();
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc_smem_u32(&s_tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_arrive(), cluster_wait();
+  tc_fence_after_sync();
+  griddep_launch();
+  const uint32_t tmem = s_tmem;
+  volatile uint32_t* stop = &s_stop;
+
+  if (warp == 0 && lane == 0) {
+    uint32_t slot = 0, phase = 0, uses = 0;
+    bool ok = true;
+    for (uint32_t tile = pair; tile < s.tiles && ok; tile += pairs) {
+      const int n0 = tile / s.n_tiles * (2 * TM) + rank * TM, t0 = tile % s.n_tiles * s.cols + rank * half;
+      for (uint32_t k = 0; k < s.steps; k++) {
+        if (!wait_bar(empty + slot, phase ^ 1, stop, s.err)) {
+          ok = false;
+          break;
+        }
+        const uint32_t bar = map_cluster(tc_smem_u32(full + slot), 0), dst = ring + slot * stage;
+        if (rank == 0) tc_mbar_expect_tx(tc_smem_u32(full + slot), 2 * stage);
+        tma_load_pair(dst, &map_w, k * TK, n0, bar);
+        tma_load_pair(dst + TM * TK, &map_x, k * TK, t0, bar);
+        uses++;
+        if (++slot == s.stages) slot = 0, phase ^= 1;
+      }
+    }
+    // the last products release their slots in both CTAs: neither ends before
+    for (uint32_t i = 0; i < min(uses, s.stages) && ok; i++) {
+      if (slot-- == 0) slot = s.stages - 1, phase ^= 1;
+      ok = wait_bar(empty + slot, phase, stop, s.err);
+    }
+    if (!ok) {  // gave up: copies in flight end within this time
+      const long long t = clock64();
+      while (clock64() - t < 4000000LL) {
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    const uint32_t idesc = idesc_i8(2 * TM, s.cols);
+    uint32_t slot = 0, phase = 0, buf = 0, turn = 0;
+    bool ok = true;
+    for (uint32_t tile = pair; tile < s.tiles && ok; tile += pairs) {
+      ok = wait_bar(acc_free + buf, turn ^ 1, stop, s.err);
+      tc_fence_after_sync();
+      for (uint32_t k = 0; k < s.steps && ok; k++) {
+        if (!(ok = wait_bar(full + slot, phase, stop, s.err))) break;
+        tc_fence_after_sync();
+        const uint64_t da = operand_desc(ring + slot * stage), db = operand_desc(ring + slot * stage + TM * TK);
+#pragma unroll
+        for (int i = 0; i < 4; i++) mma_i8_pair(tmem + buf * 256, da + 2 * i, db + 2 * i, idesc, k > 0 || i > 0);
+        commit_pair(tc_smem_u32(empty + slot));
+        if (++slot == s.stages) slot = 0, phase ^= 1;
+      }
+      commit_pair(tc_smem_u32(acc_full + buf));
+      if (++buf == 2) buf = 0, turn ^= 1;
+    }
+  } else if (warp >= 4) {
+    const uint32_t e = warp - 4;
+    uint32_t buf = 0, turn = 0;
+    for (uint32_t tile = pair; tile < s.tiles; tile += pairs) {
+      const uint32_t n = tile / s.n_tiles * (2 * TM) + rank * TM + 32 * e + lane, t0 = tile % s.n_tiles * s.cols;
+      const uint32_t tokens = min(s.cols, a.n_tokens - t0);
+      const bool live = n < a.n_out;
+      const float sw = live ? a.w_scale[n] : 0.f, bias = live && a.bias ? a.bias[n] : 0.f;
+      for (uint32_t t = lane; t < s.cols; t += 32) s_x[e][t] = t < tokens ? a.x_scale[t0 + t] : 0.f;
+      __syncwarp();
+      const bool good = wait_bar(acc_full + buf, turn, stop, s.err);
+      __syncwarp();
+      tc_fence_after_sync();
+      T* y = (T*)a.y + (uint64_t)t0 * a.y_stride + n;
+      for (uint32_t c = 0; c < s.cols; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32(tmem + (e << 21) + buf * 256 + c, r);
+        if (c + 32 >= s.cols) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                             map_cluster(tc_smem_u32(acc_free + buf), 0))
+                         : "memory");
+        }
+        if (!live || !good) continue;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          if (c + i < tokens) {
+            float v = __fmul_rn(__fmul_rn((float)(int)r[i], s_x[e][c + i]), sw);
+            if (a.bias) v = __fadd_rn(v, bias);
+            Act<T>::put(y, v);
+          }
+          y += a.y_stride;
+        }
+      }
+      __syncwarp();
+      if (++buf == 2) buf = 0, turn ^= 1;
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_arrive(), cluster_wait();
+  if (warp == 2) {
+    tc_fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
 // Tensor map of 8-bit rows, copied in boxes of 128 elements x box_rows.
 int rows_map(CUtensorMap* map, const int8_t* p, uint64_t n_cols, uint64_t n_rows, uint64_t stride, uint32_t box_rows) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -308,6 +498,37 @@ int run_split(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   return RF_OK;
 }
 
+template <class T>
+int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
+  PairArgs s{};
+  s.a = a, s.err = err;
+  s.n_tiles = (a.n_tokens + 255) / 256;
+  s.cols = ((a.n_tokens + s.n_tiles - 1) / s.n_tiles + 31) / 32 * 32;
+  s.n_tiles = (a.n_tokens + s.cols - 1) / s.cols;
+  s.steps = (a.n_in + TK - 1) / TK;
+  const uint64_t tiles = (uint64_t)((a.n_out + 2 * TM - 1) / (2 * TM)) * s.n_tiles;
+  if (tiles > 0x7fffffffull) return set_error(RF_EINVAL, "%u tokens x %u channels are too many for one call", a.n_tokens, a.n_out);
+  s.tiles = (uint32_t)tiles;
+  // the whole of an SM's shared memory, also where fewer stages would do: two pairs never share an SM's tensor memory
+  const uint32_t stage = (TM + s.cols / 2) * TK;
+  s.stages = std::min(208u * 1024 / stage, kMaxStages);
+  CUtensorMap mx{}, mw{};
+  RF_TRY(rows_map(&mx, a.x, a.n_in, a.n_tokens, a.x_stride, s.cols / 2));
+  RF_TRY(rows_map(&mw, a.w, a.n_in, a.n_out, a.w_stride, TM));
+  const size_t smem = 209 * 1024;
+  auto* k = i8_pair_kernel<T>;
+  RF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const uint32_t pairs = std::min<uint32_t>(s.tiles, std::max(1, num_sms() / 2));
+  RF_CUDA(launch_k(Launch{st, true}, k, dim3(2 * pairs), dim3(256), smem, s, mx, mw));
+  return RF_OK;
+}
+
+template <class T>
+int run(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
+  const uint64_t pair_tiles = (uint64_t)((a.n_out + 2 * TM - 1) / (2 * TM)) * ((a.n_tokens + 255) / 256);
+  return pair_tiles >= (uint64_t)num_sms() / 2 && a.n_tokens > 128 ? run_pair<T>(st, a, err) : run_split<T>(st, a, err);
+}
+
 int check_operand(const char* name, const int8_t* p, uint64_t* stride, uint32_t n_in) {
   if (!*stride) *stride = n_in;
   if (*stride < n_in)
@@ -347,9 +568,9 @@ int rf_i8_matmul(const int8_t* x, const float* x_scale, const int8_t* w, const f
   RF_TRY(verify_error_ptr(&err));
   const cudaStream_t st = (cudaStream_t)stream;
   switch (act_type) {
-    case RF_ACT_F32: return run_split<float>(st, a, err);
-    case RF_ACT_F16: return run_split<__half>(st, a, err);
-    default: return run_split<__nv_bfloat16>(st, a, err);
+    case RF_ACT_F32: return run<float>(st, a, err);
+    case RF_ACT_F16: return run<__half>(st, a, err);
+    default: return run<__nv_bfloat16>(st, a, err);
   }
 }
 

@@ -49,7 +49,8 @@ SHAPES = [(1, 1, 1), (1, 6144, 4096), (2, 130, 16), (3, 127, 17), (7, 1000, 4096
           (48, 1000, 640), (64, 4096, 4096), (65, 28672, 512), (100, 333, 333), (128, 4096, 4096), (129, 384, 4096),
           (200, 5000, 96), (255, 130, 4096), (256, 2048, 2048), (257, 4097, 1023), (333, 4096, 4096), (400, 1, 100),
           (513, 700, 65536), (600, 6144, 4096), (1000, 5555, 777), (2048, 4096, 1024), (2049, 14336, 272),
-          (4096, 4096, 64), (3, 128256, 512), (1, 64, 65536), (16, 40, 65536)]
+          (4096, 4096, 64), (3, 128256, 512), (1, 64, 65536), (16, 40, 65536),
+          (130, 20000, 300), (257, 10001, 333), (384, 12800, 128), (145, 37900, 1000), (4000, 300, 64), (9000, 200, 50)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -64,7 +65,7 @@ def test_shapes(t, n, k, dtype):
     assert verify_error_word() == 0
 
 
-@pytest.mark.parametrize("t,n,k", [(1, 300, 500), (12, 300, 500), (300, 300, 500), (700, 4200, 500)])
+@pytest.mark.parametrize("t,n,k", [(1, 300, 500), (12, 300, 500), (300, 300, 500), (700, 9000, 500)])
 @pytest.mark.parametrize("pad", [0, 16, 48])
 def test_strides(t, n, k, pad):
     """Slices of wider buffers: rows of y between others' columns stay as they are, one element off alignment too."""
