@@ -248,18 +248,20 @@ __global__ void __launch_bounds__(128)
 // A pair of CTAs (cta_group::2) has 256 channels x `cols` tokens: each holds 128 rows of W and half of the tokens'
 // rows of X in its shared memory, and the sums of its channels in its tensor memory, so an SM reads 256 rows a step
 // for 128 x 256 sums where a CTA alone reads 384.  At 8 bits that is what bounds it: 64 bytes a cycle and SM would
-// feed the tensor cores' full rate.  Pairs stay and go from tile to tile; two accumulators, so that warps 4 to 7 write one out
+// feed the tensor cores' full rate.  Pairs stay and go from tile to tile; two accumulators, so that warps 4 to 11 write one out
 // while the next fills.  Tokens' tiles come first in the order, so that a W tile is read by all of them at about one time.
 //
 //   warp 0  copies (both CTAs, completing on the first one's barriers)
 //   warp 1  tcgen05.mma (the first CTA, for both)
-//   warps 4 - 7  results
+//   warps 4 - 11  results
 // ---------------------------------------------------------------------------
 struct PairArgs {
   MatmulArgs a;
   uint32_t cols, n_tiles, tiles, stages, steps;
+  bool wide;  // y takes whole 4-byte words
   unsigned* err;
 };
+constexpr int kPairThreads = 384;
 
 __device__ __forceinline__ uint32_t map_cluster(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -305,20 +307,84 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t (&r)[32]) {
   for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
 }
 
+// Products of pairs of f32 in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
 template <class T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256)
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Sums r of 32 tokens (rows of y from y on) of the channel nw + lane, a warp's 32 channels whole.  Of 16-bit outputs the
+// lanes 2i and 2i + 1 exchange one each, so that each stores two channels of one token.
+template <class T>
+__device__ __forceinline__ void put_columns(T* y, uint64_t stride, uint32_t nw, uint32_t lane, const uint32_t (&r)[32],
+                                            const float* sx, float sw, bool add, float bias) {
+  const float2 w2 = make_float2(sw, sw);
+  y += sizeof(T) == 4 ? nw + lane : nw + (lane & 30) + (lane & 1) * stride;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(sx + i);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int j = i + 2 * h;
+      float2 v = make_float2((float)(int)r[j], (float)(int)r[j + 1]);
+      v = mul2(mul2(v, h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)), w2);
+      if (add) v.x = __fadd_rn(v.x, bias), v.y = __fadd_rn(v.y, bias);
+      if constexpr (sizeof(T) == 4) {
+        Act<T>::put(y, v.x);
+        Act<T>::put(y + stride, v.y);
+      } else {
+        const bool odd = lane & 1;
+        const float other = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1);
+        *reinterpret_cast<uint32_t*>(y) = pack2<T>(odd ? other : v.x, odd ? v.y : other);
+      }
+      y += 2 * stride;
+    }
+  }
+}
+// The same for one channel (at y) and `count` tokens.
+template <class T>
+__device__ __forceinline__ void put_columns_any(T* y, uint64_t stride, uint32_t count, const uint32_t (&r)[32],
+                                                const float* sx, float sw, bool add, float bias) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) {
+    if (i < count) {
+      float v = __fmul_rn(__fmul_rn((float)(int)r[i], sx[i]), sw);
+      if (add) v = __fadd_rn(v, bias);
+      Act<T>::put(y, v);
+    }
+    y += stride;
+  }
+}
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
     i8_pair_kernel(const PairArgs s, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w) {
   extern __shared__ uint8_t dyn[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
   __shared__ uint32_t s_tmem, s_stop;
-  __shared__ __align__(16) float s_x[4][256];
+  __shared__ __align__(16) float s_x[8][256];
   const MatmulArgs& a = s.a;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1, pair = blockIdx.x >> 1;
   const uint32_t pairs = gridDim.x >> 1, half = s.cols / 2;
   const uint32_t ring = (tc_smem_u32(dyn) + 1023) & ~1023u, stage = (TM + half) * TK;
   if (tid == 0) {
     for (uint32_t i = 0; i < s.stages; i++) tc_mbar_init(tc_smem_u32(full + i), 1), tc_mbar_init(tc_smem_u32(empty + i), 1);
-    for (int i = 0; i < 2; i++) tc_mbar_init(tc_smem_u32(acc_full + i), 1), tc_mbar_init(tc_smem_u32(acc_free + i), 8);
+    for (int i = 0; i < 2; i++) tc_mbar_init(tc_smem_u32(acc_full + i), 1), tc_mbar_init(tc_smem_u32(acc_free + i), 16);
     tc_fence_barrier_init();
     s_stop = 0;
   }
@@ -383,42 +449,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256)
       if (++buf == 2) buf = 0, turn ^= 1;
     }
   } else if (warp >= 4) {
-    const uint32_t e = warp - 4;
+    const uint32_t e = warp & 3, set = (warp - 4) >> 2;  // channels 32 e on, every other 32 columns
+    float* sx = s_x[warp - 4];
     uint32_t buf = 0, turn = 0;
     for (uint32_t tile = pair; tile < s.tiles; tile += pairs) {
-      const uint32_t n = tile / s.n_tiles * (2 * TM) + rank * TM + 32 * e + lane, t0 = tile % s.n_tiles * s.cols;
+      const uint32_t nw = tile / s.n_tiles * (2 * TM) + rank * TM + 32 * e, n = nw + lane, t0 = tile % s.n_tiles * s.cols;
       const uint32_t tokens = min(s.cols, a.n_tokens - t0);
-      const bool live = n < a.n_out;
+      const bool live = n < a.n_out, whole = s.wide && nw + 32 <= a.n_out;
       const float sw = live ? a.w_scale[n] : 0.f, bias = live && a.bias ? a.bias[n] : 0.f;
-      for (uint32_t t = lane; t < s.cols; t += 32) s_x[e][t] = t < tokens ? a.x_scale[t0 + t] : 0.f;
+      for (uint32_t t = lane; t < s.cols; t += 32) sx[t] = t < tokens ? a.x_scale[t0 + t] : 0.f;
       __syncwarp();
       const bool good = wait_bar(acc_full + buf, turn, stop, s.err);
       __syncwarp();
       tc_fence_after_sync();
-      T* y = (T*)a.y + (uint64_t)t0 * a.y_stride + n;
-      for (uint32_t c = 0; c < s.cols; c += 32) {
+      for (uint32_t c = 32 * set; c < s.cols; c += 64) {
         uint32_t r[32];
         tmem_ld_32(tmem + (e << 21) + buf * 256 + c, r);
-        if (c + 32 >= s.cols) {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0)
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                             map_cluster(tc_smem_u32(acc_free + buf), 0))
-                         : "memory");
-        }
-        if (!live || !good) continue;
-#pragma unroll
-        for (int i = 0; i < 32; i++) {
-          if (c + i < tokens) {
-            float v = __fmul_rn(__fmul_rn((float)(int)r[i], s_x[e][c + i]), sw);
-            if (a.bias) v = __fadd_rn(v, bias);
-            Act<T>::put(y, v);
-          }
-          y += a.y_stride;
-        }
+        if (!good || c >= tokens) continue;
+        T* y = (T*)a.y + (uint64_t)(t0 + c) * a.y_stride;
+        if (whole && c + 32 <= tokens)
+          put_columns<T>(y, a.y_stride, nw, lane, r, sx + c, sw, a.bias != nullptr, bias);
+        else if (live)
+          put_columns_any<T>(y + n, a.y_stride, min(32u, tokens - c), r, sx + c, sw, a.bias != nullptr, bias);
       }
+      tc_fence_before_sync();
       __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                         map_cluster(tc_smem_u32(acc_free + buf), 0))
+                     : "memory");
       if (++buf == 2) buf = 0, turn ^= 1;
     }
   }
@@ -509,6 +568,7 @@ int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   const uint64_t tiles = (uint64_t)((a.n_out + 2 * TM - 1) / (2 * TM)) * s.n_tiles;
   if (tiles > 0x7fffffffull) return set_error(RF_EINVAL, "%u tokens x %u channels are too many for one call", a.n_tokens, a.n_out);
   s.tiles = (uint32_t)tiles;
+  s.wide = aligned_to(a.y, 4) && a.y_stride * sizeof(T) % 4 == 0;
   // the whole of an SM's shared memory, also where fewer stages would do: two pairs never share an SM's tensor memory
   const uint32_t stage = (TM + s.cols / 2) * TK;
   s.stages = std::min(208u * 1024 / stage, kMaxStages);
@@ -519,7 +579,7 @@ int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   auto* k = i8_pair_kernel<T>;
   RF_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const uint32_t pairs = std::min<uint32_t>(s.tiles, std::max(1, num_sms() / 2));
-  RF_CUDA(launch_k(Launch{st, true}, k, dim3(2 * pairs), dim3(256), smem, s, mx, mw));
+  RF_CUDA(launch_k(Launch{st, true}, k, dim3(2 * pairs), dim3(kPairThreads), smem, s, mx, mw));
   return RF_OK;
 }
 
