@@ -60,35 +60,72 @@ __device__ __forceinline__ int next_child(const int32_t* parent, int n, int node
   return n;
 }
 
+// ---- clusters ---------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// 64 bits to `p`'s place in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ void push64(const void* p, uint32_t rank, uint64_t v) {
+  asm volatile(
+      "{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "st.shared::cluster.b64 [a], %2; }" ::"r"((uint32_t)__cvta_generic_to_shared(p)),
+      "r"(rank), "l"(v)
+      : "memory");
+}
+
+// E elements of a row from x on as f32, zeros from `end` on.
+template <class T, int E>
+__device__ __forceinline__ void load_piece(const T* row, uint32_t x, uint32_t end, float (&v)[E]) {
+  if constexpr (E == Act<T>::kVec) {
+    if (x + E <= end) {
+      Act<T>::unpack(ld_once(row + x), v);
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) v[e] = x + e < end ? Act<T>::get(row + x + e) : 0.f;
+}
+
 // ---------------------------------------------------------------------------
-// Sampling: a CTA a sequence.  Warp 0 walks; a pass over the vocabulary (each warp a run of it) gives the sums.
+// Sampling: a cluster a sequence.
+//
+// Every CTA gathers the drafts and walks until sums are needed; a pass over the vocabulary gives them, a run of it
+// for each CTA and each of its warps, and the CTAs' sums go to all of them.  What comes next is CTA 0's to say: the others follow
+// it, so that all meet at the same barriers whatever they read.  A chain takes one pass, and with it one meeting; each further
+// draft of a node that is refused takes one more.  The bytes of the last rows bound a batch (64 sequences, 128256 tokens, f32:
+// 65.7 MB), latency a sequence: two dependent reads, the walk, the pass, the search of one warp.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   WalkArgs w;
   const void *target, *draft;
   uint64_t target_stride, draft_stride;
   const float *accept_u, *next_u;
+  uint32_t ctas, run;  // CTAs a cluster, elements of a warp's run
 };
 
-constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kMaxCluster = 8;
 
-struct Pass {  // what a pass sums: target row, draft row, share a of q to take off, or drafts that are certain
-  int node, refused;  // refused: index of the last child tried (drafts without probabilities: those up to it are out)
+struct Pass {  // what a pass sums up: rows of `node`, the share a of q that is off; certain drafts: those up to `refused` are out
+  int32_t node, refused;
   double a;
 };
+// What follows a pass.  kLast: the token, or, where nothing is left, a pass over all of the target's row (kWhole).
+enum Next : uint32_t { kMore, kLast, kWhole };
 
-template <class T>
+template <class T, int E>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   __shared__ Drafts s;
   __shared__ float s_u[kMaxDrafts], s_p[kMaxDrafts], s_q[kMaxDrafts];
   __shared__ int32_t s_path[kMaxDrafts];  // draft j's place among the tokens that stand, or -1
-  __shared__ double s_seg[kSampleWarps];
-  __shared__ Pass s_pass;
-  __shared__ int s_token, s_final;
+  __shared__ int32_t s_out[kMaxDrafts];   // certain drafts: the tokens that are out
+  __shared__ double s_seg[kSampleWarps], s_sum[2][kMaxCluster];
+  __shared__ Pass s_pass;       // from CTA 0 (the first one from the CTA itself)
+  __shared__ uint64_t s_next[2];  // CTA 0's word on what follows a pass: Next, and the tokens that stand
+  __shared__ int s_n_out;
+  const WalkArgs& w = a.w;
+  const uint32_t b = blockIdx.x / a.ctas, rank = blockIdx.x % a.ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (a.ctas > 1) cluster_arrive();
   griddep_launch();
   griddep_wait();
-  const WalkArgs& w = a.w;
-  const uint32_t b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = w.vocab;
   const int count = draft_count(w, b), n = max(count, 0);
   if (count < 0 && tid == 0) atomicOr(w.err, kVerifyRange);
   auto p_row = [&](int node) { return (const T*)a.target + ((uint64_t)b * (w.n_tokens + 1) + node + 1) * a.target_stride; };
@@ -101,162 +138,264 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     s_p[j] = parent < -1 ? 0.f : fmaxf(Act<T>::get(p_row(parent) + token), 0.f);
     s_q[j] = parent < -1 || !a.draft ? 1.f : Act<T>::get(q_row(parent) + token);
   }
-  if (tid == 0) s_token = -1;
   __syncthreads();
-
-  // weight of token x in a pass
-  auto weight = [&](const Pass& ps, const T* p, const T* q, uint32_t x) {
-    const double px = Act<T>::get(p + x);
-    if (q) return fmax(fma(-ps.a, (double)Act<T>::get(q + x), px), 0.0);
-    for (int j = 0; j <= ps.refused; j++)
-      if (s.parent[j] == ps.node && s.token[j] == (int)x) return 0.0;
-    return fmax(px, 0.0);
-  };
-  const uint32_t per = (V + kSampleWarps - 1) / kSampleWarps, x0 = min(warp * per, V), x1 = min(x0 + per, V);
+  if (a.ctas > 1) cluster_wait();  // all have begun: their shared memory may be written
 
   // the walk's state, in every thread of warp 0
   int node = -1, last = -1, taken = 0, tried = 0;
   double off = 0.0, mass = 1.0;
-  bool fallback = false;
-  while (true) {
-    if (warp == 0) {
-      bool final = true;
-      while (!fallback) {
-        const int j = next_child(s.parent, n, node, last, lane);
-        if (j >= n) break;
-        last = j;
-        double left = s_p[j];
-        const double qc = s_q[j];
-        if (tried) {
-          if (a.draft) {
-            left = fmax(fma(-off, qc, left), 0.0);
-          } else {
-            for (int i = 0; i < j; i++)
-              if (s.parent[i] == node && s.token[i] == s.token[j]) left = 0.0;
-          }
-        }
-        if ((double)s_u[j] * qc * mass < left) {
-          if (lane == 0) s_path[j] = taken;
-          __syncwarp();
-          node = j, taken++, tried = 0, off = 0.0, mass = 1.0;
+  Next next = kLast;
+  auto walk = [&]() {  // until sums are needed
+    bool final = true;
+    while (true) {
+      const int j = next_child(s.parent, n, node, last, lane);
+      if (j >= n) break;
+      last = j;
+      double left = s_p[j];
+      const double qc = s_q[j];
+      if (tried) {
+        if (a.draft) {
+          left = fmax(fma(-off, qc, left), 0.0);
         } else {
-          off += mass;
-          tried++;
-          final = next_child(s.parent, n, node, last, lane) >= n;
-          break;
+          bool out = false;
+          for (int i = lane; i < j; i += 32) out |= s.parent[i] == node && s.token[i] == s.token[j];
+          if (__any_sync(0xffffffffu, out)) left = 0.0;
         }
       }
-      if (lane == 0) {
-        s_pass = Pass{node, tried ? last : -1, off};
-        s_final = final;
+      if ((double)s_u[j] * qc * mass < left) {
+        if (lane == 0) s_path[j] = taken;
+        __syncwarp();
+        node = j, taken++, tried = 0, off = 0.0, mass = 1.0;
+      } else {
+        off += mass;
+        tried++;
+        final = next_child(s.parent, n, node, last, lane) >= n;
+        break;
       }
     }
+    next = !final ? kMore : tried ? kLast : kWhole;
+    if (lane == 0) s_pass = Pass{node, tried ? last : -1, off};
+  };
+  if (warp == 0) walk();
+  const uint32_t x0 = min((rank * kSampleWarps + warp) * a.run, w.vocab), x1 = min(x0 + a.run, w.vocab);
+  int token = -1, stand = 0;
+  uint32_t turn = 0;
+  while (true) {
+    if (tid == 0) s_n_out = 0;
     __syncthreads();
     const Pass ps = s_pass;
-    const bool final = s_final;
     const T *p = p_row(ps.node), *q = a.draft && ps.a > 0.0 ? q_row(ps.node) : nullptr;
+    if (!a.draft && ps.refused >= 0) {
+      for (int j = tid; j <= min(ps.refused, n - 1); j += kSampleThreads)
+        if (s.parent[j] == ps.node) s_out[atomicAdd(&s_n_out, 1)] = s.token[j];
+      __syncthreads();
+    }
+    const int n_out = s_n_out;
+    auto weights = [&](uint32_t x, double (&v)[E]) {
+      float pf[E], qf[E];
+      load_piece<T, E>(p, x, x1, pf);
+      if (q) {
+        load_piece<T, E>(q, x, x1, qf);
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = fmax(fma(-ps.a, (double)qf[e], (double)pf[e]), 0.0);
+      } else {
+        for (int i = 0; i < n_out; i++)
+#pragma unroll
+          for (int e = 0; e < E; e++)
+            if (s_out[i] == (int)(x + e)) pf[e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = (double)fmaxf(pf[e], 0.f);
+      }
+    };
     double sum = 0.0;
-    for (uint32_t x = x0 + lane; x < x1; x += 32) sum += weight(ps, p, q, x);
+#pragma unroll 4
+    for (uint32_t x = x0 + lane * E; x < x1; x += 32 * E) {
+      double v[E];
+      weights(x, v);
+#pragma unroll
+      for (int e = 0; e < E; e++) sum += v[e];
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_seg[warp] = sum;
     __syncthreads();
-    mass = 0.0;
-    int lastseg = -1;
-    for (int i = 0; i < kSampleWarps; i++) {
-      if (s_seg[i] > 0.0) lastseg = i;
-      mass += s_seg[i];
+    if (tid < a.ctas) {
+      double all = 0.0;
+      for (int i = 0; i < kSampleWarps; i++) all += s_seg[i];
+      const uint64_t word = (uint64_t)next | (uint64_t)(uint32_t)taken << 32;
+      if (a.ctas == 1) {
+        s_sum[turn][0] = all, s_next[turn] = word;
+      } else {
+        push64(&s_sum[turn][rank], tid, __double_as_longlong(all));
+        if (rank == 0) push64(&s_next[turn], tid, word);
+      }
     }
-    if (!final) {
-      __syncthreads();  // s_seg is read before the next pass writes it
-      continue;
-    }
-    if (lastseg < 0) {
-      if (fallback || ps.refused < 0) break;  // the target's row itself has nothing
-      fallback = true;  // nothing is left of it (p equals q): all of it counts again
-      tried = 0, off = 0.0, last = n;
+    __syncwarp();
+    if (a.ctas > 1)
+      cluster_arrive(), cluster_wait();
+    else
       __syncthreads();
+    mass = 0.0;
+    for (uint32_t r = 0; r < a.ctas; r++) mass += s_sum[turn][r];
+    const Next now = (Next)(uint32_t)s_next[turn];
+    stand = (int)(s_next[turn] >> 32);
+    if (now == kMore || (now == kLast && !(mass > 0.0))) {
+      if (rank == 0 && warp == 0) {
+        if (now == kMore) {
+          walk();
+        } else {
+          next = kWhole;
+          if (lane == 0) s_pass = Pass{ps.node, -1, 0.0};
+        }
+        __syncwarp();
+        if (lane > 0 && lane < a.ctas) {
+          push64(&s_pass.node, lane, (uint64_t)(uint32_t)s_pass.node | (uint64_t)(uint32_t)s_pass.refused << 32);
+          push64(&s_pass.a, lane, __double_as_longlong(s_pass.a));
+        }
+        __syncwarp();
+      }
+      if (a.ctas > 1) cluster_arrive(), cluster_wait();
+      turn ^= 1;
       continue;
     }
-    // the token: first the warp whose run it lies in, then the place
+    // the token: the CTA, the warp and the place where the sum passes the aim
+    if (!(mass > 0.0)) break;  // the target's row has nothing: token -1
     const double aim = (double)fmaxf(a.next_u[b], 0.f) * mass;
     double before = 0.0;
-    int seg = 0;
-    for (; seg < lastseg; seg++) {
-      if (before + s_seg[seg] > aim) break;
-      before += s_seg[seg];
-    }
-    if ((int)warp == seg) {
+    uint32_t owner = 0, some = 0;
+    for (uint32_t r = 0; r < a.ctas; r++)
+      if (s_sum[turn][r] > 0.0) some = r;  // the sums' last bits may leave the aim behind the end: the last that has any
+    for (; owner < some && !(before + s_sum[turn][owner] > aim); owner++) before += s_sum[turn][owner];
+    if (owner != rank) break;
+    uint32_t seg = 0, full = 0;
+    for (uint32_t i = 0; i < kSampleWarps; i++)
+      if (s_seg[i] > 0.0) full = i;
+    for (; seg < full && !(before + s_seg[seg] > aim); seg++) before += s_seg[seg];
+    if (warp == seg) {
       int found = -1, latest = -1;
-      for (uint32_t y = x0; y < x1 && found < 0; y += 32) {
-        const double v = y + lane < x1 ? weight(ps, p, q, y + lane) : 0.0;
-        double cum = v;
+      for (uint32_t x = x0; x < x1 && found < 0; x += 32 * E) {
+        double v[E], own = 0.0;
+        weights(x + lane * E, v);
+        int high = -1;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          own += v[e];
+          if (v[e] > 0.0) high = (int)(x + lane * E) + e;
+        }
+        double cum = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const double c = __shfl_up_sync(0xffffffffu, cum, o);
           if (lane >= (uint32_t)o) cum += c;
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, v > 0.0 && before + cum > aim), some = __ballot_sync(0xffffffffu, v > 0.0);
-        if (hit) found = (int)y + __ffs(hit) - 1;
-        if (some) latest = (int)y + 31 - __clz(some);
+        double at = before + (cum - own);
+        int mine = -1;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          at += v[e];
+          if (mine < 0 && v[e] > 0.0 && at > aim) mine = (int)(x + lane * E) + e;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, mine >= 0), any = __ballot_sync(0xffffffffu, high >= 0);
+        if (hit) found = __shfl_sync(0xffffffffu, mine, __ffs(hit) - 1);
+        if (any) latest = __shfl_sync(0xffffffffu, high, 31 - __clz(any));
         before += __shfl_sync(0xffffffffu, cum, 31);
       }
-      if (lane == 0) s_token = found >= 0 ? found : latest;  // the sums' last bits may leave the aim behind the end
+      token = found >= 0 ? found : latest;
     }
     break;
   }
-  __syncthreads();
-  if (warp == 0 && lane == 0) {
-    if (s_token < 0) atomicOr(w.err, kVerifyRange);
-    w.n_accepted[b] = taken;
-    w.out_tokens[(uint64_t)b * (w.n_tokens + 1) + taken] = count < 0 ? -1 : s_token;
-    s_final = taken;
+  // CTA 0 writes the walk, the warp that found it the token
+  int32_t* out = w.out_tokens + (uint64_t)b * (w.n_tokens + 1);
+  if (rank == 0) {
+    if (tid == 0) {
+      w.n_accepted[b] = stand;
+      if (!(mass > 0.0)) atomicOr(w.err, kVerifyRange);
+      if (!(mass > 0.0) || count < 0) out[stand] = -1;
+    }
+    for (int j = tid; j < (int)w.n_tokens; j += kSampleThreads) {
+      const int place = j < n ? s_path[j] : -1;
+      if (place >= 0) out[place] = s.token[j];
+      if (w.positions) w.positions[(uint64_t)b * w.n_tokens + j] = place >= 0 ? w.hist[b] + place : -1;
+      if (j >= stand) out[j + 1] = -1;
+    }
   }
-  __syncthreads();
-  taken = s_final;
-  for (int j = tid; j < (int)w.n_tokens; j += kSampleThreads) {
-    const int place = j < n ? s_path[j] : -1;
-    if (place >= 0) w.out_tokens[(uint64_t)b * (w.n_tokens + 1) + place] = s.token[j];
-    if (w.positions) w.positions[(uint64_t)b * w.n_tokens + j] = place >= 0 ? w.hist[b] + place : -1;
-    if (j >= taken) w.out_tokens[(uint64_t)b * (w.n_tokens + 1) + j + 1] = -1;
-  }
+  if (token >= 0 && count >= 0 && lane == 0) out[stand] = token;
 }
 
 // ---------------------------------------------------------------------------
-// Greedy: the best token of every row, then the walk.
+// Greedy: the best token of every row (a cluster a row), then the walk.
 // ---------------------------------------------------------------------------
 struct BestArgs {
   WalkArgs w;
   const void* logits;
   uint64_t stride;
   int32_t* best;
+  uint32_t ctas, run;  // CTAs a cluster, elements of one's run
 };
 
-// Larger numbers have larger keys, of equal numbers the lower index; NaN counts as the least.
+constexpr int kBestThreads = 256;
+
+// Larger numbers have larger keys, of equal numbers the lower index.
 __device__ __forceinline__ uint64_t best_key(float v, uint32_t x) {
   const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
-  const uint32_t key = v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return (uint64_t)key << 32 | (uint32_t)~x;
+  return (uint64_t)((b & 0x80000000u) ? ~b : b | 0x80000000u) << 32 | (uint32_t)~x;
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) best_kernel(BestArgs a) {
-  __shared__ uint64_t s_best[8];
+template <class T, int E>
+__global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
+  __shared__ uint64_t s_best[kBestThreads / 32], s_cta[kMaxCluster];
+  const uint32_t row_at = blockIdx.x / a.ctas, rank = blockIdx.x % a.ctas, tid = threadIdx.x;
+  if (a.ctas > 1) cluster_arrive();
   griddep_launch();
   griddep_wait();
-  const uint32_t rows = a.w.n_tokens + 1, b = blockIdx.x / rows, r = blockIdx.x - b * rows, tid = threadIdx.x;
-  if ((int)r > max(draft_count(a.w, b), 0)) return;  // behind the sequence's last draft
-  const T* row = (const T*)a.logits + (uint64_t)blockIdx.x * a.stride;
-  uint64_t best = 0;
-  for (uint32_t x = tid; x < a.w.vocab; x += 256) best = max(best, best_key(Act<T>::get(row + x), x));
+  const uint32_t rows = a.w.n_tokens + 1, b = row_at / rows, r = row_at - b * rows;
+  if (a.ctas > 1) cluster_wait();
+  const bool live = (int)r <= max(draft_count(a.w, b), 0);  // not behind the sequence's last draft
+  const T* row = (const T*)a.logits + (uint64_t)row_at * a.stride;
+  const uint32_t x0 = min(rank * a.run, a.w.vocab), x1 = min(x0 + a.run, a.w.vocab);
+  float top = -INFINITY;
+  uint32_t at = ~0u;
+  constexpr int U = E == 1 ? 4 : 2;  // loads in flight
+  if (live)
+    for (uint32_t x = x0 + tid * E; x < x1; x += U * kBestThreads * E) {
+      float v[U][E];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const uint32_t y = x + u * kBestThreads * E;
+        if (E > 1 && y + E <= x1) {
+          load_piece<T, E>(row, y, x1, v[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e++) v[u][e] = y + e < x1 ? Act<T>::get(row + y + e) : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (v[u][e] > top) top = v[u][e], at = x + u * kBestThreads * E + e;
+    }
+  uint64_t best = at == ~0u ? 0 : best_key(top, at);  // 0: nothing above -infinity
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((tid & 31) == 0) s_best[tid >> 5] = best;
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < 8; i++) best = max(best, s_best[i]);
-    a.best[blockIdx.x] = (int32_t)~(uint32_t)best;
+    for (int i = 1; i < kBestThreads / 32; i++) best = max(best, s_best[i]);
+    if (a.ctas > 1) push64(&s_cta[rank], 0, best);
   }
+  __syncwarp();
+  if (a.ctas > 1) cluster_arrive(), cluster_wait();
+  if (rank || tid || !live) return;
+  if (a.ctas > 1)
+    for (uint32_t i = 0; i < a.ctas; i++) best = max(best, s_cta[i]);
+  uint32_t x = ~(uint32_t)best;
+  if (!best) {  // -infinity and NaN alone: the first -infinity, or 0
+    for (x = 0; x < a.w.vocab && !(Act<T>::get(row + x) == -INFINITY); x++) {
+    }
+    if (x == a.w.vocab) x = 0;
+  }
+  a.best[row_at] = (int32_t)x;
 }
 
 __global__ void __launch_bounds__(128) greedy_walk_kernel(BestArgs a) {
@@ -299,6 +438,30 @@ __global__ void __launch_bounds__(128) greedy_walk_kernel(BestArgs a) {
     if (w.positions) w.positions[(uint64_t)b * w.n_tokens + j] = place >= 0 ? w.hist[b] + place : -1;
     if (j >= taken) w.out_tokens[(uint64_t)b * (w.n_tokens + 1) + j + 1] = -1;
   }
+}
+
+// CTAs a cluster: as many as still give all of `units` a place at once (two an SM).
+uint32_t cluster_size(uint32_t units) {
+  uint32_t c = kMaxCluster;
+  while (c > 1 && (uint64_t)units * c > 2ull * num_sms()) c /= 2;
+  return c;
+}
+
+template <class Args>
+cudaError_t launch_clusters(cudaStream_t st, void (*k)(Args), uint32_t units, uint32_t ctas, int threads, const Args& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(units * ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, a);
 }
 
 int check_walk(int type, uint32_t vocab, uint32_t n_seqs, uint32_t n_tokens, const void* rows, uint64_t* stride,
@@ -347,9 +510,15 @@ int rf_verify_drafts(const void* target, const void* draft, int prob_type, uint3
   a.target_stride = target_stride, a.draft_stride = draft_stride;
   a.accept_u = accept_u, a.next_u = next_u;
   RF_TRY(verify_error_ptr(&a.w.err));
-  const Launch L{(cudaStream_t)stream, true};
-  auto* k = prob_type == RF_ACT_F32 ? sample_kernel<float> : prob_type == RF_ACT_F16 ? sample_kernel<__half> : sample_kernel<__nv_bfloat16>;
-  RF_CUDA(launch_k(L, k, dim3(n_seqs), dim3(kSampleThreads), 0, a));
+  const uint32_t es = act_bytes(prob_type);
+  const bool vec = aligned_to(target, 16) && target_stride * es % 16 == 0 && aligned_to(draft, 16) && draft_stride * es % 16 == 0;
+  a.ctas = cluster_size(n_seqs);
+  const uint32_t warps = a.ctas * kSampleWarps, unit = 16 / es;
+  a.run = ((vocab + warps - 1) / warps + unit - 1) / unit * unit;
+  auto* k = prob_type == RF_ACT_F32   ? (vec ? sample_kernel<float, 4> : sample_kernel<float, 1>)
+            : prob_type == RF_ACT_F16 ? (vec ? sample_kernel<__half, 8> : sample_kernel<__half, 1>)
+                                      : (vec ? sample_kernel<__nv_bfloat16, 8> : sample_kernel<__nv_bfloat16, 1>);
+  RF_CUDA(launch_clusters((cudaStream_t)stream, k, n_seqs, a.ctas, kSampleThreads, a));
   return RF_OK;
 }
 
@@ -366,10 +535,15 @@ int rf_verify_greedy(const void* logits, int logit_type, uint32_t vocab, uint32_
   a.w = WalkArgs{tokens, parent, n_draft, hist_len, out_tokens, n_accepted, positions, vocab, n_tokens, nullptr};
   a.logits = logits, a.stride = logits_stride, a.best = best;
   RF_TRY(verify_error_ptr(&a.w.err));
-  const Launch L{(cudaStream_t)stream, true};
-  auto* k = logit_type == RF_ACT_F32 ? best_kernel<float> : logit_type == RF_ACT_F16 ? best_kernel<__half> : best_kernel<__nv_bfloat16>;
-  RF_CUDA(launch_k(L, k, dim3(n_seqs * (n_tokens + 1)), dim3(256), 0, a));
-  RF_CUDA(launch_k(L, greedy_walk_kernel, dim3(n_seqs), dim3(128), 0, a));
+  const uint32_t es = act_bytes(logit_type), rows = n_seqs * (n_tokens + 1), unit = 16 / es;
+  const bool vec = aligned_to(logits, 16) && logits_stride * es % 16 == 0;
+  a.ctas = cluster_size(rows);
+  a.run = ((vocab + a.ctas - 1) / a.ctas + unit - 1) / unit * unit;
+  auto* k = logit_type == RF_ACT_F32   ? (vec ? best_kernel<float, 4> : best_kernel<float, 1>)
+            : logit_type == RF_ACT_F16 ? (vec ? best_kernel<__half, 8> : best_kernel<__half, 1>)
+                                       : (vec ? best_kernel<__nv_bfloat16, 8> : best_kernel<__nv_bfloat16, 1>);
+  RF_CUDA(launch_clusters((cudaStream_t)stream, k, rows, a.ctas, kBestThreads, a));
+  RF_CUDA(launch_k(Launch{(cudaStream_t)stream, true}, greedy_walk_kernel, dim3(n_seqs), dim3(128), 0, a));
   return RF_OK;
 }
 
