@@ -40,15 +40,17 @@ __device__ __forceinline__ int draft_count(const WalkArgs& a, uint32_t b) {
   const int n = a.n_draft ? a.n_draft[b] : (int)a.n_tokens;
   return n < 0 || (uint32_t)n > a.n_tokens ? -1 : n;
 }
-// Parent and token of draft j; a parent of -2 and the error bit where either is out of range.
-__device__ __forceinline__ void draft_at(const WalkArgs& a, uint32_t b, int j, int* parent, int* token) {
+// Parent and token of draft j; a parent of -2 behind the last of n, and, with the error bit, where either is out of range.
+// The count is looked at last, so that it arrives with the rest.
+__device__ __forceinline__ void draft_at(const WalkArgs& a, uint32_t b, int j, int n, int* parent, int* token) {
   const uint64_t at = (uint64_t)b * a.n_tokens + j;
   *parent = a.parent ? a.parent[at] : j - 1;
   *token = a.tokens[at];
   if (*parent < -1 || *parent >= j || *token < 0 || (uint32_t)*token >= a.vocab) {
-    atomicOr(a.err, kVerifyRange);
+    if (j < n) atomicOr(a.err, kVerifyRange);
     *parent = -2, *token = 0;
   }
+  if (j >= n) *parent = -2;
 }
 // One warp: the first draft behind `last` whose parent is `node`, or n.
 __device__ __forceinline__ int next_child(const int32_t* parent, int n, int node, int last, uint32_t lane) {
@@ -112,12 +114,12 @@ struct Pass {  // what a pass sums up: rows of `node`, the share a of q that is 
 enum Next : uint32_t { kMore, kLast, kWhole };
 
 template <class T, int E>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a) {
   __shared__ Drafts s;
   __shared__ float s_u[kMaxDrafts], s_p[kMaxDrafts], s_q[kMaxDrafts];
   __shared__ int32_t s_path[kMaxDrafts];  // draft j's place among the tokens that stand, or -1
   __shared__ int32_t s_out[kMaxDrafts];   // certain drafts: the tokens that are out
-  __shared__ double s_seg[kSampleWarps], s_sum[2][kMaxCluster];
+  __shared__ double s_seg[kSampleWarps], s_part[kSampleWarps], s_sum[2][kMaxCluster];
   __shared__ Pass s_pass;       // from CTA 0 (the first one from the CTA itself)
   __shared__ uint64_t s_next[2];  // CTA 0's word on what follows a pass: Next, and the tokens that stand
   __shared__ int s_n_out;
@@ -127,12 +129,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   griddep_launch();
   griddep_wait();
   const int count = draft_count(w, b), n = max(count, 0);
-  if (count < 0 && tid == 0) atomicOr(w.err, kVerifyRange);
   auto p_row = [&](int node) { return (const T*)a.target + ((uint64_t)b * (w.n_tokens + 1) + node + 1) * a.target_stride; };
   auto q_row = [&](int node) { return (const T*)a.draft + ((uint64_t)b * w.n_tokens + node + 1) * a.draft_stride; };
-  for (int j = tid; j < n; j += kSampleThreads) {
+  for (int j = tid; j < (int)w.n_tokens; j += kSampleThreads) {
     int parent, token;
-    draft_at(w, b, j, &parent, &token);
+    draft_at(w, b, j, n, &parent, &token);
     s.parent[j] = parent, s.token[j] = token, s_path[j] = -1;
     s_u[j] = a.accept_u[(uint64_t)b * w.n_tokens + j];
     s_p[j] = parent < -1 ? 0.f : fmaxf(Act<T>::get(p_row(parent) + token), 0.f);
@@ -191,32 +192,51 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
       __syncthreads();
     }
     const int n_out = s_n_out;
-    auto weights = [&](uint32_t x, double (&v)[E]) {
-      float pf[E], qf[E];
-      load_piece<T, E>(p, x, x1, pf);
-      if (q) {
-        load_piece<T, E>(q, x, x1, qf);
+    // what is left of the tokens from x on, out of their numbers in p and q; NaN counts as 0 in all of this
+    auto strike = [&](uint32_t x, float (&pf)[E]) {
+      for (int i = 0; i < n_out; i++)
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = fmax(fma(-ps.a, (double)qf[e], (double)pf[e]), 0.0);
-      } else {
-        for (int i = 0; i < n_out; i++)
+        for (int e = 0; e < E; e++)
+          if (s_out[i] == (int)(x + e)) pf[e] = 0.f;
+    };
+    auto weight = [&](float pf, float qf) { return q ? fma(-ps.a, (double)qf, (double)pf) : (double)pf; };
+    auto weights = [&](uint32_t x, uint32_t to, double (&v)[E]) {
+      float pf[E], qf[E] = {};
+      load_piece<T, E>(p, x, to, pf);
+      if (q) load_piece<T, E>(q, x, to, qf);
+      strike(x, pf);
 #pragma unroll
-          for (int e = 0; e < E; e++)
-            if (s_out[i] == (int)(x + e)) pf[e] = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; e++) v[e] = (double)fmaxf(pf[e], 0.f);
+      for (int e = 0; e < E; e++) {
+        const double r = weight(pf[e], qf[e]);
+        v[e] = r > 0.0 ? r : 0.0;
       }
     };
-    double sum = 0.0;
-#pragma unroll 4
-    for (uint32_t x = x0 + lane * E; x < x1; x += 32 * E) {
-      double v[E];
-      weights(x, v);
+    auto sum_run = [&](uint32_t from, uint32_t to) {  // a warp's sum of what is left of a run
+      double sums[2] = {};
+      constexpr int U = E == 1 ? 4 : 8 / E;  // pieces of a lane in flight
+      for (uint32_t x = from + lane * E; x < to; x += U * 32 * E) {
+        float pf[U][E], qf[U][E] = {};
 #pragma unroll
-      for (int e = 0; e < E; e++) sum += v[e];
-    }
+        for (int u = 0; u < U; u++) load_piece<T, E>(p, x + u * 32 * E, to, pf[u]);
+        if (q)
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          for (int u = 0; u < U; u++) load_piece<T, E>(q, x + u * 32 * E, to, qf[u]);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          strike(x + u * 32 * E, pf[u]);
+#pragma unroll
+          for (int e = 0; e < E; e++) {
+            const double r = weight(pf[u][e], qf[u][e]);
+            if (r > 0.0) sums[e & 1] += r;
+          }
+        }
+      }
+      double sum = sums[0] + sums[1];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      return sum;
+    };
+    const double sum = sum_run(x0, x1);
     if (lane == 0) s_seg[warp] = sum;
     __syncthreads();
     if (tid < a.ctas) {
@@ -267,15 +287,25 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
       if (s_sum[turn][r] > 0.0) some = r;  // the sums' last bits may leave the aim behind the end: the last that has any
     for (; owner < some && !(before + s_sum[turn][owner] > aim); owner++) before += s_sum[turn][owner];
     if (owner != rank) break;
-    uint32_t seg = 0, full = 0;
-    for (uint32_t i = 0; i < kSampleWarps; i++)
-      if (s_seg[i] > 0.0) full = i;
-    for (; seg < full && !(before + s_seg[seg] > aim); seg++) before += s_seg[seg];
-    if (warp == seg) {
+    // the run, then, by all warps again, the part of it
+    auto pick = [&](const double* sums) {
+      uint32_t i = 0, full = 0;
+      for (uint32_t j = 0; j < kSampleWarps; j++)
+        if (sums[j] > 0.0) full = j;
+      for (; i < full && !(before + sums[i] > aim); i++) before += sums[i];
+      return i;
+    };
+    const uint32_t seg = pick(s_seg), y0 = min((rank * kSampleWarps + seg) * a.run, w.vocab), y1 = min(y0 + a.run, w.vocab);
+    const uint32_t part = ((a.run + kSampleWarps - 1) / kSampleWarps + E - 1) / E * E;
+    const uint32_t z0 = min(y0 + warp * part, y1), z1 = min(z0 + part, y1);
+    const double fine = sum_run(z0, z1);
+    if (lane == 0) s_part[warp] = fine;
+    __syncthreads();
+    if (warp == pick(s_part)) {
       int found = -1, latest = -1;
-      for (uint32_t x = x0; x < x1 && found < 0; x += 32 * E) {
+      for (uint32_t x = z0; x < z1 && found < 0; x += 32 * E) {
         double v[E], own = 0.0;
-        weights(x + lane * E, v);
+        weights(x + lane * E, z1, v);
         int high = -1;
 #pragma unroll
         for (int e = 0; e < E; e++) {
@@ -305,6 +335,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     break;
   }
   // CTA 0 writes the walk, the warp that found it the token
+  if (count < 0 && tid == 0) atomicOr(w.err, kVerifyRange);
   int32_t* out = w.out_tokens + (uint64_t)b * (w.n_tokens + 1);
   if (rank == 0) {
     if (tid == 0) {
@@ -333,7 +364,7 @@ struct BestArgs {
   uint32_t ctas, run;  // CTAs a cluster, elements of one's run
 };
 
-constexpr int kBestThreads = 256;
+constexpr int kBestThreads = 512;
 
 // Larger numbers have larger keys, of equal numbers the lower index.
 __device__ __forceinline__ uint64_t best_key(float v, uint32_t x) {
@@ -355,7 +386,7 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
   const uint32_t x0 = min(rank * a.run, a.w.vocab), x1 = min(x0 + a.run, a.w.vocab);
   float top = -INFINITY;
   uint32_t at = ~0u;
-  constexpr int U = E == 1 ? 4 : 2;  // loads in flight
+  constexpr int U = 4;  // loads in flight
   if (live)
     for (uint32_t x = x0 + tid * E; x < x1; x += U * kBestThreads * E) {
       float v[U][E];
@@ -411,7 +442,7 @@ __global__ void __launch_bounds__(128) greedy_walk_kernel(BestArgs a) {
   const int32_t* best = a.best + (uint64_t)b * (w.n_tokens + 1);
   for (int j = tid; j < n; j += 128) {
     int parent, token;
-    draft_at(w, b, j, &parent, &token);
+    draft_at(w, b, j, n, &parent, &token);
     s.parent[j] = parent >= -1 && best[parent + 1] == token ? parent : -2;  // only those that would stand
     s.token[j] = token, s_path[j] = -1;
   }
