@@ -12,7 +12,7 @@
 
 #include "rf_act.cuh"
 #include "rf_device.cuh"
-#include "rf_tc.cuh"
+#include "rf_ring.cuh"
 #include "rf_verify.h"
 
 namespace rf {
@@ -29,23 +29,6 @@ struct MatmulArgs {
 };
 
 // ---- waits, tensor memory, copies -------------------------------------------------------
-// Bounded wait for the phase of `bar` with `parity`; false once any wait of the CTA gave up.
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
-  const long long t0 = clock64();
-  while (!tc_mbar_try_wait(bar, parity)) {
-    if (*stop) return false;
-    if (clock64() - t0 > 2000000000LL) {
-      *stop = 1;
-      atomicOr(err, kVerifyTimeout);
-      return false;
-    }
-  }
-  return true;
-}
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
-  const uint32_t b = tc_smem_u32(bar);
-  return tc_mbar_try_wait(b, parity) || wait_slow(b, parity, stop, err);
-}
 // The value of lane 0, which the compiler then keeps in a uniform register, as descriptors want.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
 // True in one lane of the (whole) warp, the same one every time.
