@@ -93,7 +93,7 @@ __device__ __forceinline__ void load_piece(const T* row, uint32_t x, uint32_t en
 // Every CTA gathers the drafts and walks until sums are needed; a pass over the vocabulary gives them, a run of it
 // for each CTA and each of its warps, and the CTAs' sums go to all of them.  What comes next is CTA 0's to say: the others follow
 // it, so that all meet at the same barriers whatever they read.  A chain takes one pass, and with it one meeting; each further
-// draft of a node that is refused takes one more.  The bytes of the last rows bound a batch (64 sequences, 128256 tokens, f32:
+// draft of a node that is refused takes one more (of drafts that were certain, all of a node's together one).  The bytes of the last rows bound a batch (64 sequences, 128256 tokens, f32:
 // 65.7 MB), latency a sequence: two dependent reads, the walk, the pass, the search of one warp.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
@@ -129,6 +129,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
   griddep_launch();
   griddep_wait();
   const int count = draft_count(w, b), n = max(count, 0);
+  const float u_next = a.next_u[b];  // wanted last, asked for first
+  const int hist = w.positions ? w.hist[b] : 0;
   auto p_row = [&](int node) { return (const T*)a.target + ((uint64_t)b * (w.n_tokens + 1) + node + 1) * a.target_stride; };
   auto q_row = [&](int node) { return (const T*)a.draft + ((uint64_t)b * w.n_tokens + node + 1) * a.draft_stride; };
   for (int j = tid; j < (int)w.n_tokens; j += kSampleThreads) {
@@ -144,10 +146,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
 
   // the walk's state, in every thread of warp 0
   int node = -1, last = -1, taken = 0, tried = 0;
-  double off = 0.0, mass = 1.0;
+  double off = 0.0, mass = 1.0, gone = 0.0;
+  bool whole = false;  // certain drafts: mass comes from the sum of the node's whole row
   Next next = kLast;
   auto walk = [&]() {  // until sums are needed
-    bool final = true;
+    bool final = true, masked = true;
+    if (!a.draft && tried) mass = fmax(mass - gone, 0.0);  // the whole row's sum has come
     while (true) {
       const int j = next_child(s.parent, n, node, last, lane);
       if (j >= n) break;
@@ -166,16 +170,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       if ((double)s_u[j] * qc * mass < left) {
         if (lane == 0) s_path[j] = taken;
         __syncwarp();
-        node = j, taken++, tried = 0, off = 0.0, mass = 1.0;
-      } else {
+        node = j, taken++, tried = 0, off = 0.0, mass = 1.0, whole = false;
+        continue;
+      }
+      tried++;
+      final = next_child(s.parent, n, node, last, lane) >= n;
+      if (a.draft) {
         off += mass;
-        tried++;
-        final = next_child(s.parent, n, node, last, lane) >= n;
+        break;
+      }
+      if (final) break;
+      // certain drafts: the sum of what is left is that of the whole row without the tokens that are out
+      if (whole) {
+        mass = fmax(mass - left, 0.0);
+      } else {
+        gone = left, whole = true, masked = false;
         break;
       }
     }
     next = !final ? kMore : tried ? kLast : kWhole;
-    if (lane == 0) s_pass = Pass{node, tried ? last : -1, off};
+    if (lane == 0) s_pass = Pass{node, tried && masked ? last : -1, off};
   };
   if (warp == 0) walk();
   const uint32_t x0 = min((rank * kSampleWarps + warp) * a.run, w.vocab), x1 = min(x0 + a.run, w.vocab);
@@ -280,7 +294,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
     }
     // the token: the CTA, the warp and the place where the sum passes the aim
     if (!(mass > 0.0)) break;  // the target's row has nothing: token -1
-    const double aim = (double)fmaxf(a.next_u[b], 0.f) * mass;
+    const double aim = (double)fmaxf(u_next, 0.f) * mass;
     double before = 0.0;
     uint32_t owner = 0, some = 0;
     for (uint32_t r = 0; r < a.ctas; r++)
@@ -346,7 +360,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
     for (int j = tid; j < (int)w.n_tokens; j += kSampleThreads) {
       const int place = j < n ? s_path[j] : -1;
       if (place >= 0) out[place] = s.token[j];
-      if (w.positions) w.positions[(uint64_t)b * w.n_tokens + j] = place >= 0 ? w.hist[b] + place : -1;
+      if (w.positions) w.positions[(uint64_t)b * w.n_tokens + j] = place >= 0 ? hist + place : -1;
       if (j >= stand) out[j + 1] = -1;
     }
   }
