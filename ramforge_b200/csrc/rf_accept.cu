@@ -13,6 +13,7 @@
 // Products and sums are taken in 64 bits: p and q are at most 32-bit numbers, so u q is exact, and which side of a
 // border a number lies on does not depend on the order of the sums.
 #include <algorithm>
+#include <type_traits>
 
 #include "rf_act.cuh"
 #include "rf_device.cuh"
@@ -386,6 +387,19 @@ __device__ __forceinline__ uint64_t best_key(float v, uint32_t x) {
   return (uint64_t)((b & 0x80000000u) ? ~b : b | 0x80000000u) << 32 | (uint32_t)~x;
 }
 
+// The largest of 16 bytes' numbers; NaN where all of them are.
+template <class T>
+__device__ __forceinline__ float piece_top(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    const T2* h = reinterpret_cast<const T2*>(&u);
+    const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(Act<T>::get(&m.x), Act<T>::get(&m.y));
+  }
+}
+
 template <class T, int E>
 __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
   __shared__ uint64_t s_best[kBestThreads / 32], s_cta[kMaxCluster];
@@ -398,28 +412,49 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
   const bool live = (int)r <= max(draft_count(a.w, b), 0);  // not behind the sequence's last draft
   const T* row = (const T*)a.logits + (uint64_t)row_at * a.stride;
   const uint32_t x0 = min(rank * a.run, a.w.vocab), x1 = min(x0 + a.run, a.w.vocab);
+  // the largest number and the first piece that has it, which is kept: one comparison a piece
   float top = -INFINITY;
   uint32_t at = ~0u;
-  constexpr int U = 4;  // loads in flight
-  if (live)
-    for (uint32_t x = x0 + tid * E; x < x1; x += U * kBestThreads * E) {
-      float v[U][E];
+  constexpr int U = 4, STEP = kBestThreads * E;  // loads in flight
+  if constexpr (E > 1) {
+    uint4 kept = make_uint4(0, 0, 0, 0);
+    auto look = [&](uint4 u, uint32_t x) {
+      const float v = piece_top<T>(u);
+      if (v > top) top = v, at = x, kept = u;
+    };
+    const uint32_t end = live ? x0 + (x1 - x0) / E * E : x0;
+    for (uint32_t x = x0 + tid * E; x < end; x += U * STEP) {
+      uint4 u[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const uint32_t y = x + u * kBestThreads * E;
-        if (E > 1 && y + E <= x1) {
-          load_piece<T, E>(row, y, x1, v[u]);
-        } else {
+      for (int i = 0; i < U; i++)
+        if (x + i * STEP < end) u[i] = ld_once(row + x + i * STEP);
 #pragma unroll
-          for (int e = 0; e < E; e++) v[u][e] = y + e < x1 ? Act<T>::get(row + y + e) : -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int e = 0; e < E; e++)
-          if (v[u][e] > top) top = v[u][e], at = x + u * kBestThreads * E + e;
+      for (int i = 0; i < U; i++)
+        if (x + i * STEP < end) look(u[i], x + i * STEP);
     }
+    if (at != ~0u) {
+      float v[E];
+      Act<T>::unpack(kept, v);
+      int first = 0;
+#pragma unroll
+      for (int e = E - 1; e >= 0; e--)
+        if (v[e] == top) first = e;
+      at += first;
+    }
+    if (live && tid < x1 - end) {  // the row's end, less than a piece
+      const float v = Act<T>::get(row + end + tid);
+      if (v > top) top = v, at = end + tid;
+    }
+  } else if (live) {
+    for (uint32_t x = x0 + tid; x < x1; x += U * STEP) {
+      float v[U];
+#pragma unroll
+      for (int i = 0; i < U; i++) v[i] = x + i * STEP < x1 ? Act<T>::get(row + x + i * STEP) : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < U; i++)
+        if (v[i] > top) top = v[i], at = x + i * STEP;
+    }
+  }
   uint64_t best = at == ~0u ? 0 : best_key(top, at);  // 0: nothing above -infinity
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -436,7 +471,7 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
     for (uint32_t i = 0; i < a.ctas; i++) best = max(best, s_cta[i]);
   uint32_t x = ~(uint32_t)best;
   if (!best) {  // -infinity and NaN alone: the first -infinity, or 0
-    for (x = 0; x < a.w.vocab && !(Act<T>::get(row + x) == -INFINITY); x++) {
+    for (x = 0; x < a.w.vocab && Act<T>::get(row + x) != -INFINITY; x++) {
     }
     if (x == a.w.vocab) x = 0;
   }
@@ -485,10 +520,10 @@ __global__ void __launch_bounds__(128) greedy_walk_kernel(BestArgs a) {
   }
 }
 
-// CTAs a cluster: as many as still give all of `units` a place at once (two an SM).
-uint32_t cluster_size(uint32_t units) {
+// CTAs a cluster: as many as still give all of `units` a place at once (per_sm an SM).
+uint32_t cluster_size(uint32_t units, uint32_t per_sm) {
   uint32_t c = kMaxCluster;
-  while (c > 1 && (uint64_t)units * c > 2ull * num_sms()) c /= 2;
+  while (c > 1 && (uint64_t)units * c > (uint64_t)per_sm * num_sms()) c /= 2;
   return c;
 }
 
@@ -557,7 +592,7 @@ int rf_verify_drafts(const void* target, const void* draft, int prob_type, uint3
   RF_TRY(verify_error_ptr(&a.w.err));
   const uint32_t es = act_bytes(prob_type);
   const bool vec = aligned_to(target, 16) && target_stride * es % 16 == 0 && aligned_to(draft, 16) && draft_stride * es % 16 == 0;
-  a.ctas = cluster_size(n_seqs);
+  a.ctas = cluster_size(n_seqs, 2);
   const uint32_t warps = a.ctas * kSampleWarps, unit = 16 / es;
   a.run = ((vocab + warps - 1) / warps + unit - 1) / unit * unit;
   auto* k = prob_type == RF_ACT_F32   ? (vec ? sample_kernel<float, 4> : sample_kernel<float, 1>)
@@ -582,7 +617,7 @@ int rf_verify_greedy(const void* logits, int logit_type, uint32_t vocab, uint32_
   RF_TRY(verify_error_ptr(&a.w.err));
   const uint32_t es = act_bytes(logit_type), rows = n_seqs * (n_tokens + 1), unit = 16 / es;
   const bool vec = aligned_to(logits, 16) && logits_stride * es % 16 == 0;
-  a.ctas = cluster_size(rows);
+  a.ctas = cluster_size(rows, 2);
   a.run = ((vocab + a.ctas - 1) / a.ctas + unit - 1) / unit * unit;
   auto* k = logit_type == RF_ACT_F32   ? (vec ? best_kernel<float, 4> : best_kernel<float, 1>)
             : logit_type == RF_ACT_F16 ? (vec ? best_kernel<__half, 8> : best_kernel<__half, 1>)
