@@ -62,7 +62,7 @@ class Codes:
         assert (self.q[:, self.cols:] == 99).all()
 
 
-SHAPES = [(1, 1), (1, 7), (3, 8), (2, 33), (5, 64), (17, 255), (4, 256), (1, 4096), (33, 4096), (9, 4097), (2, 5000),
+SHAPES = [(1, 1), (1, 7), (3, 8), (2, 33), (5, 64), (17, 255), (4, 256), (1, 4096), (33, 4096), (1000, 4096), (1500, 4095), (700, 1001), (1300, 129), (900, 500), (800, 14336), (9, 4097), (2, 5000),
           (3, 14336), (2, 16384), (2, 16385), (1, 32768), (1, 40001), (2, 65536), (700, 1024), (300, 96)]
 
 
