@@ -38,7 +38,7 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 // 32 columns of the thread's lane (32 * (warp % 4) + lane).
-__device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ask_32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -50,6 +50,9 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
+}
+// What was asked for is there; the registers pass through so that no use moves above the wait.
+__device__ __forceinline__ void tmem_have(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
@@ -129,13 +132,14 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Sums r of 32 tokens (rows of y from y on) of the channel nw + lane, a warp's 32 channels whole.  Of 16-bit outputs the
-// lanes 2i and 2i + 1 exchange one each, so that each stores two channels of one token.
-template <class T>
-__device__ __forceinline__ void put_columns(T* y, uint64_t stride, uint32_t nw, uint32_t lane, const uint32_t (&r)[32],
-                                            const float* sx, float sw, bool add, float bias) {
+// Sums r of 32 tokens (rows of y from y on) of the channel nw + lane, a warp's 32 channels whole.  Of 16-bit outputs
+// that lie in whole words (`wide`) the lanes 2i and 2i + 1 exchange one each, so that each stores two channels of one token.
+template <class T, bool WIDE>
+__device__ __forceinline__ void put_columns_as(T* y, uint64_t stride, uint32_t nw, uint32_t lane, const uint32_t (&r)[32],
+                                               const float* sx, float sw, bool add, float bias) {
   const float2 w2 = make_float2(sw, sw);
-  y += sizeof(T) == 4 ? nw + lane : nw + (lane & 30) + (lane & 1) * stride;
+  constexpr bool PAIR = sizeof(T) == 2 && WIDE;
+  y += PAIR ? nw + (lane & 30) + (lane & 1) * stride : nw + lane;
 #pragma unroll
   for (int i = 0; i < 32; i += 4) {
     const float4 x = *reinterpret_cast<const float4*>(sx + i);
@@ -145,17 +149,25 @@ __device__ __forceinline__ void put_columns(T* y, uint64_t stride, uint32_t nw, 
       float2 v = make_float2((float)(int)r[j], (float)(int)r[j + 1]);
       v = mul2(mul2(v, h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)), w2);
       if (add) v.x = __fadd_rn(v.x, bias), v.y = __fadd_rn(v.y, bias);
-      if constexpr (sizeof(T) == 4) {
-        Act<T>::put(y, v.x);
-        Act<T>::put(y + stride, v.y);
-      } else {
+      if constexpr (PAIR) {
         const bool odd = lane & 1;
         const float other = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1);
         *reinterpret_cast<uint32_t*>(y) = pack2<T>(odd ? other : v.x, odd ? v.y : other);
+      } else {
+        Act<T>::put(y, v.x);
+        Act<T>::put(y + stride, v.y);
       }
       y += 2 * stride;
     }
   }
+}
+template <class T>
+__device__ __forceinline__ void put_columns(T* y, uint64_t stride, uint32_t nw, uint32_t lane, const uint32_t (&r)[32],
+                                            const float* sx, float sw, bool add, float bias, bool wide) {
+  if (sizeof(T) == 2 && !wide)
+    put_columns_as<T, false>(y, stride, nw, lane, r, sx, sw, add, bias);
+  else
+    put_columns_as<T, true>(y, stride, nw, lane, r, sx, sw, add, bias);
 }
 // The same for one channel (at y) and `count` tokens.
 template <class T>
@@ -287,7 +299,7 @@ __global__ void __launch_bounds__(256)
   const uint32_t e = warp & 3;
   for (uint32_t c = 32 * (warp >> 2); c < tokens; c += 64) {
     uint32_t r[32];
-    tmem_ld_32(tmem + (e << 21) + c, r);
+    tmem_ask_32(tmem + (e << 21) + c, r), tmem_have(r);
     if (s.split > 1) {
 #pragma unroll
       for (int i = 0; i < 32; i++)
@@ -297,8 +309,8 @@ __global__ void __launch_bounds__(256)
       const uint32_t nw = n0 + 32 * e, n = nw + lane;
       const float sw = s_w[32 * e + lane], bias = s_b[32 * e + lane];
       T* y = (T*)a.y + (uint64_t)c * a.y_stride;
-      if (s.wide && nw + 32 <= a.n_out && c + 32 <= tokens)
-        put_columns<T>(y, a.y_stride, nw, lane, r, s_x + c, sw, a.bias != nullptr, bias);
+      if (nw + 32 <= a.n_out && c + 32 <= tokens)
+        put_columns<T>(y, a.y_stride, nw, lane, r, s_x + c, sw, a.bias != nullptr, bias, s.wide);
       else if (n < a.n_out)
         put_columns_any<T>(y + n, a.y_stride, min(32u, tokens - c), r, s_x + c, sw, a.bias != nullptr, bias);
     }
@@ -468,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
     for (uint32_t tile = pair; tile < s.tiles; tile += pairs) {
       const uint32_t nw = tile / s.n_tiles * (2 * TM) + rank * TM + 32 * e, n = nw + lane, t0 = tile % s.n_tiles * s.cols;
       const uint32_t tokens = min(s.cols, a.n_tokens - t0);
-      const bool live = n < a.n_out, whole = s.wide && nw + 32 <= a.n_out;
+      const bool live = n < a.n_out;
       const float sw = live ? a.w_scale[n] : 0.f, bias = live && a.bias ? a.bias[n] : 0.f;
       for (uint32_t t = lane; t < s.cols; t += 32) sx[t] = t < tokens ? a.x_scale[t0 + t] : 0.f;
       __syncwarp();
@@ -477,20 +489,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
       tc_fence_after_sync();
       for (uint32_t c = 32 * set; c < s.cols; c += 64) {
         uint32_t r[32];
-        tmem_ld_32(tmem + (e << 21) + buf * 256 + c, r);
-        if (!good || c >= tokens) continue;
+        tmem_ask_32(tmem + (e << 21) + buf * 256 + c, r), tmem_have(r);
         T* y = (T*)a.y + (uint64_t)(t0 + c) * a.y_stride;
-        if (whole && c + 32 <= tokens)
-          put_columns<T>(y, a.y_stride, nw, lane, r, sx + c, sw, a.bias != nullptr, bias);
-        else if (live)
+        if (good && nw + 32 <= a.n_out && c + 32 <= tokens)
+          put_columns<T>(y, a.y_stride, nw, lane, r, sx + c, sw, a.bias != nullptr, bias, s.wide);
+        else if (good && live && c < tokens)
           put_columns_any<T>(y + n, a.y_stride, min(32u, tokens - c), r, sx + c, sw, a.bias != nullptr, bias);
+        __syncwarp();
       }
       tc_fence_before_sync();
       __syncwarp();
+      // what the arrival hands over is tensor memory, which the fence above orders; released to the whole cluster it would
+      // wait for the results' stores as well (2048 x 8192 x 512: 18.2 us, 16.3 so)
       if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                         map_cluster(tc_smem_u32(acc_free + buf), 0))
-                     : "memory");
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_cluster(tc_smem_u32(acc_free + buf), 0)) : "memory");
       if (++buf == 2) buf = 0, turn ^= 1;
     }
   }
