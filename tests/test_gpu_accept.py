@@ -132,7 +132,8 @@ def same(got, want):
 @pytest.mark.parametrize("seqs,t,vocab,tree,ragged", [
     (1, 1, 1, False, False), (1, 4, 7, False, False), (40, 5, 33, False, True), (40, 12, 50, True, True),
     (3, 1, 1000, False, False), (60, 9, 257, True, False), (7, 40, 4000, True, True), (2, 8, 32000, False, True),
-    (5, 3, 50257, True, False), (2, 16, 128256, True, False), (1, 8, 128256, False, False), (150, 3, 600, False, True),
+    (5, 3, 50257, True, False), (2, 16, 128256, True, False), (1, 8, 128256, False, False),
+    (7, 4, 70001, True, True), (8, 4, 70001, True, True), (130, 2, 3001, False, False), (300, 2, 101, True, True), (150, 3, 600, False, True),
     (2, 300, 31, True, False), (1, 1024, 20, False, False), (1, 1024, 20, True, False)])
 def test_walks(seqs, t, vocab, tree, ragged, draft, dtype):
     for seed in range(3 if vocab < 5000 else 1):
