@@ -493,7 +493,8 @@ int rf_dequantize_i8(const int8_t* q, const float* scale, void* out, int act_typ
 /* y[t][n] = (sum_k x[t][k] w[n][k]) * x_scale[t] * w_scale[n] + bias[n] for t < n_tokens, n < n_out:
  * the sum in whole numbers, exact; then f32 in the order written, rounded to act_type.
  * bias: n_out f32, or NULL.  x [n_tokens][n_in] and w [n_out][n_in] int8 (any codes, -128 too)
- * with 16-byte aligned rows (strides multiples of 16); n_in 1..65536; y rows at any
+ * with 16-byte aligned rows (strides multiples of 16); the 16 bytes that hold a row's last
+ * code are read whole, so they belong to the buffer.  n_in 1..65536; y rows at any
  * stride >= n_out.  y overlaps no input. */
 int rf_i8_matmul(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const float* bias, void* y,
                  int act_type, uint32_t n_tokens, uint32_t n_out, uint32_t n_in, uint64_t x_stride, uint64_t w_stride,

@@ -190,8 +190,9 @@ constexpr uint32_t TM = 128, TK = 128;  // channels of a tile, elements of a ste
 // One tile a cluster, its elements split over the cluster's CTAs: i8_split_kernel.
 //
 // A CTA has 128 channels x `cols` tokens and a run of the steps; warp 0 copies 128 bytes of each row a step through a
-// ring of `stages`, warp 1 multiplies, and the CTAs' sums meet in shared memory, where each CTA adds and writes its
-// share of the tile.  Tensor memory is given back before the CTAs wait for one another, so that no two clusters can
+// ring of `stages`, warp 1 multiplies, and each CTA's sums go to the shared memory of the CTA that finishes their
+// tokens.  (9 tokens through 128256 x 4096: 82 us, 0.98 of the copy rate; short calls are bound by their fixed parts, some 5 us of
+// launch, first tile and meeting.)  Tensor memory is given back before the CTAs wait for one another, so that no two clusters can
 // wait for each other's columns, and taken only after the kernel before has ended, whose CTAs may still need it.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMaxStages = 12;
@@ -349,8 +350,9 @@ __global__ void __launch_bounds__(256)
 //
 // A pair of CTAs (cta_group::2) has 256 channels x `cols` tokens: each holds 128 rows of W and half of the tokens'
 // rows of X in its shared memory, and the sums of its channels in its tensor memory, so an SM reads 256 rows a step
-// for 128 x 256 sums where a CTA alone reads 384.  At 8 bits that is what bounds it: 64 bytes a cycle and SM would
-// feed the tensor cores' full rate.  Pairs stay and go from tile to tile; two accumulators, so that warps 4 to 11 write one out
+// for 128 x 256 sums where a CTA alone reads 384 (4096 x 28672 x 4096: 303 us with pairs, 691 with CTAs of their own, one wave of
+// tiles after the other).  At the tensor cores' full rate a step of 128 elements takes 512 cycles and 32 KB, 64 bytes a cycle and
+// SM.  Long products are bound by the power cap's clock (3.2 PFLOP/s), short ones (n_in below about 1000) by the results.  Pairs stay and go from tile to tile; two accumulators, so that warps 4 to 11 write one out
 // while the next fills.  Tokens' tiles come first in the order, so that a W tile is read by all of them at about one time.
 //
 //   warp 0  copies (both CTAs, completing on the first one's barriers)
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) i8_few_kernel(MatmulArgs a) {
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const uint32_t n0 = blockIdx.x * 16;
   griddep_launch();
-  if (tid < 16 && n0 + tid < a.n_out)  // the rows' beginnings into L2: safe before the wait
+  if (tid < 16 && n0 + tid < a.n_out && a.n_in >= 16)  // the rows' beginnings into L2: safe before the wait
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w + (n0 + tid) * a.w_stride), "r"(min(a.n_in, 4096u) & ~15u) : "memory");
   griddep_wait();
   const int8_t* w0 = a.w + min(n0 + g, a.n_out - 1) * a.w_stride;

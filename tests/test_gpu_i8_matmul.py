@@ -153,3 +153,34 @@ def test_quantised_on_the_stream_and_replayed():
     torch.cuda.synchronize()
     assert all(torch.equal(o, y) for o in outs)
     assert verify_error_word() == 0
+
+
+@pytest.mark.parametrize("t", [3, 30, 200])
+def test_products_of_rows_that_the_call_before_writes(t):
+    """Each product's rows are the quantised results of the one before, with no wait between the calls."""
+    n = 2048
+    g = gen(t + 50)
+    w = codes(g, n, n, low=-127)
+    sw = torch.full((n,), 1.0 / (73 * n ** 0.5), device="cuda")
+    x = torch.randn(t, n, device="cuda", generator=g)
+
+    def chain(wait):
+        y, outs = x.clone(), []
+        for _ in range(12):
+            q, s = torch.empty(t, n, device="cuda", dtype=torch.int8), torch.empty(t, device="cuda")
+            new = torch.empty(t, n, device="cuda")
+            quantize_i8(y.data_ptr(), q.data_ptr(), s.data_ptr(), _lib.ACT_F32, t, n)
+            if wait:
+                torch.cuda.synchronize()
+            product(q, s, w, sw, "f32", y=new)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(new)
+            y = new
+        torch.cuda.synchronize()
+        return outs
+
+    want = chain(True)
+    for _ in range(5):
+        for a, b in zip(chain(False), want):
+            assert torch.equal(a, b)

@@ -206,3 +206,36 @@ def test_rows_do_not_depend_on_their_place_and_graphs_replay():
     held.copy_(x)
     graph.replay()
     assert torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale)
+
+
+@pytest.mark.parametrize("rows,cols", [(2000, 4096), (3000, 512), (100, 4096), (1400, 4095)])
+def test_rows_that_the_call_before_writes(rows, cols):
+    """Values written by dequantize_i8 and read by norm_i8 and quantize_i8 at once, call after call with no wait
+    between them: each call begins while the one before it ends."""
+    g = gen(rows)
+    w = torch.randn(cols, device="cuda", generator=g)
+    seen = [(torch.randint(-127, 128, (rows, cols), device="cuda", generator=g, dtype=torch.int8),
+             0.001 + torch.rand(rows, device="cuda", generator=g)) for _ in range(4)]
+    values, total = torch.empty(rows, cols, device="cuda"), torch.empty(rows, cols, device="cuda")
+
+    def calls(q, scale, out, wait):
+        for fn in (lambda: dequantize_i8(q.data_ptr(), scale.data_ptr(), values.data_ptr(), _lib.ACT_F32, rows, cols),
+                   lambda: norm_i8(values.data_ptr(), w.data_ptr(), 1e-5, out[0].q.data_ptr(), out[0].scale.data_ptr(),
+                                   _lib.ACT_F32, rows, cols, add_ptr=values.data_ptr(), sum_ptr=total.data_ptr()),
+                   lambda: quantize_i8(total.data_ptr(), out[1].q.data_ptr(), out[1].scale.data_ptr(), _lib.ACT_F32,
+                                       rows, cols)):
+            fn()
+            if wait:
+                torch.cuda.synchronize()
+
+    want = [(Codes(rows, cols), Codes(rows, cols)) for _ in seen]
+    for (q, scale), out in zip(seen, want):
+        calls(q, scale, out, True)
+    got = [(Codes(rows, cols), Codes(rows, cols)) for _ in range(20)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        calls(*seen[i % 4], out, False)
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for a, b in zip(out, want[i % 4]):
+            assert torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale), i
