@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
     };
     auto sum_run = [&](uint32_t from, uint32_t to) {  // a warp's sum of what is left of a run
       double sums[2] = {};
-      constexpr int U = E == 1 ? 4 : 8 / E;  // pieces of a lane in flight
+      constexpr int U = E == 1 ? 8 : 8 / E;  // pieces of a lane in flight
       for (uint32_t x = from + lane * E; x < to; x += U * 32 * E) {
         float pf[U][E], qf[U][E] = {};
 #pragma unroll
@@ -377,7 +377,7 @@ struct BestArgs {
   const void* logits;
   uint64_t stride;
   int32_t* best;
-  uint32_t ctas, run;  // CTAs a cluster, elements of one's run
+  uint32_t ctas;  // CTAs a cluster
 };
 
 constexpr int kBestThreads = 512;
@@ -401,59 +401,58 @@ __device__ __forceinline__ float piece_top(const uint4& u) {
   }
 }
 
-template <class T, int E>
+template <class T>
 __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
+  constexpr uint32_t E = Act<T>::kVec;
   __shared__ uint64_t s_best[kBestThreads / 32], s_cta[kMaxCluster];
   const uint32_t row_at = blockIdx.x / a.ctas, rank = blockIdx.x % a.ctas, tid = threadIdx.x;
   if (a.ctas > 1) cluster_arrive();
   griddep_launch();
   griddep_wait();
-  const uint32_t rows = a.w.n_tokens + 1, b = row_at / rows, r = row_at - b * rows;
+  const uint32_t rows = a.w.n_tokens + 1, b = row_at / rows, r = row_at - b * rows, V = a.w.vocab;
   if (a.ctas > 1) cluster_wait();
   const bool live = (int)r <= max(draft_count(a.w, b), 0);  // not behind the sequence's last draft
   const T* row = (const T*)a.logits + (uint64_t)row_at * a.stride;
-  const uint32_t x0 = min(rank * a.run, a.w.vocab), x1 = min(x0 + a.run, a.w.vocab);
-  // the largest number and the first piece that has it, which is kept: one comparison a piece
+
+  // The row's whole 16-byte pieces, a run of them for each CTA; what lies before and behind them one by one.
+  const uint32_t lead = min((uint32_t)((16 - ((uintptr_t)row & 15)) & 15) / (uint32_t)sizeof(T), V), pieces = (V - lead) / E;
+  const uint32_t p0 = (uint64_t)pieces * rank / a.ctas, p1 = (uint64_t)pieces * (rank + 1) / a.ctas, tail = lead + pieces * E;
   float top = -INFINITY;
   uint32_t at = ~0u;
-  constexpr int U = 4, STEP = kBestThreads * E;  // loads in flight
-  if constexpr (E > 1) {
+  if (live) {
+    if (rank == 0 && tid < lead) {
+      const float v = Act<T>::get(row + tid);
+      if (v > top) top = v, at = tid;
+    }
+    // the largest number and the first piece that has it, which is kept: one comparison a piece
+    float most = -INFINITY;
+    uint32_t piece = 0;
     uint4 kept = make_uint4(0, 0, 0, 0);
-    auto look = [&](uint4 u, uint32_t x) {
-      const float v = piece_top<T>(u);
-      if (v > top) top = v, at = x, kept = u;
-    };
-    const uint32_t end = live ? x0 + (x1 - x0) / E * E : x0;
-    for (uint32_t x = x0 + tid * E; x < end; x += U * STEP) {
+    constexpr int U = 4;  // loads in flight
+    for (uint32_t p = p0 + tid; p < p1; p += U * kBestThreads) {
       uint4 u[U];
 #pragma unroll
       for (int i = 0; i < U; i++)
-        if (x + i * STEP < end) u[i] = ld_once(row + x + i * STEP);
+        if (p + i * kBestThreads < p1) u[i] = ld_once(row + lead + (uint64_t)(p + i * kBestThreads) * E);
 #pragma unroll
       for (int i = 0; i < U; i++)
-        if (x + i * STEP < end) look(u[i], x + i * STEP);
+        if (p + i * kBestThreads < p1) {
+          const float v = piece_top<T>(u[i]);
+          if (v > most) most = v, piece = p + i * kBestThreads, kept = u[i];
+        }
     }
-    if (at != ~0u) {
+    if (most > top) {
       float v[E];
       Act<T>::unpack(kept, v);
-      int first = 0;
+      uint32_t first = 0;
 #pragma unroll
       for (int e = E - 1; e >= 0; e--)
-        if (v[e] == top) first = e;
-      at += first;
+        if (v[e] == most) first = e;
+      top = most, at = lead + piece * E + first;
     }
-    if (live && tid < x1 - end) {  // the row's end, less than a piece
-      const float v = Act<T>::get(row + end + tid);
-      if (v > top) top = v, at = end + tid;
-    }
-  } else if (live) {
-    for (uint32_t x = x0 + tid; x < x1; x += U * STEP) {
-      float v[U];
-#pragma unroll
-      for (int i = 0; i < U; i++) v[i] = x + i * STEP < x1 ? Act<T>::get(row + x + i * STEP) : -INFINITY;
-#pragma unroll
-      for (int i = 0; i < U; i++)
-        if (v[i] > top) top = v[i], at = x + i * STEP;
+    if (rank == a.ctas - 1 && tid < V - tail) {
+      const float v = Act<T>::get(row + tail + tid);
+      if (v > top) top = v, at = tail + tid;
     }
   }
   uint64_t best = at == ~0u ? 0 : best_key(top, at);  // 0: nothing above -infinity
@@ -622,13 +621,9 @@ int rf_verify_greedy(const void* logits, int logit_type, uint32_t vocab, uint32_
   a.w = WalkArgs{tokens, parent, n_draft, hist_len, out_tokens, n_accepted, positions, vocab, n_tokens, nullptr};
   a.logits = logits, a.stride = logits_stride, a.best = best;
   RF_TRY(verify_error_ptr(&a.w.err));
-  const uint32_t es = act_bytes(logit_type), rows = n_seqs * (n_tokens + 1), unit = 16 / es;
-  const bool vec = aligned_to(logits, 16) && logits_stride * es % 16 == 0;
+  const uint32_t rows = n_seqs * (n_tokens + 1);
   a.ctas = cluster_size(rows, 2);
-  a.run = ((vocab + a.ctas - 1) / a.ctas + unit - 1) / unit * unit;
-  auto* k = logit_type == RF_ACT_F32   ? (vec ? best_kernel<float, 4> : best_kernel<float, 1>)
-            : logit_type == RF_ACT_F16 ? (vec ? best_kernel<__half, 8> : best_kernel<__half, 1>)
-                                       : (vec ? best_kernel<__nv_bfloat16, 8> : best_kernel<__nv_bfloat16, 1>);
+  auto* k = logit_type == RF_ACT_F32 ? best_kernel<float> : logit_type == RF_ACT_F16 ? best_kernel<__half> : best_kernel<__nv_bfloat16>;
   RF_CUDA(launch_clusters((cudaStream_t)stream, k, rows, a.ctas, kBestThreads, a));
   RF_CUDA(launch_k(Launch{(cudaStream_t)stream, true}, greedy_walk_kernel, dim3(n_seqs), dim3(128), 0, a));
   return RF_OK;

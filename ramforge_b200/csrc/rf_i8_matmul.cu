@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "rf_act.cuh"
 #include "rf_device.cuh"
@@ -592,7 +593,7 @@ int run_split(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
 }
 
 // The tile's columns are those for which a model of the call says it is fastest: 256 elements take a pair 0.2 us and
-// 1.8 ns a column, at least 0.28 (333 tokens, 4096 x 4096: 14.5 us with tiles of 192, 11.8 with 128, 11.1 with 96; 128 tokens, 28672 x
+// 1.8 ns a column, at least 0.28, and a tile no less than its results, 12.5 ns a column (333 tokens, 4096 x 4096: 14.5 us with tiles of 192, 11.8 with 128, 11.1 with 96; 128 tokens, 28672 x
 // 4096: 25.3 with 128, 28.9 with 64, which goes round twice).
 template <class T>
 int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
@@ -602,7 +603,7 @@ int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   double best = 1e30;
   for (uint32_t cols = 256; cols >= 32; cols -= 32) {
     const uint64_t rounds = (m_tiles * ((a.n_tokens + cols - 1) / cols) + pairs - 1) / pairs;
-    const double us = (double)rounds * std::max(0.28, 0.2 + 0.0018 * cols);
+    const double us = (double)rounds * std::max(std::ceil(a.n_in / 256.0) * std::max(0.28, 0.2 + 0.0018 * cols), 0.0125 * cols);
     if (us < best) best = us, s.cols = cols;
   }
   s.n_tiles = (a.n_tokens + s.cols - 1) / s.cols;
@@ -718,8 +719,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) i8_few_kernel(MatmulArgs a) {
 template <class T>
 int run(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   // one token, 4096 x 4096: 6.0 us in i8_few_kernel and 7.0 in i8_split_kernel, 2048 x 2048: 3.1 and 6.0; its loads do not
-  // keep up with a ring's where a warp has many runs or an SM many CTAs (6144 x 4096: 10.9 and 8.8)
-  if (a.n_tokens <= 8 && a.n_in <= 8192 && (uint64_t)a.n_out * a.n_in <= 18u << 20) {
+  // keep up with a ring's where a warp has many runs or an SM many CTAs (6144 x 4096: 10.9 and 8.8; 86720 x 128: 32.9 and 6.6)
+  if (a.n_tokens <= 8 && a.n_in <= 8192 && (uint64_t)a.n_out * a.n_in <= 18u << 20 && a.n_out <= 48u * num_sms()) {
     RF_CUDA(launch_k(Launch{st, true}, i8_few_kernel<T>, dim3((a.n_out + 15) / 16), dim3(32 * kFewWarps), 0, a));
     return RF_OK;
   }
