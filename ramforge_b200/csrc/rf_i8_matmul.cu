@@ -480,13 +480,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
     const uint32_t e = warp & 3, set = (warp - 4) >> 2;  // channels 32 e on, every other 32 columns
     float* sx = s_x[warp - 4];
     uint32_t buf = 0, turn = 0;
+    // scales and bias of a tile, asked for while the one before is written
+    float sw_next = 0.f, bias_next = 0.f, x_next[8];
+    auto ask = [&](uint32_t tile) {
+      const uint32_t n = tile / s.n_tiles * (2 * TM) + rank * TM + 32 * e + lane, t0 = tile % s.n_tiles * s.cols;
+      const bool live = tile < s.tiles && n < a.n_out;
+      sw_next = live ? a.w_scale[n] : 0.f;
+      bias_next = live && a.bias ? a.bias[n] : 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) {
+        const uint32_t t = 32 * i + lane;
+        x_next[i] = tile < s.tiles && t < s.cols && t0 + t < a.n_tokens ? a.x_scale[t0 + t] : 0.f;
+      }
+    };
+    ask(pair);
     for (uint32_t tile = pair; tile < s.tiles; tile += pairs) {
       const uint32_t nw = tile / s.n_tiles * (2 * TM) + rank * TM + 32 * e, n = nw + lane, t0 = tile % s.n_tiles * s.cols;
       const uint32_t tokens = min(s.cols, a.n_tokens - t0);
       const bool live = n < a.n_out;
-      const float sw = live ? a.w_scale[n] : 0.f, bias = live && a.bias ? a.bias[n] : 0.f;
-      for (uint32_t t = lane; t < s.cols; t += 32) sx[t] = t < tokens ? a.x_scale[t0 + t] : 0.f;
+      const float sw = sw_next, bias = bias_next;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) sx[32 * i + lane] = x_next[i];
       __syncwarp();
+      ask(tile + pairs);
       const bool good = wait_bar(acc_full + buf, turn, stop, s.err);
       __syncwarp();
       tc_fence_after_sync();
