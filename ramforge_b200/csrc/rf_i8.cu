@@ -15,6 +15,7 @@
 
 #include "rf_act.cuh"
 #include "rf_device.cuh"
+#include "rf_pair.cuh"
 #include "rf_ring.cuh"
 #include "rf_verify.h"
 
@@ -65,16 +66,54 @@ __device__ __forceinline__ void store8_wide(float* p, const float (&v)[8]) {
                : "memory");
 }
 
-// What a row's numbers become before the reduction.
+// What a row's numbers become before the reduction, in pairs: instructions bound the kernels that keep HBM busy (7 issue
+// slots of 10 full where each number was by itself).
 template <int MODE>
-__device__ __forceinline__ float combine(float x, float y) {
-  if constexpr (MODE == kSwiglu)
-    // exponential and quotient to a few units of the 24th bit: a code holds 8, and the few that lie that near to a
+__device__ __forceinline__ float2 combine2(float2 x, float2 y) {
+  if constexpr (MODE == kSwiglu) {
+    // exponential and reciprocal to a few units of the 24th bit: a code holds 8, and the few that lie that near to a
     // border go to either side
-    return __fdividef(x, 1.f + __expf(-x)) * y;
-  else
-    return __fadd_rn(x, y);
+    float2 e = pair_mul(x, make_float2(-1.44269504f, -1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    e = pair_add(e, make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    return pair_mul(pair_mul(x, e), y);
+  } else {
+    return pair_add(x, y);
+  }
 }
+template <int MODE>
+__device__ __forceinline__ void combine8(float (&v)[8], const float (&y)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float2 r = combine2<MODE>(make_float2(v[j], v[j + 1]), make_float2(y[j], y[j + 1]));
+    v[j] = r.x, v[j + 1] = r.y;
+  }
+}
+__device__ __forceinline__ void multiply8(float (&v)[8], const float (&w)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float2 r = pair_mul(make_float2(v[j], v[j + 1]), make_float2(w[j], w[j + 1]));
+    v[j] = r.x, v[j + 1] = r.y;
+  }
+}
+// The largest magnitude of top and eight numbers; NaN where one is.
+__device__ __forceinline__ float top8(float top, const float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2)
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(v[j])), "f"(fabsf(v[j + 1])));
+  return top;
+}
+// Sum of squares in 64 bits, in two chains.
+struct Squares {
+  double a = 0, b = 0;
+  __device__ __forceinline__ void add8(const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) a = fma((double)v[j], (double)v[j], a), b = fma((double)v[j + 1], (double)v[j + 1], b);
+  }
+};
 
 // A row's scale and what its codes are made with, out of its largest magnitude (as bits: a NaN's are above every
 // number's) and sum of squares.
@@ -94,24 +133,29 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top, double ss, uint32_t 
   s.inv = s.wild || s.scale == 0.f ? 0.f : __fdiv_rn(1.f, s.scale);
   return s;
 }
-// Low byte: the code.  Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even.
+// Eight codes.  Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and leaves it in the low byte.  None is over 127:
+// |y| * (1 / scale) is at most 127 (1 + 3 * 2^-24).
 template <int MODE>
-__device__ __forceinline__ uint32_t code_bits(float v, const RowScale& s) {
-  const float y = MODE == kNorm ? __fmul_rn(v, s.r) : v;
-  const uint32_t c = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(y, s.inv), -127.f), 127.f), 12582912.f));
-  return s.wild ? 0u : c;
+__device__ __forceinline__ void codes8(const float (&v)[8], const RowScale& s, uint32_t (&c)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float2 y = make_float2(v[j], v[j + 1]);
+    if constexpr (MODE == kNorm) y = pair_mul(y, make_float2(s.r, s.r));
+    // one by one: a product of pairs and the sum behind it came out as one fused operation, with one rounding in place of the
+    // format's two
+    y.x = __fmul_rn(y.x, s.inv), y.y = __fmul_rn(y.y, s.inv);
+    y = pair_add(y, make_float2(12582912.f, 12582912.f));
+    c[j] = __float_as_uint(y.x), c[j + 1] = __float_as_uint(y.y);
+  }
 }
 template <int MODE>
 __device__ __forceinline__ void store_codes8(int8_t* q, const float (&v)[8], const RowScale& s) {
-  uint32_t b[2];
+  uint32_t c[8], b[2];
+  codes8<MODE>(v, s, c);
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    uint32_t c[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) c[j] = code_bits<MODE>(v[4 * h + j], s);
-    b[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-  }
-  *reinterpret_cast<uint2*>(q) = make_uint2(b[0], b[1]);
+  for (int h = 0; h < 2; h++)
+    b[h] = __byte_perm(__byte_perm(c[4 * h], c[4 * h + 1], 0x0040), __byte_perm(c[4 * h + 2], c[4 * h + 3], 0x0040), 0x5410);
+  *reinterpret_cast<uint2*>(q) = s.wild ? make_uint2(0, 0) : make_uint2(b[0], b[1]);
 }
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -159,12 +203,9 @@ __global__ void __launch_bounds__(1024) rows_cta_kernel(RowsArgs a) {
     float u[PER][8];
     load(y, u);
 #pragma unroll
-    for (int p = 0; p < PER; p++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[p][j] = combine<MODE>(v[p][j], u[p][j]);
+    for (int p = 0; p < PER; p++) combine8<MODE>(v[p], u[p]);
   }
-  double ss = 0;
-  uint32_t top = 0;
+  Squares sq;
   if constexpr (MODE == kNorm) {
     if (a.sum) {
       T* sum = (T*)a.sum + row * a.sum_stride;
@@ -179,24 +220,20 @@ __global__ void __launch_bounds__(1024) rows_cta_kernel(RowsArgs a) {
         }
     }
 #pragma unroll
-    for (int p = 0; p < PER; p++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) ss = fma((double)v[p][j], (double)v[p][j], ss);
+    for (int p = 0; p < PER; p++) sq.add8(v[p]);
     if (a.w) {
       float w[PER][8];
       load(a.w, w);
 #pragma unroll
-      for (int p = 0; p < PER; p++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[p][j] = __fmul_rn(v[p][j], w[p][j]);
+      for (int p = 0; p < PER; p++) multiply8(v[p], w[p]);
     }
   }
+  float most = 0.f;
 #pragma unroll
-  for (int p = 0; p < PER; p++)
-#pragma unroll
-    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[p][j]) & 0x7fffffffu);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if constexpr (MODE == kNorm) ss = warp_sum(ss);
+  for (int p = 0; p < PER; p++) most = top8(most, v[p]);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+  double ss = 0;
+  if constexpr (MODE == kNorm) ss = warp_sum(sq.a + sq.b);
   if (lane == 0) s_top[warp] = top, s_ss[warp] = ss;
   __syncthreads();
   const bool in = lane < (nt >> 5);
@@ -210,9 +247,11 @@ __global__ void __launch_bounds__(1024) rows_cta_kernel(RowsArgs a) {
     if constexpr (VEC) {
       if (place(p, 0) < n) store_codes8<MODE>(q + place(p, 0), v[p], s);
     } else {
+      uint32_t c[8];
+      codes8<MODE>(v[p], s, c);
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (place(p, j) < n) q[place(p, j)] = (int8_t)code_bits<MODE>(v[p][j], s);
+        if (place(p, j) < n) q[place(p, j)] = s.wild ? 0 : (int8_t)c[j];
     }
 }
 
@@ -263,9 +302,8 @@ __global__ void __launch_bounds__(1024) rows_ring_kernel(RowsArgs a, uint32_t n_
   uint32_t slot = 0, phase = 0, turn = 0;
   for (uint64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
     const bool ok = wait_bar(full + slot, phase, &s_stop, err);
-    float v[2][8];
-    double ss = 0;
-    uint32_t top = 0;
+    float v[2][8], most = 0.f;
+    Squares sq;
 #pragma unroll
     for (int p = 0; p < 2; p++) {
 #pragma unroll
@@ -281,23 +319,19 @@ __global__ void __launch_bounds__(1024) rows_ring_kernel(RowsArgs a, uint32_t n_
 #pragma unroll
         for (int i = 0; i < W; i++) u[i] = *reinterpret_cast<const uint4*>(src + n + i * V);
         unpack8<T>(u, y);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[p][j] = combine<MODE>(v[p][j], y[j]);
+        combine8<MODE>(v[p], y);
       }
       if constexpr (MODE == kNorm) {
         if (a.sum && ok) store8<T>((T*)a.sum + row * a.sum_stride + at[p], v[p]);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          ss = fma((double)v[p][j], (double)v[p][j], ss);
-          v[p][j] = __fmul_rn(v[p][j], w[p][j]);
-        }
+        sq.add8(v[p]);
+        multiply8(v[p], w[p]);
       }
-#pragma unroll
-      for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[p][j]) & 0x7fffffffu);
+      most = top8(most, v[p]);
     }
     __syncwarp();
-    top = __reduce_max_sync(0xffffffffu, top);
-    if constexpr (MODE == kNorm) ss = warp_sum(ss);
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    double ss = 0;
+    if constexpr (MODE == kNorm) ss = warp_sum(sq.a + sq.b);
     if (lane == 0) s_top[turn][warp] = top, s_ss[turn][warp] = ss;
     __syncthreads();  // all have read the slot, too
     if (tid == 0 && ok && row + (uint64_t)kRowStages * gridDim.x < n_rows) fetch(row + (uint64_t)kRowStages * gridDim.x, slot);
@@ -370,17 +404,15 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
   uint64_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
   load(row);
   for (; row < n_rows; row += step) {
-    float v[PER][8];
-    uint32_t top = 0;
-    double ss = 0;
+    float v[PER][8], most = 0.f;
+    Squares sq;
 #pragma unroll
     for (int p = 0; p < PER; p++) {
       values(nx, p, v[p]);
       if (a.y) {
         float y[8];
         values(ny, p, y);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[p][j] = combine<MODE>(v[p][j], y[j]);
+        combine8<MODE>(v[p], y);
       }
     }
     load(row + step);
@@ -397,8 +429,7 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
               if (place(p, j) < n) Act<T>::put(sum + place(p, j), v[p][j]);
           }
         }
-#pragma unroll
-        for (int j = 0; j < 8; j++) ss = fma((double)v[p][j], (double)v[p][j], ss);
+        sq.add8(v[p]);
         if (a.w) {
           if constexpr (VEC) {
             if (place(p, 0) < n) {
@@ -416,11 +447,11 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
           }
         }
       }
-#pragma unroll
-      for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[p][j]) & 0x7fffffffu);
+      most = top8(most, v[p]);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if constexpr (MODE == kNorm) ss = warp_sum(ss);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    double ss = 0;
+    if constexpr (MODE == kNorm) ss = warp_sum(sq.a + sq.b);
     const RowScale s = row_scale<MODE>(top, ss, n, a.eps);
     if (lane == 0) a.scale[row] = s.scale;
     int8_t* q = a.q + row * a.q_stride;
@@ -429,9 +460,11 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
       if constexpr (VEC) {
         if (place(p, 0) < n) store_codes8<MODE>(q + place(p, 0), v[p], s);
       } else {
+        uint32_t c[8];
+        codes8<MODE>(v[p], s, c);
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          if (place(p, j) < n) q[place(p, j)] = (int8_t)code_bits<MODE>(v[p][j], s);
+          if (place(p, j) < n) q[place(p, j)] = s.wild ? 0 : (int8_t)c[j];
       }
   }
 }
@@ -525,9 +558,18 @@ __global__ void __launch_bounds__(256) values_i8_kernel(ValuesArgs a) {
 #pragma unroll
     for (int i = 0; i < U; i++) {
       if (at + i * step >= a.pieces) break;
+      // a byte under the exponent of 2^23 is 2^23 + 128 + code, the sum with the bias's negative exact
+      const uint32_t w[2] = {u[i].x ^ 0x80808080u, u[i].y ^ 0x80808080u};
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = __fmul_rn((float)(int8_t)((j < 4 ? u[i].x : u[i].y) >> (8 * (j & 3))), scale[i]);
+      for (int j = 0; j < 8; j += 2) {
+        const uint32_t x = w[j / 4];
+        const float2 code = pair_add(make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 + (j & 3))),
+                                                 __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 + (j & 3) + 1))),
+                                     make_float2(-8388736.f, -8388736.f));
+        const float2 y = pair_mul(code, make_float2(scale[i], scale[i]));
+        v[j] = y.x, v[j + 1] = y.y;
+      }
       if constexpr (sizeof(T) == 4) {
         if (a.wide)
           store8_wide(to[i], v);

@@ -13,6 +13,7 @@
 
 #include "rf_act.cuh"
 #include "rf_device.cuh"
+#include "rf_pair.cuh"
 #include "rf_ring.cuh"
 #include "rf_verify.h"
 
@@ -112,14 +113,6 @@ __device__ __forceinline__ void put4(const MatmulArgs& a, uint32_t t, uint32_t n
   }
 }
 
-// Products of pairs of f32 in one instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-  return d;
-}
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -148,7 +141,7 @@ __device__ __forceinline__ void put_columns_as(T* y, uint64_t stride, uint32_t n
     for (int h = 0; h < 2; h++) {
       const int j = i + 2 * h;
       float2 v = make_float2((float)(int)r[j], (float)(int)r[j + 1]);
-      v = mul2(mul2(v, h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)), w2);
+      v = pair_mul(pair_mul(v, h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)), w2);
       if (add) v.x = __fadd_rn(v.x, bias), v.y = __fadd_rn(v.y, bias);
       if constexpr (PAIR) {
         const bool odd = lane & 1;
