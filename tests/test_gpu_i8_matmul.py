@@ -112,9 +112,13 @@ def test_a_token_does_not_depend_on_the_batch():
     g = gen(8)
     x, w = codes(g, 700, 4096, low=-127), codes(g, 4096, 4096, low=-127)
     sx, sw = torch.rand(700, device="cuda", generator=g), torch.rand(4096, device="cuda", generator=g) / 4096
-    y = product(x, sx, w, sw, "bf16")
-    for at, m in ((0, 1), (5, 12), (100, 100), (0, 300), (690, 10)):
-        assert torch.equal(product(x[at:at + m], sx[at:], w, sw, "bf16"), y[at:at + m])
+    bias = torch.randn(4096, device="cuda", generator=g)
+    for dtype, b in (("bf16", None), ("f32", None), ("f32", bias)):
+        y = product(x, sx, w, sw, dtype, b)
+        for at, m in ((0, 1), (5, 12), (3, 64), (100, 100), (0, 300), (690, 10)):
+            assert torch.equal(product(x[at:at + m], sx[at:], w, sw, dtype, b), y[at:at + m]), (dtype, m)
+        few = product(x[:3, :1024], sx, w[:, :1024], sw, dtype, b)  # small enough for the kernel of few tokens
+        assert torch.equal(few, product(x[:200, :1024], sx, w[:, :1024], sw, dtype, b)[:3])
 
 
 def test_quantised_on_the_stream_and_replayed():
