@@ -601,9 +601,10 @@ int run_split(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   return RF_OK;
 }
 
-// The tile's columns are those for which a model of the call says it is fastest: 256 elements take a pair 0.2 us and
-// 1.8 ns a column, at least 0.28, and a tile no less than its results, 12.5 ns a column (333 tokens, 4096 x 4096: 14.5 us with tiles of 192, 11.8 with 128, 11.1 with 96; 128 tokens, 28672 x
-// 4096: 25.3 with 128, 28.9 with 64, which goes round twice).
+// The tile's columns are those for which a model of the call says it is fastest: 256 elements take a pair
+// 0.2 us and 1.8 ns a column, at least 0.28, and a tile's results 0.6 us and 9 ns a column; the longer of the two
+// counts in each round, and the results of the last one besides.  333 tokens, 4096 x 4096: 14.7 us with tiles of
+// 192, 11.8 with 128, 11.2 with 96, 15.7 with 64 (two rounds); 3718 tokens, 6016 x 192: 37.4 with 32, 24.6 with 64, 19.7 with 128, 17.1 with 256.
 template <class T>
 int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   PairArgs s{};
@@ -612,7 +613,8 @@ int run_pair(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
   double best = 1e30;
   for (uint32_t cols = 256; cols >= 32; cols -= 32) {
     const uint64_t rounds = (m_tiles * ((a.n_tokens + cols - 1) / cols) + pairs - 1) / pairs;
-    const double us = (double)rounds * std::max(std::ceil(a.n_in / 256.0) * std::max(0.28, 0.2 + 0.0018 * cols), 0.0125 * cols);
+    const double results = 0.6 + 0.009 * cols;
+    const double us = (double)rounds * std::max(std::ceil(a.n_in / 256.0) * std::max(0.28, 0.2 + 0.0018 * cols), results) + results;
     if (us < best) best = us, s.cols = cols;
   }
   s.n_tiles = (a.n_tokens + s.cols - 1) / s.cols;
