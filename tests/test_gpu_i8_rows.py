@@ -239,3 +239,116 @@ def test_rows_that_the_call_before_writes(rows, cols):
     for i, out in enumerate(got):
         for a, b in zip(out, want[i % 4]):
             assert torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale), i
+
+
+def placed(rows, cols, gap, lead, dt, seed):
+    """A [rows, cols] view `lead` elements into a buffer, `gap` apart; everything beside the rows is NaN."""
+    buf = torch.full((lead + rows * (cols + gap),), float("nan"), device="cuda", dtype=dt)
+    view = buf[lead:].view(rows, cols + gap)[:, :cols]
+    view.copy_(torch.randn(rows, cols, device="cuda", generator=gen(seed)))
+    return buf, view
+
+
+def beside_is_nan(buf, view):
+    mask = torch.ones_like(buf, dtype=torch.bool)
+    lead = view.storage_offset()
+    mask[lead:].view(view.shape[0], view.stride(0))[:, :view.shape[1]] = False
+    return bool(buf[mask].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("rows,cols,gap,leads", [
+    (2500, 601, 0, (0, 0)), (2500, 601, 0, (3, 6)), (1000, 4095, 0, (1, 0)), (1000, 4093, 2, (5, 2)),
+    (2600, 522, 1, (2, 7)), (1000, 4096, 4, (4, 0)), (4000, 515, 6, (7, 3)), (950, 4094, 1, (6, 1)), (320, 14335, 0, (1, 2))])
+def test_many_rows_at_any_place(rows, cols, gap, leads, in_place, dtype):
+    """Rows that begin anywhere within 16 bytes, the two inputs at different places, NaN in all that lies beside them."""
+    code, dt = ACT[dtype]
+    xb, x = placed(rows, cols, gap, leads[0], dt, rows + cols)
+    ab, add = placed(rows, cols, gap, leads[1], dt, rows + cols + 1)
+    if in_place:
+        tb, total = xb, x
+    else:
+        tb, total = placed(rows, cols, gap, leads[0], dt, 1)
+    w = 1 + 0.5 * torch.randn(cols, device="cuda", generator=gen(cols))
+    s, y = norm_rows(f32(x), f32(add), f32(w), 1e-5)
+    out = Codes(rows, cols, pad=-cols % 8 + 8)
+    norm_i8(x.data_ptr(), w.data_ptr(), 1e-5, out.q.data_ptr(), out.scale.data_ptr(), code, rows, cols,
+            add_ptr=add.data_ptr(), sum_ptr=total.data_ptr(), x_stride=x.stride(0), add_stride=add.stride(0),
+            sum_stride=total.stride(0), q_stride=out.q.stride(0))
+    c, scale = rows_of(y)
+    out.same(c, scale)
+    assert torch.equal(total.cpu(), torch.from_numpy(s).to(dt))
+    assert beside_is_nan(tb, total) and beside_is_nan(ab, add) and beside_is_nan(xb, x)
+    for to in ACT:
+        vb, values = placed(rows, cols, gap, leads[1], ACT[to][1], 2)
+        dequantize_i8(out.q.data_ptr(), out.scale.data_ptr(), values.data_ptr(), ACT[to][0], rows, cols,
+                      q_stride=out.q.stride(0), out_stride=values.stride(0))
+        assert torch.equal(values.cpu(), torch.from_numpy(c.astype(F) * scale[:, None]).to(ACT[to][1]))
+        assert beside_is_nan(vb, values)
+    # no second input, no weights
+    norm_i8(add.data_ptr(), 0, 1e-6, out.q.data_ptr(), out.scale.data_ptr(), code, rows, cols, x_stride=add.stride(0),
+            q_stride=out.q.stride(0))
+    out.same(*rows_of(norm_rows(f32(add), None, None, 1e-6)[1]))
+    quantize_i8(add.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(), code, rows, cols, x_stride=add.stride(0),
+                q_stride=out.q.stride(0))
+    out.same(*rows_of(f32(add)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(2500, 601), (1000, 4095), (330, 14335), (4000, 515)])
+def test_many_rows_are_as_alone(rows, cols, dtype):
+    """A row's codes are the same in a call of many rows and in one of its own, wild rows among them."""
+    code, dt = ACT[dtype]
+    gu = torch.randn(rows, 2 * cols, device="cuda", generator=gen(rows)).to(dt)
+    gu[7, 3], gu[rows - 1, cols - 1], gu[11, 2 * cols - 1] = float("nan"), float("inf"), float("-inf")
+    gu[12] = 0
+    es, wide = gu.element_size(), -(-cols // 8) * 8
+    many, one = Codes(rows, cols, pad=wide - cols), Codes(rows, cols, pad=wide - cols)
+    swiglu_i8(gu.data_ptr(), gu.data_ptr() + cols * es, many.q.data_ptr(), many.scale.data_ptr(), code, rows, cols,
+              gate_stride=2 * cols, up_stride=2 * cols, q_stride=wide)
+    looked = [0, 1, 7, 11, 12, rows // 2, rows - 2, rows - 1]
+    for r in looked:
+        at = gu.data_ptr() + 2 * r * cols * es
+        swiglu_i8(at, at + cols * es, one.q[r].data_ptr(), one.scale[r:].data_ptr(), code, 1, cols)
+    assert torch.equal(many.q[looked], one.q[looked]) and (many.q[:, cols:] == 99).all()
+    assert torch.equal(many.scale[looked].view(torch.int32), one.scale[looked].view(torch.int32))
+    assert many.scale[[7, 11, rows - 1]].isnan().all() and not many.q[[7, 11, 12, rows - 1], :cols].any()
+
+
+@pytest.mark.parametrize("rows,cols", [(1400, 4095), (2500, 601), (700, 1999), (400, 7001)])
+def test_rows_at_any_place_that_the_call_before_writes(rows, cols):
+    """The same chain with codes in whole eights and rows of values at any place, and SwiGLU of neighbours."""
+    g = gen(rows)
+    wide = -(-cols // 8) * 8
+    w = torch.randn(cols, device="cuda", generator=g)
+    seen = [(torch.randint(-127, 128, (rows, wide), device="cuda", generator=g, dtype=torch.int8),
+             0.001 + torch.rand(rows, device="cuda", generator=g)) for _ in range(4)]
+    values, total = torch.empty(rows, cols, device="cuda"), torch.empty(rows, cols, device="cuda")
+
+    def calls(q, scale, out, wait):
+        for fn in (lambda: dequantize_i8(q.data_ptr(), scale.data_ptr(), values.data_ptr(), _lib.ACT_F32, rows, cols,
+                                         q_stride=wide),
+                   lambda: norm_i8(values.data_ptr(), w.data_ptr(), 1e-5, out[0].q.data_ptr(), out[0].scale.data_ptr(),
+                                   _lib.ACT_F32, rows, cols, add_ptr=values.data_ptr(), sum_ptr=total.data_ptr(),
+                                   q_stride=wide),
+                   lambda: swiglu_i8(total.data_ptr(), values.data_ptr(), out[1].q.data_ptr(),
+                                     out[1].scale.data_ptr(), _lib.ACT_F32, rows, cols, q_stride=wide)):
+            fn()
+            if wait:
+                torch.cuda.synchronize()
+
+    def outputs():
+        return Codes(rows, cols, pad=wide - cols), Codes(rows, cols, pad=wide - cols)
+
+    want = [outputs() for _ in seen]
+    for (q, scale), out in zip(seen, want):
+        calls(q, scale, out, True)
+    got = [outputs() for _ in range(20)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        calls(*seen[i % 4], out, False)
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for a, b in zip(out, want[i % 4]):
+            assert torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale), i
