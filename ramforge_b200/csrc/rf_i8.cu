@@ -261,24 +261,31 @@ __global__ void __launch_bounds__(1024) rows_cta_kernel(RowsArgs a) {
 
 // ---- many rows, aligned -------------------------------------------------------------------
 // CTAs stay and go from row to row.  Rows come into a ring in shared memory by bulk copies, which go on while a row is
-// reduced and coded; 16 elements a thread, for a norm 32 (instructions bound it, and those for each row and warp are as many as for 16
-// elements: 4001 x 4096 bf16 with residual and sum 23.0 us with 16, 21.8 with 32, 5.3 TB/s), the norm's weights in registers.
-// SwiGLU of 2048 x 14336: 29.2 us, with one CTA of 896 threads an SM.  The next kernel is let in with the last row: from the first
-// one on, its waiting CTAs slowed chains of calls (norms of 8192 x 2001 f32 and the values back: 87 us, 67 so).
+// reduced and coded; 32 elements a thread, a norm's weights in registers.  Instructions bound it, and those for each row and
+// warp are as many as for 16 elements: 4001 x 4096 bf16 with residual and sum 23.0 us with 16 elements, 21.4 with 32 (5.4
+// TB/s).  Where rows are so long that an SM has one CTA, two teams of its warps have a ring each, so that one asks for data
+// while the other reduces: SwiGLU of 2048 x 14336 29.0 us without, 26.9 with them (5.5 TB/s).  The next kernel is let in with
+// the last row: from the first one on, its waiting CTAs slowed chains of calls (norms of 8192 x 2001 f32 and the values
+// back: 87 us, 67 so).
 constexpr int kRowStages = 3;
-constexpr uint32_t kRingBytes = 220 * 1024;
+constexpr uint32_t kRingBytes = 224 * 1024;
 
-template <class T, int MODE, int PER>
-__global__ void __launch_bounds__(2048 / PER) rows_ring_kernel(RowsArgs a, uint32_t n_rows, unsigned* err) {
-  extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ uint64_t full[kRowStages];
-  __shared__ double s_ss[2][32];
-  __shared__ uint32_t s_top[2][32], s_stop;
-  const uint32_t n = a.n_cols, tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31;
+template <class T, int MODE, int PER, int TEAMS>
+__global__ void __launch_bounds__(2048 / PER * TEAMS) rows_ring_kernel(RowsArgs a, uint32_t n_rows, uint32_t stages, unsigned* err) {
+  extern __shared__ __align__(128) uint8_t rings[];
+  __shared__ uint64_t fulls[TEAMS][kRowStages];
+  __shared__ double s_sss[TEAMS][2][32];
+  __shared__ uint32_t s_tops[TEAMS][2][32], s_stop;
+  const uint32_t n = a.n_cols, nt = blockDim.x / TEAMS, team = threadIdx.x / nt, tid = threadIdx.x - team * nt, warp = tid >> 5, lane = tid & 31;
+  const uint32_t first = blockIdx.x * TEAMS + team, step = gridDim.x * TEAMS;
   const uint32_t bytes = n * sizeof(T), stage = (a.y ? 2 : 1) * bytes;
   constexpr int V = Act<T>::kVec, W = 8 / V;
-  if (tid == 0) {
-    for (int i = 0; i < kRowStages; i++) tc_mbar_init(tc_smem_u32(full + i), 1);
+  uint8_t* ring = rings + team * stages * stage;
+  uint64_t* full = fulls[team];
+  auto &s_ss = s_sss[team];
+  auto &s_top = s_tops[team];
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < TEAMS * kRowStages; i++) tc_mbar_init(tc_smem_u32(fulls[0] + i), 1);
     tc_fence_barrier_init();
     s_stop = 0;
   }
@@ -291,8 +298,8 @@ __global__ void __launch_bounds__(2048 / PER) rows_ring_kernel(RowsArgs a, uint3
     if (a.y) tc_bulk_copy_g2s(dst + bytes, (const T*)a.y + row * a.y_stride, bytes, bar);
   };
   if (tid == 0)
-    for (int i = 0; i < kRowStages; i++)
-      if (blockIdx.x + (uint64_t)i * gridDim.x < n_rows) fetch(blockIdx.x + (uint64_t)i * gridDim.x, i);
+    for (uint32_t i = 0; i < stages; i++)
+      if (first + (uint64_t)i * step < n_rows) fetch(first + (uint64_t)i * step, i);
   uint32_t at[PER];
 #pragma unroll
   for (int p = 0; p < PER; p++) at[p] = (tid + p * nt) * 8;
@@ -308,8 +315,8 @@ __global__ void __launch_bounds__(2048 / PER) rows_ring_kernel(RowsArgs a, uint3
       }
   }
   uint32_t slot = 0, phase = 0, turn = 0;
-  for (uint64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
-    if (row + gridDim.x >= n_rows) griddep_launch();
+  for (uint64_t row = first; row < n_rows; row += step) {
+    if (row + step >= n_rows) griddep_launch();
     const bool ok = wait_bar(full + slot, phase, &s_stop, err);
     float v[PER][8], most = 0.f;
     Squares sq;
@@ -342,8 +349,11 @@ __global__ void __launch_bounds__(2048 / PER) rows_ring_kernel(RowsArgs a, uint3
     double ss = 0;
     if constexpr (MODE == kNorm) ss = warp_sum(sq.a + sq.b);
     if (lane == 0) s_top[turn][warp] = top, s_ss[turn][warp] = ss;
-    __syncthreads();  // all have read the slot, too
-    if (tid == 0 && ok && row + (uint64_t)kRowStages * gridDim.x < n_rows) fetch(row + (uint64_t)kRowStages * gridDim.x, slot);
+    if constexpr (TEAMS == 1)  // all have read the slot, too
+      __syncthreads();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(nt) : "memory");
+    if (tid == 0 && ok && row + (uint64_t)stages * step < n_rows) fetch(row + (uint64_t)stages * step, slot);
     __syncwarp();
     const bool in = lane < (nt >> 5);
     top = __reduce_max_sync(0xffffffffu, in ? s_top[turn][lane] : 0u);
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(2048 / PER) rows_ring_kernel(RowsArgs a, uint3
         if (at[p] < n) store_codes8<MODE>(a.q + row * a.q_stride + at[p], v[p], s);
     }
     turn ^= 1;
-    if (++slot == kRowStages) slot = 0, phase ^= 1;
+    if (++slot == stages) slot = 0, phase ^= 1;
   }
   if (*(volatile uint32_t*)&s_stop) {  // gave up: copies in flight end within this time
     const long long t = clock64();
@@ -795,20 +805,27 @@ cudaError_t launch_rows_as(const Launch& L, const RowsArgs& a, uint32_t n_rows, 
       if (per > 2) k = rows_warp_kernel<T, MODE, 4, VEC>;
     return launch_k(L, k, dim3(std::min((n_rows + 7) / 8, sms * 4)), dim3(256), 0, a, n_rows);
   }
-  // CTAs that stay, per_sm of them on each SM: as many as the threads' registers (TH threads) and shared memory have room for
-  auto ring = [&](auto* k, uint32_t threads, uint32_t smem, uint32_t per_sm) {
+  // CTAs that stay, per_sm of them on each SM: as many as its registers and shared memory have room for
+  auto ring = [&](auto* k, uint32_t threads, uint32_t smem, uint32_t per_sm, auto... more) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-    return e != cudaSuccess ? e : launch_k(L, k, dim3(sms * per_sm), dim3(threads), smem, a, n_rows, err);
+    return e != cudaSuccess ? e : launch_k(L, k, dim3(sms * per_sm), dim3(threads), smem, a, n_rows, more..., err);
   };
   if constexpr (VEC) {
-    constexpr uint32_t PER = MODE == kNorm ? 4 : 2, TH = MODE == kNorm ? 512 : 1152;
-    const uint32_t threads = ((eights + PER - 1) / PER + 31) / 32 * 32, smem = kRowStages * (a.y ? 2 : 1) * a.n_cols * (uint32_t)sizeof(T);
-    const uint32_t per_sm = std::min(std::min(TH / threads, kRingBytes / smem), 8u);
-    // a norm: 4001 x 4096 bf16 with residual and sum 21.8 us, 35 with a CTA a row (600 rows: 6.5 and 8.2); SwiGLU of
-    // 5000 x 4096: 21.1 and 16.8, of 1800 x 14336, where an SM has room for one CTA of the other kernel, 27.0 and 31.5
-    const uint32_t some = MODE == kNorm ? std::min(per_sm, n_rows / sms) : per_sm;
-    if (threads <= 2048 / PER && some && (MODE == kNorm ? n_rows >= 4 * sms : a.n_cols > 8192 && n_rows > 2 * sms * per_sm))
-      return ring(rows_ring_kernel<T, MODE, PER>, threads, smem, some);
+    // A norm: 4001 x 4096 bf16 with residual and sum 21.4 us, 35 with a CTA a row (600 rows: 6.5 and 8.2).  SwiGLU of 5000 x
+    // 4096: 21.1 and 16.8; of 2048 x 14336, where an SM has room for one CTA of the other kernel, 26.9 with two teams, 29.0
+    // with one of 16 elements a thread (16384 columns, of which four rows have no room), 36 with a CTA a row.
+    const uint32_t threads = ((eights + 3) / 4 + 31) / 32 * 32, stage = (a.y ? 2 : 1) * a.n_cols * (uint32_t)sizeof(T);
+    const uint32_t stages = std::min(kRingBytes / (2 * stage), (uint32_t)kRowStages);  // of each of two teams
+    if (threads <= 512 && n_rows >= 4 * sms) {
+      if constexpr (MODE == kNorm) {
+        const uint32_t per_sm = std::min(std::min(std::min(512 / threads, kRingBytes / (kRowStages * stage)), 8u), n_rows / sms);
+        if (per_sm) return ring(rows_ring_kernel<T, MODE, 4, 1>, threads, kRowStages * stage, per_sm, kRowStages);
+      } else if (a.n_cols > 8192) {
+        if (stages >= 2) return ring(rows_ring_kernel<T, MODE, 4, 2>, 2 * threads, 2 * stages * stage, 1, stages);
+        if (kRowStages * stage <= kRingBytes)
+          return ring(rows_ring_kernel<T, MODE, 2, 1>, 2 * threads, kRowStages * stage, 1, kRowStages);
+      }
+    }
   } else if (shift) {
     constexpr uint32_t PER = 2, TH = MODE == kNorm ? 1024 : 1280;
     const uint32_t es = sizeof(T), lanes = PER * kOwnLanes, threads = (shift_eights(a.n_cols) + lanes - 1) / lanes * 32;

@@ -352,3 +352,22 @@ def test_rows_at_any_place_that_the_call_before_writes(rows, cols):
     for i, out in enumerate(got):
         for a, b in zip(out, want[i % 4]):
             assert torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale), i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(700, 8200), (900, 11008), (620, 14336), (640, 16384), (597, 9216)])
+def test_many_long_rows_are_as_alone(rows, cols, dtype):
+    """Long rows, of which an SM has few at a time: codes and scales as in calls of one row, for SwiGLU and plain rows."""
+    code, dt = ACT[dtype]
+    x = torch.randn(rows, cols, device="cuda", generator=gen(rows)).to(dt)
+    up = torch.randn(rows, cols, device="cuda", generator=gen(cols)).to(dt)
+    up[5, cols - 1], x[rows - 3, 0], x[9] = float("inf"), float("nan"), 0
+    gated, plain, one = Codes(rows, cols), Codes(rows, cols), Codes(rows, cols)
+    swiglu_i8(x.data_ptr(), up.data_ptr(), gated.q.data_ptr(), gated.scale.data_ptr(), code, rows, cols)
+    quantize_i8(x.data_ptr(), plain.q.data_ptr(), plain.scale.data_ptr(), code, rows, cols)
+    plain.same(*rows_of(f32(x)))
+    for r in range(rows):
+        swiglu_i8(x[r].data_ptr(), up[r].data_ptr(), one.q[r].data_ptr(), one.scale[r:].data_ptr(), code, 1, cols)
+    assert torch.equal(gated.q, one.q)
+    assert torch.equal(gated.scale.view(torch.int32), one.scale.view(torch.int32))
+    assert gated.scale[[5, rows - 3]].isnan().all() and not gated.q[[5, 9, rows - 3]].any()
