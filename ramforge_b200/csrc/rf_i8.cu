@@ -812,8 +812,8 @@ cudaError_t launch_rows_as(const Launch& L, const RowsArgs& a, uint32_t n_rows, 
   };
   if constexpr (VEC) {
     // A norm: 4001 x 4096 bf16 with residual and sum 21.4 us, 35 with a CTA a row (600 rows: 6.5 and 8.2).  SwiGLU of 5000 x
-    // 4096: 21.1 and 16.8; of 2048 x 14336, where an SM has room for one CTA of the other kernel, 26.9 with two teams, 29.0
-    // with one of 16 elements a thread (16384 columns, of which four rows have no room), 36 with a CTA a row.
+    // 4096: 21.1 and 16.8; of 1800 x 14336, where an SM has room for one CTA of the other kernel, 25.0 with two teams, 26.7
+    // with one of 16 elements a thread (kept for rows of which an SM has no room for four), 31.5 with a CTA a row.
     const uint32_t threads = ((eights + 3) / 4 + 31) / 32 * 32, stage = (a.y ? 2 : 1) * a.n_cols * (uint32_t)sizeof(T);
     const uint32_t stages = std::min(kRingBytes / (2 * stage), (uint32_t)kRowStages);  // of each of two teams
     if (threads <= 512 && n_rows >= 4 * sms) {
