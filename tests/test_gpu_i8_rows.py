@@ -371,3 +371,20 @@ def test_many_long_rows_are_as_alone(rows, cols, dtype):
     assert torch.equal(gated.q, one.q)
     assert torch.equal(gated.scale.view(torch.int32), one.scale.view(torch.int32))
     assert gated.scale[[5, rows - 3]].isnan().all() and not gated.q[[5, 9, rows - 3]].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [295, 296, 591, 592, 593])
+@pytest.mark.parametrize("cols,lead", [(64, 3), (65, 0), (100, 1), (301, 5), (513, 2), (1023, 7), (1025, 1), (2801, 3)])
+def test_counts_at_which_the_kernel_changes(rows, cols, lead, dtype):
+    code, dt = ACT[dtype]
+    xb, x = placed(rows, cols, 0, lead, dt, rows + cols)
+    ab, add = placed(rows, cols, 1, 0, dt, rows + cols + 1)
+    out, out2 = Codes(rows, cols, pad=-cols % 8 + 8), Codes(rows, cols, pad=-cols % 8 + 8)
+    norm_i8(x.data_ptr(), 0, 1e-5, out.q.data_ptr(), out.scale.data_ptr(), code, rows, cols, add_ptr=add.data_ptr(),
+            x_stride=x.stride(0), add_stride=add.stride(0), q_stride=out.q.stride(0))
+    quantize_i8(add.data_ptr(), out2.q.data_ptr(), out2.scale.data_ptr(), code, rows, cols, x_stride=add.stride(0),
+                q_stride=out2.q.stride(0))
+    out.same(*rows_of(norm_rows(f32(x), f32(add), None, 1e-5)[1]))
+    out2.same(*rows_of(f32(add)))
+    assert beside_is_nan(xb, x) and beside_is_nan(ab, add)
