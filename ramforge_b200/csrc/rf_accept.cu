@@ -94,7 +94,8 @@ __device__ __forceinline__ void load_piece(const T* row, uint32_t x, uint32_t en
 // Every CTA gathers the drafts and walks until sums are needed; a pass over the vocabulary gives them, a run of it
 // for each CTA and each of its warps, and the CTAs' sums go to all of them.  What comes next is CTA 0's to say: the others follow
 // it, so that all meet at the same barriers whatever they read.  A chain takes one pass, and with it one meeting; each further
-// draft of a node that is refused takes one more (of drafts that were certain, all of a node's together one).  The bytes of the last rows bound a batch (64 sequences, 128256 tokens, f32:
+// draft of a node that is refused takes one more (of drafts that were certain, all of a node's together one, and another
+// wherever less than a sixteenth of the last sum is left: a difference of sums keeps too few bits there).  The bytes of the last rows bound a batch (64 sequences, 128256 tokens, f32:
 // 65.7 MB), latency a sequence: two dependent reads, the walk, the pass, the search of one warp.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
@@ -148,13 +149,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
 
   // the walk's state, in every thread of warp 0
   int node = -1, last = -1, taken = 0, tried = 0;
-  double off = 0.0, mass = 1.0, gone = 0.0;
+  double off = 0.0, mass = 1.0, gone = 0.0, base = 0.0;  // base: certain drafts, the sum that mass is a difference of
   bool whole = false;  // certain drafts: mass comes from the sum of the node's whole row
   Next next = kLast;
   auto walk = [&]() {  // until sums are needed
     bool final = true, masked = true;
-    if (!a.draft && tried) mass = fmax(mass - gone, 0.0);  // the whole row's sum has come
+    if (!a.draft && tried) base = mass, mass -= gone, gone = 0.0;  // the sum has come
     while (true) {
+      // certain drafts: what is left has lost four bits as a difference, so it is summed up by itself
+      if (mass < base / 16) {
+        final = false;
+        break;
+      }
       const int j = next_child(s.parent, n, node, last, lane);
       if (j >= n) break;
       last = j;
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       if ((double)s_u[j] * qc * mass < left) {
         if (lane == 0) s_path[j] = taken;
         __syncwarp();
-        node = j, taken++, tried = 0, off = 0.0, mass = 1.0, whole = false;
+        node = j, taken++, tried = 0, off = 0.0, mass = 1.0, base = 0.0, whole = false;
         continue;
       }
       tried++;
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       if (final) break;
       // certain drafts: the sum of what is left is that of the whole row without the tokens that are out
       if (whole) {
-        mass = fmax(mass - left, 0.0);
+        mass -= left;
       } else {
         gone = left, whole = true, masked = false;
         break;
