@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256)
   if (warp == 0) {
     uint32_t slot = 0, phase = 0, k = k0;
     for (; k < k1; k++) {
-      if (!__all_sync(~0u, wait_bar(empty + slot, phase ^ 1, stop, s.err))) break;
+      if (!wait_bar_warp(empty + slot, phase ^ 1, stop, s.err)) break;
       if (elect_one()) {
         const uint32_t bar = tc_smem_u32(full + slot), dst = ring + slot * stage;
         tc_mbar_expect_tx(bar, stage);
@@ -269,8 +269,7 @@ __global__ void __launch_bounds__(256)
     const uint32_t idesc = idesc_i8(TM, s.cols);
     uint32_t slot = 0, phase = 0;
     for (uint32_t k = k0; k < k1; k++) {
-      const bool ok = wait_bar(full + slot, phase, stop, s.err);
-      if (!__all_sync(~0u, ok)) break;
+      if (!wait_bar_warp(full + slot, phase, stop, s.err)) break;
       tc_fence_after_sync();
       const uint32_t at = uniform(ring + slot * stage);
       const uint64_t da = operand_desc(at), db = operand_desc(at + TM * TK);
@@ -285,7 +284,7 @@ __global__ void __launch_bounds__(256)
     if (elect_one()) tc_commit(tc_smem_u32(&done));
   }
   __syncwarp();
-  const bool good = wait_bar(&done, 0, stop, s.err);
+  const bool good = wait_bar_warp(&done, 0, stop, s.err);
   if (!good) tc_mbar_wait(tc_smem_u32(&done), 0);
   tc_fence_after_sync();
 
@@ -419,7 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
     for (uint32_t tile = pair; tile < s.tiles && ok; tile += pairs) {
       const int n0 = tile / s.n_tiles * (2 * TM) + rank * TM, t0 = tile % s.n_tiles * s.cols + rank * half;
       for (uint32_t k = 0; k < s.steps; k++) {
-        if (!(ok = __all_sync(~0u, wait_bar(empty + slot, phase ^ 1, stop, s.err)))) break;
+        if (!(ok = wait_bar_warp(empty + slot, phase ^ 1, stop, s.err))) break;
         if (elect_one()) {
           const uint32_t bar = map_cluster(tc_smem_u32(full + slot), 0), dst = ring + slot * stage;
           if (rank == 0) tc_mbar_expect_tx(tc_smem_u32(full + slot), 2 * stage);
@@ -436,7 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
     // the last products release their slots in both CTAs: neither ends before
     for (uint32_t i = 0; i < min(uses, s.stages) && ok; i++) {
       if (slot-- == 0) slot = s.stages - 1, phase ^= 1;
-      ok = wait_bar(empty + slot, phase, stop, s.err);
+      ok = wait_bar_warp(empty + slot, phase, stop, s.err);
     }
     if (!ok) {  // gave up: copies in flight end within this time
       const long long t = clock64();
@@ -448,10 +447,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
     uint32_t slot = 0, phase = 0, buf = 0, turn = 0;
     bool ok = true;
     for (uint32_t tile = pair; tile < s.tiles && ok; tile += pairs) {
-      ok = __all_sync(~0u, wait_bar(acc_free + buf, turn ^ 1, stop, s.err));
+      ok = wait_bar_warp(acc_free + buf, turn ^ 1, stop, s.err);
       tc_fence_after_sync();
       for (uint32_t k = 0; k < s.steps && ok; k++) {
-        if (!(ok = __all_sync(~0u, wait_bar(full + slot, phase, stop, s.err)))) break;
+        if (!(ok = wait_bar_warp(full + slot, phase, stop, s.err))) break;
         tc_fence_after_sync();
         const uint32_t at = uniform(ring + slot * stage);
         if (elect_one()) {
@@ -496,7 +495,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
       for (uint32_t i = 0; i < 8; i++) sx[32 * i + lane] = x_next[i];
       __syncwarp();
       ask(tile + pairs);
-      const bool good = wait_bar(acc_full + buf, turn, stop, s.err);
+      const bool good = wait_bar_warp(acc_full + buf, turn, stop, s.err);
       __syncwarp();
       tc_fence_after_sync();
       for (uint32_t c = 32 * set; c < s.cols; c += 64) {

@@ -23,5 +23,10 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   const uint32_t b = tc_smem_u32(bar);
   return tc_mbar_try_wait(b, parity) || wait_slow(b, parity, stop, err);
 }
+// The same by a whole warp, one answer for all of it: a phase may end between two lanes' last looks, and a warp that works as one
+// afterwards (shuffles, tensor memory, tcgen05) must not part there.
+__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* stop, unsigned* err) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, stop, err));
+}
 
 }  // namespace rf
