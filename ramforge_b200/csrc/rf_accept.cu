@@ -425,14 +425,16 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
   const uint32_t p0 = (uint64_t)pieces * rank / a.ctas, p1 = (uint64_t)pieces * (rank + 1) / a.ctas, tail = lead + pieces * E;
   float top = -INFINITY;
   uint32_t at = ~0u;
+  // whether a later number is taken for the one held: a larger one, -infinity as the first, no NaN
+  auto better = [](float v, float held, bool none) { return v > held || (none && v == -INFINITY); };
   if (live) {
     if (rank == 0 && tid < lead) {
       const float v = Act<T>::get(row + tid);
-      if (v > top) top = v, at = tid;
+      if (better(v, top, true)) top = v, at = tid;
     }
     // the largest number and the first piece that has it, which is kept: one comparison a piece
     float most = -INFINITY;
-    uint32_t piece = 0;
+    uint32_t piece = ~0u;
     uint4 kept = make_uint4(0, 0, 0, 0);
     constexpr int U = 4;  // loads in flight
     for (uint32_t p = p0 + tid; p < p1; p += U * kBestThreads) {
@@ -440,14 +442,19 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
 #pragma unroll
       for (int i = 0; i < U; i++)
         if (p + i * kBestThreads < p1) u[i] = ld_once(row + lead + (uint64_t)(p + i * kBestThreads) * E);
+      float v[U];
 #pragma unroll
       for (int i = 0; i < U; i++)
         if (p + i * kBestThreads < p1) {
-          const float v = piece_top<T>(u[i]);
-          if (v > most) most = v, piece = p + i * kBestThreads, kept = u[i];
+          v[i] = piece_top<T>(u[i]);
+          if (v[i] > most) most = v[i], piece = p + i * kBestThreads, kept = u[i];
         }
+      if (piece == ~0u)  // none of them above -infinity
+#pragma unroll
+        for (int i = U - 1; i >= 0; i--)
+          if (p + i * kBestThreads < p1 && v[i] == -INFINITY) piece = p + i * kBestThreads, kept = u[i];
     }
-    if (most > top) {
+    if (piece != ~0u && better(most, top, at == ~0u)) {
       float v[E];
       Act<T>::unpack(kept, v);
       uint32_t first = 0;
@@ -458,10 +465,10 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
     }
     if (rank == a.ctas - 1 && tid < V - tail) {
       const float v = Act<T>::get(row + tail + tid);
-      if (v > top) top = v, at = tail + tid;
+      if (better(v, top, at == ~0u)) top = v, at = tail + tid;
     }
   }
-  uint64_t best = at == ~0u ? 0 : best_key(top, at);  // 0: nothing above -infinity
+  uint64_t best = at == ~0u ? 0 : best_key(top, at);  // 0: NaN alone
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((tid & 31) == 0) s_best[tid >> 5] = best;
@@ -475,13 +482,7 @@ __global__ void __launch_bounds__(kBestThreads) best_kernel(BestArgs a) {
   if (rank || tid || !live) return;
   if (a.ctas > 1)
     for (uint32_t i = 0; i < a.ctas; i++) best = max(best, s_cta[i]);
-  uint32_t x = ~(uint32_t)best;
-  if (!best) {  // -infinity and NaN alone: the first -infinity, or 0
-    for (x = 0; x < a.w.vocab && Act<T>::get(row + x) != -INFINITY; x++) {
-    }
-    if (x == a.w.vocab) x = 0;
-  }
-  a.best[row_at] = (int32_t)x;
+  a.best[row_at] = best ? (int32_t)~(uint32_t)best : 0;
 }
 
 __global__ void __launch_bounds__(128) greedy_walk_kernel(BestArgs a) {

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from ramforge_b200 import verify_error_word
+from ramforge_b200 import _lib, verify_error_word, verify_greedy
 
 from .test_gpu_accept import Case, same, torch
 
@@ -25,3 +25,78 @@ def test_little_left_behind_certain_drafts():
     assert (w[1] == 0).all() and not np.isin(w[0][:, 0], c.tokens).any()
     same(c.run(), w)
     assert verify_error_word() == 0
+
+
+def graph_us(fn, calls=20):
+    """Microseconds of a call among others, the least of five."""
+    fn(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(calls):
+            fn(torch.cuda.current_stream().cuda_stream)
+    times = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3 / calls)
+    return min(times)
+
+
+def greedy_rows(logits, vocab, stride):
+    code = {torch.float32: _lib.ACT_F32, torch.float16: _lib.ACT_F16, torch.bfloat16: _lib.ACT_BF16}[logits.dtype]
+    n = logits.shape[0]
+    best, out, count = (torch.full((n,), -7, device="cuda", dtype=torch.int32) for _ in range(3))
+
+    def call(stream=0):
+        verify_greedy(logits.data_ptr(), code, vocab, n, 0, 0, best.data_ptr(), out.data_ptr(), count.data_ptr(),
+                      logits_stride=stride, stream=stream)
+    call()
+    assert torch.equal(best, out) and not count.any()
+    return best, call
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,gap", [(9, 128256, 0), (9, 50257, 0), (300, 50257, 3), (1, 131, 0), (12, 4097, 2),
+                                            (400, 9, 1)])
+def test_greedy_rows_of_nan_and_infinities(rows, vocab, gap, dtype):
+    """Rows with nothing above -infinity: the first -infinity wherever it lies, 0 where there is none; largest numbers
+    more than once, in front of every place that a thread or a 16-byte piece may begin at."""
+    rs = np.random.RandomState(rows + vocab)
+    logits = torch.full((rows, vocab + gap), float("nan"), device="cuda", dtype=dtype)
+    want = np.zeros(rows, np.int64)
+    for r in range(rows):
+        kind, at = r % 3, rs.randint(vocab)
+        if kind == 0:      # NaN, and one -infinity or more behind it
+            want[r] = at
+            logits[r, at] = logits[r, rs.randint(at, vocab)] = -float("inf")
+            if r % 2:
+                logits[r, at:vocab] = -float("inf")
+        elif kind == 1:    # NaN alone
+            want[r] = 0
+        else:              # two equal numbers between them
+            want[r] = at
+            logits[r, at] = logits[r, rs.randint(at, vocab)] = -3.0
+            logits[r, rs.randint(vocab)] = -float("inf") if rs.rand() < 0.5 else float("nan")
+            held = logits[r, :vocab].float().cpu().numpy()
+            want[r] = np.where(np.isnan(held), -np.inf, held).argmax() if (held == -3).any() else (
+                np.flatnonzero(held == -np.inf)[0] if (held == -np.inf).any() else 0)
+    best, _ = greedy_rows(logits, vocab, vocab + gap)
+    np.testing.assert_array_equal(best.cpu().numpy(), want)
+    assert verify_error_word() == 0
+
+
+@pytest.mark.parametrize("rows", [9, 300])
+def test_greedy_rows_of_nan_take_no_longer(rows):
+    """What is in a row does not show in the time: NaN alone, or one -infinity at its end, as numbers."""
+    vocab = 128256
+    logits = torch.randn(rows, vocab, device="cuda", dtype=torch.bfloat16)
+    usual = graph_us(greedy_rows(logits, vocab, vocab)[1])
+    logits.fill_(float("nan"))
+    empty = graph_us(greedy_rows(logits, vocab, vocab)[1])
+    logits[:, -1] = -float("inf")
+    late = graph_us(greedy_rows(logits, vocab, vocab)[1])
+    assert max(empty, late) < 3 * usual, (usual, empty, late)
