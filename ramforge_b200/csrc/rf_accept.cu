@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       if ((double)s_u[j] * qc * mass < left) {
         if (lane == 0) s_path[j] = taken;
         __syncwarp();
-        node = j, taken++, tried = 0, off = 0.0, mass = 1.0, base = 0.0, whole = false;
+        node = j, taken++, tried = 0, off = 0.0, mass = 1.0, base = 0.0, whole = false, final = true;
         continue;
       }
       tried++;

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from ramforge_b200 import _lib, verify_error_word, verify_greedy
+from ramforge_b200 import _lib, verify_drafts, verify_error_word, verify_greedy
 
 from .test_gpu_accept import Case, same, torch
 
@@ -100,3 +100,21 @@ def test_greedy_rows_of_nan_take_no_longer(rows):
     logits[:, -1] = -float("inf")
     late = graph_us(greedy_rows(logits, vocab, vocab)[1])
     assert max(empty, late) < 3 * usual, (usual, empty, late)
+
+
+def test_a_leaf_behind_refused_drafts_takes_one_pass():
+    """Certain drafts behind the history: the last one stands after one or after two were refused, and nothing follows
+    it.  Either way the row of the history is summed up once and the last draft's once, so the times are alike."""
+    vocab = 4000000  # passes of 40 us each, beside which nothing else shows
+    p = torch.softmax(torch.randn(1, 4, vocab, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)), -1)
+    out, count = torch.full((4,), -7, device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+    tokens, parent = torch.tensor([5, 6, 7], device="cuda", dtype=torch.int32), torch.full((3,), -1, device="cuda", dtype=torch.int32)
+    u_next = torch.full((1,), 0.5, device="cuda")
+    times = []
+    for refused in (1, 2):
+        u = torch.where(torch.arange(3, device="cuda") < refused, 0.99, 0.0)
+        times.append(graph_us(lambda st: verify_drafts(
+            p.data_ptr(), 0, _lib.ACT_F32, vocab, 1, 3, tokens.data_ptr(), u.data_ptr(), u_next.data_ptr(), out.data_ptr(),
+            count.data_ptr(), parent_ptr=parent.data_ptr(), stream=st)))
+        assert count.item() == 1 and out[0].item() == 5 + refused and out[2:].tolist() == [-1, -1]
+    assert times[1] < 1.2 * times[0], times
