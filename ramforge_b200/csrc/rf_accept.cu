@@ -602,7 +602,8 @@ int rf_verify_drafts(const void* target, const void* draft, int prob_type, uint3
   a.accept_u = accept_u, a.next_u = next_u;
   RF_TRY(verify_error_ptr(&a.w.err));
   const uint32_t es = act_bytes(prob_type);
-  const bool vec = aligned_to(target, 16) && target_stride * es % 16 == 0 && aligned_to(draft, 16) && draft_stride * es % 16 == 0;
+  const bool vec = aligned_to(target, 16) && target_stride * es % 16 == 0 &&
+                   (!a.draft || (aligned_to(draft, 16) && draft_stride * es % 16 == 0));
   // Clusters of 16 for long rows, as far as the GPU has room for them at once (7, one for most of its processing clusters):
   // a tree of 24 over 128256 tokens 13.6 us with 8, 11.3 with 16, over 32000 9.1 and 9.3.
   a.ctas = n_seqs <= 7 && vocab >= 65536 ? kMostCtas : cluster_size(n_seqs, 2);

@@ -118,3 +118,23 @@ def test_a_leaf_behind_refused_drafts_takes_one_pass():
             count.data_ptr(), parent_ptr=parent.data_ptr(), stream=st)))
         assert count.item() == 1 and out[0].item() == 5 + refused and out[2:].tolist() == [-1, -1]
     assert times[1] < 1.2 * times[0], times
+
+
+@pytest.mark.parametrize("seqs,t", [(64, 4), (50, 0)])
+def test_rows_at_a_padded_stride_without_a_draft(seqs, t):
+    """Rows of an odd vocabulary at 16-byte places take no longer than rows of an even one, where no draft has rows."""
+    stride, times = 50264, []
+    p = torch.softmax(torch.randn(seqs, t + 1, stride, device="cuda", generator=torch.Generator(device="cuda").manual_seed(t)), -1)
+    out = torch.empty(seqs, t + 1, device="cuda", dtype=torch.int32)
+    count, tokens = torch.empty(seqs, device="cuda", dtype=torch.int32), torch.full((seqs, t), 9, device="cuda", dtype=torch.int32)
+    u, u_next = torch.full((seqs, t), 0.5, device="cuda"), torch.full((seqs,), 0.5, device="cuda")
+    for vocab in (50264, 50257):
+        times.append(graph_us(lambda st: verify_drafts(
+            p.data_ptr(), 0, _lib.ACT_F32, vocab, seqs, t, tokens.data_ptr(), u.data_ptr(), u_next.data_ptr(),
+            out.data_ptr(), count.data_ptr(), target_stride=stride, stream=st)))
+        row = p[:, 0, :vocab].double()
+        row[:, 9] = 0 if t else row[:, 9]
+        cum = row.cumsum(-1)
+        want = torch.searchsorted(cum, 0.5 * cum[:, -1:], right=True)[:, 0]
+        assert not count.any() and torch.equal(out[:, 0].long(), want)
+    assert times[1] < 1.15 * times[0], times
