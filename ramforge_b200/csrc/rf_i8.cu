@@ -9,7 +9,8 @@
 // launch, loads and one reduction the short ones.  Maximum and sum of squares need one reduction together, since
 // rounding is monotonic: max |f32(f32(s w) r)| = f32(max |f32(s w)| r).
 //
-// Launched to begin while the kernel before ends, as rf_verify.cu's are; what that one may write is read by plain loads.
+// Launched to begin while the kernel before ends, as rf_verify.cu's are; what that one may write, a norm's weights among it (rows back
+// in f32 are such), is read by plain loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(2048 / PER * TEAMS) rows_ring_kernel(RowsArgs 
 #pragma unroll
       for (int j = 0; j < 8; j += 4) {
         float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-        if (a.w && at[p] < n) f = __ldg(reinterpret_cast<const float4*>(a.w + at[p] + j));
+        if (a.w && at[p] < n) f = *reinterpret_cast<const float4*>(a.w + at[p] + j);
         w[p][j] = f.x, w[p][j + 1] = f.y, w[p][j + 2] = f.z, w[p][j + 3] = f.w;
       }
   }
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(2048 / PER) rows_shift_kernel(RowsArgs a, uint
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const uint32_t e = (tid + p * nt) * 8 + j;
-        f[p][j] = a.w && e < n ? __ldg(a.w + e) : 1.f;
+        f[p][j] = a.w && e < n ? a.w[e] : 1.f;
       }
 #pragma unroll
     for (int p = 0; p < PER; p++)
@@ -672,6 +673,12 @@ __global__ void __launch_bounds__(1024) rows_shift_cta_kernel(RowsArgs a) {
 
 // ---- many short rows: a warp a row ---------------------------------------------------
 // PER eights a lane, or, where rows are not aligned, every 32nd element; the next row's are asked for before a row is worked on.
+// *p where `on`, else 1 and nothing is read.  A plain load of C++ would stay behind the stores of the sums.
+__device__ __forceinline__ float weight_if(bool on, const float* p) {
+  float w = 1.f;
+  asm volatile("{ .reg .pred q; setp.ne.u32 q, %2, 0;\n\t@q ld.global.f32 %0, [%1]; }" : "+f"(w) : "l"(p), "r"((uint32_t)on));
+  return w;
+}
 template <class T, int MODE, int PER, bool VEC>
 __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_rows) {
   griddep_launch();
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
             if (place(p, 0) < n) {
 #pragma unroll
               for (int j = 0; j < 8; j += 4) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(a.w + place(p, j)));
+                const float4 f = *reinterpret_cast<const float4*>(a.w + place(p, j));
                 v[p][j] = __fmul_rn(v[p][j], f.x), v[p][j + 1] = __fmul_rn(v[p][j + 1], f.y);
                 v[p][j + 2] = __fmul_rn(v[p][j + 2], f.z), v[p][j + 3] = __fmul_rn(v[p][j + 3], f.w);
               }
@@ -757,7 +764,7 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
           } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-              if (place(p, j) < n) v[p][j] = __fmul_rn(v[p][j], __ldg(a.w + place(p, j)));
+              v[p][j] = __fmul_rn(v[p][j], weight_if(place(p, j) < n, a.w + place(p, j)));
           }
         }
       }
