@@ -481,8 +481,8 @@ int rf_verify_error_word(uint32_t* word);
 int rf_norm_i8(const void* x, const void* add, void* sum, int act_type, uint32_t n_rows, uint32_t n_cols,
                uint64_t x_stride, uint64_t add_stride, uint64_t sum_stride, const float* weight, float eps, int8_t* q,
                uint64_t q_stride, float* scale, void* stream);
-/* y = gate / (1 + exp(-gate)) * up (the SwiGLU of compute.rs:347) as 8-bit rows; y within |gate| + 10
- * units of f32's last place, 0 for gate below -87.  gate and up may be slices of one projection's rows. */
+/* y = gate / (1 + exp(-gate)) * up (the SwiGLU of compute.rs:347) as 8-bit rows; y within
+ * (1.25 |gate| + 12) 2^-24 of its size, 0 for gate below -87.34.  gate and up may be slices of one projection's rows. */
 int rf_swiglu_i8(const void* gate, const void* up, int act_type, uint32_t n_rows, uint32_t n_cols, uint64_t gate_stride,
                  uint64_t up_stride, int8_t* q, uint64_t q_stride, float* scale, void* stream);
 /* Rows as they are into the format (weights: one row a channel), and back: out = code * scale. */
