@@ -476,8 +476,9 @@ int rf_verify_error_word(uint32_t* word);
 /* s = x + add in f32 (add NULL: s = x), rounded to act_type in sum (may be NULL, or x or add itself with the same
  * stride); then the rows y = (s * weight) * (1 / sqrt(mean(s^2) + eps)) of the f32 sums s
  * as 8-bit rows: products and reciprocal root rounded to f32, the mean in 64 bits, so that
- * the codes do not depend on how the work was split.  weight: n_cols f32, NULL: ones.  A row of
- * zeros with eps 0 counts as one that is not finite. */
+ * how the work was split shows only where the last bits of that mean decide how the root is
+ * rounded.  weight: n_cols f32, NULL: ones.  With eps 0 a row of zeros, or of numbers so small
+ * that the root is beyond f32, counts as one that is not finite. */
 int rf_norm_i8(const void* x, const void* add, void* sum, int act_type, uint32_t n_rows, uint32_t n_cols,
                uint64_t x_stride, uint64_t add_stride, uint64_t sum_stride, const float* weight, float eps, int8_t* q,
                uint64_t q_stride, float* scale, void* stream);
@@ -523,8 +524,9 @@ int rf_i8_matmul(const int8_t* x, const float* x_scale, const int8_t* w, const f
  * stand changes them to a = a + S (0 at first), r = max(p - a q, 0), S = sum r (certain drafts:
  * r(c) = 0).  Where none is left, the next token is the least x with r(0) + ... + r(x) > next_u[b] * S, S = sum r
  * (r = p again where nothing of it is left; numbers below 0 and NaN in p count as 0).  Products and sums in 64
- * bits.  accept_u [n_seqs][n_tokens] and next_u [n_seqs] are uniform in [0, 1).  A row of the target
- * without a number above 0 gives the token -1 and raises the error word. */
+ * bits: beside a draft's rows, what refusals leave of p below some 2^-48 of it is rounding.  accept_u
+ * [n_seqs][n_tokens] and next_u [n_seqs] are uniform in [0, 1).  A row of the target without a number above 0
+ * gives the token -1 and raises the error word. */
 int rf_verify_drafts(const void* target, const void* draft, int prob_type, uint32_t vocab, uint32_t n_seqs,
                      uint32_t n_tokens, uint64_t target_stride, uint64_t draft_stride, const int32_t* tokens,
                      const int32_t* parent, const int32_t* n_draft, const float* accept_u, const float* next_u,

@@ -10,8 +10,9 @@
 // (p_k = r_k / S_k, and (p_k - q)+ = (p - a_k q - S_k q)+ / S_k).  When no more are left, the next token is the least
 // x with r(0) + ... + r(x) > u S.  Drafts without probabilities are certain of their token: q is 1 there.
 //
-// Products and sums are taken in 64 bits: p and q are at most 32-bit numbers, so u q is exact, and which side of a
-// border a number lies on does not depend on the order of the sums.
+// Products and sums are taken in 64 bits: p and q are at most 32-bit numbers, so u q is exact, and on which side of a
+// border a number lies depends on the order of the sums (which follows the number of CTAs a sequence) only where their last
+// bits decide.  r is one fused operation, but a and S are sums: what 2^-48 of p and less is left of it is rounding.
 #include <algorithm>
 #include <type_traits>
 

@@ -2,8 +2,8 @@
 // rows into the format, and the rows back.  The product of such rows with an 8-bit matrix is in rf_i8_matmul.cu.
 //
 // The format (rfcuda.h) fixes every rounding from the row's f32 numbers to its codes, and the norm's are fixed up to
-// the sum of squares, which is taken in 64 bits: its order does not show in the 32-bit reciprocal root, so a row's
-// codes do not depend on how the row was split over threads.
+// the sum of squares, which is taken in 64 bits: how the row was split over threads shows in a row's codes only where the
+// last of those bits decide how the 32-bit reciprocal root is rounded (one sum in some 2^25 lies that near to a border).
 //
 // One read and one write of each element, a handful of operations between: HBM bounds the long calls, latency of
 // launch, loads and one reduction the short ones.  Maximum and sum of squares need one reduction together, since
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(2048 / PER) rows_shift_kernel(RowsArgs a, uint
 
 // ---- rows that are not aligned, without a norm: a CTA a row -------------------------------------
 // The eights of rows_shift_kernel straight from global memory: where there is no sum of squares the instructions are few
-// enough that more threads hide the loads better than the ring does, up to rows that leave one CTA an SM.
+// enough that more threads hide the loads as well as the ring does, or better; launch_rows_as has both sides.
 template <class T, int MODE, int PER>
 __global__ void __launch_bounds__(1024) rows_shift_cta_kernel(RowsArgs a) {
   constexpr int V = Act<T>::kVec, W = 8 / V;
@@ -673,7 +673,8 @@ __global__ void __launch_bounds__(1024) rows_shift_cta_kernel(RowsArgs a) {
 
 // ---- many short rows: a warp a row ---------------------------------------------------
 // PER eights a lane, or, where rows are not aligned, every 32nd element; the next row's are asked for before a row is worked on.
-// *p where `on`, else 1 and nothing is read.  A plain load of C++ would stay behind the stores of the sums.
+// *p where `on`, else 1 and nothing is read.  A plain load of C++ would stay behind the stores of the sums (4000 x 501 f32 with
+// residual and sum: 9.7 us, 8.1 so).
 __device__ __forceinline__ float weight_if(bool on, const float* p) {
   float w = 1.f;
   asm volatile("{ .reg .pred q; setp.ne.u32 q, %2, 0;\n\t@q ld.global.f32 %0, [%1]; }" : "+f"(w) : "l"(p), "r"((uint32_t)on));
@@ -793,7 +794,9 @@ __global__ void __launch_bounds__(256) rows_warp_kernel(RowsArgs a, uint32_t n_r
 template <class T, int MODE, bool VEC>
 cudaError_t launch_cta(const Launch& L, const RowsArgs& a, uint32_t n_rows) {
   const uint32_t eights = (a.n_cols + 7) / 8;
-  // 16 elements a thread, more where 1024 threads do not suffice
+  // 16 elements a thread, more where 1024 threads do not suffice: those do not fit the 64 registers that 1024 threads have, so norms
+  // and single elements of more than 16384 columns (aligned SwiGLU and plain rows: 32768) go through local memory.  300 rows with residual and sum,
+  // bf16: 16384 columns 13.6 us, 20480 28.5, 40960 105, 40961 313; SwiGLU of 300 x 20480 9.1, x 40960 18.9.
   const uint32_t per = eights <= 2048 ? 2 : eights <= 4096 ? 4 : 8;
   const uint32_t threads = std::max(32u, ((eights + per - 1) / per + 31) / 32 * 32);
   auto* k = per == 2 ? rows_cta_kernel<T, MODE, 2, VEC> : per == 4 ? rows_cta_kernel<T, MODE, 4, VEC> : rows_cta_kernel<T, MODE, 8, VEC>;
@@ -812,7 +815,10 @@ cudaError_t launch_rows_as(const Launch& L, const RowsArgs& a, uint32_t n_rows, 
       if (per > 2) k = rows_warp_kernel<T, MODE, 4, VEC>;
     return launch_k(L, k, dim3(std::min((n_rows + 7) / 8, sms * 4)), dim3(256), 0, a, n_rows);
   }
-  // CTAs that stay, per_sm of them on each SM: as many as its registers and shared memory have room for
+  // CTAs that stay, per_sm of them on each SM.  What is counted is their threads and the shared memory they ask for, not the 384 to
+  // 896 bytes that the kernel has besides and the 1 KB that each CTA takes: at the widths at which that makes one too many
+  // the last ones run when the others have ended (norm of 4000 rows with residual, f32: 14.3 us with 1152 columns, 11.6 with
+  // 1200; 25.8 with 2368, 20.2 with 2392).
   auto ring = [&](auto* k, uint32_t threads, uint32_t smem, uint32_t per_sm, auto... more) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
     return e != cudaSuccess ? e : launch_k(L, k, dim3(sms * per_sm), dim3(threads), smem, a, n_rows, more..., err);
@@ -839,12 +845,18 @@ cudaError_t launch_rows_as(const Launch& L, const RowsArgs& a, uint32_t n_rows, 
     const uint32_t stage = shift_x_bytes(a.n_cols, es) + (a.y ? shift_y_bytes(a.n_cols, es) : 0);
     const uint32_t smem = kRowStages * stage + (MODE == kNorm ? (shift_eights(a.n_cols) + 1) * 8 * 4 : 0);
     const uint32_t some = std::min(std::min(std::min(TH / threads, kRingBytes / smem), 16u), n_rows / sms);
-    // a norm of 4001 x 4095 bf16: 32.8 us, element by element in a CTA a row 61.4; SwiGLU of 2048 x 14335: 40.7 and 91.2
+    // A norm in the ring and element by element in a CTA a row, bf16: 4001 x 4095 32.8 us and 61.4, 296 x 1025 3.8 and 4.4, 592 x
+    // 1023 4.3 and 5.2 (444 x 1023, a CTA a row by the rule: 4.1 and 6.2).  SwiGLU in the ring and a CTA a row, bf16: 2048 x
+    // 14335 40.7 and 91.2 (by elements); 4000 x 2799 16.4 and 15.8, x 2801 15.7 and 15.5, x 4095 22.7 and 23.9; 592 x 4095 5.6 and
+    // 5.5; 296 x 4097 3.3 both, x 8191 5.9 and 6.2.  Plain rows, bf16: 4000 x 2801 12.9 and 11.2 (10.0 with two eights), x 4095 18.6
+    // and 17.5 (14.8); 296 x 8191 3.4 and 2.7: there the ring comes too early.
     const uint32_t least = (MODE == kNorm ? a.n_cols < 1024 : a.n_cols <= 4096) ? 4 * sms : 2 * sms;
     if (threads <= 2048 / PER && some && n_rows >= least && (MODE == kNorm || a.n_cols > 2800))
       return ring(rows_shift_kernel<T, MODE, PER>, threads, smem, some);
     if constexpr (MODE != kNorm) {
-      // SwiGLU of 2500 x 1279 bf16: 6.9 us with an eight a thread, 7.4 with two, 8.1 in the ring; 1200 x 8191: 30.4, 25.4 and 16.1
+      // SwiGLU of 2500 x 1279 bf16: 6.9 us with an eight a thread, 7.4 with two, 8.1 in the ring; 1200 x 4097: 8.9, 9.5 and 8.9;
+      // 1200 x 8191: 24.8 (12.4 with 592 rows) and 16.1 (9.4) in the ring; 592 x 515: 2.6 with an eight a thread, 3.2 by elements,
+      // 592 x 509: 2.6 and 3.4 (by elements by the rule).
       const uint32_t one = (shift_eights(a.n_cols) + kOwnLanes - 1) / kOwnLanes * 32;
       if (a.n_cols >= 512 && a.n_cols <= 4096) return launch_k(L, rows_shift_cta_kernel<T, MODE, 1>, dim3(n_rows), dim3(one), 0, a);
       if (a.n_cols >= 512 && threads <= 1024) return launch_k(L, rows_shift_cta_kernel<T, MODE, 2>, dim3(n_rows), dim3(threads), 0, a);

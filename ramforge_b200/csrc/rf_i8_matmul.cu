@@ -602,7 +602,8 @@ int run_split(cudaStream_t st, const MatmulArgs& a, unsigned* err) {
 
 // The tile's columns are those for which a model of the call says it is fastest: 256 elements take a pair
 // 0.2 us and 1.8 ns a column, at least 0.28, and a tile's results 0.6 us and 9 ns a column; the longer of the two
-// counts in each round, and the results of the last one besides.  333 tokens, 4096 x 4096: 14.7 us with tiles of
+// counts in each round, and the results of the last one besides; the bytes of W are not in it (128 tokens, 128256 x 4096: 50 us by
+// the model, 87 measured, 86 by the bytes).  333 tokens, 4096 x 4096: 14.7 us with tiles of
 // 192, 11.8 with 128, 11.2 with 96, 15.7 with 64 (two rounds); 3718 tokens, 6016 x 192: 37.4 with 32, 24.6 with 64,
 // 19.7 with 128, 17.1 with 256.
 template <class T>
