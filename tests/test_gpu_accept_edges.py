@@ -28,7 +28,7 @@ def test_little_left_behind_certain_drafts():
 
 
 def graph_us(fn, calls=20):
-    """Microseconds of a call among others, the least of five."""
+    """Microseconds of a call among others, the least of fifteen."""
     fn(torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -36,7 +36,7 @@ def graph_us(fn, calls=20):
         for _ in range(calls):
             fn(torch.cuda.current_stream().cuda_stream)
     times = []
-    for _ in range(5):
+    for _ in range(15):
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         a.record()
         graph.replay()
